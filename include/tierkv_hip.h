@@ -47,6 +47,7 @@ extern "C" {
 
 #define TIERKV_DTYPE_F16 0
 #define TIERKV_DTYPE_BF16 1
+#define TIERKV_DTYPE_F32 2 /* logits of tierkv_sample_tokens only */
 
 #define TIERKV_WARM_REF_U8 0
 #define TIERKV_WARM_ABSMAX_I8 1
@@ -417,6 +418,102 @@ typedef struct TierkvDecodeStep {
 
 TIERKV_API int32_t tierkv_decode_step(const TierkvDecodeStep* step, void* stream);
 TIERKV_API int64_t tierkv_decode_step_size(void);
+
+/* ---------------------------------------------------------------------- */
+/* A serving step over requests of different lengths.  The reference serves
+ * one sequence per table (tierkv_policy.py:1768-1816, modeling_llama.py:
+ * 419-456); these take a batch whose requests bring different numbers of new
+ * tokens, packed as rows: request b's are rows [cu[b], cu[b + 1]). */
+
+/* Table entries of the new tokens' blocks, and where each packed row goes.
+ * new_tokens int32 [batch] (device) tokens per request, >= 0.  The open block
+ * (open_blocks[b] != 0, last, HOT, not full) is filled first, then new HOT
+ * blocks are popped from hot_free [hot_slots] in (request, block) order;
+ * block_table / block_states / block_lengths [batch, table_stride],
+ * seq_num_blocks, open_blocks and ctl are updated as by tierkv_runtime_append
+ * (a request without new tokens keeps all of its words).  Outputs:
+ *   slots     int32 [num_rows] slot * block_size + position of each row, -1
+ *             for rows behind the last request
+ *   positions int32 [num_rows] the row's position in its request, or -1
+ *   cu_tokens int32 [batch + 1] first row of each request
+ *   context   int32 [batch] tokens each request holds after the step
+ * All or nothing: when the stack or a table row is too short, a length is
+ * negative or there are more tokens than num_rows (error bit 16), the tables
+ * stay as they are, every row is -1, cu_tokens is 0 and ctl[3] is 0.
+ * batch <= 4096.  slots, positions and workspace 16-byte aligned; workspace:
+ * tierkv_slot_map_workspace_bytes(batch) bytes, no initialisation needed. */
+TIERKV_API int64_t tierkv_slot_map_workspace_bytes(int32_t batch);
+TIERKV_API int32_t tierkv_build_slot_map(
+    const int32_t* new_tokens, int32_t batch, int32_t num_rows,
+    int32_t* block_table, int32_t* block_states, int32_t* block_lengths, int64_t table_stride,
+    int32_t* seq_num_blocks, int32_t* open_blocks, const int32_t* hot_free, int64_t hot_slots, int32_t* ctl,
+    int32_t block_size, int32_t* slots, int32_t* positions, int32_t* cu_tokens, int32_t* context,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Copy packed K/V rows into HOT slots: row r of key / value [num_rows,
+ * kv_heads, head_dim] (fp16 or bf16, element strides, head_dim contiguous)
+ * becomes row slots[r] = slot * block_size + position of hot_k / hot_v, in
+ * fp16 (bf16 values past its range become infinities).  Rows whose slot is
+ * negative or outside the pool are skipped; slots that are written are
+ * distinct.  write_hot_tokens (tierkv_policy.py:934-967) by rows. */
+TIERKV_API int32_t tierkv_write_slots(
+    const void* key, int64_t k_stride_t, int64_t k_stride_h, const void* value, int64_t v_stride_t, int64_t v_stride_h,
+    int32_t dtype, const int32_t* slots, int32_t num_rows, void* hot_k, void* hot_v, int64_t hot_slots,
+    int32_t num_kv_heads, int32_t block_size, int32_t head_dim, void* stream);
+
+/* Attention of several query tokens per request over the tiered cache.
+ * Request b's query rows [cu_tokens[b], cu_tokens[b + 1]) are the last n_b of
+ * the L_b tokens that its row of the tables holds (valid tokens of all blocks
+ * below its block count, evicted ones included); row i sees the tokens up to
+ * its own, ordinals 0 .. L_b - n_b + i, with the tiers, WARM formats and COLD
+ * modes of tierkv_decode_attention.  A row that sees nothing becomes 0; rows
+ * of out behind the last request are not written.
+ *   query  [num_rows, num_heads, head_dim], fp16 / bf16, element strides that
+ *          are multiples of 8, head_dim contiguous, 16-byte aligned
+ *   out    [num_rows, num_heads, head_dim] contiguous, the query's dtype
+ *   max_tokens  an upper bound of the requests' new tokens (num_rows will do):
+ *          with it small calls launch less; rows past it are not computed
+ * head_dim a multiple of 8 up to 128, block_size up to 64, any GQA group.
+ * The same inputs give the same bits on every call.  workspace: as
+ * tierkv_decode_attention's (one buffer may serve both, in stream order), at
+ * least tierkv_extend_workspace_bytes(...) bytes, zero-filled before its
+ * first use; the error word is set as there when a block is skipped. */
+TIERKV_API int64_t tierkv_extend_workspace_bytes(int32_t batch, int32_t num_rows, int32_t max_tokens,
+                                                 int32_t num_heads, int32_t num_kv_heads, int32_t num_blocks,
+                                                 int32_t block_size, int32_t head_dim);
+TIERKV_API int32_t tierkv_extend_attention(
+    const void* query, int64_t q_stride_t, int64_t q_stride_h, int32_t query_dtype, void* out,
+    const int32_t* cu_tokens, int32_t num_rows, int32_t max_tokens,
+    const int32_t* block_table, const int32_t* block_states, const int32_t* block_lengths, int64_t table_stride,
+    const int32_t* seq_num_blocks, int32_t num_blocks,
+    const void* hot_k, const void* hot_v, int64_t hot_slots,
+    const void* warm_k, const void* warm_v, int64_t warm_slots,
+    const void* k_scale, const void* k_zero, const void* v_scale, const void* v_zero,
+    int32_t warm_format, int32_t cold_mode,
+    int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t block_size, int32_t head_dim, float scaling,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Next tokens from logits [batch, vocab] (fp16, bf16 or fp32, rows
+ * row_stride elements apart) and one random number in [0, 1) per row.
+ * Weights are whole numbers W_i = rint(2^42 exp((x_i - max x) / T)), 0 for
+ * -inf and NaN.  Of the tokens in the order (logit descending, index
+ * ascending): the first top_k (off when <= 0); of these those whose sum of
+ * weights before them is below top_p times their total, one at least (off
+ * when >= 1); of these those with W_i >= 2^42 min(min_p, 1).  tokens[b] is
+ * the smallest index whose running sum of what is left, in index order,
+ * exceeds floor(uniforms[b] * total); probs (or NULL) gets W / total.
+ * temperature <= 0 (or NaN) takes the first of the largest logits, with
+ * probability 1; a row with no logit above -inf gives token -1, probability
+ * 0.  Each limit is a device array [batch] or, where that is NULL, one value
+ * for all rows.  vocab <= 2^20.  The same inputs give the same tokens on
+ * every call.  workspace: tierkv_sample_workspace_bytes(batch, vocab) bytes,
+ * 16-byte aligned, no initialisation needed. */
+TIERKV_API int64_t tierkv_sample_workspace_bytes(int32_t batch, int32_t vocab);
+TIERKV_API int32_t tierkv_sample_tokens(
+    const void* logits, int32_t dtype, int64_t row_stride, int32_t batch, int32_t vocab, const float* uniforms,
+    const float* temperature, float temperature_all, const int32_t* top_k, int32_t top_k_all,
+    const float* top_p, float top_p_all, const float* min_p, float min_p_all,
+    int64_t* tokens, float* probs, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------- */
 /* Block scores.  Per-block probability mass from softmax probabilities

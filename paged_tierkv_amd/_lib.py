@@ -27,6 +27,7 @@ TIERKV_ERR_STATE = 5
 
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
+DTYPE_F32 = 2
 WARM_REF_U8 = 0
 WARM_ABSMAX_I8 = 1
 COLD_ZERO_LOGIT = 0
@@ -150,6 +151,34 @@ SIGNATURES = {
     "tierkv_block_mass_from_probs": (c_int32, [_P, _P, _P, c_int32, c_int32, c_int32, c_int32, _P]),
     "tierkv_block_scores_from_sums": (c_int32, [_P, c_int64, _P, c_int64, _P, c_int32, c_int32, c_int32, _P]),
     "tierkv_tier_labels": (c_int32, [_P, _P, _P, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, _P]),
+    "tierkv_slot_map_workspace_bytes": (c_int64, [c_int32]),
+    "tierkv_build_slot_map": (c_int32, [
+        _P, c_int32, c_int32,
+        _P, _P, _P, c_int64,
+        _P, _P, _P, c_int64, _P,
+        c_int32, _P, _P, _P, _P,
+        _P, c_int64, _P]),
+    "tierkv_write_slots": (c_int32, [
+        _P, c_int64, c_int64, _P, c_int64, c_int64,
+        c_int32, _P, c_int32, _P, _P, c_int64,
+        c_int32, c_int32, c_int32, _P]),
+    "tierkv_extend_workspace_bytes": (c_int64, [c_int32] * 8),
+    "tierkv_extend_attention": (c_int32, [
+        _P, c_int64, c_int64, c_int32, _P,
+        _P, c_int32, c_int32,
+        _P, _P, _P, c_int64, _P, c_int32,
+        _P, _P, c_int64,
+        _P, _P, c_int64,
+        _P, _P, _P, _P,
+        c_int32, c_int32,
+        c_int32, c_int32, c_int32, c_int32, c_int32, c_float,
+        _P, c_int64, _P]),
+    "tierkv_sample_workspace_bytes": (c_int64, [c_int32, c_int32]),
+    "tierkv_sample_tokens": (c_int32, [
+        _P, c_int32, c_int64, c_int32, c_int32, _P,
+        _P, c_float, _P, c_int32,
+        _P, c_float, _P, c_float,
+        _P, _P, _P, c_int64, _P]),
     "tierkv_bm_create": (c_int32, [c_int32, POINTER(c_void_p)]),
     "tierkv_bm_destroy": (None, [_P]),
     "tierkv_bm_allocate_block": (c_int32, [_P, c_int32, _I32P]),

@@ -53,6 +53,11 @@ HIP_SOURCES = {
     # MFMA accumulators in ordinary VGPRs: the logits are consumed by VALU
     # code right away, and accumulators in AGPRs cost a copy per element.
     "prefill_score.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    # As above: logits and outputs are scaled by VALU code every tile.
+    "extend_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "slot_map.hip": [],
+    # Weights are whole numbers that follow from one product and one rounding.
+    "sampling.hip": ["-ffp-contract=off"],
 }
 CXX_SOURCES = ["block_manager.cpp"]
 

@@ -1,11 +1,14 @@
 """Python entry points of the demotion, promotion, block-score and label
-kernels (C ABI in include/tierkv_hip.h).
+kernels, and of a serving step's slot map, K/V row write and token choice (C
+ABI in include/tierkv_hip.h).
 
 All tensors are GPU tensors; index arrays are int32.  Launches are
 asynchronous on the current stream.
 """
 
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
@@ -221,3 +224,170 @@ def prefill_block_mass(query_states: torch.Tensor, key_states: torch.Tensor, blo
         tokens, dim, int(block_size), float(scaling), _lib.ptr(ws), need, _lib.stream_of(q.device))
     _lib.check(rc, "tierkv_prefill_block_mass")
     return out
+
+
+# One scratch buffer per (operator, device, stream), as the prefill scores':
+# launches on one stream are ordered; launches on different streams may
+# overlap and never share it.  A captured call takes scratch of its own from
+# its graph's memory, so that graphs replayed on different streams, and eager
+# calls beside them, share none.
+_scratch_ws: dict = {}
+
+
+def _scratch(name: str, device, need: int) -> torch.Tensor:
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(max(need, 256), dtype=torch.uint8, device=device)
+    key = (name, device.index, _lib.stream_of(device))
+    ws = _scratch_ws.get(key)
+    if ws is None or ws.numel() < need:
+        ws = _scratch_ws[key] = torch.empty(max(need, 256), dtype=torch.uint8, device=device)
+    return ws
+
+
+class SlotMap(NamedTuple):
+    """``build_slot_map``'s outputs (all int32, on the tables' device)."""
+
+    slots: torch.Tensor       # [num_tokens] slot * block_size + position of each packed row, -1 behind the last request
+    positions: torch.Tensor   # [num_tokens] the row's position in its request, or -1
+    cu_tokens: torch.Tensor   # [B + 1] first packed row of each request
+    context: torch.Tensor     # [B] tokens each request holds after the step
+
+
+def _require_i32(t, name: str, shape=None) -> None:
+    _lib.require_gpu_tensor(t, name)
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor.")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}.")
+
+
+def build_slot_map(new_tokens: torch.Tensor, block_table: torch.Tensor, block_states: torch.Tensor,
+                   block_lengths: torch.Tensor, seq_num_blocks: torch.Tensor, open_blocks: torch.Tensor,
+                   hot_free: torch.Tensor, ctl: torch.Tensor, block_size: int, num_tokens: int) -> SlotMap:
+    """Table entries and slot map of a step in which request b brings
+    ``new_tokens[b]`` tokens (``tierkv_build_slot_map``): its open block is
+    filled first, then new HOT blocks are popped from ``hot_free``; the tables
+    ``[B, max_blocks]``, ``seq_num_blocks``, ``open_blocks`` ``[B]`` and ``ctl``
+    ``[4]`` are updated in place, as ``BatchedTieredKVRuntime`` holds them.
+    ``num_tokens`` is the number of packed rows (at least the lengths' sum;
+    rows behind the last request get slot -1).  All or nothing: a step that
+    does not fit changes no table, sets an error bit in ``ctl[2]`` and gives
+    every row slot -1."""
+    lib = _lib.lib()
+    _lib.require_gpu_tensor(block_table, "block_table")
+    if block_table.ndim != 2:
+        raise ValueError("block_table must be [batch, max_blocks].")
+    batch, stride = (int(x) for x in block_table.shape)
+    for name, t in (("block_table", block_table), ("block_states", block_states), ("block_lengths", block_lengths)):
+        _require_i32(t, name, (batch, stride))
+    for name, t in (("new_tokens", new_tokens), ("seq_num_blocks", seq_num_blocks), ("open_blocks", open_blocks)):
+        _require_i32(t, name, (batch,))
+    _require_i32(hot_free, "hot_free")
+    _require_i32(ctl, "ctl", (4,))
+    device = block_table.device
+    tensors = (new_tokens, block_states, block_lengths, seq_num_blocks, open_blocks, hot_free, ctl)
+    if any(t.device != device for t in tensors):
+        raise ValueError("the slot map's tensors must be on one device.")
+    rows = int(num_tokens)
+    if rows < 0:
+        raise ValueError("num_tokens must not be negative.")
+    new = lambda n: torch.empty(n, dtype=torch.int32, device=device)
+    out = SlotMap(new(rows), new(rows), new(batch + 1), new(batch))
+    need = int(lib.tierkv_slot_map_workspace_bytes(batch))
+    with torch.cuda.device(device):
+        ws = _scratch("slot_map", device, need)
+        rc = lib.tierkv_build_slot_map(
+            _lib.ptr(new_tokens), batch, rows, _lib.ptr(block_table), _lib.ptr(block_states), _lib.ptr(block_lengths),
+            stride, _lib.ptr(seq_num_blocks), _lib.ptr(open_blocks), _lib.ptr(hot_free), int(hot_free.numel()),
+            _lib.ptr(ctl), int(block_size), _lib.ptr(out.slots), _lib.ptr(out.positions), _lib.ptr(out.cu_tokens),
+            _lib.ptr(out.context), _lib.ptr(ws), int(ws.numel()), _lib.stream_of(device))
+    _lib.check(rc, "tierkv_build_slot_map")
+    return out
+
+
+def write_slots(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, hot_k: torch.Tensor,
+                hot_v: torch.Tensor) -> None:
+    """Copy packed K/V rows ``[N, kv_heads, head_dim]`` (fp16 / bf16, any
+    strides with head_dim contiguous, e.g. columns of a fused projection) into
+    the HOT pool rows ``slots`` (``build_slot_map``; negative: skipped)."""
+    lib = _lib.lib()
+    _check_tiles(hot_k, "hot_k", torch.float16)
+    _check_tiles(hot_v, "hot_v", torch.float16)
+    kv_heads, bs, dim = (int(x) for x in hot_k.shape[1:])
+    if hot_v.shape != hot_k.shape:
+        raise ValueError("K and V pools must have identical shapes.")
+    _lib.require_gpu_tensor(key, "key")
+    _lib.require_gpu_tensor(value, "value")
+    if key.dtype not in (torch.float16, torch.bfloat16) or value.dtype != key.dtype:
+        raise ValueError("key and value must share an fp16 / bf16 dtype.")
+    if key.ndim != 3 or value.shape != key.shape or tuple(key.shape[1:]) != (kv_heads, dim):
+        raise ValueError("key and value must be [tokens, kv_heads, head_dim] of the pools' geometry.")
+    rows = int(key.shape[0])
+    _require_i32(slots, "slots", (rows,))
+    device = hot_k.device
+    if any(t.device != device for t in (key, value, slots, hot_v)):
+        raise ValueError("rows, slots and pools must be on one device.")
+    if rows == 0:
+        return
+    k = key if key.stride(-1) == 1 or dim == 1 else key.contiguous()
+    v = value if value.stride(-1) == 1 or dim == 1 else value.contiguous()
+    with torch.cuda.device(device):
+        rc = lib.tierkv_write_slots(
+            _lib.ptr(k), k.stride(0), k.stride(1), _lib.ptr(v), v.stride(0), v.stride(1),
+            _lib.DTYPE_BF16 if k.dtype == torch.bfloat16 else _lib.DTYPE_F16, _lib.ptr(slots), rows,
+            _lib.ptr(hot_k), _lib.ptr(hot_v), int(hot_k.shape[0]), kv_heads, bs, dim, _lib.stream_of(device))
+    _lib.check(rc, "tierkv_write_slots")
+
+
+_LOGIT_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+
+
+def _limit(x, name: str, batch: int, device, dtype, low=None, high=None):
+    """A sampling limit: (device tensor or None, value for all rows)."""
+    if isinstance(x, torch.Tensor):
+        if x.device != device or tuple(x.shape) != (batch,):
+            raise ValueError(f"{name} must be a number or one value per row on the logits' device.")
+        return x.to(dtype).contiguous(), 0
+    if x != x or (low is not None and x < low) or (high is not None and x > high):
+        raise ValueError(f"{name} is out of range.")
+    return None, x
+
+
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Next tokens of logits ``[B, vocab]`` (fp16 / bf16 / fp32) with one random
+    number in [0, 1) per row (``tierkv_sample_tokens``): temperature, then the
+    first ``top_k`` tokens (0: all), of these the smallest set of the likeliest
+    that holds ``top_p`` of their probability, of these those at least
+    ``min_p`` times as likely as the likeliest; equal logits rank by index.
+    The token is the first, in index order, whose running sum of what is left
+    exceeds the random number's share.  Each limit is a number or a tensor
+    ``[B]``; temperature 0 takes the likeliest token.  Returns (int64 tokens
+    [B], fp32 probabilities [B] the tokens were drawn with); a row without a
+    logit above -inf gives token -1."""
+    lib = _lib.lib()
+    _lib.require_gpu_tensor(logits, "logits")
+    _lib.require_gpu_tensor(uniforms, "uniforms")
+    if logits.ndim != 2 or logits.dtype not in _LOGIT_DTYPES or not logits.numel():
+        raise ValueError("logits must be fp16, bf16 or fp32 [batch, vocab].")
+    batch, vocab = (int(x) for x in logits.shape)
+    device = logits.device
+    if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (batch,) or uniforms.device != device:
+        raise ValueError("uniforms must be one fp32 number per row on the logits' device.")
+    t, t_all = _limit(temperature, "temperature", batch, device, torch.float32, low=0.0)
+    k, k_all = _limit(top_k, "top_k", batch, device, torch.int32)
+    p, p_all = _limit(top_p, "top_p", batch, device, torch.float32, low=0.0)
+    m, m_all = _limit(min_p, "min_p", batch, device, torch.float32, low=0.0, high=1.0)
+    x = logits if logits.stride(1) == 1 and (batch == 1 or logits.stride(0) >= vocab) else logits.contiguous()
+    u = uniforms.contiguous()
+    tokens = torch.empty(batch, dtype=torch.int64, device=device)
+    probs = torch.empty(batch, dtype=torch.float32, device=device)
+    need = int(lib.tierkv_sample_workspace_bytes(batch, vocab))
+    with torch.cuda.device(device):
+        ws = _scratch("sample", device, need)
+        rc = lib.tierkv_sample_tokens(
+            _lib.ptr(x), _LOGIT_DTYPES[x.dtype], x.stride(0), batch, vocab, _lib.ptr(u),
+            _lib.ptr(t), float(t_all), _lib.ptr(k), min(max(int(k_all), 0), 0x7fffffff), _lib.ptr(p), float(p_all),
+            _lib.ptr(m), float(m_all), _lib.ptr(tokens), _lib.ptr(probs), _lib.ptr(ws), int(ws.numel()),
+            _lib.stream_of(device))
+    _lib.check(rc, "tierkv_sample_tokens")
+    return tokens, probs

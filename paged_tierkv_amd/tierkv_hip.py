@@ -534,3 +534,151 @@ def _launch(lib, args, device, ws) -> None:
             raise RuntimeError(f"TierKV decode skipped blocks with out-of-range slot/state (flag {word}).")
 
 
+def tierkv_extend_attention(
+    query_states: torch.Tensor,
+    cu_tokens: torch.Tensor,
+    block_table: torch.Tensor,
+    block_states: torch.Tensor,
+    block_lengths: torch.Tensor,
+    hot_k_pool: torch.Tensor,
+    hot_v_pool: torch.Tensor,
+    warm_k_pool: torch.Tensor,
+    warm_v_pool: torch.Tensor,
+    k_scale: torch.Tensor,
+    k_zero: torch.Tensor | None,
+    v_scale: torch.Tensor,
+    v_zero: torch.Tensor | None,
+    num_blocks: int,
+    num_key_value_groups: int,
+    scaling: float,
+    *,
+    cold_mode: str = "zero_logit",
+    seq_num_blocks=None,
+    max_tokens: int | None = None,
+    workspace: DecodeWorkspace | None = None,
+    out: torch.Tensor | None = None,
+):
+    """Attention of several new tokens per request over the tiered cache.
+
+    Request b's query rows, ``query_states[cu_tokens[b]:cu_tokens[b + 1]]`` of
+    packed rows ``[N, H, D]``, are its last tokens, already in the cache
+    (``kernels.build_slot_map`` and ``write_slots`` put them there); each sees
+    the request's tokens up to itself.  Tables are ``[B, max_blocks]``; pools,
+    formats, ``cold_mode``, ``seq_num_blocks`` and ``workspace`` are those of
+    ``tierkv_decode_attention``.  ``max_tokens`` bounds the requests' new
+    tokens where the caller knows it.  Returns ``[N, H, D]`` (``out`` when
+    given; rows behind the last request are left as they were).  The same
+    inputs give the same bits on every call."""
+    lib = _lib.lib()
+    if query_states.ndim != 3:
+        raise ValueError("query_states must be packed rows [tokens, num_heads, head_dim].")
+    if not query_states.is_cuda:
+        raise ValueError("TierKV attention requires GPU (HIP) tensors.")
+    if query_states.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("TierKV attention supports fp16/bf16 query tensors only.")
+    if block_table.ndim != 2:
+        raise ValueError("block_table must be [batch, max_blocks].")
+    if int(num_blocks) <= 0:
+        raise ValueError("num_blocks must be positive.")
+    if int(num_blocks) > block_table.shape[-1]:
+        raise ValueError("num_blocks exceeds the provided block table length.")
+    if cold_mode not in _COLD_MODES:
+        raise ValueError('cold_mode must be "zero_logit" or "masked".')
+    rows, num_heads, head_dim = (int(x) for x in query_states.shape)
+    batch = int(block_table.shape[0])
+    device = query_states.device
+    ints = [("block_table", block_table), ("block_states", block_states), ("block_lengths", block_lengths)]
+    for name, t in ints + [("cu_tokens", cu_tokens)]:
+        _lib.require_gpu_tensor(t, name)
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor.")
+    if any(t.shape != block_table.shape for _, t in ints):
+        raise ValueError("block_states and block_lengths must have the block table's shape.")
+    if tuple(cu_tokens.shape) != (batch + 1,):
+        raise ValueError("cu_tokens needs one entry per request and one more.")
+    pools = (hot_k_pool, hot_v_pool, warm_k_pool, warm_v_pool)
+    for name, t in zip(("hot_k_pool", "hot_v_pool", "warm_k_pool", "warm_v_pool"), pools):
+        _lib.require_gpu_tensor(t, name)
+        if t.ndim != 4 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [slots, kv_heads, block_size, head_dim] tensor.")
+    if hot_k_pool.dtype != torch.float16 or hot_v_pool.dtype != torch.float16:
+        raise ValueError("HOT pools must be fp16.")
+    kv_heads, block_size, pool_dim = (int(x) for x in hot_k_pool.shape[1:])
+    if pool_dim != head_dim or tuple(warm_k_pool.shape[1:]) != (kv_heads, block_size, head_dim):
+        raise ValueError("pool geometry does not match the query head_dim.")
+    if hot_v_pool.shape != hot_k_pool.shape or warm_v_pool.shape != warm_k_pool.shape:
+        raise ValueError("K and V pools must have identical shapes.")
+    if warm_v_pool.dtype != warm_k_pool.dtype:
+        raise ValueError("WARM K and V pools must share a dtype.")
+    if kv_heads * int(num_key_value_groups) != num_heads:
+        raise ValueError("num_heads must equal kv_heads * num_key_value_groups.")
+    fmt = warm_format_of(warm_k_pool, k_scale)
+    slots = int(warm_k_pool.shape[0])
+    metas = (k_scale, v_scale) if fmt == _lib.WARM_ABSMAX_I8 else (k_scale, k_zero, v_scale, v_zero)
+    entries = slots * kv_heads * (1 if fmt == _lib.WARM_ABSMAX_I8 else block_size)
+    for t in metas:
+        if t is None:
+            raise ValueError("reference-format WARM pools need k_zero and v_zero.")
+        _lib.require_gpu_tensor(t, "warm metadata")
+        if not t.is_contiguous() or t.numel() != entries or t.dtype != k_scale.dtype:
+            raise ValueError("warm scale/zero tensors must be contiguous with one entry per WARM slot.")
+    if any(t.device != device for t in pools + metas + (block_table, block_states, block_lengths, cu_tokens)):
+        raise ValueError("queries, tables and pools must be on one device.")
+    q = query_states
+    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty((rows, num_heads, head_dim), device=device, dtype=q.dtype)
+    elif (out.dtype != q.dtype or tuple(out.shape) != (rows, num_heads, head_dim) or not out.is_contiguous()
+          or out.device != device):
+        raise ValueError("out must be a contiguous tensor of the query's shape, dtype and device.")
+    snb = None
+    if seq_num_blocks is not None:
+        snb = torch.as_tensor(seq_num_blocks, dtype=torch.int32, device=device).contiguous()
+        if snb.numel() != batch:
+            raise ValueError("seq_num_blocks needs one entry per sequence.")
+    bound = rows if max_tokens is None else min(int(max_tokens), rows)
+    if bound < 0:
+        raise ValueError("max_tokens must not be negative.")
+    need = int(lib.tierkv_extend_workspace_bytes(batch, rows, bound, num_heads, kv_heads, int(num_blocks), block_size,
+                                                 head_dim))
+    if need < 0:
+        raise ValueError("invalid attention geometry.")
+    with torch.cuda.device(device):
+        if workspace is None:
+            ws = stream_workspace(device)
+        else:
+            ws = workspace
+            ws.note_stream(torch.cuda.current_stream(device))
+        if ws.device != device:
+            raise ValueError("the decode workspace lives on another device.")
+        ws.reserve(need)
+        rc = lib.tierkv_extend_attention(
+            _lib.ptr(q), q.stride(0), q.stride(1), _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F16,
+            _lib.ptr(out), _lib.ptr(cu_tokens), rows, bound,
+            _lib.ptr(block_table), _lib.ptr(block_states), _lib.ptr(block_lengths), int(block_table.shape[-1]),
+            _lib.ptr(snb), int(num_blocks),
+            _lib.ptr(hot_k_pool), _lib.ptr(hot_v_pool), int(hot_k_pool.shape[0]),
+            _lib.ptr(warm_k_pool), _lib.ptr(warm_v_pool), slots,
+            _lib.ptr(k_scale), _lib.ptr(k_zero) if fmt == _lib.WARM_REF_U8 else None,
+            _lib.ptr(v_scale), _lib.ptr(v_zero) if fmt == _lib.WARM_REF_U8 else None,
+            fmt, _COLD_MODES[cold_mode], batch, num_heads, kv_heads, block_size, head_dim, float(scaling),
+            ws.data_ptr(), ws.nbytes, _lib.stream_of(device))
+    _lib.check(rc, "tierkv_extend_attention")
+    if _lib.env_flag("TIERKV_CHECK_ERRORS"):
+        word = ws.error_word()
+        if word:
+            raise RuntimeError(f"TierKV attention skipped blocks with out-of-range slot/state (flag {word}).")
+    return out
+
+
+def extend_workspace(device, batch: int, num_tokens: int, num_heads: int, kv_heads: int, num_blocks: int,
+                     head_dim: int, *, block_size: int = 16, max_tokens: int | None = None) -> DecodeWorkspace:
+    """A fixed workspace for ``tierkv_extend_attention`` calls of this
+    geometry, as captured steps need one."""
+    need = _lib.lib().tierkv_extend_workspace_bytes(
+        int(batch), int(num_tokens), int(num_tokens if max_tokens is None else min(max_tokens, num_tokens)),
+        int(num_heads), int(kv_heads), int(num_blocks), int(block_size), int(head_dim))
+    if need < 0:
+        raise ValueError("invalid attention geometry.")
+    return DecodeWorkspace(device, int(need), growable=False)
