@@ -505,9 +505,12 @@ TIERKV_API int32_t tierkv_extend_attention(
  * temperature <= 0 (or NaN) takes the first of the largest logits, with
  * probability 1; a row with no logit above -inf gives token -1, probability
  * 0.  Each limit is a device array [batch] or, where that is NULL, one value
- * for all rows.  vocab <= 2^20.  The same inputs give the same tokens on
- * every call.  workspace: tierkv_sample_workspace_bytes(batch, vocab) bytes,
- * 16-byte aligned, no initialisation needed. */
+ * for all rows.  vocab <= 2^20, batch <= 65536.  The same inputs give the
+ * same tokens on every call.  workspace: tierkv_sample_workspace_bytes(batch,
+ * vocab) bytes, 16-byte aligned, of which the first
+ * TIERKV_SAMPLE_COUNTER_BYTES are zero before the first call; every call
+ * leaves them so, and one workspace serves calls of any shape on one stream. */
+#define TIERKV_SAMPLE_COUNTER_BYTES 524288
 TIERKV_API int64_t tierkv_sample_workspace_bytes(int32_t batch, int32_t vocab);
 TIERKV_API int32_t tierkv_sample_tokens(
     const void* logits, int32_t dtype, int64_t row_stride, int32_t batch, int32_t vocab, const float* uniforms,

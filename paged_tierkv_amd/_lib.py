@@ -33,6 +33,7 @@ WARM_ABSMAX_I8 = 1
 COLD_ZERO_LOGIT = 0
 COLD_MASKED = 1
 DECODE_DETERMINISTIC = 0x40000000   # OR'ed into a decode call's splits hint
+SAMPLE_COUNTER_BYTES = 524288       # of a sampling workspace, zero before its first call
 
 _P = c_void_p
 _I32P = POINTER(c_int32)

@@ -234,13 +234,17 @@ def prefill_block_mass(query_states: torch.Tensor, key_states: torch.Tensor, blo
 _scratch_ws: dict = {}
 
 
-def _scratch(name: str, device, need: int) -> torch.Tensor:
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(max(need, 256), dtype=torch.uint8, device=device)
+def _scratch(name: str, device, need: int, zeros: int = 0) -> torch.Tensor:
+    """At least ``need`` bytes whose first ``zeros`` are zero when new."""
+    capturing = torch.cuda.is_current_stream_capturing()
     key = (name, device.index, _lib.stream_of(device))
-    ws = _scratch_ws.get(key)
+    ws = None if capturing else _scratch_ws.get(key)
     if ws is None or ws.numel() < need:
-        ws = _scratch_ws[key] = torch.empty(max(need, 256), dtype=torch.uint8, device=device)
+        ws = torch.empty(max(need, 256), dtype=torch.uint8, device=device)
+        if zeros:
+            ws[:zeros].zero_()
+        if not capturing:
+            _scratch_ws[key] = ws
     return ws
 
 
@@ -383,7 +387,7 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     probs = torch.empty(batch, dtype=torch.float32, device=device)
     need = int(lib.tierkv_sample_workspace_bytes(batch, vocab))
     with torch.cuda.device(device):
-        ws = _scratch("sample", device, need)
+        ws = _scratch("sample", device, need, _lib.SAMPLE_COUNTER_BYTES)
         rc = lib.tierkv_sample_tokens(
             _lib.ptr(x), _LOGIT_DTYPES[x.dtype], x.stride(0), batch, vocab, _lib.ptr(u),
             _lib.ptr(t), float(t_all), _lib.ptr(k), min(max(int(k_all), 0), 0x7fffffff), _lib.ptr(p), float(p_all),
