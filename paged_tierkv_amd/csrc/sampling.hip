@@ -14,23 +14,28 @@
 // the likeliest have weight 0.
 //
 // Bound: memory, one read of the logits, and below a few megabytes the
-// latency of the dependent steps.  No row is sorted; a row is read by up to 16
-// workgroups, whose last one to arrive (a counter per row) goes on:
-//   top-k     One pass keeps the largest logit of every group (the elements
-//             of a thread).  The k-th largest of the groups' maxima is at
-//             most the k-th largest logit, so the first k tokens lie in the
-//             groups whose maximum reaches it, a few thousand elements:
-//             those alone are read again, listed in LDS and sorted there.
-//             One launch.
-//   top-p     needs every weight: after the maximum a second pass adds counts and weights to
-//             2048 bins of the distance to the maximum.  When the bins down to the one
-//             that crosses p hold few tokens, a third pass lists them; else it
-//             lists the crossing bin's alone, which settles the border, and
-//             a fourth adds up what is kept for the draw.
-//   neither   the second pass adds up each workgroup's part of the row and the last one
-//             draws in the part that holds the token.
-// Rows that fit none of these (a million equal logits, k in the thousands) take a radix
-// select over the row by one workgroup.
+// latency of the dependent steps.  No row is sorted.  A first launch reads
+// every row with up to 16 workgroups for its largest logit; then
+//   top-k     Launch 1 also keeps the largest logit of every group (the
+//             elements of a thread).  The k-th largest of the groups' maxima
+//             is at most the k-th largest logit, so the first k tokens lie in
+//             the groups whose maximum reaches it: a second launch, one
+//             workgroup per row, reads those alone again, a few thousand
+//             elements, and lists and ranks the tokens in LDS.  (With this in
+//             launch 1, by each row's last workgroup, 256 x 128256 fp32 took
+//             77 us where the read alone takes 26: the dependent steps held
+//             back the reads of other rows.)
+//   top-p     needs every weight: a second launch adds counts and weights to
+//             2048 bins of the distance to the maximum, and the row's last
+//             workgroup to arrive (a counter per row) finds the bin where p is
+//             crossed.  When the bins down to it hold up to 512 tokens, a
+//             third launch lists and draws from them; else it lists that
+//             bin's alone, which settles the border, and a fourth adds up
+//             what is kept and draws.
+//   neither   the second launch adds up each part of the row and its last
+//             workgroup draws in the part that holds the token.
+// Rows that fit none of these (a thousand equal logits at the border, k in
+// the thousands) take a radix select over the row by one workgroup.
 
 #include "tierkv_common.h"
 
@@ -51,16 +56,14 @@ constexpr int SP_MAX_BATCH = 1 << 16;
 constexpr double SP_ONE = 4398046511104.0;   // 2^42
 constexpr float SP_REACH = 30.f;             // weights are 0 from exp(-29.81) on
 
-enum SpMode { SP_DONE = 0, SP_SUMS, SP_SHORT, SP_BORDER, SP_DRAW, SP_SLOW };
+enum SpMode { SP_DONE = 0, SP_SHORT, SP_BORDER, SP_DRAW, SP_SLOW };
 
-// A row's state between the launches (and within one, between its workgroups).
+// A row's state between the launches.
 struct SpState {
   int32_t mode;
-  int32_t top_at;       // index of the largest logit
   int32_t bin;          // the crossing bin
   uint32_t cut;         // the prefix: keys above cut, and those equal to it up to index last
   int32_t last;
-  int32_t pad;
   uint64_t above;       // weight in the bins above the crossing one
   uint64_t total;       // weight of the row
 };
@@ -82,7 +85,8 @@ struct SampleParams {
   // Workspace.
   uint32_t* counter;      // [SP_MAX_BATCH][2] arrivals and list entries of a row, zero between launches
   SpState* state;         // [batch]
-  uint64_t* part;         // [batch][parts] the parts' maxima (key, ~index), later their weights
+  uint64_t* part;         // [batch][parts] the parts' maxima (key, ~index)
+  uint64_t* weight;       // [batch][parts] the parts' weights
   uint32_t* group;        // [batch][parts * SP_THREADS] the groups' largest keys
   uint32_t* count;        // [batch][SP_BINS]
   uint64_t* mass;         // [batch][SP_BINS]
@@ -554,17 +558,41 @@ __device__ __forceinline__ bool sp_last(SpShared& sh, uint32_t* arrived, int par
 template <typename T>
 __device__ __forceinline__ int sp_part_size(const SampleParams& p) { return p.steps * SP_THREADS * int(16 / sizeof(T)); }
 
+// f(x_i, i) for this thread's elements of part c, in index order (elements
+// past the row are NaN), four vectors in flight.
+template <typename T, bool WIDE, typename F>
+__device__ __forceinline__ void sp_sweep(const SampleParams& p, int c, const T* x, F f) {
+  constexpr int VL = 16 / sizeof(T), AHEAD = 4;
+  const int base = (c * p.steps * SP_THREADS + int(threadIdx.x)) * VL;
+  for (int s = 0; s < p.steps; s += AHEAD) {
+    float v[AHEAD][VL];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int i = base + (s + a) * SP_THREADS * VL;
+      if (s + a < p.steps && i < p.vocab) sp_load_vector<T, WIDE>(x, i, p.vocab, v[a]);
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int i = base + (s + a) * SP_THREADS * VL;
+      if (s + a < p.steps && i < p.vocab) {
+#pragma unroll
+        for (int j = 0; j < VL; ++j) f(v[a][j], i + j);
+      }
+    }
+  }
+}
+
 // The first k tokens' groups, listed and drawn from; false: not this way.
 template <typename T, bool WIDE>
 __device__ __forceinline__ bool sp_top_k(SpShared& sh, const SampleParams& p, int b, const T* x, SpRow row, int k, float top_p) {
   constexpr int VL = 16 / sizeof(T), PER = SP_GROUPS / SP_THREADS;
   const int tid = threadIdx.x, groups = p.parts * SP_THREADS;
-  uint32_t* group = p.group + int64_t(b) * groups;
+  const uint32_t* group = p.group + int64_t(b) * groups;
   uint32_t key[PER], low = ~0u;
   uint64_t filled = 0, total;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    key[i] = i * SP_THREADS + tid < groups ? sp_get(group + i * SP_THREADS + tid) : 0;
+    key[i] = i * SP_THREADS + tid < groups ? group[i * SP_THREADS + tid] : 0;
     if (key[i] > SP_MINUS_INF && !(row.top - sp_value(key[i]) <= row.reach)) key[i] = 0;   // its tokens have weight 0
     if (key[i] > SP_MINUS_INF) {
       ++filled;
@@ -642,105 +670,94 @@ __device__ __forceinline__ bool sp_top_k(SpShared& sh, const SampleParams& p, in
   return true;
 }
 
-// Launch 1: the largest logit; greedy rows and rows with a top-k end here.
-template <typename T, bool WIDE>
-__global__ __launch_bounds__(SP_THREADS) void sample_max_kernel(SampleParams p) {
-  constexpr int VL = 16 / sizeof(T);
-  __shared__ SpShared sh;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int b = int(blockIdx.x) / p.parts, c = int(blockIdx.x) - b * p.parts, n = p.vocab;
-  const T* x = reinterpret_cast<const T*>(p.logits) + int64_t(b) * p.stride;
-  const SpLimits lim = sp_limits(p, b);
-  uint32_t best = 0;
-  int at = 0x7fffffff;
-  for (int s = 0; s < p.steps; ++s) {
-    const int i0 = ((c * p.steps + s) * SP_THREADS + tid) * VL;
-    float v[VL];
-    if (i0 < n) {
-      sp_load_vector<T, WIDE>(x, i0, n, v);
-#pragma unroll
-      for (int j = 0; j < VL; ++j) {
-        const uint32_t k = sp_key(v[j]);
-        if (k > best) {
-          best = k;
-          at = i0 + j;
-        }
-      }
-    }
-  }
-  if (!lim.top_k && lim.top_p < 1.f && !lim.greedy) {   // this part's share of the next launch's bins
-    for (int i = c * SP_THREADS + tid; i < SP_BINS; i += p.parts * SP_THREADS) {
-      p.mass[int64_t(b) * SP_BINS + i] = 0;
-      p.count[int64_t(b) * SP_BINS + i] = 0;
-    }
-  }
-  if (lim.top_k && !lim.greedy)
-    sp_put(p.group + (int64_t(b) * p.parts + c) * SP_THREADS + tid, best);
-  uint64_t e = sp_entry(best, at);
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    const uint64_t o = __shfl_xor(e, m, 64);
-    e = o > e ? o : e;
-  }
-  if (lane == 0) sh.wave[w] = e;
-  __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < SP_WAVES; ++i) e = sh.wave[i] > e ? sh.wave[i] : e;
-    sp_put(p.part + int64_t(b) * p.parts + c, e);
-  }
-  SpState* st = p.state + b;
-  if (!sp_last(sh, p.counter + 2 * b, p.parts)) return;
-  e = lane < p.parts ? sp_get(p.part + int64_t(b) * p.parts + lane) : 0;
+// The row's largest logit and its first index, from the parts' (every wave).
+struct SpTop {
+  uint32_t key;
+  int at;
+};
+__device__ __forceinline__ SpTop sp_top(const SampleParams& p, int b) {
+  const int lane = threadIdx.x & 63;
+  uint64_t e = lane < p.parts ? p.part[int64_t(b) * p.parts + lane] : 0;
 #pragma unroll
   for (int m = SP_PARTS / 2; m >= 1; m >>= 1) {
     const uint64_t o = __shfl_xor(e, m, 64);
     e = o > e ? o : e;
   }
   e = __shfl(e, 0, 64);
-  best = uint32_t(e >> 32);
-  at = int(~uint32_t(e));
-  int mode = SP_DONE;
-  if (best <= SP_MINUS_INF) {
-    sp_write(p, b, -1, 0.0);
-  } else if (lim.greedy) {
-    sp_write(p, b, at, 1.0);
-  } else if (lim.top_k) {
-    const SpRow row = sp_row(p, b, sp_value(best), lim.t);
-    if (!sp_top_k<T, WIDE>(sh, p, b, x, row, lim.top_k, lim.top_p)) sp_slow<T>(sh, p, b, x, row, lim.top_k, lim.top_p);
-  } else {
-    mode = SP_SUMS;
+  return SpTop{uint32_t(e >> 32), int(~uint32_t(e))};
+}
+
+// Rows that their largest logit decides; whether b is one.
+__device__ __forceinline__ bool sp_decided(const SampleParams& p, int b, const SpTop& top, const SpLimits& lim) {
+  const bool none = top.key <= SP_MINUS_INF;
+  if (none) sp_write(p, b, -1, 0.0);
+  else if (lim.greedy) sp_write(p, b, top.at, 1.0);
+  return none || lim.greedy;
+}
+
+// Launch 1: the parts' and the groups' largest logits.
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(SP_THREADS) void sample_max_kernel(SampleParams p) {
+  __shared__ uint64_t s_wave[SP_WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int b = int(blockIdx.x) / p.parts, c = int(blockIdx.x) - b * p.parts;
+  const T* x = reinterpret_cast<const T*>(p.logits) + int64_t(b) * p.stride;
+  const SpLimits lim = sp_limits(p, b);
+  uint32_t best = 0;
+  int at = 0x7fffffff;
+  sp_sweep<T, WIDE>(p, c, x, [&](float v, int i) {
+    const uint32_t k = sp_key(v);
+    if (k > best) {
+      best = k;
+      at = i;
+    }
+  });
+  if (lim.top_k && !lim.greedy) {
+    p.group[(int64_t(b) * p.parts + c) * SP_THREADS + tid] = best;
+  } else if (lim.top_p < 1.f && !lim.greedy) {   // this part's share of the next launch's bins
+    for (int i = c * SP_THREADS + tid; i < SP_BINS; i += p.parts * SP_THREADS) {
+      p.mass[int64_t(b) * SP_BINS + i] = 0;
+      p.count[int64_t(b) * SP_BINS + i] = 0;
+    }
   }
+  uint64_t e = sp_entry(best, at);
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) {
+    const uint64_t o = __shfl_xor(e, m, 64);
+    e = o > e ? o : e;
+  }
+  if (lane == 0) s_wave[w] = e;
+  __syncthreads();
   if (tid == 0) {
-    st->mode = mode;
-    st->top_at = at;
+    for (int i = 1; i < SP_WAVES; ++i) e = s_wave[i] > e ? s_wave[i] : e;
+    p.part[int64_t(b) * p.parts + c] = e;
   }
 }
 
-template <typename T>
-__device__ __forceinline__ SpRow sp_row_again(const SampleParams& p, int b, const T* x, const SpLimits& lim) {
-  return sp_row(p, b, sp_load(x, p.state[b].top_at), lim.t);
+// Rows with a top-k, a workgroup each.
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(SP_THREADS) void sample_top_k_kernel(SampleParams p) {
+  __shared__ SpShared sh;
+  const int b = blockIdx.x;
+  const T* x = reinterpret_cast<const T*>(p.logits) + int64_t(b) * p.stride;
+  const SpLimits lim = sp_limits(p, b);
+  const SpTop top = sp_top(p, b);
+  if (sp_decided(p, b, top, lim) || !lim.top_k) return;
+  const SpRow row = sp_row(p, b, sp_value(top.key), lim.t);
+  if (!sp_top_k<T, WIDE>(sh, p, b, x, row, lim.top_k, lim.top_p)) sp_slow<T>(sh, p, b, x, row, lim.top_k, lim.top_p);
 }
 
-// This part's weight under the prefix (cut, last) to p.part; the last part's
+// This part's weight under the prefix (cut, last) to p.weight; the last part's
 // workgroup draws.
 template <typename T, bool WIDE>
 __device__ __forceinline__ void sp_draw_parts(SpShared& sh, const SampleParams& p, int b, int c, const T* x, const SpRow& row,
                               uint32_t cut, int last) {
-  constexpr int VL = 16 / sizeof(T);
   const int tid = threadIdx.x, n = p.vocab;
   uint64_t sum = 0;
-  for (int s = 0; s < p.steps; ++s) {
-    const int i0 = ((c * p.steps + s) * SP_THREADS + tid) * VL;
-    float v[VL];
-    if (i0 < n) {
-      sp_load_vector<T, WIDE>(x, i0, n, v);
-#pragma unroll
-      for (int j = 0; j < VL; ++j) sum += sp_kept<T>(row, v[j], i0 + j, cut, last);
-    }
-  }
+  sp_sweep<T, WIDE>(p, c, x, [&](float v, int i) { sum += sp_kept<T>(row, v, i, cut, last); });
   uint64_t total;
   sp_scan(sh, sum, &total);
-  uint64_t* part = p.part + int64_t(b) * p.parts;
+  uint64_t* part = p.weight + int64_t(b) * p.parts;
   if (tid == 0) sp_put(part + c, total);
   if (!sp_last(sh, p.counter + 2 * b, p.parts)) return;
   const int lane = tid & 63;
@@ -766,16 +783,23 @@ __device__ __forceinline__ void sp_draw_parts(SpShared& sh, const SampleParams& 
 // the maximum and the bin where p is crossed; without one the draw.
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(SP_THREADS) void sample_sum_kernel(SampleParams p) {
-  constexpr int VL = 16 / sizeof(T);
   __shared__ SpShared sh;
   const int tid = threadIdx.x;
   const int b = int(blockIdx.x) / p.parts, c = int(blockIdx.x) - b * p.parts, n = p.vocab;
   SpState* st = p.state + b;
-  if (st->mode != SP_SUMS) return;
   const T* x = reinterpret_cast<const T*>(p.logits) + int64_t(b) * p.stride;
   const SpLimits lim = sp_limits(p, b);
-  const SpRow row = sp_row_again(p, b, x, lim);
+  const SpTop top = sp_top(p, b);
+  if (lim.top_k || top.key <= SP_MINUS_INF || lim.greedy) {
+    if (c == 0) {
+      sp_decided(p, b, top, lim);
+      if (tid == 0) st->mode = SP_DONE;
+    }
+    return;
+  }
+  const SpRow row = sp_row(p, b, sp_value(top.key), lim.t);
   if (!(lim.top_p < 1.f)) {
+    if (c == 0 && tid == 0) st->mode = SP_DONE;
     sp_draw_parts<T, WIDE>(sh, p, b, c, x, row, 0, n);
     return;
   }
@@ -784,22 +808,14 @@ __global__ __launch_bounds__(SP_THREADS) void sample_sum_kernel(SampleParams p) 
     sh.count[i] = 0;
   }
   __syncthreads();
-  for (int s = 0; s < p.steps; ++s) {
-    const int i0 = ((c * p.steps + s) * SP_THREADS + tid) * VL;
-    float v[VL];
-    if (i0 < n) {
-      sp_load_vector<T, WIDE>(x, i0, n, v);
-#pragma unroll
-      for (int j = 0; j < VL; ++j) {
-        const uint64_t wt = row.weight(v[j]);
-        if (wt) {
-          const int bin = row.bin(v[j]);
-          atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[bin]), (unsigned long long)wt);
-          atomicAdd(&sh.count[bin], 1u);
-        }
-      }
+  sp_sweep<T, WIDE>(p, c, x, [&](float v, int) {
+    const uint64_t wt = row.weight(v);
+    if (wt) {
+      const int bin = row.bin(v);
+      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[bin]), (unsigned long long)wt);
+      atomicAdd(&sh.count[bin], 1u);
     }
-  }
+  });
   __syncthreads();
   uint64_t* mass = p.mass + int64_t(b) * SP_BINS;
   uint32_t* count = p.count + int64_t(b) * SP_BINS;
@@ -844,42 +860,33 @@ __global__ __launch_bounds__(SP_THREADS) void sample_sum_kernel(SampleParams p) 
 // Launch 3: the tokens down to the crossing bin, or that bin's.
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(SP_THREADS) void sample_list_kernel(SampleParams p) {
-  constexpr int VL = 16 / sizeof(T);
   __shared__ SpShared sh;
   const int tid = threadIdx.x;
-  const int b = int(blockIdx.x) / p.parts, c = int(blockIdx.x) - b * p.parts, n = p.vocab;
+  const int b = int(blockIdx.x) / p.parts, c = int(blockIdx.x) - b * p.parts;
   SpState* st = p.state + b;
   const int mode = st->mode;
-  if (mode != SP_SHORT && mode != SP_BORDER && mode != SP_SLOW) return;
+  if (mode == SP_DONE) return;
   const T* x = reinterpret_cast<const T*>(p.logits) + int64_t(b) * p.stride;
   const SpLimits lim = sp_limits(p, b);
-  const SpRow row = sp_row_again(p, b, x, lim);
+  const SpRow row = sp_row(p, b, sp_value(sp_top(p, b).key), lim.t);
   if (mode == SP_SLOW) {
-    if (c == 0) sp_slow<T>(sh, p, b, x, row, 0, lim.top_p);
+    if (c == 0) sp_slow<T>(sh, p, b, x, row, 0, lim.top_p);   // (the draw's launch passes such rows by)
     return;
   }
   const int hi = st->bin, lo = mode == SP_BORDER ? hi : 0;
   if (tid == 0) sh.n = 0;
   __syncthreads();
-  for (int s = 0; s < p.steps; ++s) {
-    const int i0 = ((c * p.steps + s) * SP_THREADS + tid) * VL;
-    float v[VL];
-    if (i0 < n) {
-      sp_load_vector<T, WIDE>(x, i0, n, v);
-#pragma unroll
-      for (int j = 0; j < VL; ++j) {
-        const uint32_t key = sp_key(v[j]);
-        if (key > SP_MINUS_INF) {
-          const int bin = row.bin(v[j]);
-          // (tokens of weight 0 lie in the last bins, uncounted)
-          if (bin >= lo && bin <= hi && row.weight(v[j]) > 0) {
-            const uint32_t at = atomicAdd(&sh.n, 1u);
-            if (at < uint32_t(SP_LIST)) sh.list[at] = sp_entry(key, i0 + j);
-          }
-        }
+  sp_sweep<T, WIDE>(p, c, x, [&](float v, int i) {
+    const uint32_t key = sp_key(v);
+    if (key > SP_MINUS_INF) {
+      const int bin = row.bin(v);
+      // (tokens of weight 0 lie in the last bins, uncounted)
+      if (bin >= lo && bin <= hi && row.weight(v) > 0) {
+        const uint32_t at = atomicAdd(&sh.n, 1u);
+        if (at < uint32_t(SP_LIST)) sh.list[at] = sp_entry(key, i);
       }
     }
-  }
+  });
   __syncthreads();
   uint64_t* list = p.list + int64_t(b) * SP_LIST;
   uint32_t* listed = p.counter + 2 * b + 1;
@@ -937,14 +944,14 @@ __global__ __launch_bounds__(SP_THREADS) void sample_draw_kernel(SampleParams p)
   if (st->mode != SP_DRAW) return;
   const T* x = reinterpret_cast<const T*>(p.logits) + int64_t(b) * p.stride;
   const SpLimits lim = sp_limits(p, b);
-  const SpRow row = sp_row_again(p, b, x, lim);
+  const SpRow row = sp_row(p, b, sp_value(sp_top(p, b).key), lim.t);
   sp_draw_parts<T, WIDE>(sh, p, b, c, x, row, st->cut, st->last);
 }
 
 // ---- host --------------------------------------------------------------------
 
 struct SpLayout {
-  int64_t state, part, group, count, mass, list, total;
+  int64_t state, part, weight, group, count, mass, list, total;
 };
 
 static SpLayout sp_layout(int64_t batch) {
@@ -956,7 +963,8 @@ static SpLayout sp_layout(int64_t batch) {
   l.count = up(l.state + batch * int64_t(sizeof(SpState)));
   l.mass = up(l.count + batch * SP_BINS * 4);
   l.part = up(l.mass + batch * SP_BINS * 8);
-  l.group = up(l.part + batch * SP_PARTS * 8);
+  l.weight = up(l.part + batch * SP_PARTS * 8);
+  l.group = up(l.weight + batch * SP_PARTS * 8);
   l.list = up(l.group + batch * SP_GROUPS * 4);
   l.total = up(l.list + batch * SP_LIST * 8);
   return l;
@@ -967,8 +975,11 @@ static void sp_launch(const SampleParams& p, hipStream_t stream) {
   const dim3 grid(uint32_t(p.batch) * uint32_t(p.parts)), block(SP_THREADS);
   hipLaunchKernelGGL((sample_max_kernel<T, WIDE>), grid, block, 0, stream, p);
   // One value for all rows says which launches none of them needs.
-  if (!p.top_k && p.top_k_all > 0 && p.top_k_all < p.vocab) return;
-  if (!p.temperature && !(p.temperature_all > 0.f)) return;
+  const bool all_top_k = !p.top_k && p.top_k_all > 0 && p.top_k_all < p.vocab;
+  const bool all_greedy = !p.temperature && !(p.temperature_all > 0.f);
+  if (p.top_k || all_top_k || all_greedy)
+    hipLaunchKernelGGL((sample_top_k_kernel<T, WIDE>), dim3(p.batch), block, 0, stream, p);
+  if (all_top_k || all_greedy) return;
   hipLaunchKernelGGL((sample_sum_kernel<T, WIDE>), grid, block, 0, stream, p);
   if (!p.top_p && !(p.top_p_all < 1.f)) return;
   hipLaunchKernelGGL((sample_list_kernel<T, WIDE>), grid, block, 0, stream, p);
@@ -1036,6 +1047,7 @@ extern "C" int32_t tierkv_sample_tokens(
   p.counter = reinterpret_cast<uint32_t*>(ws);
   p.state = reinterpret_cast<SpState*>(ws + l.state);
   p.part = reinterpret_cast<uint64_t*>(ws + l.part);
+  p.weight = reinterpret_cast<uint64_t*>(ws + l.weight);
   p.group = reinterpret_cast<uint32_t*>(ws + l.group);
   p.count = reinterpret_cast<uint32_t*>(ws + l.count);
   p.mass = reinterpret_cast<uint64_t*>(ws + l.mass);
