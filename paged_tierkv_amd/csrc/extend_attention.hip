@@ -52,7 +52,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int EX_THREADS = 256;
-constexpr int EX_PLAN = 512;              // threads of a plan workgroup
+constexpr int EX_PLAN = 1024;             // threads of a plan workgroup
+constexpr int EX_MAX_BATCH = 4096;        // requests per call
 constexpr int EX_SUB = 16;                // tokens per sub-tile
 constexpr int EX_NARROW = 32;             // rows of a narrow tile
 constexpr int EX_WIDE = 128;              // rows of a wide tile
@@ -63,6 +64,7 @@ constexpr float EX_LAZY = 8.f;            // log2 headroom of the running maximu
 constexpr float EX_BOOST = 6.f;           // log2 of the probabilities' factor
 constexpr float EX_NONE = -1e30f;         // running maximum before the first visible key
 constexpr float EX_LOG2E = 1.4426950408889634f;
+constexpr int EX_PAD = 16;                // spare entries behind a request's sub-tile list
 constexpr int EX_STATE_ZERO = 3;          // sub-tile of COLD tokens that enter with logit 0
 
 struct ExtendParams {
@@ -110,22 +112,32 @@ __device__ __forceinline__ int ex_uniform(int v) { return __builtin_amdgcn_readf
 // Plan
 // ---------------------------------------------------------------------------
 
-template <int NW>
-__device__ __forceinline__ int ex_scan(int v, int* sh, int* total) {
+// Inclusive prefix sums of three values over a plan workgroup; total gets the
+// three sums.
+struct Ex3 {
+  int a, b, c;
+};
+__device__ __forceinline__ Ex3 ex_scan3(Ex3 v, Ex3 (&sh)[EX_PLAN / 64], Ex3* total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int x = wave_inclusive_scan(v);
+  Ex3 x = {wave_inclusive_scan(v.a), wave_inclusive_scan(v.b), wave_inclusive_scan(v.c)};
+  __syncthreads();
   if (lane == 63) sh[w] = x;
   __syncthreads();
-  int before = 0, all = 0;
+  Ex3 all = {0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    const int t = sh[i];
-    before += i < w ? t : 0;
-    all += t;
+  for (int i = 0; i < EX_PLAN / 64; ++i) {
+    const Ex3 t = sh[i];
+    if (i < w) {
+      x.a += t.a;
+      x.b += t.b;
+      x.c += t.c;
+    }
+    all.a += t.a;
+    all.b += t.b;
+    all.c += t.c;
   }
-  __syncthreads();
   *total = all;
-  return x + before;
+  return x;
 }
 
 // Query rows of request b: its packed range, clamped to the rows there are.
@@ -136,30 +148,36 @@ __device__ __forceinline__ int2 ex_rows(const ExtendParams& p, int b) {
 
 __device__ __forceinline__ int ex_tiles(int rows) { return rows <= EX_NARROW ? (rows > 0) : (rows + EX_WIDE - 1) / EX_WIDE; }
 
-// Sub-tiles that a tile's last row sees, within one of each sub-tile
-// behind it: exact when the tokens after it fill whole sub-tiles.
-__device__ __forceinline__ int ex_work(const int4 s, int tile, bool wide, int groups) {
-  if (s.x == 0) return 1;
-  const int rows = s.w * groups;
+// Sub-tiles that a tile's last row sees (of `subs`), within one of each
+// sub-tile behind it: exact when the tokens after it fill whole sub-tiles.
+__device__ __forceinline__ int ex_work(int subs, int rows, int tile, bool wide, int groups) {
   const int last = wide ? min((tile + 1) * EX_WIDE, rows) - 1 : rows - 1;
-  const int hidden = s.w - 1 - last / groups;
-  return max(s.x - hidden / EX_SUB, 1);
+  const int hidden = (rows - 1) / groups - last / groups;
+  return max(subs - hidden / EX_SUB, 1);
 }
 
+// Items of one tile: its work in parts of at most per_item sub-tiles.
+__device__ __forceinline__ int ex_parts(int work, int per_item) { return min((work + per_item - 1) / per_item, 32767); }
+
 __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
-  constexpr int NW = EX_PLAN / 64;
-  __shared__ int sh[NW];
+  __shared__ Ex3 sh[EX_PLAN / 64];
   __shared__ int s_last;
+  __shared__ int2 s_tile[EX_MAX_BATCH];   // a request's first tile, its sub-tiles
+  __shared__ int s_rows[EX_MAX_BATCH];    // its query rows per kv head
+  __shared__ float s_work[EX_PLAN / 64];
   const int tid = threadIdx.x, b = blockIdx.x;
   int nb = p.num_blocks;
   if (p.seq_nblocks) nb = min(max(p.seq_nblocks[b], 0), p.num_blocks);
   const int64_t row = int64_t(b) * p.stride;
   const int n = ex_rows(p, b).y;
-  // Tokens of the row first: COLD sub-tiles need the distance to its end.
-  int len_sum = 0;
-  for (int i = tid; i < nb; i += EX_PLAN) len_sum += min(max(p.lengths[row + i], 0), p.bs);
-  int tokens;
-  ex_scan<NW>(len_sum, sh, &tokens);
+  int tokens = 0;
+  Ex3 total;
+  if (p.cold_zero) {   // COLD sub-tiles need the distance to the row's end
+    int sum = 0;
+    for (int i = tid; i < nb; i += EX_PLAN) sum += min(max(p.lengths[row + i], 0), p.bs);
+    ex_scan3({sum, 0, 0}, sh, &total);
+    tokens = total.a;
+  }
   int at = 0, ordinal = 0, cold = 0;   // sub-tiles, tokens and COLD tokens before this chunk
   int4* out = p.subtile + int64_t(b) * p.subs_per_seq;
   for (int i0 = 0; i0 < nb; i0 += EX_PLAN) {
@@ -170,10 +188,6 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
       state = p.states[row + i];
       slot = p.table[row + i];
     }
-    int total;
-    const int first = ordinal + ex_scan<NW>(len, sh, &total) - len;
-    ordinal += total;
-    int mine_cold = 0;
     if (len > 0) {
       if (state == HOT || state == WARM) {
         const int64_t slots = state == HOT ? p.hot_slots : p.warm_slots;
@@ -182,24 +196,32 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
       } else if (state != COLD) {
         atomicOr(p.err, 2);
       } else if (p.cold_zero) {
-        // Seen by every row: a count.  Else a sub-tile of zeros, masked like others.
-        if (first + len <= tokens - n + 1) mine_cold = len;
-        else keep = 1;
+        keep = 2;          // a count when every row sees it (known below), else a sub-tile of zeros
       }
     }
-    const int count = keep ? (len + EX_SUB - 1) / EX_SUB : 0;
-    const int pos = at + ex_scan<NW>(count, sh, &total) - count;
-    at += total;
-    ex_scan<NW>(mine_cold, sh, &total);
-    cold += total;
+    int count = keep ? (len + EX_SUB - 1) / EX_SUB : 0;
+    Ex3 s = ex_scan3({len, keep == 2 ? 0 : count, 0}, sh, &total);
+    const int first = ordinal + s.a - len;
+    int pos = at + s.b - (keep == 2 ? 0 : count);
+    ordinal += total.a;
+    if (p.cold_zero) {
+      const bool all_see = keep == 2 && first + len <= tokens - n + 1;
+      if (all_see) count = 0;
+      const Ex3 z = ex_scan3({count, all_see ? len : 0, 0}, sh, &total);
+      pos = at + z.a - count;
+      at += total.a;
+      cold += total.b;
+    } else {
+      at += total.b;
+    }
     const int code = state == COLD ? EX_STATE_ZERO : state;
     for (int j = 0; j < count; ++j)
       out[pos + j] = make_int4(slot, min(len - j * EX_SUB, EX_SUB) | (code << 8) | (j << 16), first + j * EX_SUB, 0);
   }
   if (tid == 0) {
-    // Relaxed agent-scope stores: the last workgroup reads them from another XCD's cache.
+    // Agent-scope stores: the last workgroup may read them from another XCD.
     int32_t* s = reinterpret_cast<int32_t*>(p.seq + b);
-    const int v[4] = {at, tokens, cold, n};
+    const int v[4] = {at, ordinal, cold, n};
     for (int k = 0; k < 4; ++k) __hip_atomic_store(s + k, v[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __builtin_amdgcn_s_waitcnt(0);
     s_last = __hip_atomic_fetch_add(p.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == gridDim.x;
@@ -207,79 +229,76 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
   __syncthreads();
   if (!s_last) return;
   if (tid == 0) __hip_atomic_store(p.arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  auto seq_of = [&](int i) -> int4 {
-    int32_t* s = reinterpret_cast<int32_t*>(p.seq + i);
-    int4 v;
-    v.x = __hip_atomic_load(s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    v.y = 0;
-    v.z = 0;
-    v.w = __hip_atomic_load(s + 3, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return v;
-  };
-  // Total work, then sub-tiles per item.
+  // The requests' tiles and an upper bound of the sum of the tiles' works:
+  // each is at most g(t) = max(f(t), 1) with f linear, g is convex, and a
+  // convex sum lies below its chord's.
+  const int G = p.groups;
   float work = 0.f;
-  for (int i = tid; i < p.batch; i += EX_PLAN) {
-    const int4 s = seq_of(i);
-    const int tiles = ex_tiles(s.w * p.groups);
-    const bool wide = s.w * p.groups > EX_NARROW;
-    // At least the sum of the tiles' works: each is at most g(t) = max(f(t), 1)
-    // with f linear, g is convex, and a convex sum lies below its chord's.
+  int tiles_all = 0;
+  for (int i0 = 0; i0 < p.batch; i0 += EX_PLAN) {
+    const int i = i0 + tid;
+    int rows = 0, subs = 0;
+    if (i < p.batch) {
+      int32_t* s = reinterpret_cast<int32_t*>(p.seq + i);
+      subs = __hip_atomic_load(s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      rows = __hip_atomic_load(s + 3, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) * G;
+    }
+    const int tiles = ex_tiles(rows);
+    const bool wide = rows > EX_NARROW;
     if (tiles > 0) {
       auto g = [&](int t) {
-        const float last = wide ? float(t + 1) * EX_WIDE : float(s.w * p.groups);
-        return fmaxf(float(s.x) + 1.f - fmaxf(float(s.w) - 1.f - last / float(p.groups), 0.f) / EX_SUB, 1.f);
+        const float last = wide ? float(t + 1) * EX_WIDE : float(rows);
+        return fmaxf(float(subs) + 1.f - fmaxf((float(rows) - last) / float(G) - 1.f, 0.f) / EX_SUB, 1.f);
       };
       work += 0.5f * (g(0) + g(tiles - 1)) * float(tiles);
     }
+    const Ex3 s = ex_scan3({tiles, 0, 0}, sh, &total);
+    if (i < p.batch) {
+      s_tile[i] = make_int2(tiles_all + s.a - tiles, subs);
+      s_rows[i] = rows;
+    }
+    tiles_all += total.a;
   }
-  __shared__ float s_work[NW];
   work = wave_sum(work);
   if ((tid & 63) == 0) s_work[tid >> 6] = work;
   __syncthreads();
   work = 0.f;
-  for (int i = 0; i < NW; ++i) work += s_work[i];
+  for (int i = 0; i < EX_PLAN / 64; ++i) work += s_work[i];
   work = work * 1.001f + 1.f;   // the rounding of these sums
   const int target = max(EX_TARGET / p.kv_heads, 1);
-  const int per_item = max(EX_MIN_SUBS, (int(ceilf(work / float(target))) + 3) & ~3);
-  // Items, request by request; each request's longest tiles first.
+  const int per_item = max(EX_MIN_SUBS, (int(ceilf(work / float(target))) + 7) & ~7);
+  // Items, tile by tile; each request's longest tiles first.
   int items = 0, cuts = 0, partials = 0;
-  for (int i0 = 0; i0 < p.batch; i0 += EX_PLAN) {
-    const int i = i0 + tid;
-    int4 s = make_int4(0, 0, 0, 0);
-    if (i < p.batch) s = seq_of(i);
-    const int tiles = ex_tiles(s.w * p.groups);
-    const bool wide = s.w * p.groups > EX_NARROW;
-    int mine = 0, mine_cut = 0, mine_part = 0;
-    for (int t = 0; t < tiles; ++t) {
-      const int parts = min((ex_work(s, t, wide, p.groups) + per_item - 1) / per_item, 32767);
-      mine += parts;
-      if (parts > 1) {
-        ++mine_cut;
-        mine_part += parts;
+  for (int f0 = 0; f0 < tiles_all; f0 += EX_PLAN) {
+    const int f = f0 + tid;
+    int i = 0, t = 0, parts = 0;
+    bool wide = false;
+    if (f < tiles_all) {
+      int lo = 0, hi = p.batch;           // the last request whose first tile is at most f and that has tiles
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_tile[mid].x <= f) lo = mid;
+        else hi = mid;
       }
+      i = lo;
+      const int rows = s_rows[i], tiles = ex_tiles(rows);
+      wide = rows > EX_NARROW;
+      t = tiles - 1 - (f - s_tile[i].x);
+      parts = ex_parts(ex_work(s_tile[i].y, rows, t, wide, G), per_item);
     }
-    int total;
-    int at_item = items + ex_scan<NW>(mine, sh, &total) - mine;
-    items += total;
-    int at_cut = cuts + ex_scan<NW>(mine_cut, sh, &total) - mine_cut;
-    cuts += total;
-    int at_part = partials + ex_scan<NW>(mine_part, sh, &total) - mine_part;
-    partials += total;
-    for (int t = tiles - 1; t >= 0; --t) {
-      const int parts = min((ex_work(s, t, wide, p.groups) + per_item - 1) / per_item, 32767);
+    const int cut = parts > 1 ? 1 : 0;
+    const Ex3 s = ex_scan3({parts, cut, cut ? parts : 0}, sh, &total);
+    const int at_item = items + s.a - parts, at_cut = cuts + s.b - cut, at_part = partials + s.c - (cut ? parts : 0);
+    items += total.a;
+    cuts += total.b;
+    partials += total.c;
+    if (parts > 0) {
       // The host's bounds hold for packed ranges that do not overlap; items of others may be left out (-1).
-      const bool fits = at_item + parts <= p.max_items &&
-                        (parts == 1 || (at_cut < p.max_cut && at_part + parts <= p.max_part));
+      const bool fits = at_item + parts <= p.max_items && (!cut || (at_cut < p.max_cut && at_part + parts <= p.max_part));
       for (int k = 0; k < parts; ++k)
         if (at_item + k < p.max_items)
-          p.item[at_item + k] = make_int4(fits ? i : -1, t | (wide ? 1 << 30 : 0), k | (parts << 16),
-                                          parts > 1 ? at_part + k : -1);
-      if (parts > 1) {
-        if (at_cut < p.max_cut) p.cut[at_cut] = make_int2(at_part, fits ? at_item : -1);
-        ++at_cut;
-        at_part += parts;
-      }
-      at_item += parts;
+          p.item[at_item + k] = make_int4(fits ? i : -1, t | (wide ? 1 << 30 : 0), k | (parts << 16), cut ? at_part + k : -1);
+      if (cut && at_cut < p.max_cut) p.cut[at_cut] = make_int2(at_part, fits ? at_item : -1);
     }
   }
   if (tid == 0) {
@@ -304,42 +323,56 @@ struct ExStage {
   static constexpr int UD = DL < 8 ? DL : 8;     // dims per unit
   uint4 k[NPK];
   uint4 v[4][U];
-  float kmeta[NPK][2];    // REF_U8: zero and scale of the piece's token; absmax: scale in [0][0]
-  float vmeta[4][2];      // REF_U8: of key 4g + j; absmax: scale in [0][0]
+  uint32_t kmeta[NPK];    // REF_U8: zero (low half) and scale of the piece's token; absmax: scale (fp32) in [0]
+  uint32_t vmeta[4];      // REF_U8: of key 4g + j; absmax: scale in [0]
 };
+
+// The sub-tile list is read through the constant address space: uniform
+// scalar loads, which do not wait behind the tile loads in flight.
+typedef int ex_int4 __attribute__((ext_vector_type(4)));
+typedef const __attribute__((address_space(4))) ex_int4* ExList;
 
 struct ExSub {
   int slot, valid, state, sub, ordinal;
 };
 
-__device__ __forceinline__ ExSub ex_sub(const int4* list, int i, int end) {
+// Sub-tile i of a list; from `end` on an empty one.  (Lists have EX_PAD spare
+// entries behind them, which may be read.)
+__device__ __forceinline__ ExSub ex_sub(ExList list, int i, int end) {
+  const ex_int4 v = list[i];
   ExSub s;
-  s.valid = 0;
-  s.state = EX_STATE_ZERO;
-  s.slot = s.sub = 0;
-  s.ordinal = 0;
-  if (i < end) {
-    const int4 v = list[i];
-    s.slot = ex_uniform(v.x);
-    const int y = ex_uniform(v.y);
-    s.valid = y & 0xff;
-    s.state = (y >> 8) & 0xff;
-    s.sub = y >> 16;
-    s.ordinal = ex_uniform(v.z);
-  }
+  const bool in = i < end;
+  s.slot = in ? v.x : 0;
+  s.valid = in ? v.y & 0xff : 0;
+  s.state = in ? (v.y >> 8) & 0xff : EX_STATE_ZERO;
+  s.sub = in ? v.y >> 16 : 0;
+  s.ordinal = in ? v.z : 0;
   return s;
 }
 
-// Whether every row of an item sees every key of the TK keys from sub-tile `at` on.
+// What a tile of TK keys needs for its masks.
 template <int TK>
-__device__ __forceinline__ bool ex_whole(const int4* list, int at, int end, int lim_min) {
-  bool whole = true;
+struct ExMask {
+  int valid[TK / 16], ordinal[TK / 16];
+  // Whether every row of the item (from the limit lim_min on) sees every key.
+  __device__ __forceinline__ bool whole(int lim_min) const {
+    bool w = true;
+#pragma unroll
+    for (int i = 0; i < TK / 16; ++i) w = w && valid[i] == EX_SUB && ordinal[i] + EX_SUB - 1 <= lim_min;
+    return w;
+  }
+};
+
+template <int TK>
+__device__ __forceinline__ ExMask<TK> ex_mask(ExList list, int at, int end) {
+  ExMask<TK> m;
 #pragma unroll
   for (int i = 0; i < TK / 16; ++i) {
     const ExSub s = ex_sub(list, at + i, end);
-    whole = whole && s.valid == EX_SUB && s.ordinal + EX_SUB - 1 <= lim_min;
+    m.valid[i] = s.valid;
+    m.ordinal[i] = s.ordinal;
   }
-  return whole;
+  return m;
 }
 
 template <int DP, int WF>
@@ -351,12 +384,15 @@ __device__ __forceinline__ void ex_load(const ExtendParams& p, int h, const ExSu
   const int t0 = s.sub * EX_SUB;
   const int64_t tile = (int64_t(s.slot) * p.kv_heads + h) * bs;   // the block's first row of this head
   const int n = lane & 15, g = lane >> 4;
+  // Uniform bases and 32-bit offsets within the block.
   if (s.state == HOT) {
+    const char* kb = reinterpret_cast<const char*>(p.hot_k + tile * D);
+    const char* vb = reinterpret_cast<const char*>(p.hot_v + tile * D);
 #pragma unroll
     for (int i = 0; i < St::NPK; ++i) {
       const int x = lane + 64 * i, r = min(t0 + x / (DP / 8), bs - 1);
       const int c = x % (DP / 8);
-      st.k[i] = *reinterpret_cast<const uint4*>(p.hot_k + (tile + r) * D + (c * 8 < D ? c * 8 : 0));
+      st.k[i] = *reinterpret_cast<const uint4*>(kb + uint32_t(r * D + (c * 8 < D ? c * 8 : 0)) * 2u);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -364,7 +400,7 @@ __device__ __forceinline__ void ex_load(const ExtendParams& p, int h, const ExSu
 #pragma unroll
       for (int u = 0; u < St::U; ++u) {
         const int d = St::DL * n + 8 * u;
-        const __half* src = p.hot_v + (tile + r) * D + (d < D ? d : 0);
+        const char* src = vb + uint32_t(r * D + (d < D ? d : 0)) * 2u;
         if constexpr (St::UD == 8) st.v[j][u] = *reinterpret_cast<const uint4*>(src);
         else {
           const uint2 w = *reinterpret_cast<const uint2*>(src);
@@ -375,16 +411,18 @@ __device__ __forceinline__ void ex_load(const ExtendParams& p, int h, const ExSu
     }
     return;
   }
+  const uint8_t* kb = p.warm_k + tile * D;
+  const uint8_t* vb = p.warm_v + tile * D;
 #pragma unroll
   for (int i = 0; i < St::NPK; ++i) {
     const int x = lane + 64 * i, r = min(t0 + x / (DP / 8), bs - 1);
     const int c = x % (DP / 8);
-    const uint2 w = *reinterpret_cast<const uint2*>(p.warm_k + (tile + r) * D + (c * 8 < D ? c * 8 : 0));
+    const uint2 w = *reinterpret_cast<const uint2*>(kb + uint32_t(r * D + (c * 8 < D ? c * 8 : 0)));
     st.k[i].x = w.x;
     st.k[i].y = w.y;
     if constexpr (WF == TIERKV_WARM_REF_U8) {
-      st.kmeta[i][0] = __half2float(reinterpret_cast<const __half*>(p.k_zero)[tile + r]);
-      st.kmeta[i][1] = __half2float(reinterpret_cast<const __half*>(p.k_scale)[tile + r]);
+      const uint32_t z = (reinterpret_cast<const uint16_t*>(p.k_zero) + tile)[uint32_t(r)];
+      st.kmeta[i] = z | uint32_t((reinterpret_cast<const uint16_t*>(p.k_scale) + tile)[uint32_t(r)]) << 16;
     }
   }
 #pragma unroll
@@ -393,7 +431,7 @@ __device__ __forceinline__ void ex_load(const ExtendParams& p, int h, const ExSu
 #pragma unroll
     for (int u = 0; u < St::U; ++u) {
       const int d = St::DL * n + 8 * u;
-      const uint8_t* src = p.warm_v + (tile + r) * D + (d < D ? d : 0);
+      const uint8_t* src = vb + uint32_t(r * D + (d < D ? d : 0));
       if constexpr (St::UD == 8) {
         const uint2 w = *reinterpret_cast<const uint2*>(src);
         st.v[j][u].x = w.x;
@@ -403,41 +441,35 @@ __device__ __forceinline__ void ex_load(const ExtendParams& p, int h, const ExSu
       }
     }
     if constexpr (WF == TIERKV_WARM_REF_U8) {
-      st.vmeta[j][0] = __half2float(reinterpret_cast<const __half*>(p.v_zero)[tile + r]);
-      st.vmeta[j][1] = __half2float(reinterpret_cast<const __half*>(p.v_scale)[tile + r]);
+      const uint32_t z = (reinterpret_cast<const uint16_t*>(p.v_zero) + tile)[uint32_t(r)];
+      st.vmeta[j] = z | uint32_t((reinterpret_cast<const uint16_t*>(p.v_scale) + tile)[uint32_t(r)]) << 16;
     }
   }
   if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
     const int64_t m = int64_t(s.slot) * p.kv_heads + h;
-    st.kmeta[0][0] = reinterpret_cast<const float*>(p.k_scale)[m];
-    st.vmeta[0][0] = reinterpret_cast<const float*>(p.v_scale)[m];
+    st.kmeta[0] = reinterpret_cast<const uint32_t*>(p.k_scale)[m];
+    st.vmeta[0] = reinterpret_cast<const uint32_t*>(p.v_scale)[m];
   }
 }
 
-// LDS of one key tile of TK keys.
+// LDS of one key tile of TK keys.  Rows are 16 bytes longer than their data:
+// the 16 lanes that read one chunk column of 16 rows then touch all 64 banks
+// (4 r, 36 r and 20 r banks apart: distinct multiples of 4), and every access
+// of a lane is one base address with a constant offset.  (With the chunks
+// swizzled by exclusive-or instead each needs its own address register, 36 of
+// them at D = 128, and the tile loop spilled.)
 template <int DP, int TK>
 struct ExTile {
-  // K rows of DP halves; 16-byte chunk c of row r at chunk c ^ swizzle(r): the
-  // 16 lanes that read one chunk column of 16 rows touch all 64 banks.
-  uint4 k[TK * DP / 8];
-  // V^T rows of TK halves; chunk c of row d at c ^ swizzle(d).
-  uint4 v[DP * TK / 8];
-  float kscale[TK];       // factor of each key's logits (REF_U8; absmax: one per sub-tile)
+  uint4 k[TK * (DP / 8 + 1)];   // K rows of DP halves
+  uint4 v[DP * (TK / 8 + 1)];   // V^T rows of TK halves
+  float kscale[TK];             // factor of each key's logits (REF_U8; absmax: one per sub-tile)
 };
 
 template <int DP>
-__device__ __forceinline__ int ex_k_at(int r, int c) {
-  constexpr int C = DP / 8;
-  const int s = C >= 16 ? (r & 15) : ((r >> 1) & 7);
-  return r * C + (c ^ s);
-}
+__device__ __forceinline__ int ex_k_at(int r, int c) { return r * (DP / 8 + 1) + c; }
 
 template <int TK>
-__device__ __forceinline__ int ex_v_at(int d, int c) {
-  constexpr int C = TK / 8;
-  const int s = C == 8 ? (((d >> 1) ^ (d >> 4)) & 7) : (((d >> 2) ^ (d >> 4)) & 3);
-  return d * C + (c ^ s);
-}
+__device__ __forceinline__ int ex_v_at(int d, int c) { return d * (TK / 8 + 1) + c; }
 
 // Byte b of a word as a float (v_cvt_f32_ubyte).
 template <int B>
@@ -462,9 +494,10 @@ __device__ __forceinline__ uint32_t ex_max_u16(uint32_t a, uint32_t b) {
 // tile; returns the largest magnitude bits of its V (two halves).
 template <int DP, int WF, int TK>
 __device__ __forceinline__ uint32_t ex_store(const ExtendParams& p, const ExSub& s, const ExStage<DP>& st, int at,
-                                         ExTile<DP, TK>& t) {
+                                         bool check, ExTile<DP, TK>& t) {
   typedef ExStage<DP> St;
   const int lane = threadIdx.x & 63, D = p.D;
+  const bool plain = s.valid == EX_SUB && D == DP;   // nothing to clear
   const int n = lane & 15, g = lane >> 4;
   const bool zero = s.state == EX_STATE_ZERO, hot = s.state == HOT;
 #pragma unroll
@@ -484,7 +517,7 @@ __device__ __forceinline__ uint32_t ex_store(const ExtendParams& p, const ExSub&
         b -= off;
       } else {
         off = f16x4{1024, 1024, 1024, 1024};
-        const _Float16 z = _Float16(st.kmeta[i][0]);
+        const _Float16 z = as_f16x2(st.kmeta[i])[0];
         a = u8x4_plus1024(v.x) - off;
         b = u8x4_plus1024(v.y) - off;
         a -= f16x4{z, z, z, z};
@@ -492,14 +525,21 @@ __device__ __forceinline__ uint32_t ex_store(const ExtendParams& p, const ExSub&
       }
       const uint2 lo = __builtin_bit_cast(uint2, a), hi = __builtin_bit_cast(uint2, b);
       v = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {   // (see ex_step: the factors of the logits are not negative)
+        const uint32_t sign = __uint_as_float(st.kmeta[0]) < 0.f ? 0x80008000u : 0u;
+        v.x ^= sign;
+        v.y ^= sign;
+        v.z ^= sign;
+        v.w ^= sign;
+      }
     }
     t.k[ex_k_at<DP>(at * EX_SUB + r, c)] = v;
     if constexpr (WF == TIERKV_WARM_REF_U8) {
-      if (c == 0) t.kscale[at * EX_SUB + r] = (zero || hot) ? 1.f : st.kmeta[i][1];
+      if (c == 0) t.kscale[at * EX_SUB + r] = (zero || hot) ? 1.f : half_hi(st.kmeta[i]);
     }
   }
   if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
-    if (lane == 0) t.kscale[at] = (zero || hot) ? 1.f : st.kmeta[0][0];
+    if (lane == 0) t.kscale[at] = (zero || hot) ? 1.f : fabsf(__uint_as_float(st.kmeta[0]));
   }
   // V^T: the lane's four keys side by side, for each of its dims.
   uint2* const dst = reinterpret_cast<uint2*>(t.v);
@@ -507,18 +547,25 @@ __device__ __forceinline__ uint32_t ex_store(const ExtendParams& p, const ExSub&
   uint32_t largest = 0;
   auto put = [&](int d, uint2 o) {
     dst[ex_v_at<TK>(d, chunk) * 2 + piece] = o;
-    largest = ex_max_u16(largest, ex_max_u16(o.x & 0x7fff7fffu, o.y & 0x7fff7fffu));
+    if (check) largest = ex_max_u16(largest, ex_max_u16(o.x & 0x7fff7fffu, o.y & 0x7fff7fffu));
   };
 #pragma unroll
   for (int u = 0; u < St::U; ++u) {
     uint32_t w[4][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const bool off = zero || 4 * g + j >= s.valid || St::DL * n + 8 * u >= D;
-      w[j][0] = off ? 0u : st.v[j][u].x;
-      w[j][1] = off ? 0u : st.v[j][u].y;
-      w[j][2] = off ? 0u : st.v[j][u].z;
-      w[j][3] = off ? 0u : st.v[j][u].w;
+      w[j][0] = st.v[j][u].x;
+      w[j][1] = st.v[j][u].y;
+      w[j][2] = st.v[j][u].z;
+      w[j][3] = st.v[j][u].w;
+    }
+    if (zero || (hot && !plain)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool off = zero || 4 * g + j >= s.valid || St::DL * n + 8 * u >= D;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[j][i] = off ? 0u : w[j][i];
+      }
     }
     if (zero || hot) {
 #pragma unroll
@@ -533,11 +580,11 @@ __device__ __forceinline__ uint32_t ex_store(const ExtendParams& p, const ExSub&
       for (int j = 0; j < 4; ++j) {
         const bool off = 4 * g + j >= s.valid || St::DL * n + 8 * u >= D;
         if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
-          mul[j] = off ? 0.f : st.vmeta[0][0];
+          mul[j] = off ? 0.f : __uint_as_float(st.vmeta[0]);
           add[j] = -128.f * mul[j];
         } else {
-          mul[j] = off ? 0.f : st.vmeta[j][1];
-          add[j] = off ? 0.f : st.vmeta[j][0];
+          mul[j] = off ? 0.f : half_hi(st.vmeta[j]);
+          add[j] = off ? 0.f : half_lo(st.vmeta[j]);
         }
       }
 #pragma unroll
@@ -626,49 +673,66 @@ struct ExAcc {
   float m, l;
 };
 
-// One key tile: logits, online softmax, output.
-//   end[i]  keys of sub-tile i that this lane's row sees (bounds on the key's
-//           place in the sub-tile), used unless every row sees the whole tile
-template <int DP, int WF, int TK>
-__device__ __forceinline__ void ex_step(const ExTile<DP, TK>& t, const f16x8 (&q)[DP / 16], float qscale,
-                                        const int (&end)[TK / 16], bool whole, ExAcc<DP>& a) {
-  constexpr int KT = TK / 32;
+// Logits of one key tile, S^T = K Q^T, unscaled.
+template <int DP, int TK>
+__device__ __forceinline__ void ex_logits(const ExTile<DP, TK>& t, const f16x8 (&q)[DP / 16], f32x16 (&s)[TK / 32]) {
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
-  f32x16 s[KT];
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    s[kt] = f32x16{};
+  for (int kt = 0; kt < TK / 32; ++kt) s[kt] = f32x16{};
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
+  for (int kk = 0; kk < DP / 16; ++kk) {
+#pragma unroll
+    for (int kt = 0; kt < TK / 32; ++kt) {
       const f16x8 k = __builtin_bit_cast(f16x8, t.k[ex_k_at<DP>(kt * 32 + col, kk * 2 + h)]);
       s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[kk], s[kt], 0, 0, 0);
     }
   }
-  // Logits in units of log 2.
+}
+
+// Online softmax and output of one key tile.
+//   end[i]  keys of sub-tile i that this lane's row sees (bounds on the key's
+//           place in the sub-tile), used unless every row sees the whole tile
+// The factor of a sub-tile's logits (K scale, softmax scale) is not negative,
+// so the largest logit is the factor times the largest unscaled one and the
+// factor's product joins the exponential's subtraction (absmax; the reference
+// format has a factor per key and takes the product first, as masked tiles do).
+template <int DP, int WF, int TK>
+__device__ __forceinline__ void ex_softmax(const ExTile<DP, TK>& t, float qscale, const int (&end)[TK / 16], bool whole,
+                                           f32x16 (&s)[TK / 32], ExAcc<DP>& a) {
+  constexpr int KT = TK / 32;
+  const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+  float c[KT * 2];
+  if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
+#pragma unroll
+    for (int sub = 0; sub < KT * 2; ++sub) c[sub] = t.kscale[sub] * qscale;
+  } else {
+#pragma unroll
+    for (int sub = 0; sub < KT * 2; ++sub) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        s[sub / 2][(sub & 1) * 8 + r] *= t.kscale[sub * 16 + 8 * (r >> 2) + 4 * h + (r & 3)] * qscale;
+      c[sub] = 1.f;
+    }
+  }
+  if (!whole) {
+#pragma unroll
+    for (int sub = 0; sub < KT * 2; ++sub) {
+      const int e = end[sub] - 4 * h;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const int i = (sub & 1) * 8 + r;
+        s[sub / 2][i] = (8 * (r >> 2) + (r & 3)) < e ? s[sub / 2][i] * c[sub] : -INFINITY;
+      }
+      c[sub] = 1.f;
+    }
+  }
   float mx = EX_NONE;
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
+  for (int sub = 0; sub < KT * 2; ++sub) {
+    float m = s[sub / 2][(sub & 1) * 8];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int sub = kt * 2 + half;
-      if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
-        const float c = t.kscale[sub] * qscale;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) s[kt][half * 8 + r] *= c;
-      } else {
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          s[kt][half * 8 + r] *= t.kscale[sub * 16 + 8 * (r >> 2) + 4 * h + (r & 3)] * qscale;
-      }
-      if (!whole) {
-        const int e = end[sub] - 4 * h;
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          s[kt][half * 8 + r] = (8 * (r >> 2) + (r & 3)) < e ? s[kt][half * 8 + r] : -INFINITY;
-      }
-#pragma unroll
-      for (int r = 0; r < 8; ++r) mx = fmaxf(mx, s[kt][half * 8 + r]);
-    }
+    for (int r = 1; r < 8; ++r) m = fmaxf(m, s[sub / 2][(sub & 1) * 8 + r]);
+    mx = fmaxf(mx, m * c[sub]);
   }
   mx = fmaxf(mx, xor32_f(mx));
   // A row is re-based when its own maximum asks for it, so its bits do not
@@ -683,24 +747,21 @@ __device__ __forceinline__ void ex_step(const ExTile<DP, TK>& t, const f16x8 (&q
 #pragma unroll
       for (int r = 0; r < 16; ++r) a.o[dt][r] *= alpha;
   }
-  const float base = a.m - EX_BOOST;
+  const float base = EX_BOOST - a.m;
   f16x8 pr[KT * 2];
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
+  for (int sub = 0; sub < KT * 2; ++sub) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const float e = __builtin_amdgcn_exp2f(s[kt][half * 8 + r] - base);
-        a.l += e;
-        pr[kt * 2 + half][r] = _Float16(e);
-      }
+    for (int r = 0; r < 8; ++r) {
+      const float e = __builtin_amdgcn_exp2f(fmaf(s[sub / 2][(sub & 1) * 8 + r], c[sub], base));
+      a.l += e;
+      pr[sub][r] = _Float16(e);
     }
   }
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt) {
+  for (int sub = 0; sub < TK / 16; ++sub) {
 #pragma unroll
-    for (int sub = 0; sub < TK / 16; ++sub) {
+    for (int dt = 0; dt < DP / 32; ++dt) {
       const f16x8 v = __builtin_bit_cast(f16x8, t.v[ex_v_at<TK>(dt * 32 + col, sub * 2 + h)]);
       a.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pr[sub], a.o[dt], 0, 0, 0);
     }
@@ -715,8 +776,9 @@ __device__ __forceinline__ uint32_t ex_out2(float a, float b) {
 
 template <int DP>
 constexpr int ex_lds_bytes() {
-  return int(sizeof(ExTile<DP, 64>)) > 4 * int(sizeof(ExTile<DP, 32>)) ? int(sizeof(ExTile<DP, 64>))
-                                                                       : 4 * int(sizeof(ExTile<DP, 32>));
+  const int wide = 2 * int(sizeof(ExTile<DP, 64>)), narrow = 4 * int(sizeof(ExTile<DP, 32>));
+  const int merge = 4 * 32 * (DP + 4 + 2) * 4;
+  return wide > narrow ? (wide > merge ? wide : merge) : (narrow > merge ? narrow : merge);
 }
 
 // An item: query rows of one tile, sub-tiles [part / parts) of what it sees.
@@ -736,7 +798,8 @@ __device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, 
   const int rows = n * G;
   const int row_first = tile * EX_WIDE, row_last = min(row_first + RW * 32, rows) - 1;
   const int lim_min = seq.y - n + row_first / G, lim_max = seq.y - n + row_last / G;
-  const int4* list = p.subtile + int64_t(b) * p.subs_per_seq;
+  const int4* raw_list = p.subtile + int64_t(b) * p.subs_per_seq;
+  const ExList list = (ExList)(uintptr_t)raw_list;
 
   // This lane's row.
   const int r = row_first + (RW == 4 ? w * 32 : 0) + col;
@@ -744,7 +807,7 @@ __device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, 
   const int tok = live ? r / G : 0, head = h * G + (live ? r - tok * G : 0);
   const int lim = live ? seq.y - n + tok : -1;
   f16x8 q[DP / 16];
-  float qscale = p.scale_log2;
+  float qscale = fabsf(p.scale_log2);       // (its sign goes to the query)
   {
     const QT* src = reinterpret_cast<const QT*>(p.q) + int64_t(q0 + tok) * p.qs_t + int64_t(head) * p.qs_h;
     uint4 raw[DP / 16];
@@ -783,6 +846,10 @@ __device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, 
       for (int kk = 0; kk < DP / 16; ++kk) q[kk] = __builtin_bit_cast(f16x8, raw[kk]);
     }
   }
+  if (p.scale_log2 < 0.f) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) q[kk] = -q[kk];
+  }
   ExAcc<DP> a;
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) a.o[dt] = f32x16{};
@@ -793,64 +860,99 @@ __device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, 
     a.l = half == 0 ? float(seq.z) * exp2f(EX_BOOST) : 0.f;
   }
 
-  const int visible = ex_uniform(ex_visible(list, seq.x, lim_max));
-  const int chunk = ((visible + parts - 1) / parts + 3) & ~3;
+  const int visible = ex_uniform(ex_visible(raw_list, seq.x, lim_max));
+  constexpr int ROUND = RW == 4 ? 4 : 8;
+  const int chunk = ((visible + parts - 1) / parts + ROUND - 1) & ~(ROUND - 1);
   const int lo = min(part * chunk, visible), hi = min(lo + chunk, visible);
 
-  ExTile<DP, TK>* tiles = reinterpret_cast<ExTile<DP, TK>*>(lds);
-  ExTile<DP, TK>& mine = tiles[RW == 4 ? 0 : w];
+  // Wide: two tiles in LDS, so that a round has one barrier: the next tile is
+  // stored while this one's matrix products run, and the one after it loads.
+  // Narrow: a tile per wave, stored between its steps in the wave's own order.
   constexpr int STEP = TK / 16 * KW;        // sub-tiles per round of the workgroup
+  ExTile<DP, TK>* tiles = reinterpret_cast<ExTile<DP, TK>*>(lds);
   const int first = RW == 4 ? lo : lo + w * (TK / 16);
   ExStage<DP> st[NS];
   ExSub sub[NS];
-  int wild = 0;
-  auto load = [&](int at) {
+  bool wild = false;
+  auto find = [&](int at) {
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      sub[i] = ex_sub(list, at + (RW == 4 ? w : i), hi);
-      ex_load<DP, WF>(p, h, sub[i], st[i]);
-    }
+    for (int i = 0; i < NS; ++i) sub[i] = ex_sub(list, min(at, hi) + (RW == 4 ? w : i), hi);
   };
-  if (first < hi) load(first);
-  for (int at = first; at < hi; at += STEP) {
-    const bool whole = ex_whole<TK>(list, at, hi, lim_min);
-    int end[TK / 16];
+  auto load = [&]() {
 #pragma unroll
-    for (int i = 0; i < TK / 16; ++i) {
-      const ExSub s = ex_sub(list, at + i, hi);
-      end[i] = min(s.valid, lim - s.ordinal + 1);
-    }
-    if constexpr (RW == 4) __syncthreads();           // every wave has read the tile before
+    for (int i = 0; i < NS; ++i) ex_load<DP, WF>(p, h, sub[i], st[i]);
+  };
+  auto store = [&](ExTile<DP, TK>& t, const ExSub (&of)[NS], bool whole) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-      const uint32_t largest = ex_store<DP, WF, TK>(p, sub[i], st[i], RW == 4 ? w : i, mine);
+      const int place = RW == 4 ? w : i;
+      const uint32_t largest = ex_store<DP, WF, TK>(p, of[i], st[i], place, !whole, t);
       if (!whole && __any(ex_wild(largest))) {
-        ex_clear_wild<DP, TK>(RW == 4 ? w : i, &mine);
-        wild = 1;
+        ex_clear_wild<DP, TK>(place, &t);
+        wild = true;
       }
     }
+  };
+  if (first < hi) {
+    find(first);
+    load();
+    ExMask<TK> mask = ex_mask<TK>(list, first, hi);
+    store(tiles[RW == 4 ? 0 : w], sub, mask.whole(lim_min));
+    find(first + STEP);
+    load();
     if constexpr (RW == 4) __syncthreads();
     else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (at + STEP < hi) load(at + STEP);
-    ex_step<DP, WF, TK>(mine, q, qscale, end, whole, a);
+    int buf = 0;
+    for (int at = first; at < hi; at += STEP) {
+      const ExTile<DP, TK>& t = tiles[RW == 4 ? buf : w];
+      const bool whole = mask.whole(lim_min);
+      int end[TK / 16];
+#pragma unroll
+      for (int i = 0; i < TK / 16; ++i) end[i] = min(mask.valid[i], lim - mask.ordinal[i] + 1);
+      const ExMask<TK> next = ex_mask<TK>(list, min(at + STEP, hi), hi);
+      ExSub held[NS];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) held[i] = sub[i];
+      find(at + 2 * STEP);
+      f32x16 s[TK / 32];
+      ex_logits<DP, TK>(t, q, s);
+      if constexpr (RW == 4) {
+        if (at + STEP < hi) {
+          store(tiles[buf ^ 1], held, next.whole(lim_min));
+          load();
+        }
+        ex_softmax<DP, WF, TK>(t, qscale, end, whole, s, a);
+        __syncthreads();
+        buf ^= 1;
+      } else {
+        ex_softmax<DP, WF, TK>(t, qscale, end, whole, s, a);
+        if (at + STEP < hi) {
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          store(tiles[w], held, next.whole(lim_min));
+          load();
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+      }
+      mask = next;
+    }
   }
   // Infinities and NaN of the tiles with hidden keys, for the rows that see them.
   if constexpr (RW == 4) wild = __syncthreads_or(wild);
   if (wild) {
 #pragma unroll 1
     for (int at = first; at < hi; at += STEP) {
-      if (ex_whole<TK>(list, at, hi, lim_min)) continue;
+      if (ex_mask<TK>(list, at, hi).whole(lim_min)) continue;
 #pragma unroll 1
       for (int k = 0; k < TK / 16; ++k) {
-        const ExSub s = ex_sub(list, at + k, hi);
+        const ExSub sb = ex_sub(list, at + k, hi);
 #pragma unroll 1
-        for (int t = 0; t < min(s.valid, lim - s.ordinal + 1); ++t) {
+        for (int x = 0; x < min(sb.valid, lim - sb.ordinal + 1); ++x) {
 #pragma unroll
           for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int d = dt * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-              const float v = d < D ? ex_value<WF>(p, h, s, t, d) : 0.f;
+              const float v = d < D ? ex_value<WF>(p, h, sb, x, d) : 0.f;
               if (!(fabsf(v) < INFINITY)) a.o[dt][i] += v;
             }
         }
@@ -887,8 +989,10 @@ __device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, 
 #pragma unroll
       for (int k = 0; k < KW; ++k) {
         const float c = __builtin_amdgcn_exp2f(sml[(k * 32 + rr) * 2] - m);
-        l += sml[(k * 32 + rr) * 2 + 1] * c;
-        o += *reinterpret_cast<const f32x4*>(so + (k * 32 + rr) * (DP + 4) + d) * c;
+        if (c > 0.f) {   // (a state of no weight may hold an infinity's product)
+          l += sml[(k * 32 + rr) * 2 + 1] * c;
+          o += *reinterpret_cast<const f32x4*>(so + (k * 32 + rr) * (DP + 4) + d) * c;
+        }
       }
       const int row = row_first + rr;
       if (row >= rows || d >= D) continue;
@@ -955,39 +1059,54 @@ __global__ __launch_bounds__(EX_THREADS, 2) void extend_kernel(ExtendParams p) {
 }
 
 // Join of a cut tile's partials, in part order: a workgroup per (cut tile, kv
-// head, 32 of its rows).
+// head, 1024 / D of its rows), four dims of one row per thread.
 template <typename QT>
-__global__ __launch_bounds__(EX_THREADS) void extend_merge_kernel(ExtendParams p) {
+__global__ __launch_bounds__(EX_THREADS) void extend_merge_kernel(ExtendParams p, int32_t rows_per_wg) {
   const int c = int(blockIdx.x) / p.kv_heads, h = int(blockIdx.x) - c * p.kv_heads;
   if (c >= p.head[1]) return;
   const int2 cut = p.cut[c];
   if (cut.y < 0) return;
   const int4 it = p.item[cut.y];
   const int b = it.x, tile = it.y & 0x3fffffff, parts = it.z >> 16;
-  const int n = p.seq[b].w, G = p.groups, D = p.D;
-  const int row_first = tile * EX_WIDE, row_base = int(blockIdx.y) * 32;
-  const int q0 = ex_rows(p, b).x;
+  const int G = p.groups, D = p.D, rows = p.seq[b].w * G;
   const int D4 = D / 4;
-  for (int x = threadIdx.x; x < 32 * D4; x += EX_THREADS) {
-    const int rr = row_base + x / D4, d = 4 * (x % D4);
-    const int row = row_first + rr;
-    if (row >= n * G || rr >= p.part_rows) continue;
-    float m = EX_NONE;
-    for (int k = 0; k < parts; ++k)
-      m = fmaxf(m, p.part_ml[((int64_t(cut.x + k) * p.kv_heads + h) * p.part_rows + rr) * 2]);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    for (int k = 0; k < parts; ++k) {
-      const int64_t at = (int64_t(cut.x + k) * p.kv_heads + h) * p.part_rows + rr;
-      const float f = __builtin_amdgcn_exp2f(p.part_ml[at * 2] - m);
-      l += p.part_ml[at * 2 + 1] * f;
-      o += *reinterpret_cast<const f32x4*>(p.part_o + at * D + d) * f;
+  const int rr = int(blockIdx.y) * rows_per_wg + int(threadIdx.x) / D4, d = 4 * (int(threadIdx.x) % D4);
+  const int row = tile * EX_WIDE + rr;
+  if (int(threadIdx.x) >= rows_per_wg * D4 || rr >= p.part_rows || row >= rows) return;
+  constexpr int AHEAD = 8;   // partials loaded together
+  const int64_t step = int64_t(p.kv_heads) * p.part_rows;
+  const int64_t at = (int64_t(cut.x) * p.kv_heads + h) * p.part_rows + rr;
+  float m = EX_NONE, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < parts; k0 += AHEAD) {
+    float2 ml[AHEAD];
+    f32x4 v[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int64_t x = at + min(k0 + k, parts - 1) * step;
+      ml[k] = reinterpret_cast<const float2*>(p.part_ml)[x];
+      v[k] = *reinterpret_cast<const f32x4*>(p.part_o + x * D + d);
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    const int tk = row / G, hd = h * G + row - tk * G;
-    QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t(q0 + tk) * p.heads + hd) * D + d;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(ex_out2<QT>(o[0] * inv, o[1] * inv), ex_out2<QT>(o[2] * inv, o[3] * inv));
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) top = fmaxf(top, ml[k].x);
+    const float f0 = __builtin_amdgcn_exp2f(m - top);
+    m = top;
+    l *= f0;
+    o *= f0;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const float f = k0 + k < parts ? __builtin_amdgcn_exp2f(ml[k].x - m) : 0.f;
+      if (f > 0.f) {   // (a partial of no weight may hold an infinity's product)
+        l += ml[k].y * f;
+        o += v[k] * f;
+      }
+    }
   }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const int tk = row / G, hd = h * G + row - tk * G;
+  QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t(ex_rows(p, b).x + tk) * p.heads + hd) * D + d;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(ex_out2<QT>(o[0] * inv, o[1] * inv), ex_out2<QT>(o[2] * inv, o[3] * inv));
 }
 
 // ---------------------------------------------------------------------------
@@ -1015,7 +1134,7 @@ static ExLayout ex_layout(int64_t batch, int64_t rows, int64_t max_tokens, int64
   l.max_items = int32_t(std::min<int64_t>(tiles + target, 1 << 26));
   l.max_cut = int32_t(std::min(tiles, target));
   l.part_rows = longest * groups <= EX_NARROW ? EX_NARROW : EX_WIDE;
-  l.subs_per_seq = num_blocks * ((bs + EX_SUB - 1) / EX_SUB);
+  l.subs_per_seq = num_blocks * ((bs + EX_SUB - 1) / EX_SUB) + EX_PAD;
   const int64_t partials = l.max_cut + target;
   l.max_part = int32_t(partials);
   l.arrived = 128;
@@ -1032,11 +1151,13 @@ static ExLayout ex_layout(int64_t batch, int64_t rows, int64_t max_tokens, int64
 
 template <int DP, int WF, typename QT>
 static void ex_launch(const ExtendParams& p, hipStream_t stream) {
-  const int lds = std::max(ex_lds_bytes<DP>(), 4 * 32 * (DP + 4 + 2) * 4);
+  const int lds = ex_lds_bytes<DP>();
   hipLaunchKernelGGL(extend_plan_kernel, dim3(p.batch), dim3(EX_PLAN), 0, stream, p);
   hipLaunchKernelGGL((extend_kernel<DP, WF, QT>), dim3(p.max_items * p.kv_heads), dim3(EX_THREADS), lds, stream, p);
-  hipLaunchKernelGGL(extend_merge_kernel<QT>, dim3(p.max_cut * p.kv_heads, p.part_rows / 32), dim3(EX_THREADS), 0,
-                     stream, p);
+  const int rows_per_wg = 4 * EX_THREADS / p.D;
+  hipLaunchKernelGGL(extend_merge_kernel<QT>,
+                     dim3(p.max_cut * p.kv_heads, (p.part_rows + rows_per_wg - 1) / rows_per_wg), dim3(EX_THREADS), 0,
+                     stream, p, rows_per_wg);
 }
 
 template <int DP, int WF>
@@ -1106,6 +1227,7 @@ extern "C" int32_t tierkv_extend_attention(
     return fail(TIERKV_ERR_INVALID, "query, out, pools and workspace must be 16-byte aligned");
   if (int64_t(num_blocks) * block_size > 0x7fffffff - EX_SUB)
     return fail(TIERKV_ERR_UNSUPPORTED, "rows of 2^31 tokens or more");
+  if (batch > EX_MAX_BATCH) return fail(TIERKV_ERR_UNSUPPORTED, "more than 4096 requests");
   const int groups = num_heads / num_kv_heads;
   if (int64_t(num_rows) * groups > (int64_t(1) << 29))
     return fail(TIERKV_ERR_UNSUPPORTED, "more than 2^29 query rows per kv head");
