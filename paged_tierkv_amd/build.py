@@ -53,8 +53,9 @@ HIP_SOURCES = {
     # MFMA accumulators in ordinary VGPRs: the logits are consumed by VALU
     # code right away, and accumulators in AGPRs cost a copy per element.
     "prefill_score.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-    # As above: logits and outputs are scaled by VALU code every tile.
-    "extend_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    # As above (logits and outputs are scaled by VALU code every tile), and the
+    # tier branches of its tile loader as in the decode kernel.
+    "extend_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-simplifycfg-sink-common=false"],
     "slot_map.hip": [],
     # Weights are whole numbers that follow from one product and one rounding.
     "sampling.hip": ["-ffp-contract=off"],

@@ -350,29 +350,14 @@ __device__ __forceinline__ ExSub ex_sub(ExList list, int i, int end) {
   return s;
 }
 
-// What a tile of TK keys needs for its masks.
+// Keys of each sub-tile of a tile that a row with the given limit sees.
 template <int TK>
-struct ExMask {
-  int valid[TK / 16], ordinal[TK / 16];
-  // Whether every row of the item (from the limit lim_min on) sees every key.
-  __device__ __forceinline__ bool whole(int lim_min) const {
-    bool w = true;
-#pragma unroll
-    for (int i = 0; i < TK / 16; ++i) w = w && valid[i] == EX_SUB && ordinal[i] + EX_SUB - 1 <= lim_min;
-    return w;
-  }
-};
-
-template <int TK>
-__device__ __forceinline__ ExMask<TK> ex_mask(ExList list, int at, int end) {
-  ExMask<TK> m;
+__device__ __forceinline__ void ex_ends(ExList list, int at, int hi, int lim, int (&end)[TK / 16]) {
 #pragma unroll
   for (int i = 0; i < TK / 16; ++i) {
-    const ExSub s = ex_sub(list, at + i, end);
-    m.valid[i] = s.valid;
-    m.ordinal[i] = s.ordinal;
+    const ExSub s = ex_sub(list, at + i, hi);
+    end[i] = min(s.valid, lim - s.ordinal + 1);
   }
-  return m;
 }
 
 template <int DP, int WF>
@@ -453,15 +438,17 @@ __device__ __forceinline__ void ex_load(const ExtendParams& p, int h, const ExSu
 }
 
 // LDS of one key tile of TK keys.  Rows are 16 bytes longer than their data:
-// the 16 lanes that read one chunk column of 16 rows then touch all 64 banks
-// (4 r, 36 r and 20 r banks apart: distinct multiples of 4), and every access
-// of a lane is one base address with a constant offset.  (With the chunks
-// swizzled by exclusive-or instead each needs its own address register, 36 of
-// them at D = 128, and the tile loop spilled.)
+// eight lanes that read one chunk column of neighbouring rows then touch 32
+// banks in all (rows 4, 36 and 20 banks apart), and every access of a lane
+// is one base address with a constant offset.  (With the chunks swizzled by
+// exclusive-or each needs its own address register, 36 of them at D = 128, and
+// the tile loop spilled.)  V^T has 16 bytes more per eight rows, since the
+// lanes that store it are eight rows apart (without them 70 % of the LDS's
+// active cycles were conflicts).
 template <int DP, int TK>
 struct ExTile {
   uint4 k[TK * (DP / 8 + 1)];   // K rows of DP halves
-  uint4 v[DP * (TK / 8 + 1)];   // V^T rows of TK halves
+  uint4 v[DP * (TK / 8 + 1) + DP / 8];   // V^T rows of TK halves
   float kscale[TK];             // factor of each key's logits (REF_U8; absmax: one per sub-tile)
 };
 
@@ -469,7 +456,7 @@ template <int DP>
 __device__ __forceinline__ int ex_k_at(int r, int c) { return r * (DP / 8 + 1) + c; }
 
 template <int TK>
-__device__ __forceinline__ int ex_v_at(int d, int c) { return d * (TK / 8 + 1) + c; }
+__device__ __forceinline__ int ex_v_at(int d, int c) { return d * (TK / 8 + 1) + (d >> 3) + c; }
 
 // Byte b of a word as a float (v_cvt_f32_ubyte).
 template <int B>
@@ -666,6 +653,25 @@ __device__ __forceinline__ int ex_visible(const int4* list, int count, int limit
   return lo;
 }
 
+// The first sub-tile of [lo, hi) that is not full, or not seen by every row
+// (from the limit lim on): tiles before it need no masks.  By one wave.
+__device__ __forceinline__ int ex_full_until(const int4* list, int lo, int hi, int lim) {
+  const int lane = threadIdx.x & 63;
+  for (int i0 = lo; i0 < hi; i0 += 256) {
+    uint64_t odd[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = min(i0 + k * 64 + lane, hi - 1);
+      const int4 v = list[i];
+      odd[k] = __ballot((v.y & 0xff) != EX_SUB || v.z + EX_SUB - 1 > lim);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (odd[k]) return min(i0 + k * 64 + __ffsll((unsigned long long)odd[k]) - 1, hi);
+  }
+  return hi;
+}
+
 // The running state of 32 rows in a wave: lane (row = lane & 31, half = lane >> 5).
 template <int DP>
 struct ExAcc {
@@ -673,20 +679,39 @@ struct ExAcc {
   float m, l;
 };
 
+// Scheduling of a matrix product whose A operands come from LDS: AHEAD reads
+// go first, then one read per product, so that no product waits for a read
+// just issued (left to itself the compiler reads each operand when it is
+// due: 16 LDS latencies per product chain).
+template <int N, int AHEAD>
+__device__ __forceinline__ void ex_pace() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);   // LDS reads
+#pragma unroll
+  for (int i = 0; i < N - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);     // MFMA
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
+
 // Logits of one key tile, S^T = K Q^T, unscaled.
 template <int DP, int TK>
 __device__ __forceinline__ void ex_logits(const ExTile<DP, TK>& t, const f16x8 (&q)[DP / 16], f32x16 (&s)[TK / 32]) {
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
 #pragma unroll
   for (int kt = 0; kt < TK / 32; ++kt) s[kt] = f32x16{};
+  const uint4* const kb = t.k + ex_k_at<DP>(col, h);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int kk = 0; kk < DP / 16; ++kk) {
 #pragma unroll
     for (int kt = 0; kt < TK / 32; ++kt) {
-      const f16x8 k = __builtin_bit_cast(f16x8, t.k[ex_k_at<DP>(kt * 32 + col, kk * 2 + h)]);
+      const f16x8 k = __builtin_bit_cast(f16x8, kb[kt * 32 * (DP / 8 + 1) + kk * 2]);
       s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[kk], s[kt], 0, 0, 0);
     }
   }
+  ex_pace<DP / 16 * (TK / 32), 6>();
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // Online softmax and output of one key tile.
@@ -747,25 +772,49 @@ __device__ __forceinline__ void ex_softmax(const ExTile<DP, TK>& t, float qscale
 #pragma unroll
       for (int r = 0; r < 16; ++r) a.o[dt][r] *= alpha;
   }
+  // Probabilities of 16 keys, then their products with V^T while the next 16
+  // keys' exponentials are taken and their V is read: each region below holds
+  // DT products, DT reads and eight exponentials, and the schedule puts a
+  // share of the others behind each product.
   const float base = EX_BOOST - a.m;
-  f16x8 pr[KT * 2];
+  constexpr int DT = DP / 32, SUBS = KT * 2;
+  const uint4* const vb = t.v + ex_v_at<TK>(col, h);
+  constexpr int VROW = 32 * (TK / 8 + 1) + 4;   // 32 rows of V^T
+  f16x8 v[2][DT], pr[2];
+  auto read = [&](int sub) {
 #pragma unroll
-  for (int sub = 0; sub < KT * 2; ++sub) {
+    for (int dt = 0; dt < DT; ++dt) v[sub & 1][dt] = __builtin_bit_cast(f16x8, vb[dt * VROW + sub * 2]);
+  };
+  auto probabilities = [&](int sub) {
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const float e = __builtin_amdgcn_exp2f(fmaf(s[sub / 2][(sub & 1) * 8 + r], c[sub], base));
       a.l += e;
-      pr[sub][r] = _Float16(e);
+      pr[sub & 1][r] = _Float16(e);
+    }
+  };
+  __builtin_amdgcn_sched_barrier(0);
+  read(0);
+  probabilities(0);
+#pragma unroll
+  for (int sub = 0; sub < SUBS; ++sub) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      a.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[sub & 1][dt], pr[sub & 1], a.o[dt], 0, 0, 0);
+    if (sub + 1 < SUBS) {
+      read(sub + 1);
+      probabilities(sub + 1);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 20 / DT, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, 8 / DT, 0);
+      }
     }
   }
-#pragma unroll
-  for (int sub = 0; sub < TK / 16; ++sub) {
-#pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt) {
-      const f16x8 v = __builtin_bit_cast(f16x8, t.v[ex_v_at<TK>(dt * 32 + col, sub * 2 + h)]);
-      a.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pr[sub], a.o[dt], 0, 0, 0);
-    }
-  }
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 template <typename QT>
@@ -894,10 +943,10 @@ __device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, 
     }
   };
   if (first < hi) {
+    const int full = ex_uniform(ex_full_until(raw_list, lo, hi, lim_min));
     find(first);
     load();
-    ExMask<TK> mask = ex_mask<TK>(list, first, hi);
-    store(tiles[RW == 4 ? 0 : w], sub, mask.whole(lim_min));
+    store(tiles[RW == 4 ? 0 : w], sub, first + TK / 16 <= full);
     find(first + STEP);
     load();
     if constexpr (RW == 4) __syncthreads();
@@ -905,11 +954,7 @@ __device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, 
     int buf = 0;
     for (int at = first; at < hi; at += STEP) {
       const ExTile<DP, TK>& t = tiles[RW == 4 ? buf : w];
-      const bool whole = mask.whole(lim_min);
-      int end[TK / 16];
-#pragma unroll
-      for (int i = 0; i < TK / 16; ++i) end[i] = min(mask.valid[i], lim - mask.ordinal[i] + 1);
-      const ExMask<TK> next = ex_mask<TK>(list, min(at + STEP, hi), hi);
+      const bool whole = at + TK / 16 <= full;
       ExSub held[NS];
 #pragma unroll
       for (int i = 0; i < NS; ++i) held[i] = sub[i];
@@ -918,22 +963,22 @@ __device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, 
       ex_logits<DP, TK>(t, q, s);
       if constexpr (RW == 4) {
         if (at + STEP < hi) {
-          store(tiles[buf ^ 1], held, next.whole(lim_min));
+          store(tiles[buf ^ 1], held, at + STEP + TK / 16 <= full);
           load();
-        }
-        ex_softmax<DP, WF, TK>(t, qscale, end, whole, s, a);
-        __syncthreads();
-        buf ^= 1;
-      } else {
-        ex_softmax<DP, WF, TK>(t, qscale, end, whole, s, a);
-        if (at + STEP < hi) {
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          store(tiles[w], held, next.whole(lim_min));
-          load();
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
       }
-      mask = next;
+      int end[TK / 16] = {};
+      if (!whole) ex_ends<TK>(list, at, hi, lim, end);
+      ex_softmax<DP, WF, TK>(t, qscale, end, whole, s, a);
+      if constexpr (RW == 4) {
+        __syncthreads();
+        buf ^= 1;
+      } else if (at + STEP < hi) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        store(tiles[w], held, at + STEP + TK / 16 <= full);
+        load();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
     }
   }
   // Infinities and NaN of the tiles with hidden keys, for the rows that see them.
@@ -941,7 +986,7 @@ __device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, 
   if (wild) {
 #pragma unroll 1
     for (int at = first; at < hi; at += STEP) {
-      if (ex_mask<TK>(list, at, hi).whole(lim_min)) continue;
+      if (at + TK / 16 <= ex_full_until(raw_list, lo, hi, lim_min)) continue;
 #pragma unroll 1
       for (int k = 0; k < TK / 16; ++k) {
         const ExSub sb = ex_sub(list, at + k, hi);
