@@ -51,14 +51,15 @@ namespace tierkv {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int EX_THREADS = 256;
+constexpr int EX_THREADS = 512;
+constexpr int EX_WAVES = EX_THREADS / 64;
 constexpr int EX_PLAN = 1024;             // threads of a plan workgroup
 constexpr int EX_MAX_BATCH = 4096;        // requests per call
 constexpr int EX_SUB = 16;                // tokens per sub-tile
 constexpr int EX_NARROW = 32;             // rows of a narrow tile
-constexpr int EX_WIDE = 128;              // rows of a wide tile
-constexpr int EX_TARGET = 1024;           // workgroups that the cut aims at
-constexpr int EX_MIN_SUBS = 8;            // sub-tiles per item, at least, when a tile is cut
+constexpr int EX_WIDE = 32 * EX_WAVES;   // rows of a wide tile
+constexpr int EX_TARGET = 512;            // workgroups that the cut aims at
+constexpr int EX_MIN_SUBS = 16;           // sub-tiles per item, at least, when a tile is cut
 constexpr int EX_WS_HEAD = 256 + (1 << 16) * 4;   // the decode launches' error word and counters
 constexpr float EX_LAZY = 8.f;            // log2 headroom of the running maximum
 constexpr float EX_BOOST = 6.f;           // log2 of the probabilities' factor
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
   for (int i = 0; i < EX_PLAN / 64; ++i) work += s_work[i];
   work = work * 1.001f + 1.f;   // the rounding of these sums
   const int target = max(EX_TARGET / p.kv_heads, 1);
-  const int per_item = max(EX_MIN_SUBS, (int(ceilf(work / float(target))) + 7) & ~7);
+  const int per_item = max(EX_MIN_SUBS, (int(ceilf(work / float(target))) + 15) & ~15);
   // Items, tile by tile; each request's longest tiles first.
   int items = 0, cuts = 0, partials = 0;
   for (int f0 = 0; f0 < tiles_all; f0 += EX_PLAN) {
@@ -311,20 +312,18 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
 // Attention
 // ---------------------------------------------------------------------------
 
-// A sub-tile's K and V in registers, as loaded.
-//   k: piece x = lane + 64 i of the 16 rows' 8-element pieces (row x / (DP / 8));
-//   v: keys 4g + j (g = lane >> 4, j = 0..3), dims DL n .. DL n + DL - 1 (n = lane & 15),
-//      in units of up to 8 dims.
+// Half a sub-tile, its K or its V, in registers as loaded.
+//   K: r[i] is piece x = lane + 64 i of the 16 rows' 8-element pieces (row
+//      x / (DP / 8)), i < NPK;
+//   V: r[j] is key 4g + j (g = lane >> 4), dims DL n .. DL n + DL - 1 (n = lane & 15).
+// WARM codes fill the front of each entry.  meta: the reference format's zero
+// (low half) and scale of each entry's token, absmax: the scale (fp32) in [0].
 template <int DP>
-struct ExStage {
-  static constexpr int NPK = DP / 32;            // K pieces per lane
-  static constexpr int DL = DP / 16;             // V dims per lane
-  static constexpr int U = DL / 8 > 0 ? DL / 8 : 1;   // V units per row
-  static constexpr int UD = DL < 8 ? DL : 8;     // dims per unit
-  uint4 k[NPK];
-  uint4 v[4][U];
-  uint32_t kmeta[NPK];    // REF_U8: zero (low half) and scale of the piece's token; absmax: scale (fp32) in [0]
-  uint32_t vmeta[4];      // REF_U8: of key 4g + j; absmax: scale in [0]
+struct ExHalf {
+  static constexpr int NPK = DP / 32;
+  static constexpr int DL = DP / 16;
+  uint4 r[4];
+  uint32_t meta[4];
 };
 
 // The sub-tile list is read through the constant address space: uniform
@@ -360,80 +359,63 @@ __device__ __forceinline__ void ex_ends(ExList list, int at, int hi, int lim, in
   }
 }
 
-template <int DP, int WF>
-__device__ __forceinline__ void ex_load(const ExtendParams& p, int h, const ExSub& s, ExStage<DP>& st) {
-  typedef ExStage<DP> St;
+// KV: 0 K, 1 V.
+template <int DP, int WF, int KV>
+__device__ __forceinline__ void ex_load(const ExtendParams& p, int h, const ExSub& s, ExHalf<DP>& st) {
+  typedef ExHalf<DP> St;
   if (s.state == EX_STATE_ZERO) return;
   const int lane = threadIdx.x & 63;
   const int D = p.D, bs = p.bs;
   const int t0 = s.sub * EX_SUB;
   const int64_t tile = (int64_t(s.slot) * p.kv_heads + h) * bs;   // the block's first row of this head
-  const int n = lane & 15, g = lane >> 4;
+  constexpr int N = KV ? 4 : St::NPK;
   // Uniform bases and 32-bit offsets within the block.
-  if (s.state == HOT) {
-    const char* kb = reinterpret_cast<const char*>(p.hot_k + tile * D);
-    const char* vb = reinterpret_cast<const char*>(p.hot_v + tile * D);
+  const bool hot = s.state == HOT;
+  const char* base = hot ? reinterpret_cast<const char*>((KV ? p.hot_v : p.hot_k) + tile * D)
+                         : reinterpret_cast<const char*>((KV ? p.warm_v : p.warm_k) + tile * D);
+  uint32_t row[N], off[N];
 #pragma unroll
-    for (int i = 0; i < St::NPK; ++i) {
-      const int x = lane + 64 * i, r = min(t0 + x / (DP / 8), bs - 1);
-      const int c = x % (DP / 8);
-      st.k[i] = *reinterpret_cast<const uint4*>(kb + uint32_t(r * D + (c * 8 < D ? c * 8 : 0)) * 2u);
-    }
+  for (int i = 0; i < N; ++i) {
+    const int x = lane + 64 * i;
+    const int d = KV ? St::DL * (lane & 15) : 8 * (x % (DP / 8));
+    row[i] = uint32_t(min(t0 + (KV ? 4 * (lane >> 4) + i : x / (DP / 8)), bs - 1));
+    off[i] = row[i] * uint32_t(D) + uint32_t(d < D ? d : 0);
+  }
+  if (hot) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = min(t0 + 4 * g + j, bs - 1);
-#pragma unroll
-      for (int u = 0; u < St::U; ++u) {
-        const int d = St::DL * n + 8 * u;
-        const char* src = vb + uint32_t(r * D + (d < D ? d : 0)) * 2u;
-        if constexpr (St::UD == 8) st.v[j][u] = *reinterpret_cast<const uint4*>(src);
-        else {
-          const uint2 w = *reinterpret_cast<const uint2*>(src);
-          st.v[j][u].x = w.x;
-          st.v[j][u].y = w.y;
-        }
+    for (int i = 0; i < N; ++i) {
+      const char* src = base + off[i] * 2u;
+      if (KV && St::DL < 8) {
+        const uint2 w = *reinterpret_cast<const uint2*>(src);
+        st.r[i].x = w.x;
+        st.r[i].y = w.y;
+      } else {
+        st.r[i] = *reinterpret_cast<const uint4*>(src);
       }
     }
     return;
   }
-  const uint8_t* kb = p.warm_k + tile * D;
-  const uint8_t* vb = p.warm_v + tile * D;
 #pragma unroll
-  for (int i = 0; i < St::NPK; ++i) {
-    const int x = lane + 64 * i, r = min(t0 + x / (DP / 8), bs - 1);
-    const int c = x % (DP / 8);
-    const uint2 w = *reinterpret_cast<const uint2*>(kb + uint32_t(r * D + (c * 8 < D ? c * 8 : 0)));
-    st.k[i].x = w.x;
-    st.k[i].y = w.y;
-    if constexpr (WF == TIERKV_WARM_REF_U8) {
-      const uint32_t z = (reinterpret_cast<const uint16_t*>(p.k_zero) + tile)[uint32_t(r)];
-      st.kmeta[i] = z | uint32_t((reinterpret_cast<const uint16_t*>(p.k_scale) + tile)[uint32_t(r)]) << 16;
+  for (int i = 0; i < N; ++i) {
+    const char* src = base + off[i];
+    if (KV && St::DL < 8) {
+      st.r[i].x = *reinterpret_cast<const uint32_t*>(src);
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2*>(src);
+      st.r[i].x = w.x;
+      st.r[i].y = w.y;
     }
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int r = min(t0 + 4 * g + j, bs - 1);
-#pragma unroll
-    for (int u = 0; u < St::U; ++u) {
-      const int d = St::DL * n + 8 * u;
-      const uint8_t* src = vb + uint32_t(r * D + (d < D ? d : 0));
-      if constexpr (St::UD == 8) {
-        const uint2 w = *reinterpret_cast<const uint2*>(src);
-        st.v[j][u].x = w.x;
-        st.v[j][u].y = w.y;
-      } else {
-        st.v[j][u].x = *reinterpret_cast<const uint32_t*>(src);
-      }
-    }
-    if constexpr (WF == TIERKV_WARM_REF_U8) {
-      const uint32_t z = (reinterpret_cast<const uint16_t*>(p.v_zero) + tile)[uint32_t(r)];
-      st.vmeta[j] = z | uint32_t((reinterpret_cast<const uint16_t*>(p.v_scale) + tile)[uint32_t(r)]) << 16;
-    }
-  }
+  const void* scale = KV ? p.v_scale : p.k_scale;
   if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
-    const int64_t m = int64_t(s.slot) * p.kv_heads + h;
-    st.kmeta[0] = reinterpret_cast<const uint32_t*>(p.k_scale)[m];
-    st.vmeta[0] = reinterpret_cast<const uint32_t*>(p.v_scale)[m];
+    st.meta[0] = reinterpret_cast<const uint32_t*>(scale)[int64_t(s.slot) * p.kv_heads + h];
+  } else {
+    const void* zero = KV ? p.v_zero : p.k_zero;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t z = (reinterpret_cast<const uint16_t*>(zero) + tile)[row[i]];
+      st.meta[i] = z | uint32_t((reinterpret_cast<const uint16_t*>(scale) + tile)[row[i]]) << 16;
+    }
   }
 }
 
@@ -477,116 +459,120 @@ __device__ __forceinline__ uint32_t ex_max_u16(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
 
-// Write a loaded sub-tile into sub-tile place `at` (0 .. TK / 16 - 1) of a
-// tile; returns the largest magnitude bits of its V (two halves).
+// Write a loaded K half into sub-tile place `at` (0 .. TK / 16 - 1) of a tile.
 template <int DP, int WF, int TK>
-__device__ __forceinline__ uint32_t ex_store(const ExtendParams& p, const ExSub& s, const ExStage<DP>& st, int at,
-                                         bool check, ExTile<DP, TK>& t) {
-  typedef ExStage<DP> St;
+__device__ __forceinline__ void ex_store_k(const ExtendParams& p, const ExSub& s, const ExHalf<DP>& st, int at,
+                                           ExTile<DP, TK>& t) {
+  typedef ExHalf<DP> St;
   const int lane = threadIdx.x & 63, D = p.D;
-  const bool plain = s.valid == EX_SUB && D == DP;   // nothing to clear
-  const int n = lane & 15, g = lane >> 4;
   const bool zero = s.state == EX_STATE_ZERO, hot = s.state == HOT;
+  // The first piece's place; the next is 64 / (DP / 8) rows further.
+  uint4* const dst = t.k + ex_k_at<DP>(at * EX_SUB + lane / (DP / 8), lane % (DP / 8));
+  constexpr int NEXT = 64 / (DP / 8) * (DP / 8 + 1);
+  const bool clear = zero || (D != DP && (lane % (DP / 8)) * 8 >= D);
 #pragma unroll
   for (int i = 0; i < St::NPK; ++i) {
-    const int x = lane + 64 * i, r = x / (DP / 8), c = x % (DP / 8);
-    uint4 v = st.k[i];
-    if (zero || c * 8 >= D) {
-      v = make_uint4(0, 0, 0, 0);
-    } else if (!hot) {
+    uint4 v = st.r[i];
+    if (!zero && !hot) {
       f16x4 a, b;
-      f16x4 off;
       if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
-        a = i8x4_plus1152(v.x);
-        b = i8x4_plus1152(v.y);
-        off = f16x4{1152, 1152, 1152, 1152};
-        a -= off;
-        b -= off;
+        const f16x4 off = {1152, 1152, 1152, 1152};
+        a = i8x4_plus1152(v.x) - off;
+        b = i8x4_plus1152(v.y) - off;
       } else {
-        off = f16x4{1024, 1024, 1024, 1024};
-        const _Float16 z = as_f16x2(st.kmeta[i])[0];
-        a = u8x4_plus1024(v.x) - off;
-        b = u8x4_plus1024(v.y) - off;
-        a -= f16x4{z, z, z, z};
-        b -= f16x4{z, z, z, z};
+        const f16x4 off = {1024, 1024, 1024, 1024};
+        const _Float16 z = as_f16x2(st.meta[i])[0];
+        a = (u8x4_plus1024(v.x) - off) - f16x4{z, z, z, z};
+        b = (u8x4_plus1024(v.y) - off) - f16x4{z, z, z, z};
       }
       const uint2 lo = __builtin_bit_cast(uint2, a), hi = __builtin_bit_cast(uint2, b);
       v = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {   // (see ex_step: the factors of the logits are not negative)
-        const uint32_t sign = __uint_as_float(st.kmeta[0]) < 0.f ? 0x80008000u : 0u;
+      if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {   // (see ex_softmax: the factors of the logits are not negative)
+        const uint32_t sign = __uint_as_float(st.meta[0]) < 0.f ? 0x80008000u : 0u;
         v.x ^= sign;
         v.y ^= sign;
         v.z ^= sign;
         v.w ^= sign;
       }
     }
-    t.k[ex_k_at<DP>(at * EX_SUB + r, c)] = v;
+    if (clear) v = make_uint4(0, 0, 0, 0);
+    dst[i * NEXT] = v;
     if constexpr (WF == TIERKV_WARM_REF_U8) {
-      if (c == 0) t.kscale[at * EX_SUB + r] = (zero || hot) ? 1.f : half_hi(st.kmeta[i]);
+      if (lane % (DP / 8) == 0)
+        t.kscale[at * EX_SUB + (lane + 64 * i) / (DP / 8)] = (zero || hot) ? 1.f : half_hi(st.meta[i]);
     }
   }
   if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
-    if (lane == 0) t.kscale[at] = (zero || hot) ? 1.f : fabsf(__uint_as_float(st.kmeta[0]));
+    if (lane == 0) t.kscale[at] = (zero || hot) ? 1.f : fabsf(__uint_as_float(st.meta[0]));
   }
-  // V^T: the lane's four keys side by side, for each of its dims.
-  uint2* const dst = reinterpret_cast<uint2*>(t.v);
-  const int chunk = at * 2 + (g & 1), piece = g >> 1;
+}
+
+// The same of a V half, transposed; returns, when asked to check, the largest
+// magnitude bits of its values (two halves).
+template <int DP, int WF, int TK>
+__device__ __forceinline__ uint32_t ex_store_v(const ExtendParams& p, const ExSub& s, const ExHalf<DP>& st, int at,
+                                               bool check, ExTile<DP, TK>& t) {
+  typedef ExHalf<DP> St;
+  const int lane = threadIdx.x & 63, D = p.D;
+  const int n = lane & 15, g = lane >> 4;
+  const bool zero = s.state == EX_STATE_ZERO, hot = s.state == HOT;
+  const bool plain = s.valid == EX_SUB && D == DP;   // nothing to clear
+  // The lane's four keys side by side, for each of its dims.
+  uint2* const dst = reinterpret_cast<uint2*>(t.v + ex_v_at<TK>(St::DL * n, at * 2 + (g & 1))) + (g >> 1);
+  constexpr int NEXT = 2 * (TK / 8 + 1);             // the next dim's row
   uint32_t largest = 0;
-  auto put = [&](int d, uint2 o) {
-    dst[ex_v_at<TK>(d, chunk) * 2 + piece] = o;
+  auto put = [&](int i, uint2 o) {
+    dst[i * NEXT] = o;
     if (check) largest = ex_max_u16(largest, ex_max_u16(o.x & 0x7fff7fffu, o.y & 0x7fff7fffu));
   };
+  bool off[4];
 #pragma unroll
-  for (int u = 0; u < St::U; ++u) {
+  for (int j = 0; j < 4; ++j) off[j] = !plain && (zero || 4 * g + j >= s.valid || St::DL * n >= D);
+  if (zero || hot) {
     uint32_t w[4][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      w[j][0] = st.v[j][u].x;
-      w[j][1] = st.v[j][u].y;
-      w[j][2] = st.v[j][u].z;
-      w[j][3] = st.v[j][u].w;
-    }
-    if (zero || (hot && !plain)) {
+      w[j][0] = st.r[j].x;
+      w[j][1] = st.r[j].y;
+      w[j][2] = st.r[j].z;
+      w[j][3] = st.r[j].w;
+      if (!plain || zero) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool off = zero || 4 * g + j >= s.valid || St::DL * n + 8 * u >= D;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[j][i] = off ? 0u : w[j][i];
+        for (int i = 0; i < 4; ++i) w[j][i] = zero || off[j] ? 0u : w[j][i];
       }
     }
-    if (zero || hot) {
 #pragma unroll
-      for (int i = 0; i < St::UD; ++i) {
-        const uint32_t sel = (i & 1) ? 0x07060302u : 0x05040100u;
-        put(St::DL * n + 8 * u + i,
-            make_uint2(perm_b32(w[1][i / 2], w[0][i / 2], sel), perm_b32(w[3][i / 2], w[2][i / 2], sel)));
-      }
+    for (int i = 0; i < St::DL; ++i) {
+      const uint32_t sel = (i & 1) ? 0x07060302u : 0x05040100u;
+      put(i, make_uint2(perm_b32(w[1][i / 2], w[0][i / 2], sel), perm_b32(w[3][i / 2], w[2][i / 2], sel)));
+    }
+    return largest;
+  }
+  float mul[4], add[4];   // value = code' * mul + add (absmax), (code - add) * mul (reference)
+  uint32_t w[4][2];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
+      mul[j] = off[j] ? 0.f : __uint_as_float(st.meta[0]);
+      add[j] = -128.f * mul[j];
+      w[j][0] = st.r[j].x ^ 0x80808080u;
+      w[j][1] = st.r[j].y ^ 0x80808080u;
     } else {
-      float mul[4], add[4];   // value = code' * mul + add (absmax), (code - add) * mul (reference)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool off = 4 * g + j >= s.valid || St::DL * n + 8 * u >= D;
-        if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
-          mul[j] = off ? 0.f : __uint_as_float(st.vmeta[0]);
-          add[j] = -128.f * mul[j];
-        } else {
-          mul[j] = off ? 0.f : half_hi(st.vmeta[j]);
-          add[j] = off ? 0.f : half_lo(st.vmeta[j]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < St::UD; ++i) {
-        float f[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (WF == TIERKV_WARM_ABSMAX_I8)
-            f[j] = fmaf(ex_byte_at(w[j][i / 4] ^ 0x80808080u, i & 3), mul[j], add[j]);
-          else
-            f[j] = (ex_byte_at(w[j][i / 4], i & 3) - add[j]) * mul[j];
-        }
-        put(St::DL * n + 8 * u + i, make_uint2(ex_pack(f[0], f[1]), ex_pack(f[2], f[3])));
-      }
+      mul[j] = off[j] ? 0.f : half_hi(st.meta[j]);
+      add[j] = off[j] ? 0.f : half_lo(st.meta[j]);
+      w[j][0] = st.r[j].x;
+      w[j][1] = st.r[j].y;
     }
+  }
+#pragma unroll
+  for (int i = 0; i < St::DL; ++i) {
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float c = ex_byte_at(w[j][i / 4], i & 3);
+      f[j] = WF == TIERKV_WARM_ABSMAX_I8 ? fmaf(c, mul[j], add[j]) : (c - add[j]) * mul[j];
+    }
+    put(i, make_uint2(ex_pack(f[0], f[1]), ex_pack(f[2], f[3])));
   }
   return largest;
 }
@@ -600,7 +586,7 @@ __device__ __forceinline__ bool ex_wild(uint32_t w) { return (w & 0xffffu) >= 0x
 // (ex_add_wild).  Both are rare and kept out of the tile loop's registers.
 template <int DP, int TK>
 __device__ __attribute__((noinline)) void ex_clear_wild(int at, ExTile<DP, TK>* t) {
-  typedef ExStage<DP> St;
+  typedef ExHalf<DP> St;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int chunk = at * 2 + (g & 1), piece = g >> 1;
   uint2* const dst = reinterpret_cast<uint2*>(t->v);
@@ -825,19 +811,20 @@ __device__ __forceinline__ uint32_t ex_out2(float a, float b) {
 
 template <int DP>
 constexpr int ex_lds_bytes() {
-  const int wide = 2 * int(sizeof(ExTile<DP, 64>)), narrow = 4 * int(sizeof(ExTile<DP, 32>));
-  const int merge = 4 * 32 * (DP + 4 + 2) * 4;
+  const int wide = 2 * int(sizeof(ExTile<DP, 64>)), narrow = EX_WAVES * int(sizeof(ExTile<DP, 32>));
+  const int merge = EX_WAVES * 32 * (DP + 4 + 2) * 4;
   return wide > narrow ? (wide > merge ? wide : merge) : (narrow > merge ? narrow : merge);
 }
 
 // An item: query rows of one tile, sub-tiles [part / parts) of what it sees.
-//   RW  waves that hold different rows (4: wide, 1: narrow); 4 / RW waves
-//       share the rows and split the keys
-template <int DP, int WF, typename QT, int RW>
-__device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, int64_t partial) {
-  constexpr int TK = RW == 4 ? 64 : 32;
-  constexpr int NS = TK / 16 / RW;          // sub-tiles a wave stages
-  constexpr int KW = 4 / RW;
+//   WIDE  every wave holds 32 rows of its own and all share 64 keys at a time,
+//         each wave staging the K or the V of one sub-tile; else all hold the
+//         same 32 rows and each stages and takes 32 keys of its own
+template <int DP, int WF, typename QT, bool WIDE>
+__device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h, const ex_int4 it, int64_t partial) {
+  constexpr int TK = WIDE ? 64 : 32;
+  constexpr int NS = WIDE ? 1 : 4;          // halves a wave stages
+  constexpr int KW = WIDE ? 1 : EX_WAVES;   // waves that split the keys
   const int tid = threadIdx.x, lane = tid & 63, w = ex_uniform(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int b = it.x, tile = it.y & 0x3fffffff;
@@ -845,13 +832,13 @@ __device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, 
   const int4 seq = p.seq[b];
   const int q0 = ex_rows(p, b).x, n = seq.w, G = p.groups, D = p.D;
   const int rows = n * G;
-  const int row_first = tile * EX_WIDE, row_last = min(row_first + RW * 32, rows) - 1;
+  const int row_first = tile * EX_WIDE, row_last = min(row_first + (WIDE ? EX_WIDE : 32), rows) - 1;
   const int lim_min = seq.y - n + row_first / G, lim_max = seq.y - n + row_last / G;
   const int4* raw_list = p.subtile + int64_t(b) * p.subs_per_seq;
   const ExList list = (ExList)(uintptr_t)raw_list;
 
   // This lane's row.
-  const int r = row_first + (RW == 4 ? w * 32 : 0) + col;
+  const int r = row_first + (WIDE ? w * 32 : 0) + col;
   const bool live = r < rows;
   const int tok = live ? r / G : 0, head = h * G + (live ? r - tok * G : 0);
   const int lim = live ? seq.y - n + tok : -1;
@@ -910,83 +897,146 @@ __device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, 
   }
 
   const int visible = ex_uniform(ex_visible(raw_list, seq.x, lim_max));
-  constexpr int ROUND = RW == 4 ? 4 : 8;
+  constexpr int ROUND = TK / 16 * KW;       // sub-tiles per round of the workgroup
   const int chunk = ((visible + parts - 1) / parts + ROUND - 1) & ~(ROUND - 1);
   const int lo = min(part * chunk, visible), hi = min(lo + chunk, visible);
 
-  // Wide: two tiles in LDS, so that a round has one barrier: the next tile is
-  // stored while this one's matrix products run, and the one after it loads.
-  // Narrow: a tile per wave, stored between its steps in the wave's own order.
-  constexpr int STEP = TK / 16 * KW;        // sub-tiles per round of the workgroup
+  // Wide: two tiles in LDS; the next tile is stored while this one is taken,
+  // and the one after it loads.  Narrow: a tile per wave, stored between its
+  // steps in the wave's own order.
   ExTile<DP, TK>* tiles = reinterpret_cast<ExTile<DP, TK>*>(lds);
-  const int first = RW == 4 ? lo : lo + w * (TK / 16);
-  ExStage<DP> st[NS];
-  ExSub sub[NS];
+  const int first = WIDE ? lo : lo + w * (TK / 16);
+  ExHalf<DP> st[NS];
+  ExSub sub[WIDE ? 1 : 2];
   bool wild = false;
   auto find = [&](int at) {
-#pragma unroll
-    for (int i = 0; i < NS; ++i) sub[i] = ex_sub(list, min(at, hi) + (RW == 4 ? w : i), hi);
+    if constexpr (WIDE) {
+      sub[0] = ex_sub(list, min(at, hi) + (w & 3), hi);
+    } else {
+      sub[0] = ex_sub(list, min(at, hi), hi);
+      sub[1] = ex_sub(list, min(at, hi) + 1, hi);
+    }
   };
   auto load = [&]() {
+    if constexpr (WIDE) {
+      if (w < 4) ex_load<DP, WF, 0>(p, h, sub[0], st[0]);
+      else ex_load<DP, WF, 1>(p, h, sub[0], st[0]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < NS; ++i) ex_load<DP, WF>(p, h, sub[i], st[i]);
-  };
-  auto store = [&](ExTile<DP, TK>& t, const ExSub (&of)[NS], bool whole) {
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int place = RW == 4 ? w : i;
-      const uint32_t largest = ex_store<DP, WF, TK>(p, of[i], st[i], place, !whole, t);
-      if (!whole && __any(ex_wild(largest))) {
-        ex_clear_wild<DP, TK>(place, &t);
-        wild = true;
+      for (int i = 0; i < 2; ++i) {
+        ex_load<DP, WF, 0>(p, h, sub[i], st[2 * i]);
+        ex_load<DP, WF, 1>(p, h, sub[i], st[2 * i + 1]);
       }
     }
   };
-  if (first < hi) {
-    const int full = ex_uniform(ex_full_until(raw_list, lo, hi, lim_min));
-    find(first);
-    load();
-    store(tiles[RW == 4 ? 0 : w], sub, first + TK / 16 <= full);
-    find(first + STEP);
-    load();
-    if constexpr (RW == 4) __syncthreads();
-    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    int buf = 0;
-    for (int at = first; at < hi; at += STEP) {
-      const ExTile<DP, TK>& t = tiles[RW == 4 ? buf : w];
-      const bool whole = at + TK / 16 <= full;
-      ExSub held[NS];
+  auto store_v = [&](ExTile<DP, TK>& t, const ExSub& of, const ExHalf<DP>& v, int place, bool whole) {
+    const uint32_t largest = ex_store_v<DP, WF, TK>(p, of, v, place, !whole, t);
+    if (!whole && __any(ex_wild(largest))) {
+      ex_clear_wild<DP, TK>(place, &t);
+      wild = true;
+    }
+  };
+  auto store = [&](ExTile<DP, TK>& t, const auto& of, bool whole) {
+    if constexpr (WIDE) {
+      if (w < 4) ex_store_k<DP, WF, TK>(p, of[0], st[0], w, t);
+      else store_v(t, of[0], st[0], w - 4, whole);
+    } else {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) held[i] = sub[i];
-      find(at + 2 * STEP);
-      f32x16 s[TK / 32];
-      ex_logits<DP, TK>(t, q, s);
-      if constexpr (RW == 4) {
-        if (at + STEP < hi) {
-          store(tiles[buf ^ 1], held, at + STEP + TK / 16 <= full);
-          load();
-        }
+      for (int i = 0; i < 2; ++i) {
+        ex_store_k<DP, WF, TK>(p, of[i], st[2 * i], i, t);
+        store_v(t, of[i], st[2 * i + 1], i, whole);
       }
+    }
+  };
+  if constexpr (WIDE) {
+    // The two waves of a SIMD work half a tile apart: while waves 0-3 form a
+    // tile's logits, waves 4-7 take the softmax and the output of the tile
+    // before, so one's matrix products run beside the other's exponentials
+    // (in step, the products and the exponentials of all waves came one after
+    // the other: 1313 us at 2048 tokens on 32768). Waves 0-3 stage K, 4-7 V.
+    const bool idle = row_first + w * 32 >= rows;   // a wave without rows only stages
+    const int tiles_n = (hi - lo + 3) / 4, lag = w >> 2;
+    int full = 0;
+    if (tiles_n > 0) {
+      full = ex_uniform(ex_full_until(raw_list, lo, hi, lim_min));
+      find(lo);
+      load();
+      store(tiles[0], sub, lo + 4 <= full);
+      find(lo + 4);
+      load();
+      __syncthreads();
+    }
+    auto output = [&](int at, f32x16 (&s)[TK / 32], const ExTile<DP, TK>& t) {
+      const bool whole = at + 4 <= full;
       int end[TK / 16] = {};
       if (!whole) ex_ends<TK>(list, at, hi, lim, end);
       ex_softmax<DP, WF, TK>(t, qscale, end, whole, s, a);
-      if constexpr (RW == 4) {
+    };
+    // Two barriers per tile; every wave meets 2 tiles_n + 1 of them.
+    int buf = 0;
+    if (w < 4) {
+      for (int at = lo; at < hi; at += 4, buf ^= 1) {
+        f32x16 s[TK / 32];
+        if (!idle) ex_logits<DP, TK>(tiles[buf], q, s);
         __syncthreads();
-        buf ^= 1;
-      } else if (at + STEP < hi) {
+        if (at + 4 < hi) {
+          ex_store_k<DP, WF, TK>(p, sub[0], st[0], w, tiles[buf ^ 1]);
+          find(at + 8);
+          ex_load<DP, WF, 0>(p, h, sub[0], st[0]);
+        }
+        if (!idle) output(at, s, tiles[buf]);
+        __syncthreads();
+      }
+      __syncthreads();
+    } else {
+      __syncthreads();
+      for (int at = lo; at < hi; at += 4, buf ^= 1) {
+        f32x16 s[TK / 32];
+        if (!idle) ex_logits<DP, TK>(tiles[buf], q, s);
+        if (at + 4 < hi) {
+          store_v(tiles[buf ^ 1], sub[0], st[0], w - 4, at + 8 <= full);
+          find(at + 8);
+          ex_load<DP, WF, 1>(p, h, sub[0], st[0]);
+        }
+        __syncthreads();
+        if (!idle) output(at, s, tiles[buf]);
+        __syncthreads();
+      }
+    }
+  } else if (first < hi) {
+    const int full = ex_uniform(ex_full_until(raw_list, lo, hi, lim_min));
+    find(first);
+    load();
+    store(tiles[w], sub, first + TK / 16 <= full);
+    find(first + ROUND);
+    load();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int at = first; at < hi; at += ROUND) {
+      const bool whole = at + TK / 16 <= full;
+      ExSub held[2];
+      held[0] = sub[0];
+      held[1] = sub[WIDE ? 0 : 1];
+      find(at + 2 * ROUND);
+      f32x16 s[TK / 32];
+      ex_logits<DP, TK>(tiles[w], q, s);
+      int end[TK / 16] = {};
+      if (!whole) ex_ends<TK>(list, at, hi, lim, end);
+      ex_softmax<DP, WF, TK>(tiles[w], qscale, end, whole, s, a);
+      if (at + ROUND < hi) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        store(tiles[w], held, at + STEP + TK / 16 <= full);
+        store(tiles[w], held, at + ROUND + TK / 16 <= full);
         load();
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       }
     }
   }
   // Infinities and NaN of the tiles with hidden keys, for the rows that see them.
-  if constexpr (RW == 4) wild = __syncthreads_or(wild);
+  if constexpr (WIDE) wild = __syncthreads_or(wild);
   if (wild) {
+    const int full = ex_full_until(raw_list, lo, hi, lim_min);
 #pragma unroll 1
-    for (int at = first; at < hi; at += STEP) {
-      if (at + TK / 16 <= ex_full_until(raw_list, lo, hi, lim_min)) continue;
+    for (int at = first; at < hi; at += ROUND) {
+      if (at + TK / 16 <= full) continue;
 #pragma unroll 1
       for (int k = 0; k < TK / 16; ++k) {
         const ExSub sb = ex_sub(list, at + k, hi);
@@ -1088,19 +1138,16 @@ __device__ void ex_item(const ExtendParams& p, char* lds, int h, const int4 it, 
   }
 }
 
-template <int DP, int WF, typename QT>
+// MIXED: calls that may hold wide tiles; the others' kernel is without their code.
+template <int DP, int WF, typename QT, bool MIXED>
 __global__ __launch_bounds__(EX_THREADS, 2) void extend_kernel(ExtendParams p) {
   extern __shared__ __attribute__((aligned(16))) char ex_lds[];
   const int i = int(blockIdx.x) / p.kv_heads, h = int(blockIdx.x) - i * p.kv_heads;
   if (i >= p.head[0]) return;
-  int4 it = p.item[i];
-  it.x = ex_uniform(it.x);
-  it.y = ex_uniform(it.y);
-  it.z = ex_uniform(it.z);
-  it.w = ex_uniform(it.w);
+  const ex_int4 it = ((ExList)(uintptr_t)p.item)[i];
   if (it.x < 0) return;
-  if (it.y & (1 << 30)) ex_item<DP, WF, QT, 4>(p, ex_lds, h, it, it.w);
-  else ex_item<DP, WF, QT, 1>(p, ex_lds, h, it, it.w);
+  if (MIXED && (it.y & (1 << 30))) ex_item<DP, WF, QT, true>(p, ex_lds, h, it, it.w);
+  else ex_item<DP, WF, QT, false>(p, ex_lds, h, it, it.w);
 }
 
 // Join of a cut tile's partials, in part order: a workgroup per (cut tile, kv
@@ -1198,7 +1245,9 @@ template <int DP, int WF, typename QT>
 static void ex_launch(const ExtendParams& p, hipStream_t stream) {
   const int lds = ex_lds_bytes<DP>();
   hipLaunchKernelGGL(extend_plan_kernel, dim3(p.batch), dim3(EX_PLAN), 0, stream, p);
-  hipLaunchKernelGGL((extend_kernel<DP, WF, QT>), dim3(p.max_items * p.kv_heads), dim3(EX_THREADS), lds, stream, p);
+  const dim3 grid(p.max_items * p.kv_heads);
+  if (p.part_rows > EX_NARROW) hipLaunchKernelGGL((extend_kernel<DP, WF, QT, true>), grid, dim3(EX_THREADS), lds, stream, p);
+  else hipLaunchKernelGGL((extend_kernel<DP, WF, QT, false>), grid, dim3(EX_THREADS), lds, stream, p);
   const int rows_per_wg = 4 * EX_THREADS / p.D;
   hipLaunchKernelGGL(extend_merge_kernel<QT>,
                      dim3(p.max_cut * p.kv_heads, (p.part_rows + rows_per_wg - 1) / rows_per_wg), dim3(EX_THREADS), 0,
