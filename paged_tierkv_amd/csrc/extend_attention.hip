@@ -955,7 +955,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
     // (in step, the products and the exponentials of all waves came one after
     // the other: 1313 us at 2048 tokens on 32768). Waves 0-3 stage K, 4-7 V.
     const bool idle = row_first + w * 32 >= rows;   // a wave without rows only stages
-    const int tiles_n = (hi - lo + 3) / 4, lag = w >> 2;
+    const int tiles_n = (hi - lo + 3) / 4;
     int full = 0;
     if (tiles_n > 0) {
       full = ex_uniform(ex_full_until(raw_list, lo, hi, lim_min));
