@@ -25,7 +25,9 @@ Two runtimes plug in through their ``cache`` object:
 * ``runtime.BatchedTieredKVRuntime`` -- B sequences in lockstep
   (``is_batched``): prefill goes straight to the tiers, each decode step is
   one ``decode_layer`` call (fused append, attention, and on policy steps the
-  device-side tick).  Sequences must be unpadded and of equal length, the
+  device-side tick).  With ``extend_tokens`` set, a forward of several
+  tokens on a cache that holds some is one ``extend_layer`` call (a follow-up
+  prompt, drafted tokens).  Sequences must be unpadded and of equal length, the
   same restriction the reference's decode path has (batch 1, no padding,
   modeling_llama.py:70-73).
 """
@@ -250,6 +252,13 @@ def tierkv_attention_forward(self, hidden_states: torch.Tensor, position_embeddi
 def _batched_forward(self, runtime, query_states, key_states, value_states, attention_mask, input_shape, dropout,
                      kwargs):
     layer = self.layer_idx
+    if runtime.extends(int(query_states.shape[-2])):
+        # Several tokens on top of the cache: a follow-up prompt, drafted tokens.
+        if not bool(kwargs.get("tierkv_triton_mask_safe", False)):
+            raise ValueError("the batched tiered runtime extends unpadded sequences only (2-D or no attention mask).")
+        out = runtime.extend_layer(layer, query_states, key_states, value_states, self.num_key_value_groups,
+                                   self.scaling)
+        return self.o_proj(out.reshape(*input_shape, -1)), None
     if query_states.shape[-2] > 1:
         attn_output, attn_weights = _attention_interface(self)(
             self, query_states, key_states, value_states, attention_mask, scaling=self.scaling, dropout=dropout)
@@ -362,6 +371,19 @@ class DecodeGraphRunner:
         rt.cache.finish_forward()
         self.replays += 1
         return out
+
+    def sample_step(self, input_ids: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+                    min_p=0.0):
+        """One decode step and the choice of the next tokens
+        (``kernels.sample_tokens`` of the last position's logits with one
+        random number per sequence; each limit a number or a tensor [B]).
+        Returns (next token ids [B, 1], the probabilities [B] they were drawn
+        with); nothing is read back to the host."""
+        from . import kernels
+
+        logits = self.step(input_ids)[:, -1]
+        tokens, probs = kernels.sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p)
+        return tokens[:, None], probs
 
 
 def install() -> None:

@@ -17,7 +17,10 @@ resident on the device:
 * ``decode_layer`` appends the step's K/V (``tierkv_runtime_append``: new HOT
   blocks popped on the device), runs the tiered decode kernel, and on policy
   steps runs ``tierkv_runtime_tick`` (scores -> labels -> migrations on the
-  device).  The host never waits for the device inside a step.
+  device).  The host never waits for the device inside a step;
+* ``extend_layer`` takes several new tokens per sequence on top of what the
+  cache holds (a follow-up prompt, drafted tokens): slot map, row write,
+  ``tierkv_extend_attention``, and the tick by the scores of the last token.
 
 Budgets are fractions of each sequence's current block count (workload
 C5: 15 % HOT, 55 % WARM, the rest evicted), evaluated on the host from the
@@ -34,12 +37,12 @@ import numpy as np
 import torch
 
 from . import _lib, kernels
-from .tierkv_hip import DecodeWorkspace, tierkv_decode_attention
+from .tierkv_hip import DecodeWorkspace, tierkv_decode_attention, tierkv_extend_attention
 
 HOT_STATE, WARM_STATE, COLD_STATE = 0, 1, 2
 _MODES = {"hot_warm": 1, "hot_warm_cold": 2}
 ERROR_BITS = {1: "no free HOT slot", 2: "no free WARM slot", 4: "a table row is full",
-              8: "a sequence's last block was not HOT"}
+              8: "a sequence's last block was not HOT", 16: "token counts did not fit the packed rows"}
 
 
 def _ceil_div(a: int, b: int) -> int:
@@ -180,7 +183,7 @@ class BatchedTieredKVRuntime:
                  block_size: int = 16, hot_fraction: float = 0.15, warm_fraction: float = 0.55,
                  policy_mode: str = "hot_warm_cold", policy_interval: int = 64,
                  warm_format: str = "absmax_i8", cold_mode: str = "masked", device=None,
-                 prefill_scoring: str = "proxy", deterministic: bool | None = None):
+                 prefill_scoring: str = "proxy", deterministic: bool | None = None, extend_tokens: int = 0):
         if policy_mode not in _MODES:
             raise ValueError('policy_mode must be "hot_warm" or "hot_warm_cold".')
         if warm_format not in kernels.WARM_FORMATS:
@@ -189,6 +192,8 @@ class BatchedTieredKVRuntime:
             raise ValueError("policy_interval must be positive.")
         if prefill_scoring not in ("proxy", "attention"):
             raise ValueError('prefill_scoring must be "proxy" or "attention".')
+        if extend_tokens < 0:
+            raise ValueError("extend_tokens must not be negative.")
         if not (0.0 <= hot_fraction <= 1.0 and 0.0 <= warm_fraction <= 1.0):
             raise ValueError("tier fractions must lie in [0, 1].")
         self.device = torch.device(device or "cuda")
@@ -220,6 +225,10 @@ class BatchedTieredKVRuntime:
             env = os.environ.get("TIERKV_DETERMINISTIC")
             deterministic = True if env is None else env not in ("", "0")
         self.deterministic = bool(deterministic)
+        # The most tokens that a forward of several tokens may add to a cache
+        # that holds some (extend_layer); 0: such a forward is a new prompt,
+        # which replaces the cache.
+        self.extend_tokens = int(extend_tokens)
         n = self.max_blocks
         # Capacities per sequence, from the budgets: a tick reuses the slots it
         # frees (demotions take evicted WARM slots, promotions the HOT slots
@@ -228,6 +237,8 @@ class BatchedTieredKVRuntime:
         # promotions (blocks still WARM until the promotion has read them).
         hot_max = max(2, budget_blocks(self.hot_fraction, n))
         appended = _ceil_div(self.policy_interval, self.block_size) + 2
+        if self.extend_tokens:
+            appended += _ceil_div(self.extend_tokens, self.block_size) + 1
         self.hot_per_seq = min(n, hot_max + appended)
         if policy_mode == "hot_warm":
             self.warm_per_seq = n
@@ -492,6 +503,56 @@ class BatchedTieredKVRuntime:
             self.last_score_sums = sums   # the probability sums the tick ranked (kept for inspection)
             self.tick_layer(layer, sums, num_blocks)
         return out
+
+    def extends(self, query_length: int) -> bool:
+        """Whether a forward of ``query_length`` tokens adds to what the cache
+        holds (True) or is a new prompt (False)."""
+        return query_length > 1 and self.extend_tokens > 0 and self.cache.get_seq_length() > 0
+
+    def extend_layer(self, layer: int, query_states: torch.Tensor, key_states: torch.Tensor,
+                     value_states: torch.Tensor, num_key_value_groups: int, scaling: float,
+                     policy_step: bool = True) -> torch.Tensor:
+        """Several new tokens per sequence of one layer: append K/V [B, kv_heads,
+        T, D], attend with query [B, H, T, D] (rotated, as K; each token sees
+        the cache and the new tokens up to itself) and, with ``policy_step``,
+        re-tier the layer by the scores of the last token.  T is at most
+        ``extend_tokens``.  Returns the attention output [B, T, H, D]."""
+        if key_states.shape != value_states.shape or key_states.ndim != 4 or query_states.ndim != 4:
+            raise ValueError("query must be [batch, heads, tokens, head_dim], K/V [batch, kv_heads, tokens, head_dim].")
+        B, kv, T, d = (int(x) for x in key_states.shape)
+        if (B, kv, d) != (self.batch, self.kv_heads, self.head_dim) or (int(query_states.shape[0]),
+                                                                       int(query_states.shape[2])) != (B, T):
+            raise ValueError("query or K/V geometry does not match the runtime.")
+        if not 0 < T <= self.extend_tokens:
+            raise ValueError(f"extend_layer takes 1 to extend_tokens={self.extend_tokens} tokens per sequence.")
+        room = self.block_size - self._open_tokens[layer] if self._open_tokens[layer] else 0
+        if self._blocks[layer] + _ceil_div(max(T - room, 0), self.block_size) > self.max_blocks:
+            raise RuntimeError(f"{T} more tokens exceed max_seq_len={self.max_seq_len}.")
+        st = self.layers[layer]
+        rows = lambda t: t.transpose(1, 2).reshape(B * T, t.shape[1], d)   # noqa: E731
+        q, k, v = rows(query_states), rows(key_states), rows(value_states)
+        if k.dtype not in (torch.float16, torch.bfloat16):
+            k, v = k.to(torch.float16), v.to(torch.float16)
+        new = torch.full((B,), T, dtype=torch.int32, device=self.device)
+        m = kernels.build_slot_map(new, st.table, st.states, st.lengths, st.nblocks, st.open, st.hot_free, st.ctl,
+                                   self.block_size, B * T)
+        kernels.write_slots(k, v, m.slots, st.hot_k, st.hot_v)
+        num_blocks = min(self._advance_blocks(layer, T), self.max_blocks)
+        out = tierkv_extend_attention(
+            q, m.cu_tokens, st.table, st.states, st.lengths, st.hot_k, st.hot_v, st.warm_k, st.warm_v, st.k_scale,
+            st.k_zero, st.v_scale, st.v_zero, num_blocks, num_key_value_groups, scaling, cold_mode=self.cold_mode,
+            seq_num_blocks=st.nblocks, max_tokens=T)
+        if policy_step:
+            _, sums = tierkv_decode_attention(
+                query_states[:, :, -1:].contiguous(), st.table, st.states, st.lengths, st.hot_k, st.hot_v, st.warm_k,
+                st.warm_v, st.k_scale, st.k_zero, st.v_scale, st.v_zero, num_blocks, num_key_value_groups, scaling,
+                return_scores=True, cold_mode=self.cold_mode, seq_num_blocks=st.nblocks,
+                workspace=self.reserve_decode_workspace(query_states.shape[1]), deterministic=self.deterministic)
+            self.last_score_sums = sums
+            self.tick_layer(layer, sums, num_blocks)
+        if layer == self.num_layers - 1:
+            self.seq_len += T
+        return out.view(B, T, -1, d)
 
     def tick_layer(self, layer: int, score_sums: torch.Tensor, num_blocks: int) -> None:
         st = self.layers[layer]
