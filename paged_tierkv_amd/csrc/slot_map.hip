@@ -57,51 +57,67 @@ struct SlotMapParams {
   int32_t* head;    // {ok, stack top, error bits, new blocks}
 };
 
-// Inclusive prefix sum of a 64-bit value over the workgroup (waves of 64,
-// sh: one entry per wave and one for the total).
-__device__ __forceinline__ int64_t sm_scan(int64_t v, int64_t* sh, int64_t* total) {
+// Inclusive prefix sums of two 64-bit values over the workgroup.
+struct Sm2 {
+  int64_t n, need;
+};
+__device__ __forceinline__ Sm2 sm_scan(Sm2 v, Sm2* sh, Sm2* total) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  int64_t x = v;
+  Sm2 x = v;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int64_t y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
+    const int64_t a = __shfl_up(x.n, d, 64), b = __shfl_up(x.need, d, 64);
+    if (lane >= d) {
+      x.n += a;
+      x.need += b;
+    }
   }
+  __syncthreads();
   if (lane == 63) sh[w] = x;
   __syncthreads();
-  if (w == 0) {
-    int64_t t = lane < SM_WAVES ? sh[lane] : 0;
-    const int64_t own = t;
+  Sm2 all = {0, 0};
 #pragma unroll
-    for (int d = 1; d < SM_WAVES; d <<= 1) {
-      const int64_t y = __shfl_up(t, d, 64);
-      if (lane >= d) t += y;
+  for (int i = 0; i < SM_WAVES; ++i) {
+    const Sm2 t = sh[i];
+    if (i < w) {
+      x.n += t.n;
+      x.need += t.need;
     }
-    if (lane < SM_WAVES) sh[lane] = t - own;
-    if (lane == SM_WAVES - 1) sh[SM_WAVES] = t;
+    all.n += t.n;
+    all.need += t.need;
   }
-  __syncthreads();
-  x += sh[w];
-  *total = sh[SM_WAVES];
-  __syncthreads();
+  *total = all;
   return x;
 }
 
-// Tokens that request b holds: the sum of its blocks' lengths, by one wave.
-__device__ __forceinline__ int tokens_held(const SlotMapParams& p, int b) {
-  const int lane = threadIdx.x & 63;
-  const int nb = min(max(p.nblocks[b], 0), int(min(p.stride, int64_t(0x7fffffff))));
-  const int32_t* row = p.lengths + int64_t(b) * p.stride;
+// Tokens that each request of [b0, b0 + 4) holds, the sums of their blocks'
+// lengths, by the 16-lane rows of one wave (four requests of 256 blocks: two
+// memory round trips, where a wave per request in turn took eight).
+__device__ __forceinline__ void tokens_held(const SlotMapParams& p, int b0, int32_t* held) {
+  const int lane = threadIdx.x & 63, c = lane & 15, b = b0 + (lane >> 4);
   int sum = 0;
-  for (int i = lane; i < nb; i += 64) sum += min(max(row[i], 0), p.bs);
+  if (b < p.batch) {
+    const int nb = min(max(p.nblocks[b], 0), int(min(p.stride, int64_t(0x7fffffff))));
+    const int32_t* row = p.lengths + int64_t(b) * p.stride;
+    int i = c;
+    for (; i + 7 * 16 < nb; i += 8 * 16) {
+      int v[8];
 #pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
-  return sum;
+      for (int k = 0; k < 8; ++k) v[k] = row[i + k * 16];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += min(max(v[k], 0), p.bs);
+    }
+    for (; i < nb; i += 16) sum += min(max(row[i], 0), p.bs);
+  }
+#pragma unroll
+  for (int m = 8; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
+  if (c == 0 && b < p.batch) held[b] = sum;
 }
 
 // The prefix sums (one workgroup of SM_THREADS): writes cu, the requests'
-// plan entries and the head; returns whether the step fits.
-__device__ __forceinline__ bool sm_plan(const SlotMapParams& p, int64_t* sh, int* s_err) {
+// plan entries (seq) and the head; cu also to where the caller keeps it.
+__device__ __forceinline__ void sm_plan(const SlotMapParams& p, Sm2* sh, int* s_err, int4* seq, int32_t* head,
+                                        int32_t* cu) {
   const int tid = threadIdx.x, B = p.batch, bs = p.bs;
   const int nit = (B + SM_THREADS - 1) / SM_THREADS;
   int n[SM_NIT], room[SM_NIT], nb[SM_NIT];
@@ -137,11 +153,12 @@ __device__ __forceinline__ bool sm_plan(const SlotMapParams& p, int64_t* sh, int
 #pragma unroll
   for (int it = 0; it < SM_NIT; ++it) {
     if (it < nit) {
-      int64_t total;
-      cu_end[it] = tokens + sm_scan(n[it], sh, &total);
-      tokens += total;
-      first[it] = blocks + sm_scan(need[it], sh, &total) - need[it];
-      blocks += total;
+      Sm2 total;
+      const Sm2 x = sm_scan({n[it], need[it]}, sh, &total);
+      cu_end[it] = tokens + x.n;
+      first[it] = blocks + x.need - need[it];
+      tokens += total.n;
+      blocks += total.need;
     }
   }
   if (tid == 0) {
@@ -155,25 +172,25 @@ __device__ __forceinline__ bool sm_plan(const SlotMapParams& p, int64_t* sh, int
     const int b = it * SM_THREADS + tid;
     if (it < nit && b < B) {
       p.cu[b + 1] = ok ? int32_t(cu_end[it]) : 0;
-      p.seq[b] = make_int4(ok ? int32_t(first[it]) : 0, room[it], nb[it], ok ? n[it] : 0);
+      if (cu) cu[b + 1] = ok ? int32_t(cu_end[it]) : 0;
+      seq[b] = make_int4(ok ? int32_t(first[it]) : 0, room[it], nb[it], ok ? n[it] : 0);
     }
   }
   if (tid == 0) {
     p.cu[0] = 0;
-    p.head[0] = ok;
-    p.head[1] = top;
-    p.head[2] = *s_err;
-    p.head[3] = ok ? int32_t(blocks) : 0;
+    if (cu) cu[0] = 0;
+    head[0] = ok;
+    head[1] = top;
+    head[2] = *s_err;
+    head[3] = ok ? int32_t(blocks) : 0;
   }
-  return ok;
 }
 
 // Counts, open flags, the open blocks' lengths and the tokens held after the
 // step, of request b.
-__device__ __forceinline__ void sm_update(const SlotMapParams& p, int b) {
-  const int4 s = p.seq[b];
+__device__ __forceinline__ void sm_update(const SlotMapParams& p, int b, const int4 s, int held) {
   const int n = s.w, bs = p.bs;
-  p.context[b] = p.held[b] + n;
+  p.context[b] = held + n;
   if (n == 0) return;
   const int taken = min(s.y, n);
   const int need = (n - taken + bs - 1) / bs;
@@ -183,16 +200,17 @@ __device__ __forceinline__ void sm_update(const SlotMapParams& p, int b) {
   p.open[b] = last < bs ? 1 : 0;
 }
 
-__device__ __forceinline__ void sm_finish(const SlotMapParams& p) {
-  if (p.head[2]) atomicOr(p.ctl + 2, p.head[2]);
-  p.ctl[0] = p.head[0] ? p.head[1] - p.head[3] : p.ctl[0];
-  p.ctl[3] = p.head[0];
+__device__ __forceinline__ void sm_finish(const SlotMapParams& p, const int32_t* head) {
+  if (head[2]) atomicOr(p.ctl + 2, head[2]);
+  if (head[0]) p.ctl[0] = head[1] - head[3];
+  p.ctl[3] = head[0];
 }
 
 // Rows [r0, r0 + 4) of the packed step: their slots and positions, and the
 // table entries of the blocks whose first token is among them.  cu is in LDS.
-__device__ __forceinline__ void sm_rows(const SlotMapParams& p, const int32_t* cu, int r0) {
-  const int B = p.batch, bs = p.bs, top = p.head[1];
+__device__ __forceinline__ void sm_rows(const SlotMapParams& p, const int32_t* cu, const int4* seq, const int32_t* held,
+                                        int top, int r0) {
+  const int B = p.batch, bs = p.bs;
   const int total = cu[B];
   int lo = 0, hi = B;                       // cu[lo] <= r0 < cu[hi] (when r0 < total)
   while (hi - lo > 1) {
@@ -207,9 +225,9 @@ __device__ __forceinline__ void sm_rows(const SlotMapParams& p, const int32_t* c
     slot[k] = pos[k] = -1;
     if (r < total) {
       while (cu[b + 1] <= r) ++b;
-      const int4 s = p.seq[b];
+      const int4 s = seq[b];
       const int i = r - cu[b];
-      pos[k] = p.held[b] + i;
+      pos[k] = held[b] + i;
       const int64_t row = int64_t(b) * p.stride;
       if (i < s.y) {
         slot[k] = p.table[row + s.z - 1] * bs + (bs - s.y) + i;
@@ -237,38 +255,33 @@ __device__ __forceinline__ void sm_rows(const SlotMapParams& p, const int32_t* c
   }
 }
 
-// The whole step in one workgroup.
+// The whole step in one workgroup; what passes between the phases is in LDS.
 __global__ __launch_bounds__(SM_THREADS) void slot_map_kernel(SlotMapParams p) {
-  __shared__ int64_t sh[SM_WAVES + 1];
+  __shared__ Sm2 sh[SM_WAVES];
   __shared__ int s_err;
-  __shared__ int32_t s_cu[SM_MAX_BATCH + 1];
+  __shared__ int32_t s_head[4];
+  __shared__ int32_t s_cu[SM_THREADS + 1];
+  __shared__ int32_t s_held[SM_THREADS];
+  __shared__ int4 s_seq[SM_THREADS];
   const int tid = threadIdx.x;
-  for (int b = tid >> 6; b < p.batch; b += SM_WAVES) {
-    const int held = tokens_held(p, b);
-    if ((tid & 63) == 0) p.held[b] = held;
-  }
-  sm_plan(p, sh, &s_err);
+  for (int b = (tid >> 6) * 4; b < p.batch; b += SM_WAVES * 4) tokens_held(p, b, s_held);
+  sm_plan(p, sh, &s_err, s_seq, s_head, s_cu);
   __syncthreads();
-  for (int b = tid; b <= p.batch; b += SM_THREADS) s_cu[b] = p.cu[b];
-  __syncthreads();
-  for (int r = tid * 4; r < p.rows; r += SM_THREADS * 4) sm_rows(p, s_cu, r);
-  for (int b = tid; b < p.batch; b += SM_THREADS) sm_update(p, b);
-  if (tid == 0) sm_finish(p);
+  for (int r = tid * 4; r < p.rows; r += SM_THREADS * 4) sm_rows(p, s_cu, s_seq, s_held, s_head[1], r);
+  if (tid < p.batch) sm_update(p, tid, s_seq[tid], s_held[tid]);
+  if (tid == 0) sm_finish(p, s_head);
 }
 
 // First launch of a large step: workgroup 0 forms the prefix sums, the
-// others the tokens held, one wave per request.
+// others the tokens held, four requests per wave.
 __global__ __launch_bounds__(SM_THREADS) void slot_plan_kernel(SlotMapParams p) {
-  __shared__ int64_t sh[SM_WAVES + 1];
+  __shared__ Sm2 sh[SM_WAVES];
   __shared__ int s_err;
   if (blockIdx.x == 0) {
-    sm_plan(p, sh, &s_err);
+    sm_plan(p, sh, &s_err, p.seq, p.head, nullptr);
     return;
   }
-  const int b = (int(blockIdx.x) - 1) * SM_WAVES + (int(threadIdx.x) >> 6);
-  if (b >= p.batch) return;
-  const int held = tokens_held(p, b);
-  if ((threadIdx.x & 63) == 0) p.held[b] = held;
+  tokens_held(p, ((int(blockIdx.x) - 1) * SM_WAVES + (int(threadIdx.x) >> 6)) * 4, p.held);
 }
 
 // Second launch: the packed rows, and the requests' own words.
@@ -278,9 +291,10 @@ __global__ __launch_bounds__(SM_FILL) void slot_fill_kernel(SlotMapParams p) {
   for (int b = tid; b <= p.batch; b += SM_FILL) s_cu[b] = p.cu[b];
   __syncthreads();
   const int64_t r = int64_t(blockIdx.x) * SM_ROWS + tid * 4;
-  if (r < p.rows) sm_rows(p, s_cu, int(r));
-  for (int b = int(blockIdx.x) * SM_FILL + tid; b < p.batch; b += int(gridDim.x) * SM_FILL) sm_update(p, b);
-  if (blockIdx.x == 0 && tid == 0) sm_finish(p);
+  if (r < p.rows) sm_rows(p, s_cu, p.seq, p.held, p.head[1], int(r));
+  for (int b = int(blockIdx.x) * SM_FILL + tid; b < p.batch; b += int(gridDim.x) * SM_FILL)
+    sm_update(p, b, p.seq[b], p.held[b]);
+  if (blockIdx.x == 0 && tid == 0) sm_finish(p, p.head);
 }
 
 // ---------------------------------------------------------------------------
@@ -406,7 +420,7 @@ extern "C" int32_t tierkv_build_slot_map(
   if (num_rows <= 4 * SM_THREADS && batch <= SM_THREADS) {
     hipLaunchKernelGGL(slot_map_kernel, dim3(1), dim3(SM_THREADS), 0, stream, p);
   } else {
-    hipLaunchKernelGGL(slot_plan_kernel, dim3(1 + (batch + SM_WAVES - 1) / SM_WAVES), dim3(SM_THREADS), 0, stream, p);
+    hipLaunchKernelGGL(slot_plan_kernel, dim3(1 + (batch + SM_WAVES * 4 - 1) / (SM_WAVES * 4)), dim3(SM_THREADS), 0, stream, p);
     const int wgs = int((int64_t(num_rows) + SM_ROWS - 1) / SM_ROWS);
     hipLaunchKernelGGL(slot_fill_kernel, dim3(wgs > 0 ? wgs : 1), dim3(SM_FILL), 0, stream, p);
   }

@@ -236,7 +236,7 @@ _scratch_ws: dict = {}
 
 def _scratch(name: str, device, need: int, zeros: int = 0) -> torch.Tensor:
     """At least ``need`` bytes whose first ``zeros`` are zero when new."""
-    capturing = torch.cuda.is_current_stream_capturing()
+    capturing = torch.cuda.is_current_stream_capturing()   # (a capture is the current device's)
     key = (name, device.index, _lib.stream_of(device))
     ws = None if capturing else _scratch_ws.get(key)
     if ws is None or ws.numel() < need:
@@ -246,6 +246,14 @@ def _scratch(name: str, device, need: int, zeros: int = 0) -> torch.Tensor:
         if not capturing:
             _scratch_ws[key] = ws
     return ws
+
+
+def _on_device(device, call, *args) -> int:
+    """``call(*args, stream)`` with ``device`` current and its current stream."""
+    if torch.cuda.current_device() == device.index:
+        return call(*args, _lib.stream_of(device))
+    with torch.cuda.device(device):
+        return call(*args, _lib.stream_of(device))
 
 
 class SlotMap(NamedTuple):
@@ -261,7 +269,7 @@ def _require_i32(t, name: str, shape=None) -> None:
     _lib.require_gpu_tensor(t, name)
     if t.dtype != torch.int32 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor.")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}.")
 
 
@@ -281,32 +289,33 @@ def build_slot_map(new_tokens: torch.Tensor, block_table: torch.Tensor, block_st
     _lib.require_gpu_tensor(block_table, "block_table")
     if block_table.ndim != 2:
         raise ValueError("block_table must be [batch, max_blocks].")
-    batch, stride = (int(x) for x in block_table.shape)
-    for name, t in (("block_table", block_table), ("block_states", block_states), ("block_lengths", block_lengths)):
-        _require_i32(t, name, (batch, stride))
-    for name, t in (("new_tokens", new_tokens), ("seq_num_blocks", seq_num_blocks), ("open_blocks", open_blocks)):
-        _require_i32(t, name, (batch,))
-    _require_i32(hot_free, "hot_free")
-    _require_i32(ctl, "ctl", (4,))
+    shape = block_table.shape
+    batch, stride = shape
+    index = block_table.get_device()
+    for name, t, want in (("block_table", block_table, shape), ("block_states", block_states, shape),
+                          ("block_lengths", block_lengths, shape), ("new_tokens", new_tokens, shape[:1]),
+                          ("seq_num_blocks", seq_num_blocks, shape[:1]), ("open_blocks", open_blocks, shape[:1]),
+                          ("hot_free", hot_free, None), ("ctl", ctl, (4,))):
+        _require_i32(t, name, want)
+        if t.get_device() != index:
+            raise ValueError("the slot map's tensors must be on one device.")
     device = block_table.device
-    tensors = (new_tokens, block_states, block_lengths, seq_num_blocks, open_blocks, hot_free, ctl)
-    if any(t.device != device for t in tensors):
-        raise ValueError("the slot map's tensors must be on one device.")
     rows = int(num_tokens)
     if rows < 0:
         raise ValueError("num_tokens must not be negative.")
-    new = lambda n: torch.empty(n, dtype=torch.int32, device=device)
-    out = SlotMap(new(rows), new(rows), new(batch + 1), new(batch))
-    need = int(lib.tierkv_slot_map_workspace_bytes(batch))
-    with torch.cuda.device(device):
-        ws = _scratch("slot_map", device, need)
-        rc = lib.tierkv_build_slot_map(
-            _lib.ptr(new_tokens), batch, rows, _lib.ptr(block_table), _lib.ptr(block_states), _lib.ptr(block_lengths),
-            stride, _lib.ptr(seq_num_blocks), _lib.ptr(open_blocks), _lib.ptr(hot_free), int(hot_free.numel()),
-            _lib.ptr(ctl), int(block_size), _lib.ptr(out.slots), _lib.ptr(out.positions), _lib.ptr(out.cu_tokens),
-            _lib.ptr(out.context), _lib.ptr(ws), int(ws.numel()), _lib.stream_of(device))
+    # One allocation: slots and positions start at multiples of 16 bytes.
+    pad = -rows % 4
+    slots, _, positions, _, cu, context = torch.empty(2 * (rows + pad) + 2 * batch + 1, dtype=torch.int32,
+                                                      device=device).split([rows, pad, rows, pad, batch + 1, batch])
+    need = lib.tierkv_slot_map_workspace_bytes(batch)
+    ws = _scratch("slot_map", device, need)
+    ptr = _lib.ptr
+    rc = _on_device(device, lib.tierkv_build_slot_map, ptr(new_tokens), batch, rows, ptr(block_table),
+                    ptr(block_states), ptr(block_lengths), stride, ptr(seq_num_blocks), ptr(open_blocks), ptr(hot_free),
+                    hot_free.numel(), ptr(ctl), int(block_size), ptr(slots), ptr(positions), ptr(cu), ptr(context),
+                    ptr(ws), ws.numel())
     _lib.check(rc, "tierkv_build_slot_map")
-    return out
+    return SlotMap(slots, positions, cu, context)
 
 
 def write_slots(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, hot_k: torch.Tensor,
@@ -328,18 +337,19 @@ def write_slots(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, hot
         raise ValueError("key and value must be [tokens, kv_heads, head_dim] of the pools' geometry.")
     rows = int(key.shape[0])
     _require_i32(slots, "slots", (rows,))
-    device = hot_k.device
-    if any(t.device != device for t in (key, value, slots, hot_v)):
+    index = hot_k.get_device()
+    if any(t.get_device() != index for t in (key, value, slots, hot_v)):
         raise ValueError("rows, slots and pools must be on one device.")
     if rows == 0:
         return
-    k = key if key.stride(-1) == 1 or dim == 1 else key.contiguous()
-    v = value if value.stride(-1) == 1 or dim == 1 else value.contiguous()
-    with torch.cuda.device(device):
-        rc = lib.tierkv_write_slots(
-            _lib.ptr(k), k.stride(0), k.stride(1), _lib.ptr(v), v.stride(0), v.stride(1),
-            _lib.DTYPE_BF16 if k.dtype == torch.bfloat16 else _lib.DTYPE_F16, _lib.ptr(slots), rows,
-            _lib.ptr(hot_k), _lib.ptr(hot_v), int(hot_k.shape[0]), kv_heads, bs, dim, _lib.stream_of(device))
+    k = key if key.stride(2) == 1 or dim == 1 else key.contiguous()
+    v = value if value.stride(2) == 1 or dim == 1 else value.contiguous()
+    kt, kh, _ = k.stride()
+    vt, vh, _ = v.stride()
+    ptr = _lib.ptr
+    rc = _on_device(hot_k.device, lib.tierkv_write_slots, ptr(k), kt, kh, ptr(v), vt, vh,
+                    _lib.DTYPE_BF16 if k.dtype == torch.bfloat16 else _lib.DTYPE_F16, ptr(slots), rows, ptr(hot_k),
+                    ptr(hot_v), hot_k.shape[0], kv_heads, bs, dim)
     _lib.check(rc, "tierkv_write_slots")
 
 
@@ -385,13 +395,11 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     u = uniforms.contiguous()
     tokens = torch.empty(batch, dtype=torch.int64, device=device)
     probs = torch.empty(batch, dtype=torch.float32, device=device)
-    need = int(lib.tierkv_sample_workspace_bytes(batch, vocab))
-    with torch.cuda.device(device):
-        ws = _scratch("sample", device, need, _lib.SAMPLE_COUNTER_BYTES)
-        rc = lib.tierkv_sample_tokens(
-            _lib.ptr(x), _LOGIT_DTYPES[x.dtype], x.stride(0), batch, vocab, _lib.ptr(u),
-            _lib.ptr(t), float(t_all), _lib.ptr(k), min(max(int(k_all), 0), 0x7fffffff), _lib.ptr(p), float(p_all),
-            _lib.ptr(m), float(m_all), _lib.ptr(tokens), _lib.ptr(probs), _lib.ptr(ws), int(ws.numel()),
-            _lib.stream_of(device))
+    need = lib.tierkv_sample_workspace_bytes(batch, vocab)
+    ws = _scratch("sample", device, need, _lib.SAMPLE_COUNTER_BYTES)
+    ptr = _lib.ptr
+    rc = _on_device(device, lib.tierkv_sample_tokens, ptr(x), _LOGIT_DTYPES[x.dtype], x.stride(0), batch, vocab, ptr(u),
+                    ptr(t), float(t_all), ptr(k), min(max(int(k_all), 0), 0x7fffffff), ptr(p), float(p_all), ptr(m),
+                    float(m_all), ptr(tokens), ptr(probs), ptr(ws), ws.numel())
     _lib.check(rc, "tierkv_sample_tokens")
     return tokens, probs

@@ -622,7 +622,8 @@ def tierkv_extend_attention(
         _lib.require_gpu_tensor(t, "warm metadata")
         if not t.is_contiguous() or t.numel() != entries or t.dtype != k_scale.dtype:
             raise ValueError("warm scale/zero tensors must be contiguous with one entry per WARM slot.")
-    if any(t.device != device for t in pools + metas + (block_table, block_states, block_lengths, cu_tokens)):
+    index = query_states.get_device()
+    if any(t.get_device() != index for t in pools + metas + (block_table, block_states, block_lengths, cu_tokens)):
         raise ValueError("queries, tables and pools must be on one device.")
     q = query_states
     if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
@@ -634,17 +635,21 @@ def tierkv_extend_attention(
         raise ValueError("out must be a contiguous tensor of the query's shape, dtype and device.")
     snb = None
     if seq_num_blocks is not None:
-        snb = torch.as_tensor(seq_num_blocks, dtype=torch.int32, device=device).contiguous()
+        snb = seq_num_blocks
+        if not (isinstance(snb, torch.Tensor) and snb.dtype == torch.int32 and snb.get_device() == index):
+            snb = torch.as_tensor(seq_num_blocks, dtype=torch.int32, device=device)
+        snb = snb.contiguous()
         if snb.numel() != batch:
             raise ValueError("seq_num_blocks needs one entry per sequence.")
     bound = rows if max_tokens is None else min(int(max_tokens), rows)
     if bound < 0:
         raise ValueError("max_tokens must not be negative.")
-    need = int(lib.tierkv_extend_workspace_bytes(batch, rows, bound, num_heads, kv_heads, int(num_blocks), block_size,
-                                                 head_dim))
+    need = lib.tierkv_extend_workspace_bytes(batch, rows, bound, num_heads, kv_heads, int(num_blocks), block_size,
+                                             head_dim)
     if need < 0:
         raise ValueError("invalid attention geometry.")
-    with torch.cuda.device(device):
+
+    def launch():
         if workspace is None:
             ws = stream_workspace(device)
         else:
@@ -653,17 +658,22 @@ def tierkv_extend_attention(
         if ws.device != device:
             raise ValueError("the decode workspace lives on another device.")
         ws.reserve(need)
+        ptr = _lib.ptr
+        ref = fmt == _lib.WARM_REF_U8
         rc = lib.tierkv_extend_attention(
-            _lib.ptr(q), q.stride(0), q.stride(1), _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F16,
-            _lib.ptr(out), _lib.ptr(cu_tokens), rows, bound,
-            _lib.ptr(block_table), _lib.ptr(block_states), _lib.ptr(block_lengths), int(block_table.shape[-1]),
-            _lib.ptr(snb), int(num_blocks),
-            _lib.ptr(hot_k_pool), _lib.ptr(hot_v_pool), int(hot_k_pool.shape[0]),
-            _lib.ptr(warm_k_pool), _lib.ptr(warm_v_pool), slots,
-            _lib.ptr(k_scale), _lib.ptr(k_zero) if fmt == _lib.WARM_REF_U8 else None,
-            _lib.ptr(v_scale), _lib.ptr(v_zero) if fmt == _lib.WARM_REF_U8 else None,
-            fmt, _COLD_MODES[cold_mode], batch, num_heads, kv_heads, block_size, head_dim, float(scaling),
-            ws.data_ptr(), ws.nbytes, _lib.stream_of(device))
+            ptr(q), q.stride(0), q.stride(1), _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F16,
+            ptr(out), ptr(cu_tokens), rows, bound, ptr(block_table), ptr(block_states), ptr(block_lengths),
+            block_table.shape[-1], ptr(snb), int(num_blocks), ptr(hot_k_pool), ptr(hot_v_pool), hot_k_pool.shape[0],
+            ptr(warm_k_pool), ptr(warm_v_pool), slots, ptr(k_scale), ptr(k_zero) if ref else None, ptr(v_scale),
+            ptr(v_zero) if ref else None, fmt, _COLD_MODES[cold_mode], batch, num_heads, kv_heads, block_size, head_dim,
+            float(scaling), ws.data_ptr(), ws.nbytes, _lib.stream_of(device))
+        return rc, ws
+
+    if torch.cuda.current_device() == index:
+        rc, ws = launch()
+    else:
+        with torch.cuda.device(device):
+            rc, ws = launch()
     _lib.check(rc, "tierkv_extend_attention")
     if _lib.env_flag("TIERKV_CHECK_ERRORS"):
         word = ws.error_word()
