@@ -27,6 +27,23 @@ constexpr int SM_THREADS = 1024;
 constexpr int SM_WAVES = SM_THREADS / 64;
 constexpr int SM_MAX_BATCH = 4096;              // as tierkv_runtime_append
 constexpr int SM_NIT = SM_MAX_BATCH / SM_THREADS;
+// One workgroup holds a step of at most SM_ONE_BATCH requests (four per wave,
+// all lengths read at once), SM_ONE_ROWS packed rows (four per thread) and
+// tables of SM_ONE_BLOCKS blocks.  Measured with one workgroup against two
+// launches, replayed from a graph behind a 2 us copy of the tables (us):
+//   requests x new tokens x blocks   one    two
+//    1 x   1 x   16                  9.1   10.9
+//    1 x   1 x 1024                 11.4   10.4
+//   64 x  16 x   16                 11.5   12.7
+//   64 x  16 x  256                 14.7   13.2
+//   64 x  16 x 1024                 17.0   13.9
+//   64 x 700 x   16                 27.6   12.9
+//  256 x   1 x   64                 18.1   14.0
+// Outside a graph the second launch costs the host another 2 to 3 us, so the
+// limit on blocks is where one workgroup is behind by less than that.
+constexpr int SM_ONE_BATCH = 64;
+constexpr int SM_ONE_ROWS = 4 * SM_THREADS;
+constexpr int SM_ONE_BLOCKS = 256;
 constexpr int SM_FILL = 256;                    // threads of a fill workgroup
 constexpr int SM_ROWS = SM_FILL * 4;            // packed rows per fill workgroup
 
@@ -116,17 +133,18 @@ __device__ __forceinline__ void tokens_held(const SlotMapParams& p, int b0, int3
 
 // The prefix sums (one workgroup of SM_THREADS): writes cu, the requests'
 // plan entries (seq) and the head; cu also to where the caller keeps it.
+template <int NIT>
 __device__ __forceinline__ void sm_plan(const SlotMapParams& p, Sm2* sh, int* s_err, int4* seq, int32_t* head,
                                         int32_t* cu) {
   const int tid = threadIdx.x, B = p.batch, bs = p.bs;
-  const int nit = (B + SM_THREADS - 1) / SM_THREADS;
-  int n[SM_NIT], room[SM_NIT], nb[SM_NIT];
-  int64_t need[SM_NIT], cu_end[SM_NIT], first[SM_NIT];
+  const int nit = (B + SM_THREADS - 1) / SM_THREADS;   // at most NIT
+  int n[NIT], room[NIT], nb[NIT];
+  int64_t need[NIT], cu_end[NIT], first[NIT];
   const int top = min(max(p.ctl[0], 0), p.hot_slots);
   if (tid == 0) *s_err = 0;
   __syncthreads();
 #pragma unroll
-  for (int it = 0; it < SM_NIT; ++it) {
+  for (int it = 0; it < NIT; ++it) {
     n[it] = room[it] = nb[it] = 0;
     need[it] = 0;
     const int b = it * SM_THREADS + tid;
@@ -151,7 +169,7 @@ __device__ __forceinline__ void sm_plan(const SlotMapParams& p, Sm2* sh, int* s_
   }
   int64_t tokens = 0, blocks = 0;
 #pragma unroll
-  for (int it = 0; it < SM_NIT; ++it) {
+  for (int it = 0; it < NIT; ++it) {
     if (it < nit) {
       Sm2 total;
       const Sm2 x = sm_scan({n[it], need[it]}, sh, &total);
@@ -168,7 +186,7 @@ __device__ __forceinline__ void sm_plan(const SlotMapParams& p, Sm2* sh, int* s_
   __syncthreads();
   const bool ok = *s_err == 0;
 #pragma unroll
-  for (int it = 0; it < SM_NIT; ++it) {
+  for (int it = 0; it < NIT; ++it) {
     const int b = it * SM_THREADS + tid;
     if (it < nit && b < B) {
       p.cu[b + 1] = ok ? int32_t(cu_end[it]) : 0;
@@ -260,14 +278,15 @@ __global__ __launch_bounds__(SM_THREADS) void slot_map_kernel(SlotMapParams p) {
   __shared__ Sm2 sh[SM_WAVES];
   __shared__ int s_err;
   __shared__ int32_t s_head[4];
-  __shared__ int32_t s_cu[SM_THREADS + 1];
-  __shared__ int32_t s_held[SM_THREADS];
-  __shared__ int4 s_seq[SM_THREADS];
+  __shared__ int32_t s_cu[SM_ONE_BATCH + 1];
+  __shared__ int32_t s_held[SM_ONE_BATCH];
+  __shared__ int4 s_seq[SM_ONE_BATCH];
+  static_assert(SM_ONE_BATCH == SM_WAVES * 4 && SM_ONE_ROWS == SM_THREADS * 4, "one pass each");
   const int tid = threadIdx.x;
-  for (int b = (tid >> 6) * 4; b < p.batch; b += SM_WAVES * 4) tokens_held(p, b, s_held);
-  sm_plan(p, sh, &s_err, s_seq, s_head, s_cu);
+  tokens_held(p, (tid >> 6) * 4, s_held);
+  sm_plan<1>(p, sh, &s_err, s_seq, s_head, s_cu);
   __syncthreads();
-  for (int r = tid * 4; r < p.rows; r += SM_THREADS * 4) sm_rows(p, s_cu, s_seq, s_held, s_head[1], r);
+  if (tid * 4 < p.rows) sm_rows(p, s_cu, s_seq, s_held, s_head[1], tid * 4);
   if (tid < p.batch) sm_update(p, tid, s_seq[tid], s_held[tid]);
   if (tid == 0) sm_finish(p, s_head);
 }
@@ -278,7 +297,7 @@ __global__ __launch_bounds__(SM_THREADS) void slot_plan_kernel(SlotMapParams p) 
   __shared__ Sm2 sh[SM_WAVES];
   __shared__ int s_err;
   if (blockIdx.x == 0) {
-    sm_plan(p, sh, &s_err, p.seq, p.head, nullptr);
+    sm_plan<SM_NIT>(p, sh, &s_err, p.seq, p.head, nullptr);
     return;
   }
   tokens_held(p, ((int(blockIdx.x) - 1) * SM_WAVES + (int(threadIdx.x) >> 6)) * 4, p.held);
@@ -417,7 +436,7 @@ extern "C" int32_t tierkv_build_slot_map(
   p.seq = reinterpret_cast<int4*>(ws + 256);
   p.held = reinterpret_cast<int32_t*>(ws + 256 + int64_t(batch) * 16);
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  if (num_rows <= 4 * SM_THREADS && batch <= SM_THREADS) {
+  if (batch <= SM_ONE_BATCH && num_rows <= SM_ONE_ROWS && table_stride <= SM_ONE_BLOCKS) {
     hipLaunchKernelGGL(slot_map_kernel, dim3(1), dim3(SM_THREADS), 0, stream, p);
   } else {
     hipLaunchKernelGGL(slot_plan_kernel, dim3(1 + (batch + SM_WAVES * 4 - 1) / (SM_WAVES * 4)), dim3(SM_THREADS), 0, stream, p);
