@@ -14,9 +14,9 @@
 //   * extend_plan_kernel, a workgroup per request, lists the resident
 //     16-token sub-tiles of its row (slot, state, first ordinal, valid
 //     tokens); the last workgroup to finish turns the requests' query rows
-//     into tiles and cuts the tiles' key ranges into items of about equal
-//     work, about as many as the chip runs at once;
-//   * extend_kernel, a workgroup of four waves per (item, kv head);
+//     into tiles and cuts the tiles' key ranges into items where that
+//     shortens the whole;
+//   * extend_kernel, a workgroup of eight waves per (item, kv head);
 //   * extend_merge_kernel joins the items of tiles that were cut.
 //
 // Rows of a tile are (token, head of the GQA group) pairs of one kv head, so
@@ -29,8 +29,10 @@
 //                   step is key 8a + 4h + j; V^T's rows are stored in that order)
 // so probabilities never leave their registers, and a row's running maximum
 // and sum live in the two lanes that own it.  Tiles of more than 32 rows
-// ("wide") are 128 rows over four waves that share 64 keys at a time; smaller
-// ones ("narrow") give each wave its own 32 keys of the same rows, merged in LDS.
+// ("wide") are 256 rows over eight waves that share 64 keys at a time, four
+// waves half a tile ahead of the others so that one half's products run beside
+// the other's exponentials; smaller ones ("narrow") give each wave its own 32
+// keys of the same rows, merged in LDS.
 //
 // K goes to LDS as fp16 of the codes themselves (exact: |code| <= 127, or
 // code - zero, an integer below 2048 for any row whose values are not far
@@ -58,8 +60,11 @@ constexpr int EX_MAX_BATCH = 4096;        // requests per call
 constexpr int EX_SUB = 16;                // tokens per sub-tile
 constexpr int EX_NARROW = 32;             // rows of a narrow tile
 constexpr int EX_WIDE = 32 * EX_WAVES;   // rows of a wide tile
-constexpr int EX_TARGET = 512;            // workgroups that the cut aims at
+constexpr int EX_SLOTS = 256;             // workgroups that run at once: one per CU
+constexpr int EX_TARGET = 512;            // workgroups that a cut adds, at most
 constexpr int EX_MIN_SUBS = 16;           // sub-tiles per item, at least, when a tile is cut
+constexpr float EX_ITEM_COST = 8.f;       // an item's start and end, in sub-tiles' time
+constexpr float EX_PART_COST = 12.f;      // a partial's write and read, in sub-tiles' time
 constexpr int EX_WS_HEAD = 256 + (1 << 16) * 4;   // the decode launches' error word and counters
 constexpr float EX_LAZY = 8.f;            // log2 headroom of the running maximum
 constexpr float EX_BOOST = 6.f;           // log2 of the probabilities' factor
@@ -159,6 +164,22 @@ __device__ __forceinline__ int ex_work(int subs, int rows, int tile, bool wide, 
 
 // Items of one tile: its work in parts of at most per_item sub-tiles.
 __device__ __forceinline__ int ex_parts(int work, int per_item) { return min((work + per_item - 1) / per_item, 32767); }
+
+// Tile f of all: its request (the last one whose first tile is at most f, and
+// that has tiles) and its place there, the longest first.
+struct ExTileId {
+  int request, tile;
+  bool wide;
+};
+__device__ __forceinline__ ExTileId ex_tile_id(const ExtendParams& p, int f, const int2* first, const int* rows) {
+  int lo = 0, hi = p.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid].x <= f) lo = mid;
+    else hi = mid;
+  }
+  return {lo, ex_tiles(rows[lo]) - 1 - (f - first[lo].x), rows[lo] > EX_NARROW};
+}
 
 __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
   __shared__ Ex3 sh[EX_PLAN / 64];
@@ -266,8 +287,61 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
   work = 0.f;
   for (int i = 0; i < EX_PLAN / 64; ++i) work += s_work[i];
   work = work * 1.001f + 1.f;   // the rounding of these sums
-  const int target = max(EX_TARGET / p.kv_heads, 1);
-  const int per_item = max(EX_MIN_SUBS, (int(ceilf(work / float(target))) + 15) & ~15);
+  // Sub-tiles per item: each wave rates one choice.  P = longest / (w + 1) for
+  // the first eight waves, a few sizes around an even share for the others;
+  // with the items' count and the longest of them the time is the rounds over
+  // the slots, or the even share and a quarter of an item where the items are
+  // of mixed lengths and fill each other's gaps, and the cost of the partials.
+  // Measured with the whole call: 2048 tokens on 32768, 32 tiles on as many
+  // slots, are left whole, 973 us against 1221 cut in two (the tiles of a head
+  // then also walk the same keys at the same time, in one L2); a single token
+  // on 100000 in 32 parts 85 us, in 64 99; a cost of 24 per partial leaves 512
+  // tokens beside 15 single ones whole, 98 us against 78 cut in four.
+  __shared__ float s_time[EX_PLAN / 64];
+  __shared__ int s_per[EX_PLAN / 64];
+  const float slots = fmaxf(float(EX_SLOTS / p.kv_heads), 1.f);
+  const int least = max(EX_MIN_SUBS, int(ceilf(work / fmaxf(float(EX_TARGET / p.kv_heads), 1.f))));
+  {
+    const int w = tid >> 6, lane = tid & 63;
+    auto tile_work = [&](int f) {
+      const ExTileId x = ex_tile_id(p, f, s_tile, s_rows);
+      return ex_work(s_tile[x.request].y, s_rows[x.request], x.tile, x.wide, G);
+    };
+    float longest = 0.f;
+    for (int i = lane; i < p.batch; i += 64)
+      if (s_rows[i] > 0) longest = fmaxf(longest, float(s_tile[i].y));
+    longest = wave_max(longest);
+    const float share = work / slots;
+    const float f = w == 8 ? 0.34f : w == 9 ? 0.51f : w == 10 ? 0.68f : w == 11 ? 0.8f : w == 12 ? 1.02f
+                  : w == 13 ? 1.25f : w == 14 ? 1.5f : 2.f;
+    const int per = max(least, int(ceilf(w < 8 ? longest / float(w + 1) : share * f)));
+    float items = 0.f, partials = 0.f, len = 0.f;
+    for (int i = lane; i < tiles_all; i += 64) {
+      const int v = tile_work(i), k = ex_parts(v, per);
+      items += float(k);
+      if (k > 1) partials += float(k);
+      len = fmaxf(len, float(v) / float(k));
+    }
+    items = wave_sum(items);
+    partials = wave_sum(partials);
+    len = wave_max(len) + EX_ITEM_COST;
+    const float even = (work + EX_ITEM_COST * items) / slots;
+    const float time = fmaxf(len, fminf(ceilf(items / slots) * len, even + 0.25f * len)) + EX_PART_COST * partials / slots;
+    if (lane == 0) {
+      s_time[w] = time;
+      s_per[w] = per;
+    }
+  }
+  __syncthreads();
+  int per_item = s_per[0];
+  {
+    float best = s_time[0];
+    for (int i = 1; i < EX_PLAN / 64; ++i)
+      if (s_time[i] < best) {
+        best = s_time[i];
+        per_item = s_per[i];
+      }
+  }
   // Items, tile by tile; each request's longest tiles first.
   int items = 0, cuts = 0, partials = 0;
   for (int f0 = 0; f0 < tiles_all; f0 += EX_PLAN) {
@@ -275,17 +349,11 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
     int i = 0, t = 0, parts = 0;
     bool wide = false;
     if (f < tiles_all) {
-      int lo = 0, hi = p.batch;           // the last request whose first tile is at most f and that has tiles
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_tile[mid].x <= f) lo = mid;
-        else hi = mid;
-      }
-      i = lo;
-      const int rows = s_rows[i], tiles = ex_tiles(rows);
-      wide = rows > EX_NARROW;
-      t = tiles - 1 - (f - s_tile[i].x);
-      parts = ex_parts(ex_work(s_tile[i].y, rows, t, wide, G), per_item);
+      const ExTileId x = ex_tile_id(p, f, s_tile, s_rows);
+      i = x.request;
+      t = x.tile;
+      wide = x.wide;
+      parts = ex_parts(ex_work(s_tile[i].y, s_rows[i], t, wide, G), per_item);
     }
     const int cut = parts > 1 ? 1 : 0;
     const Ex3 s = ex_scan3({parts, cut, cut ? parts : 0}, sh, &total);
@@ -1151,7 +1219,7 @@ __global__ __launch_bounds__(EX_THREADS, 2) void extend_kernel(ExtendParams p) {
 }
 
 // Join of a cut tile's partials, in part order: a workgroup per (cut tile, kv
-// head, 1024 / D of its rows), four dims of one row per thread.
+// head, 4 EX_THREADS / D of its rows), four dims of one row per thread.
 template <typename QT>
 __global__ __launch_bounds__(EX_THREADS) void extend_merge_kernel(ExtendParams p, int32_t rows_per_wg) {
   const int c = int(blockIdx.x) / p.kv_heads, h = int(blockIdx.x) - c * p.kv_heads;

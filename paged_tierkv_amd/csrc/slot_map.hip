@@ -32,18 +32,17 @@ constexpr int SM_NIT = SM_MAX_BATCH / SM_THREADS;
 // tables of SM_ONE_BLOCKS blocks.  Measured with one workgroup against two
 // launches, replayed from a graph behind a 2 us copy of the tables (us):
 //   requests x new tokens x blocks   one    two
-//    1 x   1 x   16                  9.1   10.9
-//    1 x   1 x 1024                 11.4   10.4
-//   64 x  16 x   16                 11.5   12.7
-//   64 x  16 x  256                 14.7   13.2
-//   64 x  16 x 1024                 17.0   13.9
-//   64 x 700 x   16                 27.6   12.9
-//  256 x   1 x   64                 18.1   14.0
-// Outside a graph the second launch costs the host another 2 to 3 us, so the
-// limit on blocks is where one workgroup is behind by less than that.
+//    1 x  1 x   16                   6.9   10.9
+//    8 x 16 x  256                  10.1   11.8
+//   64 x  1 x   16                   9.5   12.4
+//   64 x 60 x  256                  12.4   13.0
+//   64 x 16 x 1024                  14.1   14.4
+// and with a workgroup that took several passes beyond these limits:
+//   64 x 700 x 16                   27.6   12.9
+//  256 x   1 x 64                   18.1   14.0
 constexpr int SM_ONE_BATCH = 64;
 constexpr int SM_ONE_ROWS = 4 * SM_THREADS;
-constexpr int SM_ONE_BLOCKS = 256;
+constexpr int SM_ONE_BLOCKS = 1024;
 constexpr int SM_FILL = 256;                    // threads of a fill workgroup
 constexpr int SM_ROWS = SM_FILL * 4;            // packed rows per fill workgroup
 
