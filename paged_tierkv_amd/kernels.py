@@ -353,6 +353,7 @@ def write_slots(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, hot
     _lib.check(rc, "tierkv_write_slots")
 
 
+SAMPLE_MAX_VOCAB = 1 << 20   # tierkv_sample_tokens
 _LOGIT_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
 
 
@@ -361,6 +362,8 @@ def _limit(x, name: str, batch: int, device, dtype, low=None, high=None):
     if isinstance(x, torch.Tensor):
         if x.device != device or tuple(x.shape) != (batch,):
             raise ValueError(f"{name} must be a number or one value per row on the logits' device.")
+        if dtype == torch.int32 and x.dtype != dtype:
+            x = x.clamp(0, SAMPLE_MAX_VOCAB)   # (past 32 bits too)
         return x.to(dtype).contiguous(), 0
     if x != x or (low is not None and x < low) or (high is not None and x > high):
         raise ValueError(f"{name} is out of range.")
@@ -399,7 +402,7 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     ws = _scratch("sample", device, need, _lib.SAMPLE_COUNTER_BYTES)
     ptr = _lib.ptr
     rc = _on_device(device, lib.tierkv_sample_tokens, ptr(x), _LOGIT_DTYPES[x.dtype], x.stride(0), batch, vocab, ptr(u),
-                    ptr(t), float(t_all), ptr(k), min(max(int(k_all), 0), 0x7fffffff), ptr(p), float(p_all), ptr(m),
+                    ptr(t), float(t_all), ptr(k), int(min(max(k_all, 0), SAMPLE_MAX_VOCAB)), ptr(p), float(p_all), ptr(m),
                     float(m_all), ptr(tokens), ptr(probs), ptr(ws), ws.numel())
     _lib.check(rc, "tierkv_sample_tokens")
     return tokens, probs

@@ -627,7 +627,7 @@ def tierkv_extend_attention(
         raise ValueError("queries, tables and pools must be on one device.")
     q = query_states
     if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)   # (.contiguous() keeps a misaligned start)
     if out is None:
         out = torch.empty((rows, num_heads, head_dim), device=device, dtype=q.dtype)
     elif (out.dtype != q.dtype or tuple(out.shape) != (rows, num_heads, head_dim) or not out.is_contiguous()

@@ -521,3 +521,64 @@ def test_steps_on_two_streams_do_not_mix(device):
     for i in (0, 1):
         for out, tok in res[i]:
             assert torch.equal(out, base[i]) and torch.equal(tok, base[2])
+
+
+def test_a_query_that_starts_off_a_16_byte_boundary(device):
+    s = step(31, [3, 12], [40, 25], 8, 2, 64)
+    q = s["q"].to(device)
+    flat = torch.zeros(q.numel() + 3, dtype=q.dtype, device=device)
+    flat[3:] = q.flatten()
+    assert torch.equal(call(s, device, "masked", q=flat[3:].view(q.shape)), call(s, device, "masked"))
+
+
+@pytest.mark.parametrize("new,held,heads,kv,d", [
+    ([i % 4 for i in range(1500)], [5 + i % 37 for i in range(1500)], 4, 1, 32),      # more requests than plan threads
+    ([100, 1, 70, 0, 2], [2000, 3000, 70, 50, 1], 16, 1, 64),                         # some tiles cut, others whole
+    ([70] * 40, [70 + 10 * i for i in range(40)], 16, 8, 64),                         # more tiles than run at once
+])
+def test_cuts_of_many_tiles(device, new, held, heads, kv, d):
+    s = step(32, new, held, heads, kv, d)
+    out = call(s, device, "masked")
+    rng = np.random.default_rng(32)
+    check(out, s, "masked", np.sort(rng.choice(s["cu"][-1], min(400, int(s["cu"][-1])), replace=False)))
+    assert torch.equal(out[:s["cu"][-1]], call(s, device, "masked")[:s["cu"][-1]])
+
+
+def test_limits_of_each_row_past_32_bits(device):
+    x = logits(np.random.default_rng(5), 3, 700, torch.float32, "plain").to(device)
+    u = torch.tensor([0.9, 0.5, 0.99], device=device)
+    k = torch.tensor([2 ** 32 + 1, -2 ** 40, 2 ** 31], dtype=torch.int64, device=device)   # all off
+    got = kernels.sample_tokens(x, u, top_k=k)
+    assert all(torch.equal(a, b) for a, b in zip(got, kernels.sample_tokens(x, u)))
+    assert torch.equal(kernels.sample_tokens(x, u, top_k=2 ** 40)[0], got[0])
+
+
+def test_one_graph_follows_the_requests_rows(device):
+    """A captured call replayed with other numbers of new tokens, so other tiles and cuts, beside eager work."""
+    s = step(33, [20, 20], [600, 90], 8, 2, 64)
+    ks, kz, vs, vz = (gpu(a, device) for a in s["meta"])
+    pools = [gpu(a, device) for a in (*s["hot"], *s["warm"])]
+    tables = [gpu(s[n], device) for n in ("table", "states", "lengths", "nblocks")]
+    q, cu = s["q"].to(device), gpu(s["cu"], device)
+    out = torch.empty_like(q)
+    ws = extend_workspace(device, 2, 40, 8, 2, s["table"].shape[1], 64)
+    run = lambda: tierkv_extend_attention(q, cu, *tables[:3], *pools, ks, kz, vs, vz, s["table"].shape[1], 4, s["scaling"],
+                                          cold_mode="masked", seq_num_blocks=tables[3], workspace=ws, out=out)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run()
+    torch.cuda.synchronize()
+    for rows in ([5, 30], [40, 0], [1, 1], [0, 0], [0, 33], [8, 9], [20, 20]):
+        s["cu"] = np.array([0, rows[0], sum(rows)], np.int32)
+        cu.copy_(torch.from_numpy(s["cu"]))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (out[sum(rows):] == 7.0).all()
+        if sum(rows):
+            check(out, s, "masked")
+            assert torch.equal(call(s, device, "masked")[:sum(rows)], out[:sum(rows)])   # (an eager call of its own)
