@@ -17,7 +17,9 @@
 // larger ones in two launches: the prefix sums in one workgroup beside the
 // sums of the rows of lengths in others, then the rows, four per thread.
 // Nothing is written to the tables before every read of them is done: the
-// first launch (or phase) only reads.
+// first launch (or phase) only reads.  Measured: 10.3 us in one workgroup (64
+// requests, tables of 256 blocks), 6.0 + 5.6 us in two launches (256 requests,
+// 26 700 packed rows).
 
 #include "tierkv_common.h"
 
@@ -319,7 +321,8 @@ __global__ __launch_bounds__(SM_FILL) void slot_fill_kernel(SlotMapParams p) {
 // tierkv_write_slots: row r of k / v [rows, kv_heads, D] into HOT pool row
 // slots[r] = slot * block_size + position.  A copy: bound by memory.  One
 // thread per 16 bytes of output (eight elements), so a row's reads and each
-// head's writes are whole segments.
+// head's writes are whole segments.  Measured: 16384 bf16 rows of 8 heads of
+// 128, read and written 134 MB, 21.9 us, 6.1 TB/s; 64 rows 2.8 us.
 // ---------------------------------------------------------------------------
 struct WriteSlotsParams {
   const void* src[2];
