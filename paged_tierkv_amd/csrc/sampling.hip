@@ -426,12 +426,18 @@ __device__ __forceinline__ uint32_t sp_select(SpShared& sh, const T* x, int n, d
     if (tid < SP_DIGITS) sh.hist[tid] = 0;
     __syncthreads();
     const uint32_t high = shift == 24 ? 0u : ~0u << (shift + 8);
-    for (int i = tid; i < n; i += SP_THREADS) {
-      const float v = sp_load(x, i);
-      const uint32_t k = sp_key(v);
-      if ((k & high) == prefix) {
-        const uint64_t m = measure(v, k);
-        if (m) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[(k >> shift) & 255]), (unsigned long long)m);
+    constexpr int AHEAD = 16;   // loads in flight
+    for (int i0 = tid; i0 < n; i0 += SP_THREADS * AHEAD) {
+      float v[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) v[j] = sp_load(x, min(i0 + SP_THREADS * j, n - 1));
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const uint32_t k = sp_key(v[j]);
+        if (i0 + SP_THREADS * j < n && (k & high) == prefix) {
+          const uint64_t m = measure(v[j], k);
+          if (m) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[(k >> shift) & 255]), (unsigned long long)m);
+        }
       }
     }
     if (tid == 0 && extra && (key_x & high) == prefix)
@@ -448,12 +454,21 @@ __device__ __forceinline__ uint32_t sp_select(SpShared& sh, const T* x, int n, d
 
 // Sum of measure(i) over [lo, hi) by wave segments; every thread finds the
 // segments' sums in sh.wave.  Returns the segment length.
-template <typename M>
-__device__ __forceinline__ int sp_segments(SpShared& sh, int lo, int hi, M measure) {
+template <typename T, typename M>
+__device__ __forceinline__ int sp_segments(SpShared& sh, const T* x, int lo, int hi, M measure) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int seg = (((hi - lo) + SP_WAVES * 64 - 1) / (SP_WAVES * 64)) * 64;
   uint64_t s = 0;
-  for (int i = lo + w * seg + lane; i < min(lo + (w + 1) * seg, hi); i += 64) s += measure(i);
+  const int first = lo + w * seg, end = min(first + seg, hi);
+  constexpr int AHEAD = 16;   // loads in flight (one at a time, a part of 8016 took 16 round trips)
+  for (int i0 = first + lane; i0 < end; i0 += 64 * AHEAD) {
+    float v[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) v[k] = sp_load(x, min(i0 + 64 * k, end - 1));
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (i0 + 64 * k < end) s += measure(v[k], i0 + 64 * k);
+  }
   s = sp_wave_sum(s);
   __syncthreads();
   if (lane == 0) sh.wave[w] = s;
@@ -463,17 +478,17 @@ __device__ __forceinline__ int sp_segments(SpShared& sh, int lo, int hi, M measu
 
 // The smallest index in [lo, hi) whose running sum of measure exceeds
 // target, which is below the sum over [lo, hi).
-template <typename M>
-__device__ __forceinline__ int sp_descend(SpShared& sh, int lo, int hi, uint64_t target, M measure) {
+template <typename T, typename M>
+__device__ __forceinline__ int sp_descend(SpShared& sh, const T* x, int lo, int hi, uint64_t target, M measure) {
   while (hi - lo > 64) {
-    const int seg = sp_segments(sh, lo, hi, measure);
+    const int seg = sp_segments(sh, x, lo, hi, measure);
     int w = 0;
     while (w < SP_WAVES - 1 && target >= sh.wave[w]) target -= sh.wave[w++];
     lo += w * seg;
     hi = min(lo + seg, hi);
   }
   const int lane = threadIdx.x & 63;
-  uint64_t c = lo + lane < hi ? measure(lo + lane) : 0;
+  uint64_t c = lo + lane < hi ? measure(sp_load(x, lo + lane), lo + lane) : 0;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const uint64_t y = __shfl_up(c, d, 64);
@@ -509,10 +524,7 @@ __device__ __forceinline__ void sp_slow(SpShared& sh, const SampleParams& p, int
     const uint32_t cut_k = cut;
     const uint64_t at_cut = ties >= 0 ? uint64_t(ties) * row.weight(sp_value(cut_k)) : 0;
     auto measure = [&](float v, uint32_t key) -> uint64_t { return key > cut_k || ties < 0 ? row.weight(v) : 0; };
-    sp_segments(sh, 0, n, [&](int i) {
-      const float v = sp_load(x, i);
-      return measure(v, sp_key(v));
-    });
+    sp_segments(sh, x, 0, n, [&](float v, int) { return measure(v, sp_key(v)); });
     uint64_t total = at_cut;
     for (int i = 0; i < SP_WAVES; ++i) total += sh.wave[i];
     const double thr = fmax(double(top_p) * double(total), 1.0);   // one token at least
@@ -527,18 +539,18 @@ __device__ __forceinline__ void sp_slow(SpShared& sh, const SampleParams& p, int
   // The index of the last tie kept.
   int last = n;
   if (ties >= 0) {
-    auto tie = [&](int i) -> uint64_t { return sp_key(sp_load(x, i)) == cut ? 1 : 0; };
-    sp_segments(sh, 0, n, tie);
+    auto tie = [&](float v, int) -> uint64_t { return sp_key(v) == cut ? 1 : 0; };
+    sp_segments(sh, x, 0, n, tie);
     int64_t count = 0;
     for (int i = 0; i < SP_WAVES; ++i) count += int64_t(sh.wave[i]);
-    if (ties < count) last = sp_descend(sh, 0, n, uint64_t(ties - 1), tie);
+    if (ties < count) last = sp_descend(sh, x, 0, n, uint64_t(ties - 1), tie);
   }
-  auto kept = [&](int i) -> uint64_t { return sp_kept<T>(row, sp_load(x, i), i, cut, last); };
-  sp_segments(sh, 0, n, kept);
+  auto kept = [&](float v, int i) -> uint64_t { return sp_kept<T>(row, v, i, cut, last); };
+  sp_segments(sh, x, 0, n, kept);
   uint64_t total = 0;
   for (int i = 0; i < SP_WAVES; ++i) total += sh.wave[i];
-  const int token = sp_descend(sh, 0, n, sp_target(p, b, total), kept);
-  sp_write(p, b, token, double(kept(token)) / double(total));
+  const int token = sp_descend(sh, x, 0, n, sp_target(p, b, total), kept);
+  sp_write(p, b, token, double(kept(sp_load(x, token), token)) / double(total));
 }
 
 // ---- the launches ----------------------------------------------------------
@@ -778,9 +790,9 @@ __device__ __forceinline__ void sp_draw_parts(SpShared& sh, const SampleParams& 
   const int i = past ? __ffsll((unsigned long long)past) - 1 : p.parts - 1;
   target -= __shfl(run - own, i, 64);
   const int size = sp_part_size<T>(p);
-  auto kept = [&](int e) -> uint64_t { return sp_kept<T>(row, sp_load(x, e), e, cut, last); };
-  const int token = sp_descend(sh, i * size, min((i + 1) * size, n), target, kept);
-  sp_write(p, b, token, double(kept(token)) / double(all));
+  auto kept = [&](float v, int e) -> uint64_t { return sp_kept<T>(row, v, e, cut, last); };
+  const int token = sp_descend(sh, x, i * size, min((i + 1) * size, n), target, kept);
+  sp_write(p, b, token, double(kept(sp_load(x, token), token)) / double(all));
 }
 
 // Launch 2: rows without a top-k.  With a top-p the bins of the distance to
