@@ -35,11 +35,12 @@
 //   neither   the second launch adds up each part of the row and its last
 //             workgroup draws in the part that holds the token.
 // Measured (us per launch; maxima, top-k, sums, list, draw): 1 x 32000 fp16
-// with top-k 3.7 + 13.7; 16 x 128256 bf16 with top-p 4.2, -, 14.7, 14.9, 22.2;
-// 256 x 128256 fp32, limits of each row, 23.0 (5.7 TB/s), 19.5, 16.1, 20.6,
-// 35.1 (the later launches read a row again only where its limits need it).
+// with top-k 3.6 + 13.6; 16 x 128256 bf16 with top-p 4.8, -, 14.2, 14.8, 20.6;
+// 256 x 128256 fp32, limits of each row, 23.1 (5.7 TB/s), 19.5, 16.4, 20.9,
+// 29.7 (the later launches read a row again only where its limits need it).
 // Rows that fit none of these (a thousand equal logits at the border, k in
-// the thousands) take a radix select over the row by one workgroup.
+// the thousands) take a radix select over the row by one workgroup (64 x
+// 128256 fp32 of whole numbers: 329 us with top-k 3000, 1020 with top-p 0.9).
 
 #include "tierkv_common.h"
 
