@@ -423,7 +423,10 @@ TIERKV_API int64_t tierkv_decode_step_size(void);
 /* A serving step over requests of different lengths.  The reference serves
  * one sequence per table (tierkv_policy.py:1768-1816, modeling_llama.py:
  * 419-456); these take a batch whose requests bring different numbers of new
- * tokens, packed as rows: request b's are rows [cu[b], cu[b + 1]). */
+ * tokens, packed as rows: request b's are rows [cu[b], cu[b + 1]).
+ * A call may be several launches that pass state on through its workspace:
+ * calls that share one go to one stream, and a host thread starts one only
+ * after another thread's has returned. */
 
 /* Table entries of the new tokens' blocks, and where each packed row goes.
  * new_tokens int32 [batch] (device) tokens per request, >= 0.  The open block

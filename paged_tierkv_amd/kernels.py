@@ -207,28 +207,31 @@ def prefill_block_mass(query_states: torch.Tensor, key_states: torch.Tensor, blo
         raise ValueError("key states do not match the query geometry.")
     kv_heads = int(k.shape[1])
     need = int(lib.tierkv_prefill_block_mass_full_workspace_bytes(batch, heads, kv_heads, tokens))
-    # One scratch buffer per (device, stream): launches on one stream are
-    # ordered; launches on different streams may overlap and never share it.
-    # The call passes what this shape needs, not what the buffer holds, so its
-    # summation order does not depend on earlier calls.
-    key = (q.device.index, _lib.stream_of(q.device))
-    ws = _prefill_ws.get(key)
-    if ws is None or ws.numel() < need:
-        ws = torch.empty(max(need, 256), dtype=torch.uint8, device=q.device)
-        _prefill_ws[key] = ws
+    # One scratch buffer per (device, stream): calls on one stream are enqueued
+    # whole, one after another (_lib.call_lock); launches on different streams
+    # may overlap and never share it.  The call passes what this shape needs,
+    # not what the buffer holds, so its summation order does not depend on
+    # earlier calls.
     nblk = (tokens + int(block_size) - 1) // int(block_size)
     out = torch.empty((batch, nblk), dtype=torch.float32, device=q.device)
-    rc = lib.tierkv_prefill_block_mass(
-        _lib.ptr(q), q.stride(0), q.stride(1), q.stride(2), _lib.ptr(k), k.stride(0), k.stride(1), k.stride(2),
-        _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F16, _lib.ptr(out), batch, heads, kv_heads,
-        tokens, dim, int(block_size), float(scaling), _lib.ptr(ws), need, _lib.stream_of(q.device))
+    key = (q.device.index, _lib.stream_of(q.device))
+    with _lib.call_lock:
+        ws = _prefill_ws.get(key)
+        if ws is None or ws.numel() < need:
+            ws = torch.empty(max(need, 256), dtype=torch.uint8, device=q.device)
+            _prefill_ws[key] = ws
+        rc = lib.tierkv_prefill_block_mass(
+            _lib.ptr(q), q.stride(0), q.stride(1), q.stride(2), _lib.ptr(k), k.stride(0), k.stride(1), k.stride(2),
+            _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F16, _lib.ptr(out), batch, heads, kv_heads,
+            tokens, dim, int(block_size), float(scaling), _lib.ptr(ws), need, _lib.stream_of(q.device))
     _lib.check(rc, "tierkv_prefill_block_mass")
     return out
 
 
 # One scratch buffer per (operator, device, stream), as the prefill scores':
-# launches on one stream are ordered; launches on different streams may
-# overlap and never share it.  A captured call takes scratch of its own from
+# calls on one stream are enqueued whole, one after another (_lib.call_lock);
+# launches on different streams may overlap and never share it.  A captured
+# call takes scratch of its own from
 # its graph's memory, so that graphs replayed on different streams, and eager
 # calls beside them, share none.
 _scratch_ws: dict = {}
@@ -308,12 +311,13 @@ def build_slot_map(new_tokens: torch.Tensor, block_table: torch.Tensor, block_st
     slots, _, positions, _, cu, context = torch.empty(2 * (rows + pad) + 2 * batch + 1, dtype=torch.int32,
                                                       device=device).split([rows, pad, rows, pad, batch + 1, batch])
     need = lib.tierkv_slot_map_workspace_bytes(batch)
-    ws = _scratch("slot_map", device, need)
     ptr = _lib.ptr
-    rc = _on_device(device, lib.tierkv_build_slot_map, ptr(new_tokens), batch, rows, ptr(block_table),
-                    ptr(block_states), ptr(block_lengths), stride, ptr(seq_num_blocks), ptr(open_blocks), ptr(hot_free),
-                    hot_free.numel(), ptr(ctl), int(block_size), ptr(slots), ptr(positions), ptr(cu), ptr(context),
-                    ptr(ws), ws.numel())
+    with _lib.call_lock:
+        ws = _scratch("slot_map", device, need)
+        rc = _on_device(device, lib.tierkv_build_slot_map, ptr(new_tokens), batch, rows, ptr(block_table),
+                        ptr(block_states), ptr(block_lengths), stride, ptr(seq_num_blocks), ptr(open_blocks),
+                        ptr(hot_free), hot_free.numel(), ptr(ctl), int(block_size), ptr(slots), ptr(positions), ptr(cu),
+                        ptr(context), ptr(ws), ws.numel())
     _lib.check(rc, "tierkv_build_slot_map")
     return SlotMap(slots, positions, cu, context)
 
@@ -399,10 +403,11 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     tokens = torch.empty(batch, dtype=torch.int64, device=device)
     probs = torch.empty(batch, dtype=torch.float32, device=device)
     need = lib.tierkv_sample_workspace_bytes(batch, vocab)
-    ws = _scratch("sample", device, need, _lib.SAMPLE_COUNTER_BYTES)
     ptr = _lib.ptr
-    rc = _on_device(device, lib.tierkv_sample_tokens, ptr(x), _LOGIT_DTYPES[x.dtype], x.stride(0), batch, vocab, ptr(u),
-                    ptr(t), float(t_all), ptr(k), int(min(max(k_all, 0), SAMPLE_MAX_VOCAB)), ptr(p), float(p_all), ptr(m),
-                    float(m_all), ptr(tokens), ptr(probs), ptr(ws), ws.numel())
+    with _lib.call_lock:
+        ws = _scratch("sample", device, need, _lib.SAMPLE_COUNTER_BYTES)
+        rc = _on_device(device, lib.tierkv_sample_tokens, ptr(x), _LOGIT_DTYPES[x.dtype], x.stride(0), batch, vocab,
+                        ptr(u), ptr(t), float(t_all), ptr(k), int(min(max(k_all, 0), SAMPLE_MAX_VOCAB)), ptr(p),
+                        float(p_all), ptr(m), float(m_all), ptr(tokens), ptr(probs), ptr(ws), ws.numel())
     _lib.check(rc, "tierkv_sample_tokens")
     return tokens, probs

@@ -169,9 +169,9 @@ def launch_bytes(lib, *shape) -> tuple[int, int]:
 
 
 _LIVE: "weakref.WeakSet[DecodeWorkspace]" = weakref.WeakSet()
-# Implicit workspaces, one per (device, stream): launches on one stream are
-# ordered, so they may share one; launches on different streams may overlap
-# and never share.
+# Implicit workspaces, one per (device, stream): calls on one stream are
+# enqueued whole, one after another (_lib.call_lock), so they may share one;
+# launches on different streams may overlap and never share.
 _implicit: dict = {}
 
 
@@ -262,23 +262,22 @@ def tierkv_decode_attention(
                k_scale, k_zero, v_scale, v_zero)
     det = default_deterministic() if deterministic is None else bool(deterministic)
     simple = workspace is None and seq_num_blocks is None and splits is None
-    if simple:
-        hit = _rebind(lib, query_states, statics, num_blocks, num_key_value_groups, scaling, return_scores, cold_mode,
-                      det)
+    with _lib.call_lock:
+        hit = None
+        if simple:
+            hit = _rebind(lib, query_states, statics, num_blocks, num_key_value_groups, scaling, return_scores, cold_mode,
+                          det)
         if hit is not None:
             args, out, score_sums, ws, batched = hit
-            _launch(lib, args, query_states.device, ws)
-            if score_sums is not None and not batched:
-                score_sums = score_sums[0]
-            return out, score_sums
-    args, out, score_sums, ws, batched, _ = _bind(
-        query_states, block_table, block_states, block_lengths, hot_k_pool, hot_v_pool, warm_k_pool, warm_v_pool,
-        k_scale, k_zero, v_scale, v_zero, num_blocks, num_key_value_groups, scaling, return_scores,
-        cold_mode=cold_mode, seq_num_blocks=seq_num_blocks, splits=splits, workspace=workspace, deterministic=det)
-    if simple:
-        _remember(query_states, statics, num_blocks, num_key_value_groups, scaling, return_scores, cold_mode, det,
-                  args, batched)
-    _launch(lib, args, query_states.device, ws)
+        else:
+            args, out, score_sums, ws, batched, _ = _bind(
+                query_states, block_table, block_states, block_lengths, hot_k_pool, hot_v_pool, warm_k_pool, warm_v_pool,
+                k_scale, k_zero, v_scale, v_zero, num_blocks, num_key_value_groups, scaling, return_scores,
+                cold_mode=cold_mode, seq_num_blocks=seq_num_blocks, splits=splits, workspace=workspace, deterministic=det)
+            if simple:
+                _remember(query_states, statics, num_blocks, num_key_value_groups, scaling, return_scores, cold_mode, det,
+                          args, batched)
+        _launch(lib, args, query_states.device, ws)
     if score_sums is not None and not batched:
         score_sums = score_sums[0]
     return out, score_sums
@@ -522,16 +521,17 @@ def _bind(
 
 
 def _launch(lib, args, device, ws) -> None:
-    if ws is None:
-        rc = lib.tierkv_decode_attention_noalloc(*args, _lib.stream_of(device))
-        _lib.check(rc, "tierkv_decode_attention_noalloc")
-    else:
-        rc = lib.tierkv_decode_attention(*args, _lib.stream_of(device))
-        _lib.check(rc, "tierkv_decode_attention")
-    if _lib.env_flag("TIERKV_CHECK_ERRORS"):
-        word = noalloc_error_word(device) if ws is None else ws.error_word()
-        if word:
-            raise RuntimeError(f"TierKV decode skipped blocks with out-of-range slot/state (flag {word}).")
+    with _lib.call_lock:
+        if ws is None:
+            rc = lib.tierkv_decode_attention_noalloc(*args, _lib.stream_of(device))
+            _lib.check(rc, "tierkv_decode_attention_noalloc")
+        else:
+            rc = lib.tierkv_decode_attention(*args, _lib.stream_of(device))
+            _lib.check(rc, "tierkv_decode_attention")
+        if _lib.env_flag("TIERKV_CHECK_ERRORS"):
+            word = noalloc_error_word(device) if ws is None else ws.error_word()
+            if word:
+                raise RuntimeError(f"TierKV decode skipped blocks with out-of-range slot/state (flag {word}).")
 
 
 def tierkv_extend_attention(
@@ -669,16 +669,17 @@ def tierkv_extend_attention(
             float(scaling), ws.data_ptr(), ws.nbytes, _lib.stream_of(device))
         return rc, ws
 
-    if torch.cuda.current_device() == index:
-        rc, ws = launch()
-    else:
-        with torch.cuda.device(device):
+    with _lib.call_lock:
+        if torch.cuda.current_device() == index:
             rc, ws = launch()
-    _lib.check(rc, "tierkv_extend_attention")
-    if _lib.env_flag("TIERKV_CHECK_ERRORS"):
-        word = ws.error_word()
-        if word:
-            raise RuntimeError(f"TierKV attention skipped blocks with out-of-range slot/state (flag {word}).")
+        else:
+            with torch.cuda.device(device):
+                rc, ws = launch()
+        _lib.check(rc, "tierkv_extend_attention")
+        if _lib.env_flag("TIERKV_CHECK_ERRORS"):
+            word = ws.error_word()
+            if word:
+                raise RuntimeError(f"TierKV attention skipped blocks with out-of-range slot/state (flag {word}).")
     return out
 
 

@@ -1394,24 +1394,25 @@ class CompactTieredKVTensorPool(_PoolBase):
         if need is None:
             need = needs[n] = tierkv_hip.launch_bytes(lib, st.batch, st.num_heads, st.num_kv_heads, n, st.block_size,
                                                       st.head_dim, 0, st.splits_hint)
-        ws = tierkv_hip.stream_workspace(self.device)
-        ws.reserve(*need)
-        out = torch.empty((1, 1, st.num_heads, st.head_dim), device=self.device, dtype=query_states.dtype)
-        # Host state first, as the general path records it before launching.
-        self._blocks[physical_idx] = _Block(HOT_STATE, b.slot, pos + 1)
-        tables.set(self._t_len, where[0], where[1], pos + 1)
-        pending = tables.pending
-        sent = dict(pending)
-        for i, (flat, value) in enumerate(sent.items()):
-            st.pairs[i][0], st.pairs[i][1] = flat, value
-        st.n_pairs = len(sent)
-        pending.clear()
-        st.src_k, st.src_v = key_states.data_ptr(), value_states.data_ptr()
-        st.src_tokens = key_states.shape[2]
-        job[3], job[4] = b.slot, pos
-        st.query, st.out, st.num_blocks = query_states.data_ptr(), out.data_ptr(), n
-        st.workspace, st.workspace_bytes = ws.data_ptr(), ws.nbytes
-        rc = lib.tierkv_decode_step(st_ref, _lib.stream_of(self.device))
+        with _lib.call_lock:   # no other thread replaces the workspace before the launch
+            ws = tierkv_hip.stream_workspace(self.device)
+            ws.reserve(*need)
+            out = torch.empty((1, 1, st.num_heads, st.head_dim), device=self.device, dtype=query_states.dtype)
+            # Host state first, as the general path records it before launching.
+            self._blocks[physical_idx] = _Block(HOT_STATE, b.slot, pos + 1)
+            tables.set(self._t_len, where[0], where[1], pos + 1)
+            pending = tables.pending
+            sent = dict(pending)
+            for i, (flat, value) in enumerate(sent.items()):
+                st.pairs[i][0], st.pairs[i][1] = flat, value
+            st.n_pairs = len(sent)
+            pending.clear()
+            st.src_k, st.src_v = key_states.data_ptr(), value_states.data_ptr()
+            st.src_tokens = key_states.shape[2]
+            job[3], job[4] = b.slot, pos
+            st.query, st.out, st.num_blocks = query_states.data_ptr(), out.data_ptr(), n
+            st.workspace, st.workspace_bytes = ws.data_ptr(), ws.nbytes
+            rc = lib.tierkv_decode_step(st_ref, _lib.stream_of(self.device))
         if rc != _lib.TIERKV_OK:
             # A refused step queued nothing on the device (its checks run
             # before its first launch): the ledger entry and the block's
