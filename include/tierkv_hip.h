@@ -475,12 +475,17 @@ TIERKV_API int32_t tierkv_write_slots(
  *          are multiples of 8, head_dim contiguous, 16-byte aligned
  *   out    [num_rows, num_heads, head_dim] contiguous, the query's dtype
  *   max_tokens  an upper bound of the requests' new tokens (num_rows will do):
- *          with it small calls launch less; rows past it are not computed
+ *          with it small calls launch less.  Of a request that brings more, or
+ *          whose range ends past num_rows, the first max_tokens rows that
+ *          there are see what they see in any case, the others are not
+ *          written, and bit 4 of the error word is set (nothing is launched,
+ *          and no bit set, when max_tokens or num_rows is 0)
  * head_dim a multiple of 8 up to 128, block_size up to 64, any GQA group.
  * The same inputs give the same bits on every call.  workspace: as
  * tierkv_decode_attention's (one buffer may serve both, in stream order), at
  * least tierkv_extend_workspace_bytes(...) bytes, zero-filled before its
- * first use; the error word is set as there when a block is skipped. */
+ * first use; the error word is set as there when a block is skipped, and to 4
+ * when rows are not computed (max_tokens, or packed ranges that overlap). */
 TIERKV_API int64_t tierkv_extend_workspace_bytes(int32_t batch, int32_t num_rows, int32_t max_tokens,
                                                  int32_t num_heads, int32_t num_kv_heads, int32_t num_blocks,
                                                  int32_t block_size, int32_t head_dim);

@@ -110,7 +110,7 @@ struct ExtendParams {
   int32_t* err;
   uint32_t* arrived;   // zero between launches; in the workspace's first 256 bytes, which no launch uses otherwise
   int32_t* head;       // {items, cut tiles}
-  int4* seq;           // [batch] {sub-tiles, tokens L, COLD tokens that every row sees, query rows n}
+  int4* seq;           // [batch] {sub-tiles, tokens up to the last computed row, COLD tokens that every row sees, query rows n}
   int4* subtile;       // [batch][num_blocks * subs] {slot, valid | state << 8 | sub << 16, first ordinal, 0}
   int4* item;          // [max_items] {request, tile | wide << 30, part | parts << 16, partial or -1}
   int2* cut;           // [max_cut] {first partial, item}
@@ -154,10 +154,13 @@ __device__ __forceinline__ Ex3 ex_scan3(Ex3 v, Ex3 (&sh)[EX_PLAN / 64], Ex3* tot
   return x;
 }
 
-// Query rows of request b: its packed range, clamped to the rows there are.
-__device__ __forceinline__ int2 ex_rows(const ExtendParams& p, int b) {
-  const int lo = min(max(p.cu[b], 0), p.rows), hi = min(max(p.cu[b + 1], lo), p.rows);
-  return make_int2(lo, min(hi - lo, p.max_tokens));
+// Query rows of request b that are computed (first packed row, count): at
+// most max_tokens of those that there are.  The limits of what they see come
+// from the tokens that the request brings, `all`, computed or not.
+__device__ __forceinline__ int2 ex_rows(const ExtendParams& p, int b, int* all = nullptr) {
+  const int lo = min(max(p.cu[b], 0), p.rows), end = max(p.cu[b + 1], lo);
+  if (all) *all = end - lo;
+  return make_int2(lo, min(min(end, p.rows) - lo, p.max_tokens));
 }
 
 __device__ __forceinline__ int ex_tiles(int rows) { return rows <= EX_NARROW ? (rows > 0) : (rows + EX_WIDE - 1) / EX_WIDE; }
@@ -199,7 +202,8 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
   int nb = p.num_blocks;
   if (p.seq_nblocks) nb = min(max(p.seq_nblocks[b], 0), p.num_blocks);
   const int64_t row = int64_t(b) * p.stride;
-  const int n = ex_rows(p, b).y;
+  int n_all;   // the request's new tokens, of which the first n are computed
+  const int n = ex_rows(p, b, &n_all).y;
   int tokens = 0;
   Ex3 total;
   if (p.cold_zero) {   // COLD sub-tiles need the distance to the row's end
@@ -235,7 +239,7 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
     int pos = at + s.b - (keep == 2 ? 0 : count);
     ordinal += total.a;
     if (p.cold_zero) {
-      const bool all_see = keep == 2 && first + len <= tokens - n + 1;
+      const bool all_see = keep == 2 && first + len <= tokens - n_all + 1;
       if (all_see) count = 0;
       const Ex3 z = ex_scan3({count, all_see ? len : 0, 0}, sh, &total);
       pos = at + z.a - count;
@@ -251,7 +255,8 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
   if (tid == 0) {
     // Agent-scope stores: the last workgroup may read them from another XCD.
     int32_t* s = reinterpret_cast<int32_t*>(p.seq + b);
-    const int v[4] = {at, ordinal, cold, n};
+    if (n < n_all) atomicOr(p.err, 4);
+    const int v[4] = {at, ordinal - (n_all - n), cold, n};
     for (int k = 0; k < 4; ++k) __hip_atomic_store(s + k, v[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __builtin_amdgcn_s_waitcnt(0);
     s_last = __hip_atomic_fetch_add(p.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == gridDim.x;
@@ -372,6 +377,7 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
     if (parts > 0) {
       // The host's bounds hold for packed ranges that do not overlap; items of others may be left out (-1).
       const bool fits = at_item + parts <= p.max_items && (!cut || (at_cut < p.max_cut && at_part + parts <= p.max_part));
+      if (!fits) atomicOr(p.err, 4);
       for (int k = 0; k < parts; ++k)
         if (at_item + k < p.max_items)
           p.item[at_item + k] = make_int4(fits ? i : -1, t | (wide ? 1 << 30 : 0), k | (parts << 16), cut ? at_part + k : -1);

@@ -566,9 +566,11 @@ def tierkv_extend_attention(
     the request's tokens up to itself.  Tables are ``[B, max_blocks]``; pools,
     formats, ``cold_mode``, ``seq_num_blocks`` and ``workspace`` are those of
     ``tierkv_decode_attention``.  ``max_tokens`` bounds the requests' new
-    tokens where the caller knows it.  Returns ``[N, H, D]`` (``out`` when
-    given; rows behind the last request are left as they were).  The same
-    inputs give the same bits on every call."""
+    tokens where the caller knows it; of a request that brings more, the first
+    ``max_tokens`` rows are computed and bit 4 of the workspace's error word is
+    set.  Returns ``[N, H, D]`` (``out`` when given; rows that are not computed
+    and rows behind the last request are left as they were).  The same inputs
+    give the same bits on every call."""
     lib = _lib.lib()
     if query_states.ndim != 3:
         raise ValueError("query_states must be packed rows [tokens, num_heads, head_dim].")
@@ -679,7 +681,9 @@ def tierkv_extend_attention(
         if _lib.env_flag("TIERKV_CHECK_ERRORS"):
             word = ws.error_word()
             if word:
-                raise RuntimeError(f"TierKV attention skipped blocks with out-of-range slot/state (flag {word}).")
+                what = ["skipped blocks with out-of-range slot/state"] if word & 3 else []
+                what += ["left rows out (more new tokens than max_tokens or rows)"] if word & 4 else []
+                raise RuntimeError(f"TierKV attention {' and '.join(what)} (flag {word}).")
     return out
 
 

@@ -12,8 +12,9 @@ import torch
 
 from oracle import serving
 from paged_tierkv_amd import kernels
+from paged_tierkv_amd.tierkv_hip import DecodeWorkspace
 
-from test_gpu_serving_step import call, gpu, step, tables
+from test_gpu_serving_step import call, check, gpu, step, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,42 @@ def test_threads_on_one_stream_get_their_own_results(device):
         assert len(results[i]) == 12
         for got in results[i]:
             assert all(torch.equal(g, e) for g, e in zip(got, alone[i]))
+
+
+@pytest.mark.parametrize("new,held,heads,kv,d,bound,rows", [
+    ([9, 5, 0, 20], [60, 300, 4, 20], 8, 2, 64, 6, None),            # narrow tiles
+    ([300, 3, 40], [900, 70, 41], 8, 1, 128, 37, None),              # wide tiles, one bound inside a request's second
+    ([90, 1], [2500, 3000], 16, 1, 64, 33, None),                    # cut tiles
+    ([9, 30], [60, 300], 8, 2, 64, 1, None),
+    ([9, 30], [60, 300], 8, 2, 64, None, 20),                        # packed rows that end inside a request
+    ([6, 4], [5, 4], 4, 2, 64, 3, None),                             # more new tokens than the request holds
+])
+@pytest.mark.parametrize("cold", ["masked", "zero_logit"])
+def test_rows_within_a_bound_that_is_too_low_are_right(device, new, held, heads, kv, d, bound, rows, cold):
+    """Of a request that brings more tokens than max_tokens (or than there are
+    rows), the first rows see what they see in any case, the others stay as
+    they were, and the error word tells."""
+    s = step(51 + len(new), new, held, heads, kv, d)
+    count = int(s["cu"][-1]) if rows is None else rows
+    done = np.concatenate([s["cu"][b] + np.arange(min(n, bound or n)) for b, n in enumerate(new)])
+    done = done[done < count]
+    q = s["q"].to(device)[:count]
+    out = torch.full(q.shape, 7.0, dtype=q.dtype, device=device)
+    ws = DecodeWorkspace(device)
+    call(s, device, cold, q=q, out=out, max_tokens=bound, workspace=ws)
+    assert ws.error_word() == 4
+    left = np.setdiff1d(np.arange(count), done)
+    assert (out[torch.from_numpy(left).to(device)] == 7.0).all()
+    full = torch.zeros(s["q"].shape, dtype=q.dtype, device=device)
+    full[:count] = out
+    check(full, s, cold, done)
+    call(s, device, cold, out=full, max_tokens=max(new), workspace=ws)
+    assert ws.error_word() == 0
+
+
+def test_a_bound_that_is_too_low_is_raised_when_errors_are_checked(device, monkeypatch):
+    s = step(52, [9, 5], [60, 30], 8, 2, 64)
+    monkeypatch.setenv("TIERKV_CHECK_ERRORS", "1")
+    call(s, device, "masked", max_tokens=9)
+    with pytest.raises(RuntimeError, match="max_tokens"):
+        call(s, device, "masked", max_tokens=8)
