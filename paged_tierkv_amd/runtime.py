@@ -260,6 +260,10 @@ class BatchedTieredKVRuntime:
         # so launch sizes and budgets need no device read-back.
         self._blocks = [0] * self.num_layers
         self._open_tokens = [0] * self.num_layers
+        # HOT blocks per sequence and layer, at most: exact after a prefill and
+        # for what is appended, the budget after a tick (a COLD block may rank
+        # among the HOT ones and stays COLD).
+        self._hot_bound = [0] * self.num_layers
         self.seq_len = 0              # tokens per sequence (lockstep)
         self.decode_step = 0
         self.max_demotions = self.batch * self.hot_per_seq
@@ -393,6 +397,7 @@ class BatchedTieredKVRuntime:
         st.load(dev[:m], self._meta_views)
         self._blocks[layer] = n
         self._open_tokens[layer] = 0
+        self._hot_bound[layer] = int((tiers == HOT_STATE).sum(1).max()) if n else 0
         if layer == self.num_layers - 1:
             self.seq_len = T
 
@@ -420,6 +425,7 @@ class BatchedTieredKVRuntime:
         rest = tokens - take
         if rest > 0:
             self._blocks[layer] += _ceil_div(rest, self.block_size)
+            self._hot_bound[layer] += _ceil_div(rest, self.block_size)
             last = rest - (_ceil_div(rest, self.block_size) - 1) * self.block_size
         else:
             last = self._open_tokens[layer] + take
@@ -516,7 +522,9 @@ class BatchedTieredKVRuntime:
         T, D], attend with query [B, H, T, D] (rotated, as K; each token sees
         the cache and the new tokens up to itself) and, with ``policy_step``,
         re-tier the layer by the scores of the last token.  T is at most
-        ``extend_tokens``.  Returns the attention output [B, T, H, D]."""
+        ``extend_tokens``.  Returns the attention output [B, T, H, D].
+        RuntimeError, with nothing changed, when the tokens exceed max_seq_len
+        or the free HOT slots (tokens of several calls without a tick)."""
         if key_states.shape != value_states.shape or key_states.ndim != 4 or query_states.ndim != 4:
             raise ValueError("query must be [batch, heads, tokens, head_dim], K/V [batch, kv_heads, tokens, head_dim].")
         B, kv, T, d = (int(x) for x in key_states.shape)
@@ -526,9 +534,15 @@ class BatchedTieredKVRuntime:
         if not 0 < T <= self.extend_tokens:
             raise ValueError(f"extend_layer takes 1 to extend_tokens={self.extend_tokens} tokens per sequence.")
         room = self.block_size - self._open_tokens[layer] if self._open_tokens[layer] else 0
-        if self._blocks[layer] + _ceil_div(max(T - room, 0), self.block_size) > self.max_blocks:
+        need = _ceil_div(max(T - room, 0), self.block_size)
+        if self._blocks[layer] + need > self.max_blocks:
             raise RuntimeError(f"{T} more tokens exceed max_seq_len={self.max_seq_len}.")
         st = self.layers[layer]
+        # The pools hold what one call adds between ticks.  Where more was added
+        # without one, the free stack's own count decides (a read-back).
+        if self._hot_bound[layer] + need > self.hot_per_seq and int(st.ctl[0].item()) < B * need:
+            raise RuntimeError(f"no free HOT slots for {T} more tokens in layer {layer}: re-tier it first "
+                               "(a call with policy_step, or tick_layer).")
         rows = lambda t: t.transpose(1, 2).reshape(B * T, t.shape[1], d)   # noqa: E731
         q, k, v = rows(query_states), rows(key_states), rows(value_states)
         if k.dtype not in (torch.float16, torch.bfloat16):
@@ -538,10 +552,13 @@ class BatchedTieredKVRuntime:
                                    self.block_size, B * T)
         kernels.write_slots(k, v, m.slots, st.hot_k, st.hot_v)
         num_blocks = min(self._advance_blocks(layer, T), self.max_blocks)
-        out = tierkv_extend_attention(
+        # Zeros: what a step gives that the device refuses all the same (after
+        # an earlier error that check_errors reports).
+        out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+        tierkv_extend_attention(
             q, m.cu_tokens, st.table, st.states, st.lengths, st.hot_k, st.hot_v, st.warm_k, st.warm_v, st.k_scale,
             st.k_zero, st.v_scale, st.v_zero, num_blocks, num_key_value_groups, scaling, cold_mode=self.cold_mode,
-            seq_num_blocks=st.nblocks, max_tokens=T)
+            seq_num_blocks=st.nblocks, max_tokens=T, out=out)
         if policy_step:
             _, sums = tierkv_decode_attention(
                 query_states[:, :, -1:].contiguous(), st.table, st.states, st.lengths, st.hot_k, st.hot_v, st.warm_k,
@@ -570,6 +587,7 @@ class BatchedTieredKVRuntime:
             self.max_demotions, self.max_promotions,
             self.kv_heads, self.block_size, self.head_dim, _lib.stream_of(self.device))
         _lib.check(rc, "tierkv_runtime_tick")
+        self._hot_bound[layer] = min(int(num_blocks), hot_b)
 
     # -- state and telemetry -------------------------------------------------
 
