@@ -29,6 +29,7 @@ lockstep block count.
 
 from __future__ import annotations
 
+import math
 import os
 
 from dataclasses import dataclass
@@ -194,6 +195,8 @@ class BatchedTieredKVRuntime:
             raise ValueError('prefill_scoring must be "proxy" or "attention".')
         if extend_tokens < 0:
             raise ValueError("extend_tokens must not be negative.")
+        if extend_tokens and (head_dim > 128 or head_dim % 8 or block_size > 64):
+            raise ValueError("extend_tokens needs a head_dim that is a multiple of 8 up to 128, and blocks of up to 64.")
         if not (0.0 <= hot_fraction <= 1.0 and 0.0 <= warm_fraction <= 1.0):
             raise ValueError("tier fractions must lie in [0, 1].")
         self.device = torch.device(device or "cuda")
@@ -523,14 +526,25 @@ class BatchedTieredKVRuntime:
         the cache and the new tokens up to itself) and, with ``policy_step``,
         re-tier the layer by the scores of the last token.  T is at most
         ``extend_tokens``.  Returns the attention output [B, T, H, D].
-        RuntimeError, with nothing changed, when the tokens exceed max_seq_len
-        or the free HOT slots (tokens of several calls without a tick)."""
+        A call that cannot be taken raises before anything changes: ValueError
+        for its tensors, RuntimeError when the tokens exceed max_seq_len or the
+        free HOT slots (tokens of several calls without a tick), and under
+        graph capture."""
         if key_states.shape != value_states.shape or key_states.ndim != 4 or query_states.ndim != 4:
             raise ValueError("query must be [batch, heads, tokens, head_dim], K/V [batch, kv_heads, tokens, head_dim].")
         B, kv, T, d = (int(x) for x in key_states.shape)
-        if (B, kv, d) != (self.batch, self.kv_heads, self.head_dim) or (int(query_states.shape[0]),
-                                                                       int(query_states.shape[2])) != (B, T):
+        groups = int(num_key_value_groups)
+        if ((B, kv, d) != (self.batch, self.kv_heads, self.head_dim)
+                or tuple(query_states.shape) != (B, self.kv_heads * groups, T, d)):
             raise ValueError("query or K/V geometry does not match the runtime.")
+        if query_states.dtype not in (torch.float16, torch.bfloat16) or value_states.dtype != key_states.dtype:
+            raise ValueError("extend_layer takes an fp16 / bf16 query and K/V of one dtype.")
+        if any(t.device != self.layers[layer].table.device for t in (query_states, key_states, value_states)):
+            raise ValueError("query and K/V must be on the runtime's device.")
+        if not math.isfinite(scaling):
+            raise ValueError("scaling must be finite.")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("extend_layer cannot be captured: it keeps the host's block counts.")
         if not 0 < T <= self.extend_tokens:
             raise ValueError(f"extend_layer takes 1 to extend_tokens={self.extend_tokens} tokens per sequence.")
         room = self.block_size - self._open_tokens[layer] if self._open_tokens[layer] else 0

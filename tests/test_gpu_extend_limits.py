@@ -95,3 +95,63 @@ def test_the_bound_on_hot_blocks_holds_over_steps_of_all_kinds(device):
         if T == 1:
             rt.end_step()
     rt.check_errors()
+
+
+@pytest.mark.parametrize("why", ["query fp32", "query fp64", "heads", "groups", "head_dim", "K bf16, V fp16", "query on the host",
+                                 "K/V on the host", "scaling", "tokens", "too long"])
+def test_a_call_that_is_refused_changes_nothing(device, why):
+    rt, x = runtime(device, max_seq_len=260), rand(device, 3)
+    rt.prefill_layer(0, x(2, 230), x(2, 230))
+    q, k, v, groups, scaling = x(4, 9), x(2, 9), x(2, 9), 2, 0.125
+    if why == "query fp32":
+        q = q.float()
+    if why == "query fp64":
+        q = q.double()
+    if why == "heads":
+        q = x(6, 9)
+    if why == "groups":
+        groups = 4
+    if why == "head_dim":
+        q = q[..., :32]
+    if why == "K bf16, V fp16":
+        k = k.bfloat16()
+    if why == "query on the host":
+        q = q.cpu()
+    if why == "K/V on the host":
+        k, v = k.cpu(), v.cpu()
+    if why == "scaling":
+        scaling = float("nan")
+    if why == "tokens":
+        q, k, v = x(4, 49), x(2, 49), x(2, 49)
+    if why == "too long":
+        q, k, v = x(4, 33), x(2, 33), x(2, 33)
+    before = held(rt)
+    with pytest.raises(RuntimeError if why == "too long" else ValueError):
+        rt.extend_layer(0, q, k, v, groups, scaling)
+    assert same(held(rt), before)
+    rt.extend_layer(0, x(4, 9), x(2, 9), x(2, 9), 2, 0.125)
+    rt.check_errors()
+
+
+def test_a_capture_is_refused(device):
+    rt, x = runtime(device), rand(device, 4)
+    rt.prefill_layer(0, x(2, 100), x(2, 100))
+    q, k, v = x(4, 9), x(2, 9), x(2, 9)
+    rt.extend_layer(0, q, k, v, 2, 0.125)
+    before = held(rt)
+    torch.cuda.synchronize()
+    graph, seen = torch.cuda.CUDAGraph(), None
+    with torch.cuda.graph(graph):
+        try:
+            rt.extend_layer(0, q, k, v, 2, 0.125)
+        except RuntimeError as e:
+            seen = str(e)
+        q.add(0)
+    assert seen and "captured" in seen and same(held(rt), before)
+
+
+def test_geometry_that_the_attention_does_not_take_is_refused_at_once(device):
+    for kw in (dict(head_dim=256), dict(head_dim=68), dict(block_size=128)):
+        with pytest.raises(ValueError, match="extend_tokens"):
+            runtime(device, **kw)
+    runtime(device, head_dim=256, extend_tokens=0)
