@@ -378,11 +378,16 @@ class DecodeGraphRunner:
         (``kernels.sample_tokens`` of the last position's logits with one
         random number per sequence; each limit a number or a tensor [B]).
         Returns (next token ids [B, 1], the probabilities [B] they were drawn
-        with); nothing is read back to the host."""
+        with); nothing is read back to the host.  ValueError before the step
+        when ``sample_tokens`` would not take the arguments."""
         from . import kernels
 
+        limits = [rows if rows is not None else one for rows, one in kernels._sampling_limits(
+            uniforms, temperature, top_k, top_p, min_p, self.rt.batch, self.ids.device)]
+        if self.model.config.vocab_size > kernels.SAMPLE_MAX_VOCAB:
+            raise ValueError(f"sample_step takes vocabularies of up to {kernels.SAMPLE_MAX_VOCAB} tokens.")
         logits = self.step(input_ids)[:, -1]
-        tokens, probs = kernels.sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p)
+        tokens, probs = kernels.sample_tokens(logits, uniforms, *limits)
         return tokens[:, None], probs
 
 

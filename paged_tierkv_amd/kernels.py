@@ -374,6 +374,18 @@ def _limit(x, name: str, batch: int, device, dtype, low=None, high=None):
     return None, x
 
 
+def _sampling_limits(uniforms, temperature, top_k, top_p, min_p, batch: int, device):
+    """What ``sample_tokens`` asks of its arguments beside the logits: the four
+    limits as ``_limit`` gives them."""
+    _lib.require_gpu_tensor(uniforms, "uniforms")
+    if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (batch,) or uniforms.device != device:
+        raise ValueError("uniforms must be one fp32 number per row on the logits' device.")
+    return (_limit(temperature, "temperature", batch, device, torch.float32, low=0.0),
+            _limit(top_k, "top_k", batch, device, torch.int32),
+            _limit(top_p, "top_p", batch, device, torch.float32, low=0.0),
+            _limit(min_p, "min_p", batch, device, torch.float32, low=0.0, high=1.0))
+
+
 def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Next tokens of logits ``[B, vocab]`` (fp16 / bf16 / fp32) with one random
     number in [0, 1) per row (``tierkv_sample_tokens``): temperature, then the
@@ -387,17 +399,12 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     logit above -inf gives token -1."""
     lib = _lib.lib()
     _lib.require_gpu_tensor(logits, "logits")
-    _lib.require_gpu_tensor(uniforms, "uniforms")
     if logits.ndim != 2 or logits.dtype not in _LOGIT_DTYPES or not logits.numel():
         raise ValueError("logits must be fp16, bf16 or fp32 [batch, vocab].")
     batch, vocab = (int(x) for x in logits.shape)
     device = logits.device
-    if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (batch,) or uniforms.device != device:
-        raise ValueError("uniforms must be one fp32 number per row on the logits' device.")
-    t, t_all = _limit(temperature, "temperature", batch, device, torch.float32, low=0.0)
-    k, k_all = _limit(top_k, "top_k", batch, device, torch.int32)
-    p, p_all = _limit(top_p, "top_p", batch, device, torch.float32, low=0.0)
-    m, m_all = _limit(min_p, "min_p", batch, device, torch.float32, low=0.0, high=1.0)
+    (t, t_all), (k, k_all), (p, p_all), (m, m_all) = _sampling_limits(uniforms, temperature, top_k, top_p, min_p, batch,
+                                                                      device)
     x = logits if logits.stride(1) == 1 and (batch == 1 or logits.stride(0) >= vocab) else logits.contiguous()
     u = uniforms.contiguous()
     tokens = torch.empty(batch, dtype=torch.int64, device=device)
