@@ -367,7 +367,9 @@ def _limit(x, name: str, batch: int, device, dtype, low=None, high=None):
         if x.device != device or tuple(x.shape) != (batch,):
             raise ValueError(f"{name} must be a number or one value per row on the logits' device.")
         if dtype == torch.int32 and x.dtype != dtype:
-            x = x.clamp(0, SAMPLE_MAX_VOCAB)   # (past 32 bits too)
+            # To a type that holds the bound, and bounded before it becomes 32 bits; NaN is off.
+            x = x.double().nan_to_num(nan=0.0) if x.is_floating_point() else x.long()
+            x = x.clamp(0, SAMPLE_MAX_VOCAB)
         return x.to(dtype).contiguous(), 0
     if x != x or (low is not None and x < low) or (high is not None and x > high):
         raise ValueError(f"{name} is out of range.")
