@@ -27,7 +27,8 @@ Two runtimes plug in through their ``cache`` object:
   one ``decode_layer`` call (fused append, attention, and on policy steps the
   device-side tick).  With ``extend_tokens`` set, a forward of several
   tokens on a cache that holds some is one ``extend_layer`` call (a follow-up
-  prompt, drafted tokens).  Sequences must be unpadded and of equal length, the
+  prompt; tokens stay, so drafts that may be rejected are not for it, and
+  ``cache.crop`` raises).  Sequences must be unpadded and of equal length, the
   same restriction the reference's decode path has (batch 1, no padding,
   modeling_llama.py:70-73).
 """
@@ -253,7 +254,7 @@ def _batched_forward(self, runtime, query_states, key_states, value_states, atte
                      kwargs):
     layer = self.layer_idx
     if runtime.extends(int(query_states.shape[-2])):
-        # Several tokens on top of the cache: a follow-up prompt, drafted tokens.
+        # Several tokens on top of the cache: a follow-up prompt.
         if not bool(kwargs.get("tierkv_triton_mask_safe", False)):
             raise ValueError("the batched tiered runtime extends unpadded sequences only (2-D or no attention mask).")
         out = runtime.extend_layer(layer, query_states, key_states, value_states, self.num_key_value_groups,

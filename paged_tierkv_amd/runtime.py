@@ -19,8 +19,9 @@ resident on the device:
   steps runs ``tierkv_runtime_tick`` (scores -> labels -> migrations on the
   device).  The host never waits for the device inside a step;
 * ``extend_layer`` takes several new tokens per sequence on top of what the
-  cache holds (a follow-up prompt, drafted tokens): slot map, row write,
+  cache holds (a follow-up prompt): slot map, row write,
   ``tierkv_extend_attention``, and the tick by the scores of the last token.
+  They stay: nothing takes tokens back out of the cache.
 
 Budgets are fractions of each sequence's current block count (workload
 C5: 15 % HOT, 55 % WARM, the rest evicted), evaluated on the host from the

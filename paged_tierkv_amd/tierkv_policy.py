@@ -1626,7 +1626,8 @@ class LayerRuntimeState:
 class TieredKVCache(HFCache):
     """The HF cache object of a tiered runtime (tierkv_policy.py:1487-1531):
     it counts the committed tokens; the KV itself lives in the runtime.  The
-    beam and crop hooks are no-ops."""
+    beam and crop hooks are no-ops; a batched runtime's crop raises where it
+    would shorten the cache."""
 
     is_compileable = False
 
@@ -1660,6 +1661,12 @@ class TieredKVCache(HFCache):
         return None
 
     def crop(self, max_length: int):
+        held = self.committed_seq_len
+        keep = held + max_length if max_length < 0 else max_length   # (negative: that many tokens less)
+        if keep < held and getattr(self.runtime, "is_batched", False):
+            # Its tokens are in the tables and the tiers; text generated on a
+            # cache that only counts fewer would be wrong.
+            raise NotImplementedError("the batched tiered runtime cannot shorten its cache.")
         return None
 
     def batch_repeat_interleave(self, repeats: int):
