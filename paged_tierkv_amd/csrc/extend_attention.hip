@@ -34,9 +34,16 @@
 // the other's exponentials; smaller ones ("narrow") give each wave its own 32
 // keys of the same rows, merged in LDS.
 //
-// K goes to LDS as fp16 of the codes themselves (exact: |code| <= 127, or
-// code - zero, an integer below 2048 for any row whose values are not far
-// from 0 against their spread), and the scale is applied to the logits in 32 bits.
+// K goes to LDS as fp16 of the codes themselves (exact), and the scale is
+// applied to the logits in 32 bits.  The reference format's zero point is the
+// same for all dims of a token, q . (code - zero) = q . code - zero sum q: one
+// more product step takes it off, with the zero point (fp16, exact) beside
+// the token's row of K and the query's sum in three fp16 pieces beside the
+// query, so that it is off by a 32-bit rounding.  (code - zero in fp16 was off
+// by as much as the codes are where keys lie far from 0 against their spread,
+// mean 10 and deviation 0.2, and infinite past 65504.  2048 tokens on 32768 of
+// that format take 1197 us, with code - zero 1143, with the zero point taken
+// off each logit by vector instructions 1239 to 1369.)
 // V goes to LDS as fp16 of code * scale, one rounding of at most 2^-11 of the
 // value, as the probabilities have one when they become fp16 operands.
 // Probabilities carry a factor 2^6 so that small ones stay normal fp16.
@@ -563,9 +570,8 @@ __device__ __forceinline__ void ex_store_k(const ExtendParams& p, const ExSub& s
         b = i8x4_plus1152(v.y) - off;
       } else {
         const f16x4 off = {1024, 1024, 1024, 1024};
-        const _Float16 z = as_f16x2(st.meta[i])[0];
-        a = (u8x4_plus1024(v.x) - off) - f16x4{z, z, z, z};
-        b = (u8x4_plus1024(v.y) - off) - f16x4{z, z, z, z};
+        a = u8x4_plus1024(v.x) - off;
+        b = u8x4_plus1024(v.y) - off;
       }
       const uint2 lo = __builtin_bit_cast(uint2, a), hi = __builtin_bit_cast(uint2, b);
       v = make_uint4(lo.x, lo.y, hi.x, hi.y);
@@ -580,8 +586,11 @@ __device__ __forceinline__ void ex_store_k(const ExtendParams& p, const ExSub& s
     if (clear) v = make_uint4(0, 0, 0, 0);
     dst[i * NEXT] = v;
     if constexpr (WF == TIERKV_WARM_REF_U8) {
-      if (lane % (DP / 8) == 0)
+      if (lane % (DP / 8) == 0) {
         t.kscale[at * EX_SUB + (lane + 64 * i) / (DP / 8)] = (zero || hot) ? 1.f : half_hi(st.meta[i]);
+        const uint32_t z = (zero || hot) ? 0u : st.meta[i] & 0xffffu;
+        dst[i * NEXT + DP / 8] = make_uint4(z | (z << 16), z, 0, 0);   // behind the row
+      }
     }
   }
   if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
@@ -762,14 +771,35 @@ __device__ __forceinline__ void ex_pace() {
   __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
 }
 
-// Logits of one key tile, S^T = K Q^T, unscaled.
-template <int DP, int TK>
-__device__ __forceinline__ void ex_logits(const ExTile<DP, TK>& t, const f16x8 (&q)[DP / 16], f32x16 (&s)[TK / 32]) {
+// The sum of a row's query, negated, in three fp16 pieces (the sum is below
+// 2^8, so what they miss is below 2^-26), by the lane's half 0.
+__device__ __forceinline__ f16x8 ex_sum_pieces(float qsum) {
+  asm volatile("" : "+v"(qsum));   // formed for each tile: kept over the loop they cost four registers, and it spilled
+  const float v = (threadIdx.x & 32) ? 0.f : -qsum;
+  const _Float16 a = _Float16(v), b = _Float16(v - float(a)), c = _Float16(v - float(a) - float(b));
+  return f16x8{a, b, c, 0, 0, 0, 0, 0};
+}
+
+// Logits of one key tile, S^T = K Q^T, unscaled; reference format: with the
+// zero points taken off, qsum is the sum of the row's query.
+template <int DP, int WF, int TK>
+__device__ __forceinline__ void ex_logits(const ExTile<DP, TK>& t, const f16x8 (&q)[DP / 16], float qsum,
+                                          f32x16 (&s)[TK / 32]) {
+  constexpr bool REF = WF == TIERKV_WARM_REF_U8;
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
 #pragma unroll
   for (int kt = 0; kt < TK / 32; ++kt) s[kt] = f32x16{};
   const uint4* const kb = t.k + ex_k_at<DP>(col, h);
+  f16x8 qz;
+  if constexpr (REF) qz = ex_sum_pieces(qsum);
   __builtin_amdgcn_sched_barrier(0);
+  if constexpr (REF) {
+#pragma unroll
+    for (int kt = 0; kt < TK / 32; ++kt) {
+      const f16x8 z = __builtin_bit_cast(f16x8, t.k[ex_k_at<DP>(kt * 32 + col, DP / 8)]);
+      s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(z, qz, s[kt], 0, 0, 0);
+    }
+  }
 #pragma unroll
   for (int kk = 0; kk < DP / 16; ++kk) {
 #pragma unroll
@@ -778,7 +808,7 @@ __device__ __forceinline__ void ex_logits(const ExTile<DP, TK>& t, const f16x8 (
       s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[kk], s[kt], 0, 0, 0);
     }
   }
-  ex_pace<DP / 16 * (TK / 32), 6>();
+  ex_pace<(DP / 16 + REF) * (TK / 32), 6>();
   __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -934,14 +964,18 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
       const int d = kk * 16 + half * 8;
       raw[kk] = (live && d < D) ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
     }
-    if constexpr (sizeof(QT) == 2 && !__is_same(QT, __half)) {
+    // bf16 rows become fp16, and the reference format needs their sum to fit it.
+    constexpr bool BF = !__is_same(QT, __half);
+    if constexpr (BF || WF == TIERKV_WARM_REF_U8) {
+      auto lo = [](uint32_t w) { return BF ? __uint_as_float(w << 16) : half_lo(w); };
+      auto hi = [](uint32_t w) { return BF ? __uint_as_float(w & 0xffff0000u) : half_hi(w); };
       float mx = 0.f;
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
         const uint32_t x[4] = {raw[kk].x, raw[kk].y, raw[kk].z, raw[kk].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(x[i] << 16)), fabsf(__uint_as_float(x[i] & 0xffff0000u))));
+          mx = fmaxf(mx, fmaxf(fabsf(lo(x[i])), fabsf(hi(x[i]))));
       }
       mx = fmaxf(mx, xor32_f(mx));
       // 2^-e with mx in [2^e, 2^(e + 1)), by the exponent bits; rows of
@@ -955,8 +989,8 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
         const uint32_t x[4] = {raw[kk].x, raw[kk].y, raw[kk].z, raw[kk].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          q[kk][2 * i] = _Float16(__uint_as_float(x[i] << 16) * inv);
-          q[kk][2 * i + 1] = _Float16(__uint_as_float(x[i] & 0xffff0000u) * inv);
+          q[kk][2 * i] = _Float16(lo(x[i]) * inv);
+          q[kk][2 * i + 1] = _Float16(hi(x[i]) * inv);
         }
       }
     } else {
@@ -967,6 +1001,14 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
   if (p.scale_log2 < 0.f) {
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) q[kk] = -q[kk];
+  }
+  float qsum = 0.f;
+  if constexpr (WF == TIERKV_WARM_REF_U8) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) qsum += float(q[kk][i]);
+    qsum += xor32_f(qsum);
   }
   ExAcc<DP> a;
 #pragma unroll
@@ -1059,7 +1101,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
     if (w < 4) {
       for (int at = lo; at < hi; at += 4, buf ^= 1) {
         f32x16 s[TK / 32];
-        if (!idle) ex_logits<DP, TK>(tiles[buf], q, s);
+        if (!idle) ex_logits<DP, WF, TK>(tiles[buf], q, qsum, s);
         __syncthreads();
         if (at + 4 < hi) {
           ex_store_k<DP, WF, TK>(p, sub[0], st[0], w, tiles[buf ^ 1]);
@@ -1074,7 +1116,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
       __syncthreads();
       for (int at = lo; at < hi; at += 4, buf ^= 1) {
         f32x16 s[TK / 32];
-        if (!idle) ex_logits<DP, TK>(tiles[buf], q, s);
+        if (!idle) ex_logits<DP, WF, TK>(tiles[buf], q, qsum, s);
         if (at + 4 < hi) {
           store_v(tiles[buf ^ 1], sub[0], st[0], w - 4, at + 8 <= full);
           find(at + 8);
@@ -1100,7 +1142,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
       held[1] = sub[WIDE ? 0 : 1];
       find(at + 2 * ROUND);
       f32x16 s[TK / 32];
-      ex_logits<DP, TK>(tiles[w], q, s);
+      ex_logits<DP, WF, TK>(tiles[w], q, qsum, s);
       int end[TK / 16] = {};
       if (!whole) ex_ends<TK>(list, at, hi, lim, end);
       ex_softmax<DP, WF, TK>(tiles[w], qscale, end, whole, s, a);

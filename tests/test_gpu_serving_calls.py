@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from oracle import serving
+from oracle import codec, serving
 from paged_tierkv_amd import kernels
 from paged_tierkv_amd.tierkv_hip import DecodeWorkspace
 
@@ -87,3 +87,39 @@ def test_a_bound_that_is_too_low_is_raised_when_errors_are_checked(device, monke
     call(s, device, "masked", max_tokens=9)
     with pytest.raises(RuntimeError, match="max_tokens"):
         call(s, device, "masked", max_tokens=8)
+
+
+def far_from_zero(s, rng, mean, dev):
+    """Keys of a cache in the reference format at ``mean`` +- ``dev`` in every
+    dim, HOT ones too: zero points of about -255 mean / (6 dev)."""
+    key = lambda a: (mean + dev * rng.standard_normal(a.shape)).astype(np.float16)   # noqa: E731
+    s["hot"] = (key(s["hot"][0]), s["hot"][1])
+    qk, ks, kz = codec.quantize_ref_u8(key(s["warm"][0]))
+    s["warm"], s["meta"] = (qk, s["warm"][1]), (ks, kz, *s["meta"][2:])
+    return kz
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("mean,dev", [(10, 0.2), (-30, 0.1), (100, 2.0), (100, 0.3)])
+@pytest.mark.parametrize("new,held,heads,kv,d", [([3, 5], [40, 33], 4, 2, 64), ([60, 3], [120, 40], 8, 1, 128),
+                                                 ([4], [20], 2, 1, 40)])
+def test_reference_format_keys_far_from_zero(device, new, held, heads, kv, d, mean, dev, dtype):
+    """|code - zero| well past 2048, where fp16 has no more whole numbers."""
+    rng = np.random.default_rng(int(abs(mean) + 10 * dev))
+    s = step(61, new, held, heads, kv, d, fmt="ref_u8", dtype=dtype, cold=0.1, warm=0.85)
+    assert np.abs(far_from_zero(s, rng, mean, dev).astype(np.float64)).max() > 1500
+    check(call(s, device, "masked"), s, "masked")
+
+
+@pytest.mark.parametrize("zero", [-65504.0, 65504.0, -40000.0, 255.0, 0.0])
+def test_reference_format_zero_points_over_their_whole_range(device, zero):
+    """code - zero past what fp16 holds; the logits are ordinary numbers."""
+    s = step(62, [40, 3], [90, 60], 4, 2, 64, fmt="ref_u8", cold=0, warm=0.8)
+    ks, kz, vs, vz = s["meta"]
+    scale = np.float16(2.0 ** -11 if abs(zero) > 1000 else 2.0 ** -7)
+    s["meta"] = (np.full_like(ks, scale), np.full_like(kz, zero), vs, vz)
+    mean = np.float16(-zero * float(scale))
+    s["hot"] = ((s["hot"][0].astype(np.float32) * 0.03 + mean).astype(np.float16), s["hot"][1])
+    out = call(s, device, "masked")
+    assert torch.isfinite(out.float()).all()
+    check(out, s, "masked")
