@@ -1450,7 +1450,8 @@ extern "C" int32_t tierkv_extend_attention(
   if (int64_t(num_rows) * groups > (int64_t(1) << 29))
     return fail(TIERKV_ERR_UNSUPPORTED, "more than 2^29 query rows per kv head");
   const ExLayout l = ex_layout(batch, num_rows, max_tokens, groups, num_kv_heads, num_blocks, block_size, head_dim);
-  if (int64_t(l.max_items) * num_kv_heads > 0x7fffffff) return fail(TIERKV_ERR_UNSUPPORTED, "grid too large");
+  // (a launch has fewer than 2^32 threads)
+  if (int64_t(l.max_items) * num_kv_heads > 0xffffffffll / EX_THREADS) return fail(TIERKV_ERR_UNSUPPORTED, "grid too large");
   if (workspace_bytes < l.total) return fail(TIERKV_ERR_WORKSPACE, "workspace too small");
   if (num_rows == 0 || max_tokens == 0) return TIERKV_OK;
   char* ws = reinterpret_cast<char*>(workspace);

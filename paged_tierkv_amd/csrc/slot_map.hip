@@ -464,8 +464,6 @@ extern "C" int32_t tierkv_write_slots(
   if (!key || !value || !slots || !hot_k || !hot_v) return fail(TIERKV_ERR_INVALID, "null pointer");
   if (k_stride_t < 0 || k_stride_h < 0 || v_stride_t < 0 || v_stride_h < 0)
     return fail(TIERKV_ERR_INVALID, "strides must be non-negative");
-  if (int64_t(num_rows) * num_kv_heads * head_dim > (int64_t(1) << 38))
-    return fail(TIERKV_ERR_UNSUPPORTED, "write too large for one call");
   WriteSlotsParams p{};
   p.src[0] = key;
   p.src[1] = value;
@@ -483,6 +481,9 @@ extern "C" int32_t tierkv_write_slots(
   p.hot[1] = reinterpret_cast<__half*>(hot_v);
   const bool wide = head_dim % 8 == 0 && ((k_stride_t | k_stride_h | v_stride_t | v_stride_h) & 7) == 0 &&
                     aligned16(key) && aligned16(value) && aligned16(hot_k) && aligned16(hot_v);
+  // One thread per vector or element, and fewer than 2^32 threads in a launch.
+  if (int64_t(num_rows) * num_kv_heads > (0xffffffffll - 255) / (wide ? head_dim / 8 : head_dim))
+    return fail(TIERKV_ERR_UNSUPPORTED, "write too large for one call");
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   if (dtype == TIERKV_DTYPE_BF16) launch_write<__hip_bfloat16>(p, wide, stream);
   else launch_write<__half>(p, wide, stream);
