@@ -42,7 +42,7 @@
 // query, so that it is off by a 32-bit rounding.  (code - zero in fp16 was off
 // by as much as the codes are where keys lie far from 0 against their spread,
 // mean 10 and deviation 0.2, and infinite past 65504.  2048 tokens on 32768 of
-// that format take 1197 us, with code - zero 1143, with the zero point taken
+// that format take 1178 us, with code - zero 1140, with the zero point taken
 // off each logit by vector instructions 1239 to 1369.)
 // V goes to LDS as fp16 of code * scale, one rounding of at most 2^-11 of the
 // value, as the probabilities have one when they become fp16 operands.
@@ -790,22 +790,21 @@ __device__ __forceinline__ void ex_logits(const ExTile<DP, TK>& t, const f16x8 (
 #pragma unroll
   for (int kt = 0; kt < TK / 32; ++kt) s[kt] = f32x16{};
   const uint4* const kb = t.k + ex_k_at<DP>(col, h);
-  f16x8 qz;
-  if constexpr (REF) qz = ex_sum_pieces(qsum);
   __builtin_amdgcn_sched_barrier(0);
-  if constexpr (REF) {
-#pragma unroll
-    for (int kt = 0; kt < TK / 32; ++kt) {
-      const f16x8 z = __builtin_bit_cast(f16x8, t.k[ex_k_at<DP>(kt * 32 + col, DP / 8)]);
-      s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(z, qz, s[kt], 0, 0, 0);
-    }
-  }
 #pragma unroll
   for (int kk = 0; kk < DP / 16; ++kk) {
 #pragma unroll
     for (int kt = 0; kt < TK / 32; ++kt) {
       const f16x8 k = __builtin_bit_cast(f16x8, kb[kt * 32 * (DP / 8 + 1) + kk * 2]);
       s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[kk], s[kt], 0, 0, 0);
+    }
+  }
+  if constexpr (REF) {
+    const f16x8 qz = ex_sum_pieces(qsum);
+#pragma unroll
+    for (int kt = 0; kt < TK / 32; ++kt) {
+      const f16x8 z = __builtin_bit_cast(f16x8, t.k[ex_k_at<DP>(kt * 32 + col, DP / 8)]);
+      s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(z, qz, s[kt], 0, 0, 0);
     }
   }
   ex_pace<(DP / 16 + REF) * (TK / 32), 6>();
