@@ -481,6 +481,8 @@ TIERKV_API int32_t tierkv_write_slots(
  *          written, and bit 4 of the error word is set (nothing is launched,
  *          and no bit set, when max_tokens or num_rows is 0)
  * head_dim a multiple of 8 up to 128, block_size up to 64, any GQA group.
+ * Probabilities and WARM values are rounded to fp16 once (WARM values past its
+ * range become infinite); logits, statistics and sums are 32-bit.
  * The same inputs give the same bits on every call.  workspace: as
  * tierkv_decode_attention's (one buffer may serve both, in stream order), at
  * least tierkv_extend_workspace_bytes(...) bytes, zero-filled before its

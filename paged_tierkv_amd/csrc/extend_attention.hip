@@ -45,14 +45,18 @@
 // that format take 1178 us, with code - zero 1140, with the zero point taken
 // off each logit by vector instructions 1239 to 1369.)
 // V goes to LDS as fp16 of code * scale, one rounding of at most 2^-11 of the
-// value, as the probabilities have one when they become fp16 operands.
+// value, as the probabilities have one when they become fp16 operands: the
+// matrix units take 16-bit operands at sixteen times the rate of 32-bit ones.
+// (Values past fp16's range become infinite, as the format's own
+// dequantization makes them, tierkv_policy.py:39-44.)
 // Probabilities carry a factor 2^6 so that small ones stay normal fp16.
 // bf16 queries become fp16 after division by a power of two near the row's
 // largest value, which the logits get back in 32 bits.
 //
 // Bound: the matrix products and the exponentials between them for wide tiles
-// (2048 tokens on 32768, 32 heads on 8 kv heads of 128: 988 us, 810 TFLOP/s of
-// the 1100 that a large library product reaches here; with tiles still cut in
+// (2048 tokens on 32768, 32 heads on 8 kv heads of 128: 977 us, 820 TFLOP/s of
+// the 1100 that a large library product reaches here, 8.5 other vector
+// instructions per product; with tiles still cut in
 // two, 1165, where 128-row tiles of four waves took 1297, eight waves in step
 // 1313 and one loop with branches for the two halves 1844); for narrow ones
 // the reads of the cache and a chain of plan, attention and merge (8 x 5

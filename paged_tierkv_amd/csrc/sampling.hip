@@ -38,9 +38,9 @@
 // with top-k 3.6 + 13.6; 16 x 128256 bf16 with top-p 4.8, -, 14.2, 14.8, 20.6;
 // 256 x 128256 fp32, limits of each row, 23.1 (5.7 TB/s), 19.5, 16.4, 20.9,
 // 29.7 (the later launches read a row again only where its limits need it).
-// Rows that fit none of these (a thousand equal logits at the border, k in
-// the thousands) take a radix select over the row by one workgroup (64 x
-// 128256 fp32 of whole numbers: 329 us with top-k 3000, 1020 with top-p 0.9).
+// Rows that fit none of these (a thousand equal logits at the border, k from
+// about a thousand on) take a radix select over the row by one workgroup (64 x
+// 128256 fp32 of whole numbers: 344 us with top-k 3000, 1019 with top-p 0.9).
 
 #include "tierkv_common.h"
 
@@ -1006,9 +1006,11 @@ static void sp_launch(const SampleParams& p, hipStream_t stream) {
 template <typename T>
 static void sp_dispatch(SampleParams& p, hipStream_t stream) {
   constexpr int VL = 16 / sizeof(T);
-  // Parts per row: as many as put 512 workgroups (two per CU) on the chip, and
-  // no more than eight vectors per thread, so that single rows of a large
-  // batch that need the later launches are not read by one or two workgroups.
+  // Parts per row, up to 16: as many as put 512 workgroups (two per CU) on the
+  // chip, and as give a thread no more than eight vectors (fp32 rows of up to
+  // 262144 tokens, 16-bit ones of 524288; longer rows up to 32), so that single
+  // rows of a large batch that need the later launches are not read by one or
+  // two workgroups.
   const int steps = (p.vocab + SP_THREADS * VL - 1) / (SP_THREADS * VL);
   const int want = std::min({steps, SP_PARTS, std::max((steps + 7) / 8, (512 + p.batch - 1) / p.batch)});
   p.steps = (steps + want - 1) / want;

@@ -39,7 +39,8 @@ constexpr int SM_NIT = SM_MAX_BATCH / SM_THREADS;
 //   64 x  1 x   16                   9.5   12.4
 //   64 x 60 x  256                  12.4   13.0
 //   64 x 16 x 1024                  14.1   14.4
-// and with a workgroup that took several passes beyond these limits:
+// (level at tables of 512 to 1024 blocks, half a microsecond either way:
+// 64 x 1 x 1024 14.4 and 13.9, 64 x 16 x 512 13.0 and 12.7), and with a workgroup that took several passes beyond these limits:
 //   64 x 700 x 16                   27.6   12.9
 //  256 x   1 x 64                   18.1   14.0
 constexpr int SM_ONE_BATCH = 64;
