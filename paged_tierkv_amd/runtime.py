@@ -538,7 +538,8 @@ class BatchedTieredKVRuntime:
         if ((B, kv, d) != (self.batch, self.kv_heads, self.head_dim)
                 or tuple(query_states.shape) != (B, self.kv_heads * groups, T, d)):
             raise ValueError("query or K/V geometry does not match the runtime.")
-        if query_states.dtype not in (torch.float16, torch.bfloat16) or value_states.dtype != key_states.dtype:
+        halves = (torch.float16, torch.bfloat16)   # (K/V of other types become fp16)
+        if query_states.dtype not in halves or (key_states.dtype in halves and value_states.dtype != key_states.dtype):
             raise ValueError("extend_layer takes an fp16 / bf16 query and K/V of one dtype.")
         if any(t.device != self.layers[layer].table.device for t in (query_states, key_states, value_states)):
             raise ValueError("query and K/V must be on the runtime's device.")
@@ -560,7 +561,7 @@ class BatchedTieredKVRuntime:
                                "(a call with policy_step, or tick_layer).")
         rows = lambda t: t.transpose(1, 2).reshape(B * T, t.shape[1], d)   # noqa: E731
         q, k, v = rows(query_states), rows(key_states), rows(value_states)
-        if k.dtype not in (torch.float16, torch.bfloat16):
+        if k.dtype not in halves:
             k, v = k.to(torch.float16), v.to(torch.float16)
         new = torch.full((B,), T, dtype=torch.int32, device=self.device)
         m = kernels.build_slot_map(new, st.table, st.states, st.lengths, st.nblocks, st.open, st.hot_free, st.ctl,

@@ -155,3 +155,14 @@ def test_geometry_that_the_attention_does_not_take_is_refused_at_once(device):
         with pytest.raises(ValueError, match="extend_tokens"):
             runtime(device, **kw)
     runtime(device, head_dim=256, extend_tokens=0)
+
+
+def test_keys_and_values_in_32_bits_become_fp16(device):
+    outs = []
+    for k_type, v_type in ((torch.float16,) * 2, (torch.float32,) * 2, (torch.float32, torch.float16)):
+        rt, x = runtime(device), rand(device, 5)
+        rt.prefill_layer(0, x(2, 100), x(2, 100))
+        q, k, v = x(4, 9), x(2, 9), x(2, 9)
+        outs.append(rt.extend_layer(0, q, k.to(k_type), v.to(v_type), 2, 0.125))
+        rt.check_errors()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
