@@ -47,7 +47,7 @@ extern "C" {
 
 #define TIERKV_DTYPE_F16 0
 #define TIERKV_DTYPE_BF16 1
-#define TIERKV_DTYPE_F32 2 /* logits of tierkv_sample_tokens only */
+#define TIERKV_DTYPE_F32 2 /* logits of tierkv_sample_tokens, norm weights, rows read back */
 
 #define TIERKV_WARM_REF_U8 0
 #define TIERKV_WARM_ABSMAX_I8 1
@@ -463,6 +463,77 @@ TIERKV_API int32_t tierkv_write_slots(
     const void* key, int64_t k_stride_t, int64_t k_stride_h, const void* value, int64_t v_stride_t, int64_t v_stride_h,
     int32_t dtype, const int32_t* slots, int32_t num_rows, void* hot_k, void* hot_v, int64_t hot_slots,
     int32_t num_kv_heads, int32_t block_size, int32_t head_dim, void* stream);
+
+/* Per-head norms and rotation by position of packed query and key rows, and
+ * the write of keys and values into HOT slots, in one pass.  Row r stands at
+ * positions[r] of its context (tierkv_build_slot_map gives them).  For each
+ * head of q (with q_weight) and of k (with k_weight; NULL: no norm)
+ *   x' = x * rsqrt(mean(x^2) + eps) * weight,
+ * then the pairs (a, b) of the first rotary_dim dims, (i, i + rotary_dim / 2)
+ * or (2 i, 2 i + 1) when interleaved, turn by the angle positions[r] * inv_freq[i]
+ * (formed in 64 bits) and are scaled by attention_scaling; the other dims pass.
+ *   q  [num_rows, num_heads, head_dim], k / v [num_rows, num_kv_heads, head_dim],
+ *      fp16 or bf16, element strides, head_dim contiguous; weights [head_dim],
+ *      in that dtype or fp32; inv_freq fp32 [rotary_dim / 2], rotary_dim even
+ *   q_out, k_out  contiguous rows of the same dtype (k_out may be NULL where
+ *      the keys go to pools); they do not overlap the inputs
+ *   slots NULL (then value and pools are NULL), or the pool row slot *
+ *      block_size + position of each row: k rotated and v as it is are written
+ *      there in fp16, as tierkv_write_slots does; negative and outside ones
+ *      are skipped, those written are distinct
+ * Rows whose position is negative are left out: nothing of them is written.
+ * 32-bit arithmetic, one rounding.  apply_rotary_pos_emb and write_hot_tokens
+ * (modeling_llama.py:376-377, tierkv_policy.py:934-967) by rows; the norms
+ * have no counterpart in the reference.  head_dim up to 256. */
+TIERKV_API int32_t tierkv_rotate_rows(
+    const void* query, int64_t q_stride_t, int64_t q_stride_h, void* q_out,
+    const void* key, int64_t k_stride_t, int64_t k_stride_h, void* k_out,
+    const void* value, int64_t v_stride_t, int64_t v_stride_h, int32_t dtype,
+    const int32_t* positions, int32_t num_rows,
+    const float* inv_freq, int32_t rotary_dim, int32_t interleaved, float attention_scaling,
+    const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+    const int32_t* slots, void* hot_k, void* hot_v, int64_t hot_slots,
+    int32_t num_heads, int32_t num_kv_heads, int32_t block_size, int32_t head_dim, void* stream);
+
+/* Packed K/V rows quantized into WARM slots as a step writes them: row r of
+ * key / value (as tierkv_write_slots takes them; bf16 rows become fp16 first)
+ * becomes row slots[r] = slot * block_size + position of warm_k / warm_v.
+ * Rows whose slot is negative or outside the pool are skipped; slots that are
+ * written are distinct.
+ *   REF_U8: each (row, head) by itself, the codes, scale and zero point of
+ *     tierkv_demote_to_warm.
+ *   ABSMAX_I8: a block's rows are consecutive in the call.  With p the lowest
+ *     position written of a block and s its scale (0 where p = 0, a block that
+ *     starts anew), the scale becomes s' = max(|s|, max|x| / 127) of the rows
+ *     written; the rows before p, which the block holds, become rint(code * s /
+ *     s') and those written rint(x / s').  Every other row of the block holds
+ *     nothing afterwards.
+ * write_warm_block (tierkv_policy.py:969-1002) by rows.  head_dim up to 256. */
+TIERKV_API int32_t tierkv_quantize_rows(
+    const void* key, int64_t k_stride_t, int64_t k_stride_h, const void* value, int64_t v_stride_t, int64_t v_stride_h,
+    int32_t dtype, const int32_t* slots, int32_t num_rows,
+    void* warm_k, void* warm_v, int64_t warm_slots,
+    void* k_scale, void* k_zero, void* v_scale, void* v_zero, int32_t warm_format,
+    int32_t num_kv_heads, int32_t block_size, int32_t head_dim, void* stream);
+
+/* Tokens of a tiered cache read back as packed rows.  Request b's rows
+ * [cu_tokens[b], cu_tokens[b + 1]) of out_k / out_v [num_rows, num_kv_heads,
+ * head_dim] (fp16, bf16 or fp32) become its tokens of ordinal start[b] (0 when
+ * negative), start[b] + 1, ... over the valid tokens of its blocks: HOT as
+ * they are, WARM as code * scale (ABSMAX_I8) or (code - zero) * scale (REF_U8)
+ * in 32 bits, rounded once; tokens of evicted blocks, of blocks whose slot is
+ * out of range, and past what the request holds are 0.  Rows of no request
+ * are not written.  reconstruct_layer (tierkv_policy.py:1818-1841) for a
+ * batch.  head_dim up to 256, block_size up to 64, batch up to 65535. */
+TIERKV_API int32_t tierkv_read_rows(
+    const int32_t* start, const int32_t* cu_tokens, int32_t num_rows,
+    const int32_t* block_table, const int32_t* block_states, const int32_t* block_lengths, int64_t table_stride,
+    const int32_t* seq_num_blocks, int32_t num_blocks,
+    const void* hot_k, const void* hot_v, int64_t hot_slots,
+    const void* warm_k, const void* warm_v, int64_t warm_slots,
+    const void* k_scale, const void* k_zero, const void* v_scale, const void* v_zero, int32_t warm_format,
+    void* out_k, void* out_v, int32_t out_dtype,
+    int32_t batch, int32_t num_kv_heads, int32_t block_size, int32_t head_dim, void* stream);
 
 /* Attention of several query tokens per request over the tiered cache.
  * Request b's query rows [cu_tokens[b], cu_tokens[b + 1]) are the last n_b of

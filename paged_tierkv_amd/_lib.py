@@ -163,6 +163,25 @@ SIGNATURES = {
         _P, c_int64, c_int64, _P, c_int64, c_int64,
         c_int32, _P, c_int32, _P, _P, c_int64,
         c_int32, c_int32, c_int32, _P]),
+    "tierkv_rotate_rows": (c_int32, [
+        _P, c_int64, c_int64, _P, _P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int32,
+        _P, c_int32, _P, c_int32, c_int32, c_float,
+        _P, _P, c_int32, c_float,
+        _P, _P, _P, c_int64,
+        c_int32, c_int32, c_int32, c_int32, _P]),
+    "tierkv_quantize_rows": (c_int32, [
+        _P, c_int64, c_int64, _P, c_int64, c_int64,
+        c_int32, _P, c_int32, _P, _P, c_int64,
+        _P, _P, _P, _P, c_int32,
+        c_int32, c_int32, c_int32, _P]),
+    "tierkv_read_rows": (c_int32, [
+        _P, _P, c_int32,
+        _P, _P, _P, c_int64, _P, c_int32,
+        _P, _P, c_int64,
+        _P, _P, c_int64,
+        _P, _P, _P, _P, c_int32,
+        _P, _P, c_int32,
+        c_int32, c_int32, c_int32, c_int32, _P]),
     "tierkv_extend_workspace_bytes": (c_int64, [c_int32] * 8),
     "tierkv_extend_attention": (c_int32, [
         _P, c_int64, c_int64, c_int32, _P,

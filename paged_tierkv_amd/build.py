@@ -57,6 +57,8 @@ HIP_SOURCES = {
     # tier branches of its tile loader as in the decode kernel.
     "extend_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-simplifycfg-sink-common=false"],
     "slot_map.hip": [],
+    "rotate.hip": [],
+    "read_rows.hip": [],
     # Weights are whole numbers that follow from one product and one rounding.
     "sampling.hip": ["-ffp-contract=off"],
 }

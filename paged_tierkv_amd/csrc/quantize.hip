@@ -788,6 +788,124 @@ int32_t launch_promote(const DequantJobs& q, int n_grid, hipStream_t stream) {
   return check_launch("promote_wave_kernel");
 }
 
+// ---------------------------------------------------------------------------
+// Packed rows quantized as a step writes them (tierkv_quantize_rows): row r of
+// k / v [rows, kv_heads, D] becomes row slots[r] = slot * bs + position of the
+// WARM pools.  bf16 rows become fp16 first, as where they are written HOT.
+// ---------------------------------------------------------------------------
+struct QuantRows {
+  const void* src[2];
+  int64_t st_t[2], st_h[2];
+  const int32_t* slots;
+  int32_t rows, kv_heads, bs, D;
+  int64_t pool_rows;      // warm_slots * block_size
+  uint8_t* warm[2];
+  void* scale[2];
+  void* zero[2];
+};
+
+template <typename T>
+__device__ __forceinline__ float qr_value(const QuantRows& q, int kv, int64_t r, int h, int d) {
+  const float x = to_f32<T>(reinterpret_cast<const T*>(q.src[kv])[r * q.st_t[kv] + h * q.st_h[kv] + d]);
+  return r16(x);
+}
+
+// The block that a packed row goes to, -1 for none.
+__device__ __forceinline__ int qr_block(const QuantRows& q, int64_t r) {
+  const int x = q.slots[r];
+  return x < 0 || x >= q.pool_rows ? -1 : x / q.bs;
+}
+
+// REF_U8, any layout: a 16-lane group per (row, head) of K or V.
+template <typename T>
+__global__ __launch_bounds__(QT) void quantize_rows_ref_kernel(QuantRows q) {
+  const int sub = threadIdx.x & 15, kv = blockIdx.y;
+  const int64_t x = (int64_t(blockIdx.x) * QT + threadIdx.x) >> 4;
+  const int64_t r = x / q.kv_heads;
+  const int h = int(x - r * q.kv_heads);
+  const int at = r < q.rows ? q.slots[r] : -1;
+  const bool ok = at >= 0 && at < q.pool_rows;
+  float mn = INFINITY, mx = -INFINITY;
+  if (ok) {
+    for (int d = sub; d < q.D; d += 16) {
+      const float v = qr_value<T>(q, kv, r, h, d);
+      mn = fminf(mn, v);
+      mx = fmaxf(mx, v);
+    }
+  }
+#pragma unroll
+  for (int m = 8; m >= 1; m >>= 1) {
+    mn = fminf(mn, __shfl_xor(mn, m, 16));
+    mx = fmaxf(mx, __shfl_xor(mx, m, 16));
+  }
+  if (!ok) return;
+  const int64_t row = (int64_t(at / q.bs) * q.kv_heads + h) * q.bs + at % q.bs;
+  float sc = r16(__fdiv_rn(r16(mx - mn), 255.f));
+  if (sc == 0.f) sc = 1.f;
+  const float zp = r16(-rintf(r16(__fdiv_rn(mn, sc))));
+  for (int d = sub; d < q.D; d += 16) {
+    const float t = rintf(r16(__fdiv_rn(qr_value<T>(q, kv, r, h, d), sc)));
+    q.warm[kv][row * q.D + d] = static_cast<uint8_t>(fminf(fmaxf(r16(t + zp), 0.f), 255.f));
+  }
+  if (sub == 0) {
+    reinterpret_cast<__half*>(q.scale[kv])[row] = __float2half_rn(sc);
+    reinterpret_cast<__half*>(q.zero[kv])[row] = __float2half_rn(zp);
+  }
+}
+
+// ABSMAX_I8, any layout: a wave per (row, head) of K or V, of which those of a
+// run's first row work.  A run is consecutive packed rows of one block, from
+// its lowest position p on: the block's scale becomes max(|scale|, max|x| / 127)
+// (the run's own where p = 0), the codes of the p rows before it become those
+// of the values that they stood for, and the run's rows are quantized.
+template <typename T>
+__global__ __launch_bounds__(QT) void quantize_rows_absmax_kernel(QuantRows q) {
+  const int lane = threadIdx.x & 63, kv = blockIdx.y;
+  const int64_t x = int64_t(blockIdx.x) * (QT / 64) + (threadIdx.x >> 6);
+  const int64_t r0 = x / q.kv_heads;
+  if (r0 >= q.rows) return;
+  const int h = int(x - r0 * q.kv_heads);
+  const int block = qr_block(q, r0);
+  if (block < 0 || (r0 > 0 && qr_block(q, r0 - 1) == block)) return;
+  // The run's rows, one per lane (a block holds 64 at most).
+  const bool mine = r0 + lane < q.rows && qr_block(q, r0 + lane) == block;
+  const uint64_t others = ~__ballot(mine);
+  const int n = others ? __ffsll((unsigned long long)others) - 1 : 64;
+  const int pos = lane < n ? q.slots[r0 + lane] - block * q.bs : 64;
+  int first = pos;
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) first = min(first, __shfl_xor(first, m, 64));
+  float amax = 0.f;
+  for (int i = 0; i < n; ++i)
+    for (int d = lane; d < q.D; d += 64) amax = fmaxf(amax, fabsf(qr_value<T>(q, kv, r0 + i, h, d)));
+  amax = wave_max(amax);
+  float* scale = reinterpret_cast<float*>(q.scale[kv]) + int64_t(block) * q.kv_heads + h;
+  uint8_t* codes = q.warm[kv] + (int64_t(block) * q.kv_heads + h) * q.bs * q.D;
+  const float old = first > 0 ? *scale : 0.f;
+  const float s = fmaxf(fabsf(old), __fdiv_rn(amax, 127.f));
+  auto code = [&](float v) {
+    return s != 0.f ? uint8_t(int8_t(int(fminf(fmaxf(rintf(__fdiv_rn(v, s)), -127.f), 127.f)))) : uint8_t(0);
+  };
+  if (first > 0 && s != old)
+    for (int e = lane; e < first * q.D; e += 64) codes[e] = code(float(int8_t(codes[e])) * old);
+  for (int i = 0; i < n; ++i) {
+    const int p = __shfl(pos, i, 64);
+    for (int d = lane; d < q.D; d += 64) codes[p * q.D + d] = code(qr_value<T>(q, kv, r0 + i, h, d));
+  }
+  if (lane == 0) *scale = s;
+}
+
+template <typename T>
+static void launch_quantize_rows(const QuantRows& q, int32_t warm_format, hipStream_t stream) {
+  const int64_t tiles = int64_t(q.rows) * q.kv_heads;
+  if (warm_format == TIERKV_WARM_ABSMAX_I8)
+    hipLaunchKernelGGL(quantize_rows_absmax_kernel<T>, dim3(uint32_t((tiles + QT / 64 - 1) / (QT / 64)), 2), dim3(QT), 0,
+                       stream, q);
+  else
+    hipLaunchKernelGGL(quantize_rows_ref_kernel<T>, dim3(uint32_t((tiles + QT / 16 - 1) / (QT / 16)), 2), dim3(QT), 0,
+                       stream, q);
+}
+
 }  // namespace tierkv
 
 using namespace tierkv;
@@ -918,4 +1036,55 @@ extern "C" int32_t tierkv_promote_to_hot(
   q.D = head_dim;
   q.warm_format = warm_format;
   return launch_promote(q, n, stream);
+}
+
+extern "C" int32_t tierkv_quantize_rows(
+    const void* key, int64_t k_stride_t, int64_t k_stride_h, const void* value, int64_t v_stride_t, int64_t v_stride_h,
+    int32_t dtype, const int32_t* slots, int32_t num_rows,
+    void* warm_k, void* warm_v, int64_t warm_slots,
+    void* k_scale, void* k_zero, void* v_scale, void* v_zero, int32_t warm_format,
+    int32_t num_kv_heads, int32_t block_size, int32_t head_dim, void* stream_) {
+  clear_error();
+  if (num_rows < 0) return fail(TIERKV_ERR_INVALID, "negative row count");
+  if (dtype != TIERKV_DTYPE_F16 && dtype != TIERKV_DTYPE_BF16)
+    return fail(TIERKV_ERR_INVALID, "K/V rows must be fp16 or bf16");
+  if (warm_format != TIERKV_WARM_REF_U8 && warm_format != TIERKV_WARM_ABSMAX_I8)
+    return fail(TIERKV_ERR_INVALID, "unknown warm format");
+  if (num_kv_heads <= 0 || num_kv_heads > 65536 || block_size <= 0 || block_size > 64 || head_dim <= 0 || head_dim > 256)
+    return fail(TIERKV_ERR_UNSUPPORTED, "1 to 65536 heads, block_size in [1, 64] and head_dim in [1, 256]");
+  if (warm_slots <= 0 || warm_slots * block_size > 0x7fffffff)
+    return fail(TIERKV_ERR_UNSUPPORTED, "pool rows must lie in (0, 2^31)");
+  if (num_rows == 0) return TIERKV_OK;
+  if (!key || !value || !slots || !warm_k || !warm_v || !k_scale || !v_scale)
+    return fail(TIERKV_ERR_INVALID, "null pointer");
+  if (warm_format == TIERKV_WARM_REF_U8 && (!k_zero || !v_zero))
+    return fail(TIERKV_ERR_INVALID, "reference format needs zero-point pools");
+  if (k_stride_t < 0 || k_stride_h < 0 || v_stride_t < 0 || v_stride_h < 0)
+    return fail(TIERKV_ERR_INVALID, "strides must be non-negative");
+  // A wave per (row, head) at most, and fewer than 2^32 threads in a launch's dimension.
+  if (int64_t(num_rows) * num_kv_heads > (0xffffffffll - QT) / 64)
+    return fail(TIERKV_ERR_UNSUPPORTED, "write too large for one call");
+  QuantRows q{};
+  q.src[0] = key;
+  q.src[1] = value;
+  q.st_t[0] = k_stride_t;
+  q.st_h[0] = k_stride_h;
+  q.st_t[1] = v_stride_t;
+  q.st_h[1] = v_stride_h;
+  q.slots = slots;
+  q.rows = num_rows;
+  q.kv_heads = num_kv_heads;
+  q.bs = block_size;
+  q.D = head_dim;
+  q.pool_rows = warm_slots * block_size;
+  q.warm[0] = reinterpret_cast<uint8_t*>(warm_k);
+  q.warm[1] = reinterpret_cast<uint8_t*>(warm_v);
+  q.scale[0] = k_scale;
+  q.scale[1] = v_scale;
+  q.zero[0] = k_zero;
+  q.zero[1] = v_zero;
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  if (dtype == TIERKV_DTYPE_BF16) launch_quantize_rows<__hip_bfloat16>(q, warm_format, stream);
+  else launch_quantize_rows<__half>(q, warm_format, stream);
+  return check_launch("tierkv_quantize_rows");
 }

@@ -1,6 +1,7 @@
 """Python entry points of the demotion, promotion, block-score and label
-kernels, and of a serving step's slot map, K/V row write and token choice (C
-ABI in include/tierkv_hip.h).
+kernels, and of a serving step's slot map, norm and rotation of rows, K/V row
+writes (HOT and quantized), rows read back and token choice (C ABI in
+include/tierkv_hip.h).
 
 All tensors are GPU tensors; index arrays are int32.  Launches are
 asynchronous on the current stream.
@@ -355,6 +356,213 @@ def write_slots(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, hot
                     _lib.DTYPE_BF16 if k.dtype == torch.bfloat16 else _lib.DTYPE_F16, ptr(slots), rows, ptr(hot_k),
                     ptr(hot_v), hot_k.shape[0], kv_heads, bs, dim)
     _lib.check(rc, "tierkv_write_slots")
+
+
+_HALVES = (torch.float16, torch.bfloat16)
+
+
+def _packed_rows(t, name: str, rows: int, heads: int, dim: int, dtype, index: int):
+    """Packed rows [rows, heads, dim] with the last dim contiguous (copied
+    where it is not)."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != (rows, heads, dim):
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] of the step's geometry and the rows' dtype.")
+    if t.get_device() != index:
+        raise ValueError("rows, tables and pools must be on one device.")
+    return t if t.stride(2) == 1 or dim == 1 else t.contiguous()
+
+
+def _out_rows(t, name: str, shape, dtype, device):
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be a contiguous tensor of the rows' shape, dtype and device.")
+    return t
+
+
+def _warm_pools(warm_k, warm_v, k_scale, k_zero, v_scale, v_zero, fmt: int, index: int) -> None:
+    """Check WARM pools and their metadata (``fmt``: WARM_FORMATS' value)."""
+    dtype = torch.uint8 if fmt == _lib.WARM_REF_U8 else torch.int8
+    _check_tiles(warm_k, "warm_k", dtype)
+    _check_tiles(warm_v, "warm_v", dtype)
+    if warm_v.shape != warm_k.shape:
+        raise ValueError("K and V pools must have identical shapes.")
+    slots, kv_heads, bs, _ = warm_k.shape
+    ref = fmt == _lib.WARM_REF_U8
+    metas = (k_scale, k_zero, v_scale, v_zero) if ref else (k_scale, v_scale)
+    if any(t is None for t in metas):
+        raise ValueError("WARM pools need their scales, reference-format ones their zero points.")
+    for t in metas:
+        _lib.require_gpu_tensor(t, "warm metadata")
+        if (t.dtype != (torch.float16 if ref else torch.float32) or not t.is_contiguous()
+                or t.numel() != slots * kv_heads * (bs if ref else 1)):
+            raise ValueError("WARM metadata must be contiguous: fp16 per token and head (ref_u8), fp32 per slot and "
+                             "head (absmax_i8).")
+    if any(t.get_device() != index for t in (warm_k, warm_v, *metas)):
+        raise ValueError("rows, tables and pools must be on one device.")
+
+
+def rotate_rows(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
+                q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                attention_scaling: float = 1.0, interleaved: bool = False, value: torch.Tensor | None = None,
+                slots: torch.Tensor | None = None, hot_k: torch.Tensor | None = None,
+                hot_v: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                k_out: torch.Tensor | None = None):
+    """Per-head norms and rotation by position of a step's packed rows
+    (``tierkv_rotate_rows``): ``query`` ``[N, H, D]``, ``key`` ``[N, kv_heads,
+    D]`` (fp16 / bf16, any strides with head_dim contiguous, e.g. columns of a
+    fused projection), ``positions`` int32 ``[N]`` (``build_slot_map``; rows of
+    negative ones are left out), ``inv_freq`` fp32 ``[rotary_dim / 2]``.  Where a
+    weight ``[head_dim]`` is given (the rows' dtype or fp32), the heads become
+    ``x * rsqrt(mean(x^2) + eps) * weight`` first; the first ``rotary_dim`` dims
+    turn in pairs ``(i, i + rotary_dim / 2)``, ``interleaved``: ``(2 i, 2 i + 1)``,
+    by angles formed in 64 bits, and are scaled by ``attention_scaling``.  With
+    ``value``, ``slots`` and the HOT pools, keys and values go there as
+    ``write_slots`` puts them.  Returns ``(q_out, k_out)``: contiguous rows (the
+    tensors given, which must not overlap the inputs, or new ones), ``k_out``
+    None where the keys go to pools and none is given.  Rows that are left out
+    are not written."""
+    lib = _lib.lib()
+    _lib.require_gpu_tensor(query, "query")
+    _lib.require_gpu_tensor(key, "key")
+    if query.ndim != 3 or key.ndim != 3 or query.dtype not in _HALVES:
+        raise ValueError("query and key must be fp16 / bf16 [tokens, heads, head_dim].")
+    rows, heads, dim = query.shape
+    kv_heads = key.shape[1]
+    index, device, dtype = query.get_device(), query.device, query.dtype
+    q = _packed_rows(query, "query", rows, heads, dim, dtype, index)
+    k = _packed_rows(key, "key", rows, kv_heads, dim, dtype, index)
+    _require_i32(positions, "positions", (rows,))
+    _lib.require_gpu_tensor(inv_freq, "inv_freq")
+    if inv_freq.dtype != torch.float32 or inv_freq.ndim != 1 or not inv_freq.is_contiguous() or 2 * len(inv_freq) > dim:
+        raise ValueError("inv_freq must be contiguous fp32 [rotary_dim / 2], rotary_dim at most head_dim.")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        _lib.require_gpu_tensor(w, "norm weight")
+        if (w.dtype not in (dtype, torch.float32) or w.dtype != weights[0].dtype or tuple(w.shape) != (dim,)
+                or not w.is_contiguous()):
+            raise ValueError("norm weights must be contiguous [head_dim] tensors of the rows' dtype or fp32, both alike.")
+    given = [t is not None for t in (value, slots, hot_k, hot_v)]
+    if any(given) != all(given):
+        raise ValueError("value, slots, hot_k and hot_v go together.")
+    bs, pool, v, vt, vh = 1, 0, None, 0, 0
+    if slots is not None:
+        _check_tiles(hot_k, "hot_k", torch.float16)
+        _check_tiles(hot_v, "hot_v", torch.float16)
+        if hot_v.shape != hot_k.shape or (hot_k.shape[1], hot_k.shape[3]) != (kv_heads, dim):
+            raise ValueError("K and V pools must have identical shapes, of the rows' geometry.")
+        pool, bs = hot_k.shape[0], hot_k.shape[2]
+        _require_i32(slots, "slots", (rows,))
+        v = _packed_rows(value, "value", rows, kv_heads, dim, dtype, index)
+        vt, vh, _ = v.stride()
+    on = (positions, inv_freq, *weights, *((slots, hot_k, hot_v) if slots is not None else ()))
+    if any(t.get_device() != index for t in on):
+        raise ValueError("rows, tables and pools must be on one device.")
+    q_out = _out_rows(q_out, "q_out", (rows, heads, dim), dtype, device)
+    if k_out is not None or slots is None:
+        k_out = _out_rows(k_out, "k_out", (rows, kv_heads, dim), dtype, device)
+    code = _lib.DTYPE_BF16 if dtype == torch.bfloat16 else _lib.DTYPE_F16
+    ptr = _lib.ptr
+    rc = _on_device(device, lib.tierkv_rotate_rows, ptr(q), q.stride(0), q.stride(1), ptr(q_out), ptr(k), k.stride(0),
+                    k.stride(1), ptr(k_out), ptr(v), vt, vh, code, ptr(positions), rows, ptr(inv_freq),
+                    2 * len(inv_freq), int(bool(interleaved)), float(attention_scaling), ptr(q_weight), ptr(k_weight),
+                    _lib.DTYPE_F32 if weights and weights[0].dtype == torch.float32 else code, float(eps), ptr(slots),
+                    ptr(hot_k), ptr(hot_v), pool, heads, kv_heads, bs, dim)
+    _lib.check(rc, "tierkv_rotate_rows")
+    return q_out, k_out
+
+
+def quantize_rows(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, warm_k: torch.Tensor,
+                  warm_v: torch.Tensor, k_scale: torch.Tensor, k_zero: torch.Tensor | None, v_scale: torch.Tensor,
+                  v_zero: torch.Tensor | None, warm_format: str = "ref_u8") -> None:
+    """Quantize packed K/V rows ``[N, kv_heads, head_dim]`` (as ``write_slots``
+    takes them) into the WARM pool rows ``slots`` (slot * block_size +
+    position; negative: skipped), as a step writes them
+    (``tierkv_quantize_rows``).  ``ref_u8``: each row and head by itself, as
+    ``demote_to_warm`` does.  ``absmax_i8``: a block's rows are consecutive in
+    the call; the block's scale grows where they ask for it, and the rows that
+    it holds before them are brought to the new scale."""
+    lib = _lib.lib()
+    if warm_format not in WARM_FORMATS:
+        raise ValueError('warm_format must be "absmax_i8" or "ref_u8".')
+    fmt = WARM_FORMATS[warm_format]
+    _lib.require_gpu_tensor(key, "key")
+    _lib.require_gpu_tensor(value, "value")
+    _lib.require_gpu_tensor(slots, "slots")
+    index = key.get_device()
+    _warm_pools(warm_k, warm_v, k_scale, k_zero, v_scale, v_zero, fmt, index)
+    pool, kv_heads, bs, dim = warm_k.shape
+    if key.ndim != 3 or key.dtype not in _HALVES:
+        raise ValueError("key and value must be fp16 / bf16 [tokens, kv_heads, head_dim].")
+    rows = key.shape[0]
+    k = _packed_rows(key, "key", rows, kv_heads, dim, key.dtype, index)
+    v = _packed_rows(value, "value", rows, kv_heads, dim, key.dtype, index)
+    _require_i32(slots, "slots", (rows,))
+    if slots.get_device() != index:
+        raise ValueError("rows, tables and pools must be on one device.")
+    if rows == 0:
+        return
+    ptr, ref = _lib.ptr, fmt == _lib.WARM_REF_U8
+    rc = _on_device(key.device, lib.tierkv_quantize_rows, ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0),
+                    v.stride(1), _lib.DTYPE_BF16 if k.dtype == torch.bfloat16 else _lib.DTYPE_F16, ptr(slots), rows,
+                    ptr(warm_k), ptr(warm_v), pool, ptr(k_scale), ptr(k_zero) if ref else None, ptr(v_scale),
+                    ptr(v_zero) if ref else None, fmt, kv_heads, bs, dim)
+    _lib.check(rc, "tierkv_quantize_rows")
+
+
+def read_rows(start: torch.Tensor, cu_tokens: torch.Tensor, num_tokens: int, block_table: torch.Tensor,
+              block_states: torch.Tensor, block_lengths: torch.Tensor, seq_num_blocks: torch.Tensor | None,
+              hot_k: torch.Tensor, hot_v: torch.Tensor, warm_k: torch.Tensor, warm_v: torch.Tensor,
+              k_scale: torch.Tensor, k_zero: torch.Tensor | None, v_scale: torch.Tensor, v_zero: torch.Tensor | None,
+              dtype: torch.dtype = torch.float16, out=None):
+    """Tokens of a tiered cache as packed rows (``tierkv_read_rows``): rows
+    ``cu_tokens[b]`` to ``cu_tokens[b + 1]`` (int32 ``[B + 1]``) are request b's
+    tokens from ordinal ``start[b]`` (int32 ``[B]``) on, in order; evicted ones
+    and those past what the request holds are 0.  Tables are ``[B,
+    max_blocks]``, pools and metadata those of ``tierkv_extend_attention``.
+    Returns K and V ``[num_tokens, kv_heads, head_dim]`` of ``dtype`` (fp16, bf16
+    or fp32; ``out``: a pair to write into).  Rows of no request are not
+    written."""
+    lib = _lib.lib()
+    _lib.require_gpu_tensor(block_table, "block_table")
+    if block_table.ndim != 2:
+        raise ValueError("block_table must be [batch, max_blocks].")
+    shape = block_table.shape
+    batch, stride = shape
+    index, device = block_table.get_device(), block_table.device
+    ints = [("block_table", block_table, shape), ("block_states", block_states, shape),
+            ("block_lengths", block_lengths, shape), ("start", start, shape[:1]), ("cu_tokens", cu_tokens, (batch + 1,))]
+    if seq_num_blocks is not None:
+        ints.append(("seq_num_blocks", seq_num_blocks, shape[:1]))
+    for name, t, want in ints:
+        _require_i32(t, name, want)
+        if t.get_device() != index:
+            raise ValueError("rows, tables and pools must be on one device.")
+    if dtype not in _LOGIT_DTYPES:
+        raise ValueError("dtype must be fp16, bf16 or fp32.")
+    rows = int(num_tokens)
+    if rows < 0:
+        raise ValueError("num_tokens must not be negative.")
+    _check_tiles(hot_k, "hot_k", torch.float16)
+    _check_tiles(hot_v, "hot_v", torch.float16)
+    _lib.require_gpu_tensor(warm_k, "warm_k")
+    fmt = _lib.WARM_ABSMAX_I8 if warm_k.dtype == torch.int8 else _lib.WARM_REF_U8
+    _warm_pools(warm_k, warm_v, k_scale, k_zero, v_scale, v_zero, fmt, index)
+    if hot_v.shape != hot_k.shape or warm_k.shape[1:] != hot_k.shape[1:]:
+        raise ValueError("HOT and WARM pools must have one geometry.")
+    if hot_k.get_device() != index or hot_v.get_device() != index:
+        raise ValueError("rows, tables and pools must be on one device.")
+    kv_heads, bs, dim = hot_k.shape[1:]
+    k_rows, v_rows = (None, None) if out is None else out
+    k_rows = _out_rows(k_rows, "out", (rows, kv_heads, dim), dtype, device)
+    v_rows = _out_rows(v_rows, "out", (rows, kv_heads, dim), dtype, device)
+    ptr, ref = _lib.ptr, fmt == _lib.WARM_REF_U8
+    rc = _on_device(device, lib.tierkv_read_rows, ptr(start), ptr(cu_tokens), rows, ptr(block_table), ptr(block_states),
+                    ptr(block_lengths), stride, ptr(seq_num_blocks), stride, ptr(hot_k), ptr(hot_v), hot_k.shape[0],
+                    ptr(warm_k), ptr(warm_v), warm_k.shape[0], ptr(k_scale), ptr(k_zero) if ref else None, ptr(v_scale),
+                    ptr(v_zero) if ref else None, fmt, ptr(k_rows), ptr(v_rows), _LOGIT_DTYPES[dtype], batch, kv_heads,
+                    bs, dim)
+    _lib.check(rc, "tierkv_read_rows")
+    return k_rows, v_rows
 
 
 SAMPLE_MAX_VOCAB = 1 << 20   # tierkv_sample_tokens

@@ -1,0 +1,98 @@
+"""What the entry points of rotated, quantized and read-back rows refuse,
+before any launch (CPU)."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from paged_tierkv_amd import _lib, kernels
+
+P = 4096        # a non-null, aligned address that no refused call touches
+
+
+def rotate(**kw):
+    a = dict(q=P, qt=512, qh=64, qo=P, k=P, kt=128, kh=64, ko=None, v=P, vt=128, vh=64, dtype=0, pos=P, rows=4, freq=P,
+             rot=64, pairs=0, amp=1.0, qw=None, kw=None, wt=0, eps=1e-6, slots=P, hk=P, hv=P, pool=8, heads=8, kv=2, bs=16,
+             d=64)
+    a.update(kw)
+    f = ctypes.c_float
+    return _lib.lib().tierkv_rotate_rows(
+        a["q"], a["qt"], a["qh"], a["qo"], a["k"], a["kt"], a["kh"], a["ko"], a["v"], a["vt"], a["vh"], a["dtype"], a["pos"],
+        a["rows"], a["freq"], a["rot"], a["pairs"], f(a["amp"]), a["qw"], a["kw"], a["wt"], f(a["eps"]), a["slots"], a["hk"],
+        a["hv"], a["pool"], a["heads"], a["kv"], a["bs"], a["d"], None)
+
+
+NO_POOLS = dict(v=None, slots=None, hk=None, hv=None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(q=None), 1), (dict(qo=None), 1), (dict(k=None), 1), (dict(pos=None), 1), (dict(freq=None), 1), (dict(rows=-1), 1),
+    (dict(dtype=2), 1), (dict(wt=1), 1), (dict(rot=65), 1), (dict(rot=66), 1), (dict(rot=-2), 1), (dict(qt=-1), 1),
+    (dict(vh=-8), 1), (dict(amp=float("nan")), 1), (dict(eps=-1.0), 1), (dict(eps=float("nan")), 1),
+    (dict(eps=float("inf")), 1), (dict(slots=None), 1), (dict(hv=None), 1), (dict(v=None), 1), (NO_POOLS, 1),
+    (dict(heads=0), 2), (dict(kv=0), 2), (dict(heads=65537), 2), (dict(d=0), 2), (dict(d=257), 2), (dict(bs=0), 2),
+    (dict(bs=65), 2), (dict(pool=0), 2), (dict(pool=1 << 27), 2), (dict(rows=1 << 26, heads=64), 2),
+    (dict(rows=0), 0), (dict(rows=0, q=None, **NO_POOLS), 0),
+])
+def test_rotate_rows_refusals(kw, code):
+    assert rotate(**kw) == code
+    assert code == 0 or _lib.last_error()
+
+
+def quantize(**kw):
+    a = dict(k=P, kt=128, kh=64, v=P, vt=128, vh=64, dtype=0, slots=P, rows=4, wk=P, wv=P, pool=8, ks=P, kz=P, vs=P, vz=P,
+             fmt=0, kv=2, bs=16, d=64)
+    a.update(kw)
+    return _lib.lib().tierkv_quantize_rows(
+        a["k"], a["kt"], a["kh"], a["v"], a["vt"], a["vh"], a["dtype"], a["slots"], a["rows"], a["wk"], a["wv"], a["pool"],
+        a["ks"], a["kz"], a["vs"], a["vz"], a["fmt"], a["kv"], a["bs"], a["d"], None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(k=None), 1), (dict(slots=None), 1), (dict(wv=None), 1), (dict(ks=None), 1), (dict(kz=None), 1), (dict(dtype=2), 1),
+    (dict(fmt=2), 1), (dict(rows=-1), 1), (dict(kt=-1), 1), (dict(kv=0), 2), (dict(kv=65537), 2), (dict(bs=0), 2),
+    (dict(bs=65), 2), (dict(d=257), 2), (dict(pool=0), 2), (dict(pool=1 << 27), 2), (dict(rows=1 << 26), 2),
+    (dict(rows=0), 0), (dict(rows=0, k=None, fmt=1, kz=None), 0),
+])
+def test_quantize_rows_refusals(kw, code):
+    assert quantize(**kw) == code
+
+
+def read(**kw):
+    a = dict(start=P, cu=P, rows=8, table=P, states=P, lengths=P, stride=8, snb=None, blocks=8, hk=P, hv=P, hot=4, wk=P, wv=P,
+             warm=4, ks=P, kz=P, vs=P, vz=P, fmt=0, ok=P, ov=P, dtype=0, batch=2, kv=2, bs=16, d=64)
+    a.update(kw)
+    return _lib.lib().tierkv_read_rows(
+        a["start"], a["cu"], a["rows"], a["table"], a["states"], a["lengths"], a["stride"], a["snb"], a["blocks"], a["hk"],
+        a["hv"], a["hot"], a["wk"], a["wv"], a["warm"], a["ks"], a["kz"], a["vs"], a["vz"], a["fmt"], a["ok"], a["ov"],
+        a["dtype"], a["batch"], a["kv"], a["bs"], a["d"], None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(start=None), 1), (dict(cu=None), 1), (dict(table=None), 1), (dict(ok=None), 1), (dict(rows=-1), 1),
+    (dict(batch=0), 1), (dict(blocks=0), 1), (dict(blocks=9), 1), (dict(fmt=2), 1), (dict(dtype=3), 1), (dict(hk=None), 1),
+    (dict(hot=0), 1), (dict(wk=None), 1), (dict(warm=0), 1), (dict(vz=None), 1), (dict(kv=0), 2), (dict(bs=0), 2),
+    (dict(bs=65), 2), (dict(d=257), 2), (dict(batch=65536), 2), (dict(blocks=1 << 27, stride=1 << 27), 2),
+    (dict(blocks=1 << 25, stride=1 << 25), 2), (dict(rows=0), 0), (dict(rows=0, ok=None, ov=None), 0),
+])
+def test_read_rows_refusals(kw, code):
+    assert read(**kw) == code
+
+
+def test_wrappers_refuse_cpu_tensors():
+    rows = torch.zeros((3, 2, 64), dtype=torch.float16)
+    v = torch.zeros(3, dtype=torch.int32)
+    pool = torch.zeros((2, 2, 16, 64), dtype=torch.float16)
+    codes = torch.zeros((2, 2, 16, 64), dtype=torch.int8)
+    scale = torch.zeros((2, 2))
+    with pytest.raises(ValueError, match="GPU"):
+        kernels.rotate_rows(rows, rows, v, torch.zeros(32))
+    with pytest.raises(ValueError, match="GPU"):
+        kernels.quantize_rows(rows, rows, v, codes, codes, scale, None, scale, None, "absmax_i8")
+    with pytest.raises(ValueError, match="warm_format"):
+        kernels.quantize_rows(rows, rows, v, codes, codes, scale, None, scale, None, "fp8")
+    with pytest.raises(ValueError, match="GPU"):
+        kernels.read_rows(v, v, 3, v.view(3, 1), v.view(3, 1), v.view(3, 1), v, pool, pool, codes, codes, scale, None, scale, None)
