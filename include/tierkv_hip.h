@@ -574,6 +574,38 @@ TIERKV_API int32_t tierkv_extend_attention(
     int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t block_size, int32_t head_dim, float scaling,
     void* workspace, int64_t workspace_bytes, void* stream);
 
+/* tierkv_extend_attention for requests that share prefixes, each prefix read
+ * once for the rows of all its requests.  Every row of request b sees all
+ * tokens of prefix prefix_of[b] (a row of the prefix tables; negative, or not
+ * below num_prefixes: none), then the request's own tokens as there.
+ *   prefix_of  int32 [batch] (device), requests of a prefix in any order
+ *   prefix_table / prefix_states / prefix_lengths  int32 [num_prefixes,
+ *      prefix_stride], of the same pools, with prefix_num_blocks (NULL: all
+ *      num_prefix_blocks of them) as seq_num_blocks; blocks may also be in
+ *      requests' tables, and a prefix may have no request
+ * batch + num_prefixes <= 4096.  The prefix adds no position of its own: the
+ * keys are in the cache with the positions that they were rotated by.
+ * workspace: as there, tierkv_prefix_workspace_bytes(...) bytes (2 (D + 2) * 4
+ * bytes for each row and head, and what cut tiles take).  Other arguments,
+ * limits, errors and roundings as there; the same inputs give the same bits. */
+TIERKV_API int64_t tierkv_prefix_workspace_bytes(int32_t batch, int32_t num_prefixes, int32_t num_rows,
+                                                 int32_t max_tokens, int32_t num_heads, int32_t num_kv_heads,
+                                                 int32_t num_blocks, int32_t num_prefix_blocks, int32_t block_size,
+                                                 int32_t head_dim);
+TIERKV_API int32_t tierkv_prefix_attention(
+    const void* query, int64_t q_stride_t, int64_t q_stride_h, int32_t query_dtype, void* out,
+    const int32_t* cu_tokens, int32_t num_rows, int32_t max_tokens,
+    const int32_t* block_table, const int32_t* block_states, const int32_t* block_lengths, int64_t table_stride,
+    const int32_t* seq_num_blocks, int32_t num_blocks,
+    const int32_t* prefix_of, const int32_t* prefix_table, const int32_t* prefix_states, const int32_t* prefix_lengths,
+    int64_t prefix_stride, const int32_t* prefix_num_blocks, int32_t num_prefix_blocks, int32_t num_prefixes,
+    const void* hot_k, const void* hot_v, int64_t hot_slots,
+    const void* warm_k, const void* warm_v, int64_t warm_slots,
+    const void* k_scale, const void* k_zero, const void* v_scale, const void* v_zero,
+    int32_t warm_format, int32_t cold_mode,
+    int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t block_size, int32_t head_dim, float scaling,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Next tokens from logits [batch, vocab] (fp16, bf16 or fp32, rows
  * row_stride elements apart) and one random number in [0, 1) per row.
  * Weights are whole numbers W_i = rint(2^42 exp((x_i - max x) / T)), 0 for

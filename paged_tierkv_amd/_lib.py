@@ -193,6 +193,18 @@ SIGNATURES = {
         c_int32, c_int32,
         c_int32, c_int32, c_int32, c_int32, c_int32, c_float,
         _P, c_int64, _P]),
+    "tierkv_prefix_workspace_bytes": (c_int64, [c_int32] * 10),
+    "tierkv_prefix_attention": (c_int32, [
+        _P, c_int64, c_int64, c_int32, _P,
+        _P, c_int32, c_int32,
+        _P, _P, _P, c_int64, _P, c_int32,
+        _P, _P, _P, _P, c_int64, _P, c_int32, c_int32,
+        _P, _P, c_int64,
+        _P, _P, c_int64,
+        _P, _P, _P, _P,
+        c_int32, c_int32,
+        c_int32, c_int32, c_int32, c_int32, c_int32, c_float,
+        _P, c_int64, _P]),
     "tierkv_sample_workspace_bytes": (c_int64, [c_int32, c_int32]),
     "tierkv_sample_tokens": (c_int32, [
         _P, c_int32, c_int64, c_int32, c_int32, _P,

@@ -56,6 +56,8 @@ HIP_SOURCES = {
     # As above (logits and outputs are scaled by VALU code every tile), and the
     # tier branches of its tile loader as in the decode kernel.
     "extend_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-simplifycfg-sink-common=false"],
+    # (the same kernels)
+    "prefix_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-simplifycfg-sink-common=false"],
     "slot_map.hip": [],
     "rotate.hip": [],
     "read_rows.hip": [],

@@ -571,6 +571,73 @@ def tierkv_extend_attention(
     set.  Returns ``[N, H, D]`` (``out`` when given; rows that are not computed
     and rows behind the last request are left as they were).  The same inputs
     give the same bits on every call."""
+    return _attend_packed(query_states, cu_tokens, block_table, block_states, block_lengths, hot_k_pool, hot_v_pool,
+                          warm_k_pool, warm_v_pool, k_scale, k_zero, v_scale, v_zero, num_blocks, num_key_value_groups,
+                          scaling, None, cold_mode, seq_num_blocks, max_tokens, workspace, out)
+
+
+def tierkv_prefix_attention(
+    query_states: torch.Tensor,
+    cu_tokens: torch.Tensor,
+    block_table: torch.Tensor,
+    block_states: torch.Tensor,
+    block_lengths: torch.Tensor,
+    hot_k_pool: torch.Tensor,
+    hot_v_pool: torch.Tensor,
+    warm_k_pool: torch.Tensor,
+    warm_v_pool: torch.Tensor,
+    k_scale: torch.Tensor,
+    k_zero: torch.Tensor | None,
+    v_scale: torch.Tensor,
+    v_zero: torch.Tensor | None,
+    num_blocks: int,
+    num_key_value_groups: int,
+    scaling: float,
+    prefix_of: torch.Tensor,
+    prefix_table: torch.Tensor,
+    prefix_states: torch.Tensor,
+    prefix_lengths: torch.Tensor,
+    *,
+    prefix_num_blocks=None,
+    cold_mode: str = "zero_logit",
+    seq_num_blocks=None,
+    max_tokens: int | None = None,
+    workspace: DecodeWorkspace | None = None,
+    out: torch.Tensor | None = None,
+):
+    """``tierkv_extend_attention`` for requests that share prefixes (a system
+    prompt, a document), each prefix read once for all of its requests.
+
+    ``prefix_of`` int32 ``[B]`` names each request's row of the prefix tables
+    ``[P, max_prefix_blocks]`` (negative, or not below P: no prefix), whose
+    blocks lie in the same pools; ``prefix_num_blocks``: a count ``[P]``, None:
+    whole rows.  Each query row sees every token of its request's prefix, then
+    the request's own tokens up to itself; the keys are in the cache as rotated
+    by their positions (``kernels.rotate_rows``).  Everything else is
+    ``tierkv_extend_attention``'s; a fixed workspace comes from
+    ``extend_workspace(..., prefixes=, prefix_blocks=)``."""
+    return _attend_packed(query_states, cu_tokens, block_table, block_states, block_lengths, hot_k_pool, hot_v_pool,
+                          warm_k_pool, warm_v_pool, k_scale, k_zero, v_scale, v_zero, num_blocks, num_key_value_groups,
+                          scaling, (prefix_of, prefix_table, prefix_states, prefix_lengths, prefix_num_blocks), cold_mode,
+                          seq_num_blocks, max_tokens, workspace, out)
+
+
+def _block_counts(counts, rows: int, index: int, device):
+    """Block counts [rows] as int32 on the device, None as it is."""
+    if counts is None:
+        return None
+    if not (isinstance(counts, torch.Tensor) and counts.dtype == torch.int32 and counts.get_device() == index):
+        counts = torch.as_tensor(counts, dtype=torch.int32, device=device)
+    counts = counts.contiguous()
+    if counts.numel() != rows:
+        raise ValueError("seq_num_blocks needs one entry per sequence.")
+    return counts
+
+
+def _attend_packed(query_states, cu_tokens, block_table, block_states, block_lengths, hot_k_pool, hot_v_pool, warm_k_pool,
+                   warm_v_pool, k_scale, k_zero, v_scale, v_zero, num_blocks, num_key_value_groups, scaling, prefix,
+                   cold_mode, seq_num_blocks, max_tokens, workspace, out):
+    """Both calls of packed rows; ``prefix``: None, or the prefixes' tensors."""
     lib = _lib.lib()
     if query_states.ndim != 3:
         raise ValueError("query_states must be packed rows [tokens, num_heads, head_dim].")
@@ -635,21 +702,26 @@ def tierkv_extend_attention(
     elif (out.dtype != q.dtype or tuple(out.shape) != (rows, num_heads, head_dim) or not out.is_contiguous()
           or out.device != device):
         raise ValueError("out must be a contiguous tensor of the query's shape, dtype and device.")
-    snb = None
-    if seq_num_blocks is not None:
-        snb = seq_num_blocks
-        if not (isinstance(snb, torch.Tensor) and snb.dtype == torch.int32 and snb.get_device() == index):
-            snb = torch.as_tensor(seq_num_blocks, dtype=torch.int32, device=device)
-        snb = snb.contiguous()
-        if snb.numel() != batch:
-            raise ValueError("seq_num_blocks needs one entry per sequence.")
+    snb = _block_counts(seq_num_blocks, batch, index, device)
+    pre = ()
+    if prefix is not None:
+        prefix_of, *tables, counts = prefix
+        _lib.require_gpu_tensor(prefix_of, "prefix_of")
+        if prefix_of.dtype != torch.int32 or not prefix_of.is_contiguous() or tuple(prefix_of.shape) != (batch,):
+            raise ValueError("prefix_of must be a contiguous int32 tensor with one entry per request.")
+        for name, t in zip(("prefix_table", "prefix_states", "prefix_lengths"), tables):
+            _lib.require_gpu_tensor(t, name)
+            if t.dtype != torch.int32 or not t.is_contiguous() or t.ndim != 2 or t.shape != tables[0].shape:
+                raise ValueError(f"{name} must be a contiguous int32 tensor [prefixes, max_prefix_blocks].")
+        if any(t.get_device() != index for t in (prefix_of, *tables)):
+            raise ValueError("queries, tables and pools must be on one device.")
+        prefixes, width = (int(x) for x in tables[0].shape)
+        counts = _block_counts(counts, prefixes, index, device)
+        pre = (_lib.ptr(prefix_of), *(_lib.ptr(t) for t in tables), width, _lib.ptr(counts), width, prefixes)
     bound = rows if max_tokens is None else min(int(max_tokens), rows)
     if bound < 0:
         raise ValueError("max_tokens must not be negative.")
-    need = lib.tierkv_extend_workspace_bytes(batch, rows, bound, num_heads, kv_heads, int(num_blocks), block_size,
-                                             head_dim)
-    if need < 0:
-        raise ValueError("invalid attention geometry.")
+    need = _extend_bytes(batch, rows, bound, num_heads, kv_heads, int(num_blocks), block_size, head_dim, *(pre[-1:] + pre[-2:-1]))
 
     def launch():
         if workspace is None:
@@ -662,10 +734,10 @@ def tierkv_extend_attention(
         ws.reserve(need)
         ptr = _lib.ptr
         ref = fmt == _lib.WARM_REF_U8
-        rc = lib.tierkv_extend_attention(
+        rc = (lib.tierkv_prefix_attention if pre else lib.tierkv_extend_attention)(
             ptr(q), q.stride(0), q.stride(1), _lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_F16,
             ptr(out), ptr(cu_tokens), rows, bound, ptr(block_table), ptr(block_states), ptr(block_lengths),
-            block_table.shape[-1], ptr(snb), int(num_blocks), ptr(hot_k_pool), ptr(hot_v_pool), hot_k_pool.shape[0],
+            block_table.shape[-1], ptr(snb), int(num_blocks), *pre, ptr(hot_k_pool), ptr(hot_v_pool), hot_k_pool.shape[0],
             ptr(warm_k_pool), ptr(warm_v_pool), slots, ptr(k_scale), ptr(k_zero) if ref else None, ptr(v_scale),
             ptr(v_zero) if ref else None, fmt, _COLD_MODES[cold_mode], batch, num_heads, kv_heads, block_size, head_dim,
             float(scaling), ws.data_ptr(), ws.nbytes, _lib.stream_of(device))
@@ -677,7 +749,7 @@ def tierkv_extend_attention(
         else:
             with torch.cuda.device(device):
                 rc, ws = launch()
-        _lib.check(rc, "tierkv_extend_attention")
+        _lib.check(rc, "tierkv_prefix_attention" if pre else "tierkv_extend_attention")
         if _lib.env_flag("TIERKV_CHECK_ERRORS"):
             word = ws.error_word()
             if word:
@@ -687,13 +759,26 @@ def tierkv_extend_attention(
     return out
 
 
-def extend_workspace(device, batch: int, num_tokens: int, num_heads: int, kv_heads: int, num_blocks: int,
-                     head_dim: int, *, block_size: int = 16, max_tokens: int | None = None) -> DecodeWorkspace:
-    """A fixed workspace for ``tierkv_extend_attention`` calls of this
-    geometry, as captured steps need one."""
-    need = _lib.lib().tierkv_extend_workspace_bytes(
-        int(batch), int(num_tokens), int(num_tokens if max_tokens is None else min(max_tokens, num_tokens)),
-        int(num_heads), int(kv_heads), int(num_blocks), int(block_size), int(head_dim))
+def _extend_bytes(batch, rows, bound, num_heads, kv_heads, num_blocks, block_size, head_dim, prefixes=0, prefix_blocks=0) -> int:
+    """Workspace bytes of a call of packed rows."""
+    lib = _lib.lib()
+    if prefixes or prefix_blocks:
+        need = lib.tierkv_prefix_workspace_bytes(batch, prefixes, rows, bound, num_heads, kv_heads, num_blocks,
+                                                 prefix_blocks, block_size, head_dim)
+    else:
+        need = lib.tierkv_extend_workspace_bytes(batch, rows, bound, num_heads, kv_heads, num_blocks, block_size, head_dim)
     if need < 0:
         raise ValueError("invalid attention geometry.")
-    return DecodeWorkspace(device, int(need), growable=False)
+    return int(need)
+
+
+def extend_workspace(device, batch: int, num_tokens: int, num_heads: int, kv_heads: int, num_blocks: int,
+                     head_dim: int, *, block_size: int = 16, max_tokens: int | None = None, prefixes: int = 0,
+                     prefix_blocks: int = 0) -> DecodeWorkspace:
+    """A fixed workspace for ``tierkv_extend_attention`` calls of this
+    geometry, as captured steps need one; with ``prefixes`` rows of
+    ``prefix_blocks`` blocks, for ``tierkv_prefix_attention``."""
+    need = _extend_bytes(int(batch), int(num_tokens), int(num_tokens if max_tokens is None else min(max_tokens, num_tokens)),
+                         int(num_heads), int(kv_heads), int(num_blocks), int(block_size), int(head_dim), int(prefixes),
+                         int(prefix_blocks))
+    return DecodeWorkspace(device, need, growable=False)

@@ -96,3 +96,37 @@ def test_wrappers_refuse_cpu_tensors():
         kernels.quantize_rows(rows, rows, v, codes, codes, scale, None, scale, None, "fp8")
     with pytest.raises(ValueError, match="GPU"):
         kernels.read_rows(v, v, 3, v.view(3, 1), v.view(3, 1), v.view(3, 1), v, pool, pool, codes, codes, scale, None, scale, None)
+
+
+def prefix(**kw):
+    a = dict(q=P, qt=512, qh=64, dtype=0, out=P, cu=P, rows=8, most=8, table=P, states=P, lengths=P, stride=8, snb=None,
+             blocks=8, of=P, pt=P, ps=P, pl=P, pstride=16, pnb=None, pblocks=16, prefixes=2, hk=P, hv=P, hot=4, wk=P, wv=P,
+             warm=4, ks=P, kz=P, vs=P, vz=P, fmt=0, cold=0, batch=2, heads=8, kv=2, bs=16, d=64, scaling=0.125, ws=P,
+             nbytes=1 << 40)
+    a.update(kw)
+    return _lib.lib().tierkv_prefix_attention(
+        a["q"], a["qt"], a["qh"], a["dtype"], a["out"], a["cu"], a["rows"], a["most"], a["table"], a["states"],
+        a["lengths"], a["stride"], a["snb"], a["blocks"], a["of"], a["pt"], a["ps"], a["pl"], a["pstride"], a["pnb"],
+        a["pblocks"], a["prefixes"], a["hk"], a["hv"], a["hot"], a["wk"], a["wv"], a["warm"], a["ks"], a["kz"], a["vs"],
+        a["vz"], a["fmt"], a["cold"], a["batch"], a["heads"], a["kv"], a["bs"], a["d"], ctypes.c_float(a["scaling"]), a["ws"],
+        a["nbytes"], None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(q=None), 1), (dict(ws=None), 1), (dict(rows=-1), 1), (dict(batch=0), 1), (dict(heads=7), 1), (dict(blocks=9), 1),
+    (dict(scaling=float("inf")), 1), (dict(qt=510), 1), (dict(out=P + 8), 1), (dict(of=None), 1), (dict(pt=None), 1),
+    (dict(pl=None), 1), (dict(prefixes=0), 1), (dict(pblocks=0), 1), (dict(pblocks=17), 1), (dict(prefixes=4095), 2),
+    (dict(pblocks=1 << 27, pstride=1 << 27), 2), (dict(bs=65), 2), (dict(d=136), 2), (dict(rows=1 << 28), 2),
+    (dict(rows=1 << 27, heads=2, nbytes=1 << 62), 2), (dict(nbytes=4096), 4), (dict(rows=0), 0), (dict(most=0), 0),
+])
+def test_prefix_attention_refusals(kw, code):
+    assert prefix(**kw) == code
+
+
+def test_prefix_workspace_sizes():
+    size = lambda *a: _lib.lib().tierkv_prefix_workspace_bytes(*a)   # noqa: E731
+    assert size(2, 0, 8, 8, 8, 2, 8, 8, 16, 64) < 0 and size(2, 1, 8, 8, 7, 2, 8, 8, 16, 64) < 0
+    assert size(2, 1, 8, 8, 8, 2, 8, 0, 16, 64) < 0
+    small = size(2, 1, 8, 8, 8, 2, 8, 8, 16, 64)
+    assert 0 < small <= size(2, 1, 800, 800, 8, 2, 8, 8, 16, 64) and small < size(2, 3, 8, 8, 8, 2, 8, 800, 16, 64)
+    assert prefix(nbytes=small - 1, pblocks=8, prefixes=1) == 4
