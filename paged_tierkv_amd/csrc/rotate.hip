@@ -11,14 +11,30 @@
 // fraction of a turn before it becomes 32 bits: position * f_i in 32 bits is
 // off by up to 2^-24 of the angle, 0.007 at position 120000.  Everything else
 // is 32-bit, rounded once when it is stored.
+//
+// Bound: memory.  16384 bf16 rows of 32 / 8 heads of 128 with both norms, 403
+// MB read and written, take 84 us, 4.8 TB/s (a copy of 1 GiB reaches 5.14);
+// with every head forming its own sines and cosines from one workgroup's
+// table, and the weights read again for each, the instructions bounded it
+// (22 per element, 105 us); a wave per (row, head) with a sine and a cosine
+// for each pair took 507.  A few rows take 6 us, the chain from a position to its
+// sine and cosine to the first store.
 
 #include "tierkv_common.h"
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace tierkv {
 
 constexpr int ROT_THREADS = 256;
+// Rows from which a workgroup takes four, a wave to each, instead of one.
+// Launches of 32 / 8 heads of 128, four against one: 64 rows 7.9 / 6.2 us, 512
+// 8.6 / 7.4, 1024 9.3 / 9.4, 2048 13.1 / 16.8, 16384 84 / 130; of 14 / 2 heads
+// of 64: 512 7.5 / 6.7, 1024 7.5 / 7.3, 2048 7.6 / 11.7.
+constexpr int ROT_MANY = 1024;
+constexpr int ROT_HEADS = 2;     // heads of a thread whose loads are in flight together (1: 87 us, 4: 89 us of 85)
 
 struct RotateParams {
   const void* src[3];       // q, k, v rows (v: NULL without pools)
@@ -108,10 +124,225 @@ __global__ __launch_bounds__(ROT_THREADS) void rotate_scalar_kernel(RotateParams
   for (int d = 2 * p.half + lane; d < p.D; d += 64) put(d, get(d));
 }
 
+// Two 16-bit values of a word as floats, and back in the type's rounding.
 template <typename T>
-static void launch_rotate(const RotateParams& p, bool interleaved, hipStream_t stream) {
-  const int units = p.heads + p.kv_heads * (p.src[2] ? 2 : 1);
-  const int64_t waves = int64_t(p.rows) * units;
+__device__ __forceinline__ float2 rot_two(uint32_t w) {
+  if constexpr (__is_same(T, __half)) return make_float2(half_lo(w), half_hi(w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t rot_pack(float a, float b) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  if constexpr (__is_same(T, __half)) {
+    return bits_of(__builtin_convertvector(f2{a, b}, f16x2));
+  } else {
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, bf2));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 rot_pack8(const float (&x)[8]) {
+  return make_uint4(rot_pack<T>(x[0], x[1]), rot_pack<T>(x[2], x[3]), rot_pack<T>(x[4], x[5]), rot_pack<T>(x[6], x[7]));
+}
+
+template <typename T>
+__device__ __forceinline__ void rot_unpack8(uint4 v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = rot_two<T>(w[i]);
+    x[2 * i] = t.x;
+    x[2 * i + 1] = t.y;
+  }
+}
+
+// Sum over the 2^lanes_log2 (at most 16) neighbouring lanes of a head, the
+// same in all of them: each step pairs groups that already agree.
+__device__ __forceinline__ float rot_sum(float v, int lanes_log2) {
+  auto step = [&](auto ctrl) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  if (lanes_log2 >= 1) step(std::integral_constant<int, 0xB1>{});    // quad_perm [1, 0, 3, 2]
+  if (lanes_log2 >= 2) step(std::integral_constant<int, 0x4E>{});    // quad_perm [2, 3, 0, 1]
+  if (lanes_log2 >= 3) step(std::integral_constant<int, 0x141>{});   // row_half_mirror
+  if (lanes_log2 >= 4) step(std::integral_constant<int, 0x140>{});   // row_mirror
+  return v;
+}
+
+// Head dims of whole 16-byte chunks.  A thread takes two chunks of its row's
+// heads, one head after another: those of eight pairs, chunk l and l + half /
+// 8, or 2 l and 2 l + 1 when the pairs are adjacent, so that a pair never
+// crosses threads; 2^lanes_log2 threads hold a head.  ROT_THREADS / R threads
+// share a row: they form its sines and cosines together, one each, and a
+// thread keeps its eight, times the norm's weights, in registers over all
+// heads.  R = 4, a wave to each row, where there are many rows.
+template <typename T, bool PAIRS, int R>
+__global__ __launch_bounds__(ROT_THREADS) void rotate_kernel(RotateParams p, int32_t lanes_log2) {
+  constexpr int PER_ROW = ROT_THREADS / R, MAX_HALF = 128;   // head_dim up to 256
+  constexpr int NI = ROT_HEADS;
+  __shared__ __attribute__((aligned(16))) float s_turn[2][R][MAX_HALF];
+  const int x = threadIdx.x % PER_ROW, of = threadIdx.x / PER_ROW;
+  const int64_t r = int64_t(blockIdx.x) * R + of;
+  const int pos = r < p.rows ? p.positions[r] : -1;
+  const int l = x & ((1 << lanes_log2) - 1), first = x >> lanes_log2, step = PER_ROW >> lanes_log2;
+  const int chunks = p.D / 8, turning = p.half / 8;   // turning: threads of a head whose chunks turn
+  const bool turns = l < turning;
+  const int c0 = PAIRS ? 2 * l : (turns ? l : 2 * l);
+  const int c1 = PAIRS ? 2 * l + 1 : (turns ? l + turning : 2 * l + 1);
+  const bool has0 = c0 < chunks && pos >= 0, has1 = c1 < chunks && pos >= 0;
+  if (pos >= 0) {
+    for (int i = x; i < p.half; i += PER_ROW) {
+      const float2 t = rot_turn(p, pos, i);
+      s_turn[0][of][i] = t.x;
+      s_turn[1][of][i] = t.y;
+    }
+  }
+  __syncthreads();
+  if (pos < 0) return;
+  float cs[8], sn[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    cs[e] = turns ? s_turn[0][of][8 * l + e] : 1.f;
+    sn[e] = turns ? s_turn[1][of][8 * l + e] : 0.f;
+  }
+  // The pool row of head 0, and the next head's distance.
+  const int64_t pool = p.slots ? rot_pool(p, p.slots[r], 0) : -1;
+  const int64_t pool_step = int64_t(p.bs) * p.D;
+#pragma unroll 1
+  for (int kind = 0; kind < 2; ++kind) {
+    const int heads = kind ? p.kv_heads : p.heads;
+    const void* weight = kind ? p.weight[1] : p.weight[0];
+    // y_a = (c w_a) x_a - (s w_b) x_b, y_b = (c w_b) x_b + (s w_a) x_a; the norm's factor comes last.
+    float ca[8], sa[8], cb[8], sb[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      ca[e] = cb[e] = cs[e];
+      sa[e] = sb[e] = sn[e];
+    }
+    if (weight) {
+      float w[16];
+      if (p.weight_f32) {
+        const float* src = reinterpret_cast<const float*>(weight);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          w[e] = has0 ? src[8 * c0 + e] : 0.f;
+          w[8 + e] = has1 ? src[8 * c1 + e] : 0.f;
+        }
+      } else {
+        float t[8];
+        const uint4* src = reinterpret_cast<const uint4*>(weight);
+        rot_unpack8<T>(has0 ? src[c0] : make_uint4(0, 0, 0, 0), t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = t[e];
+        rot_unpack8<T>(has1 ? src[c1] : make_uint4(0, 0, 0, 0), t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[8 + e] = t[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float wa = PAIRS ? w[2 * e] : w[e], wb = PAIRS ? w[2 * e + 1] : w[8 + e];
+        ca[e] *= wa;
+        sa[e] *= wa;
+        cb[e] *= wb;
+        sb[e] *= wb;
+      }
+    }
+    const T* src = reinterpret_cast<const T*>(kind ? p.src[1] : p.src[0]) + r * (kind ? p.st_t[1] : p.st_t[0]);
+    const int64_t src_step = kind ? p.st_h[1] : p.st_h[0];
+    T* const out = reinterpret_cast<T*>(kind ? p.k_out : p.q_out);
+#pragma unroll 1
+    for (int h0 = first; h0 < heads; h0 += step * NI) {
+      uint4 v0[NI], v1[NI];
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int h = h0 + i * step;
+        const uint4* at = reinterpret_cast<const uint4*>(src + (h < heads ? h : h0) * src_step);
+        v0[i] = has0 ? at[c0] : make_uint4(0, 0, 0, 0);
+        v1[i] = has1 ? at[c1] : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int h = h0 + i * step;
+        float v[16], t[8];
+        rot_unpack8<T>(v0[i], t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = t[e];
+        rot_unpack8<T>(v1[i], t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 + e] = t[e];
+        float factor = 1.f;
+        if (weight) {
+          float sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sum = fmaf(v[e], v[e], sum);
+          factor = 1.f / sqrtf(rot_sum(sum, lanes_log2) / float(p.D) + p.eps);
+        }
+        if (h >= heads) break;   // (a head's lanes alike)
+        float y[16];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int a = PAIRS ? 2 * e : e, b = PAIRS ? 2 * e + 1 : 8 + e;
+          if (turns) {
+            y[a] = ca[e] * v[a] - sb[e] * v[b];
+            y[b] = cb[e] * v[b] + sa[e] * v[a];
+          } else {
+            y[a] = ca[e] * v[a];
+            y[b] = cb[e] * v[b];
+          }
+        }
+        if (weight) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) y[e] *= factor;
+        }
+        const float lo[8] = {y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
+        const float hi[8] = {y[8], y[9], y[10], y[11], y[12], y[13], y[14], y[15]};
+        if (out) {
+          uint4* dst = reinterpret_cast<uint4*>(out + (r * heads + h) * p.D);
+          if (has0) dst[c0] = rot_pack8<T>(lo);
+          if (has1) dst[c1] = rot_pack8<T>(hi);
+        }
+        if (kind && pool >= 0) {
+          uint4* dst = reinterpret_cast<uint4*>(p.hot[0] + pool + h * pool_step);
+          if (has0) dst[c0] = rot_pack8<__half>(lo);
+          if (has1) dst[c1] = rot_pack8<__half>(hi);
+        }
+      }
+    }
+  }
+  if (pool < 0) return;
+  const T* src = reinterpret_cast<const T*>(p.src[2]) + r * p.st_t[2];
+  for (int h = first; h < p.kv_heads; h += step) {
+    const uint4* at = reinterpret_cast<const uint4*>(src + h * p.st_h[2]);
+    uint4* dst = reinterpret_cast<uint4*>(p.hot[1] + pool + h * pool_step);
+    float t[8];
+    if (has0) {
+      rot_unpack8<T>(at[c0], t);
+      dst[c0] = rot_pack8<__half>(t);
+    }
+    if (has1) {
+      rot_unpack8<T>(at[c1], t);
+      dst[c1] = rot_pack8<__half>(t);
+    }
+  }
+}
+
+template <typename T, bool PAIRS>
+static void launch_rotate_wide(const RotateParams& p, hipStream_t stream) {
+  int lanes_log2 = 0;
+  while ((16 << lanes_log2) < p.D) ++lanes_log2;
+  if (p.rows >= ROT_MANY)
+    hipLaunchKernelGGL((rotate_kernel<T, PAIRS, 4>), dim3((p.rows + 3) / 4), dim3(ROT_THREADS), 0, stream, p, lanes_log2);
+  else
+    hipLaunchKernelGGL((rotate_kernel<T, PAIRS, 1>), dim3(p.rows), dim3(ROT_THREADS), 0, stream, p, lanes_log2);
+}
+
+template <typename T>
+static void launch_rotate(const RotateParams& p, bool interleaved, bool wide, hipStream_t stream) {
+  if (wide && interleaved) return launch_rotate_wide<T, true>(p, stream);
+  if (wide) return launch_rotate_wide<T, false>(p, stream);
+  const int64_t waves = int64_t(p.rows) * (p.heads + p.kv_heads * (p.src[2] ? 2 : 1));
   hipLaunchKernelGGL(rotate_scalar_kernel<T>, dim3(uint32_t((waves + 3) / 4)), dim3(ROT_THREADS), 0, stream, p,
                      int32_t(interleaved));
 }
@@ -187,7 +418,13 @@ extern "C" int32_t tierkv_rotate_rows(
   p.eps = eps;
   p.amplitude = attention_scaling;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  if (dtype == TIERKV_DTYPE_BF16) launch_rotate<__hip_bfloat16>(p, interleaved != 0, stream);
-  else launch_rotate<__half>(p, interleaved != 0, stream);
+  const bool pairs = interleaved != 0;
+  // 16-byte chunks throughout, of dims that turn or pass, in pairs of chunks.
+  const int64_t strides = q_stride_t | q_stride_h | k_stride_t | k_stride_h | v_stride_t | v_stride_h;
+  const bool wide = head_dim % 8 == 0 && rotary_dim % 16 == 0 && strides % 8 == 0 && aligned16(query) &&
+                    aligned16(key) && aligned16(value) && aligned16(q_out) && aligned16(k_out) && aligned16(hot_k) &&
+                    aligned16(hot_v) && aligned16(q_weight) && aligned16(k_weight);
+  if (dtype == TIERKV_DTYPE_BF16) launch_rotate<__hip_bfloat16>(p, pairs, wide, stream);
+  else launch_rotate<__half>(p, pairs, wide, stream);
   return check_launch("tierkv_rotate_rows");
 }
