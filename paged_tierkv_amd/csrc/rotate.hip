@@ -365,8 +365,8 @@ extern "C" int32_t tierkv_rotate_rows(
   if (dtype != TIERKV_DTYPE_F16 && dtype != TIERKV_DTYPE_BF16) return fail(TIERKV_ERR_INVALID, "rows must be fp16 or bf16");
   if (weight_dtype != dtype && weight_dtype != TIERKV_DTYPE_F32)
     return fail(TIERKV_ERR_INVALID, "norm weights must have the rows' dtype or be fp32");
-  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads > 65536 || num_kv_heads > 65536 || head_dim <= 0 || head_dim > 256)
-    return fail(TIERKV_ERR_UNSUPPORTED, "1 to 65536 heads and a head_dim in [1, 256]");
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads > 65535 || num_kv_heads > 65535 || head_dim <= 0 || head_dim > 256)
+    return fail(TIERKV_ERR_UNSUPPORTED, "1 to 65535 heads and a head_dim in [1, 256]");
   if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 2 != 0)
     return fail(TIERKV_ERR_INVALID, "rotary_dim must be even and at most head_dim");
   if (!std::isfinite(attention_scaling) || !(eps >= 0.f) || !std::isfinite(eps))

@@ -335,16 +335,6 @@ struct WriteSlotsParams {
 };
 
 template <typename T>
-__device__ __forceinline__ uint4 to_half8(uint4 v);
-template <>
-__device__ __forceinline__ uint4 to_half8<__half>(uint4 v) { return v; }
-template <>
-__device__ __forceinline__ uint4 to_half8<__hip_bfloat16>(uint4 v) {
-  auto two = [](uint32_t w) { return pack_f16x2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); };
-  return make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
-}
-
-template <typename T>
 __global__ __launch_bounds__(256) void write_slots_kernel(WriteSlotsParams p, int32_t per_row) {
   const int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x;
   const int kv = blockIdx.y;

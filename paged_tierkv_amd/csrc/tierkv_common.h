@@ -203,4 +203,15 @@ template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __hip_bfloat16 from_f32<__hip_bfloat16>(float v) { return __float2bfloat16(v); }
 
+// Eight 16-bit values as fp16 (bf16 values past its range become infinities).
+template <typename T>
+__device__ __forceinline__ uint4 to_half8(uint4 v);
+template <>
+__device__ __forceinline__ uint4 to_half8<__half>(uint4 v) { return v; }
+template <>
+__device__ __forceinline__ uint4 to_half8<__hip_bfloat16>(uint4 v) {
+  auto two = [](uint32_t w) { return pack_f16x2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); };
+  return make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
+}
+
 }  // namespace tierkv

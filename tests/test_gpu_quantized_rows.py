@@ -68,6 +68,26 @@ def test_codes_match_the_oracle(device, runs, kv, d, bs, fmt, dtype):
     same(dv, pv)
 
 
+@pytest.mark.parametrize("copies", [1, 6])           # few rows and many
+@pytest.mark.parametrize("d", [8, 128])
+def test_long_runs_beside_short_ones(device, copies, d):
+    """Blocks of 64 tokens: runs of every length that start close together,
+    some of them past the next 64 rows."""
+    kinds = [(0, 1), (5, 1), (63, 1), (3, 61), (0, 64), (0, 1), (9, 1), (0, 2), (1, 63), (0, 17), (60, 4), (0, 50), (8, 1),
+             (0, 1), (2, 1), (0, 64), (0, 64), (7, 3)] * copies
+    rng = np.random.default_rng(copies)
+    order = rng.permutation(len(kinds))
+    slots = np.concatenate([order[i] * 64 + p + np.arange(n) for i, (p, n) in enumerate(kinds)])
+    k, v = (torch.from_numpy((rng.standard_normal((len(slots), 3, d)) * np.exp(rng.standard_normal((len(slots), 1, 1)))
+                              ).astype(np.float16)) for _ in range(2))
+    pk, pv = pools(rng, len(kinds), 3, 64, d, "absmax_i8"), pools(rng, len(kinds), 3, 64, d, "absmax_i8")
+    dk, dv = write(device, k.to(device), v.to(device), slots, pk, pv, "absmax_i8")
+    for rows, p in ((k, pk), (v, pv)):
+        shared_prompt.quantize_rows(rows.numpy(), slots, p["codes"], p["scale"], None)
+    same(dk, pk)
+    same(dv, pv)
+
+
 @pytest.mark.parametrize("fmt", ["absmax_i8", "ref_u8"])
 def test_a_cache_grown_token_by_token_is_the_oracle_s(device, fmt):
     """One call per token, scales that grow and stay, a row of zeros among them."""

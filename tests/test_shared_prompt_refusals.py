@@ -33,7 +33,7 @@ NO_POOLS = dict(v=None, slots=None, hk=None, hv=None)
     (dict(dtype=2), 1), (dict(wt=1), 1), (dict(rot=65), 1), (dict(rot=66), 1), (dict(rot=-2), 1), (dict(qt=-1), 1),
     (dict(vh=-8), 1), (dict(amp=float("nan")), 1), (dict(eps=-1.0), 1), (dict(eps=float("nan")), 1),
     (dict(eps=float("inf")), 1), (dict(slots=None), 1), (dict(hv=None), 1), (dict(v=None), 1), (NO_POOLS, 1),
-    (dict(heads=0), 2), (dict(kv=0), 2), (dict(heads=65537), 2), (dict(d=0), 2), (dict(d=257), 2), (dict(bs=0), 2),
+    (dict(heads=0), 2), (dict(kv=0), 2), (dict(heads=65536), 2), (dict(d=0), 2), (dict(d=257), 2), (dict(bs=0), 2),
     (dict(bs=65), 2), (dict(pool=0), 2), (dict(pool=1 << 27), 2), (dict(rows=1 << 26, heads=64), 2),
     (dict(rows=0), 0), (dict(rows=0, q=None, **NO_POOLS), 0),
 ])
@@ -53,7 +53,7 @@ def quantize(**kw):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(k=None), 1), (dict(slots=None), 1), (dict(wv=None), 1), (dict(ks=None), 1), (dict(kz=None), 1), (dict(dtype=2), 1),
-    (dict(fmt=2), 1), (dict(rows=-1), 1), (dict(kt=-1), 1), (dict(kv=0), 2), (dict(kv=65537), 2), (dict(bs=0), 2),
+    (dict(fmt=2), 1), (dict(rows=-1), 1), (dict(kt=-1), 1), (dict(kv=0), 2), (dict(kv=65536), 2), (dict(bs=0), 2),
     (dict(bs=65), 2), (dict(d=257), 2), (dict(pool=0), 2), (dict(pool=1 << 27), 2), (dict(rows=1 << 26), 2),
     (dict(rows=0), 0), (dict(rows=0, k=None, fmt=1, kz=None), 0),
 ])
