@@ -5,6 +5,202 @@
 
 namespace tierkv {
 
+__global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
+  __shared__ Ex3 sh[EX_PLAN / 64];
+  __shared__ int s_last;
+  __shared__ int2 s_tile[EX_MAX_BATCH];   // a request's first tile, its sub-tiles
+  __shared__ int s_rows[EX_MAX_BATCH];    // its query rows per kv head
+  __shared__ float s_work[EX_PLAN / 64];
+  const int tid = threadIdx.x, b = blockIdx.x;
+  int nb = p.num_blocks;
+  if (p.seq_nblocks) nb = min(max(p.seq_nblocks[b], 0), p.num_blocks);
+  const int64_t row = int64_t(b) * p.stride;
+  int n_all;   // the request's new tokens, of which the first n are computed
+  const int n = ex_rows(p, b, &n_all).y;
+  int tokens = 0;
+  Ex3 total;
+  if (p.cold_zero) {   // COLD sub-tiles need the distance to the row's end
+    int sum = 0;
+    for (int i = tid; i < nb; i += EX_PLAN) sum += min(max(p.lengths[row + i], 0), p.bs);
+    ex_scan3({sum, 0, 0}, sh, &total);
+    tokens = total.a;
+  }
+  ExWalk list;
+  ex_walk(p, p.table + row, p.states + row, p.lengths + row, nb, tokens - n_all + 1, p.subtile + int64_t(b) * p.subs_per_seq, sh, list);
+  if (tid == 0) {
+    // Agent-scope stores: the last workgroup may read them from another XCD.
+    int32_t* s = reinterpret_cast<int32_t*>(p.seq + b);
+    if (n < n_all) atomicOr(p.err, 4);
+    const int v[4] = {list.at, list.ordinal - (n_all - n), list.cold, n};
+    for (int k = 0; k < 4; ++k) __hip_atomic_store(s + k, v[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_amdgcn_s_waitcnt(0);
+    s_last = __hip_atomic_fetch_add(p.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == gridDim.x;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  if (tid == 0) __hip_atomic_store(p.arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // The requests' tiles and an upper bound of the sum of the tiles' works:
+  // each is at most g(t) = max(f(t), 1) with f linear, g is convex, and a
+  // convex sum lies below its chord's.
+  const int G = p.groups;
+  float work = 0.f;
+  int tiles_all = 0;
+  for (int i0 = 0; i0 < p.batch; i0 += EX_PLAN) {
+    const int i = i0 + tid;
+    int rows = 0, subs = 0;
+    if (i < p.batch) {
+      int32_t* s = reinterpret_cast<int32_t*>(p.seq + i);
+      subs = __hip_atomic_load(s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      rows = __hip_atomic_load(s + 3, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) * G;
+    }
+    const int tiles = ex_tiles(rows);
+    const bool wide = rows > EX_NARROW;
+    if (tiles > 0) {
+      auto g = [&](int t) {
+        const float last = wide ? float(t + 1) * EX_WIDE : float(rows);
+        return fmaxf(float(subs) + 1.f - fmaxf((float(rows) - last) / float(G) - 1.f, 0.f) / EX_SUB, 1.f);
+      };
+      work += 0.5f * (g(0) + g(tiles - 1)) * float(tiles);
+    }
+    const Ex3 s = ex_scan3({tiles, 0, 0}, sh, &total);
+    if (i < p.batch) {
+      s_tile[i] = make_int2(tiles_all + s.a - tiles, subs);
+      s_rows[i] = rows;
+    }
+    tiles_all += total.a;
+  }
+  work = wave_sum(work);
+  if ((tid & 63) == 0) s_work[tid >> 6] = work;
+  __syncthreads();
+  work = 0.f;
+  for (int i = 0; i < EX_PLAN / 64; ++i) work += s_work[i];
+  work = work * 1.001f + 1.f;   // the rounding of these sums
+  // Sub-tiles per item: each wave rates one choice.  P = longest / (w + 1) for
+  // the first eight waves, a few sizes around an even share for the others;
+  // with the items' count and the longest of them the time is the rounds over
+  // the slots, or the even share and a quarter of an item where the items are
+  // of mixed lengths and fill each other's gaps, and the cost of the partials.
+  // Measured with the whole call: 2048 tokens on 32768, 32 tiles on as many
+  // slots, are left whole, 973 us against 1221 cut in two (the tiles of a head
+  // then also walk the same keys at the same time, in one L2); a single token
+  // on 100000 in 32 parts 85 us, in 64 99; a cost of 24 per partial leaves 512
+  // tokens beside 15 single ones whole, 98 us against 78 cut in four.
+  __shared__ float s_time[EX_PLAN / 64];
+  __shared__ int s_per[EX_PLAN / 64];
+  const float slots = fmaxf(float(EX_SLOTS / p.kv_heads), 1.f);
+  const int least = max(EX_MIN_SUBS, int(ceilf(work / fmaxf(float(EX_TARGET / p.kv_heads), 1.f))));
+  {
+    const int w = tid >> 6, lane = tid & 63;
+    auto tile_work = [&](int f) {
+      const ExTileId x = ex_tile_id(p.batch, f, s_tile, s_rows);
+      return ex_work(s_tile[x.request].y, s_rows[x.request], x.tile, x.wide, G);
+    };
+    float longest = 0.f;
+    for (int i = lane; i < p.batch; i += 64)
+      if (s_rows[i] > 0) longest = fmaxf(longest, float(s_tile[i].y));
+    longest = wave_max(longest);
+    const float share = work / slots;
+    const float f = w == 8 ? 0.34f : w == 9 ? 0.51f : w == 10 ? 0.68f : w == 11 ? 0.8f : w == 12 ? 1.02f
+                  : w == 13 ? 1.25f : w == 14 ? 1.5f : 2.f;
+    const int per = max(least, int(ceilf(w < 8 ? longest / float(w + 1) : share * f)));
+    float items = 0.f, partials = 0.f, len = 0.f;
+    for (int i = lane; i < tiles_all; i += 64) {
+      const int v = tile_work(i), k = ex_parts(v, per);
+      items += float(k);
+      if (k > 1) partials += float(k);
+      len = fmaxf(len, float(v) / float(k));
+    }
+    items = wave_sum(items);
+    partials = wave_sum(partials);
+    len = wave_max(len) + EX_ITEM_COST;
+    const float even = (work + EX_ITEM_COST * items) / slots;
+    const float time = fmaxf(len, fminf(ceilf(items / slots) * len, even + 0.25f * len)) + EX_PART_COST * partials / slots;
+    if (lane == 0) {
+      s_time[w] = time;
+      s_per[w] = per;
+    }
+  }
+  __syncthreads();
+  int per_item = s_per[0];
+  {
+    float best = s_time[0];
+    for (int i = 1; i < EX_PLAN / 64; ++i)
+      if (s_time[i] < best) {
+        best = s_time[i];
+        per_item = s_per[i];
+      }
+  }
+  // Items, tile by tile; each request's longest tiles first.
+  int items = 0, cuts = 0, partials = 0;
+  for (int f0 = 0; f0 < tiles_all; f0 += EX_PLAN) {
+    const int f = f0 + tid;
+    int i = 0, t = 0, parts = 0;
+    bool wide = false;
+    if (f < tiles_all) {
+      const ExTileId x = ex_tile_id(p.batch, f, s_tile, s_rows);
+      i = x.request;
+      t = x.tile;
+      wide = x.wide;
+      parts = ex_parts(ex_work(s_tile[i].y, s_rows[i], t, wide, G), per_item);
+    }
+    const int cut = parts > 1 ? 1 : 0;
+    const Ex3 s = ex_scan3({parts, cut, cut ? parts : 0}, sh, &total);
+    const int at_item = items + s.a - parts, at_cut = cuts + s.b - cut, at_part = partials + s.c - (cut ? parts : 0);
+    items += total.a;
+    cuts += total.b;
+    partials += total.c;
+    if (parts > 0) {
+      // The host's bounds hold for packed ranges that do not overlap; items of others may be left out (-1).
+      const bool fits = at_item + parts <= p.max_items && (!cut || (at_cut < p.max_cut && at_part + parts <= p.max_part));
+      if (!fits) atomicOr(p.err, 4);
+      for (int k = 0; k < parts; ++k)
+        if (at_item + k < p.max_items)
+          p.item[at_item + k] = make_int4(fits ? i : -1, t | (wide ? 1 << 30 : 0), k | (parts << 16), cut ? at_part + k : -1);
+      if (cut && at_cut < p.max_cut) p.cut[at_cut] = make_int2(at_part, fits ? at_item : -1);
+    }
+  }
+  if (tid == 0) {
+    p.head[0] = min(items, p.max_items);
+    p.head[1] = min(cuts, p.max_cut);
+  }
+}
+
+// MIXED: calls that may hold wide tiles; the others' kernel is without their code.
+template <int DP, int WF, typename QT, bool MIXED>
+__global__ __launch_bounds__(EX_THREADS, 2) void extend_kernel(ExtendParams p) {
+  extern __shared__ __attribute__((aligned(16))) char ex_lds[];
+  const int i = int(blockIdx.x) / p.kv_heads, h = int(blockIdx.x) - i * p.kv_heads;
+  if (i >= p.head[0]) return;
+  const ex_int4 it = ((ExList)(uintptr_t)p.item)[i];
+  if (it.x < 0) return;
+  if (MIXED && (it.y & (1 << 30))) ex_item<DP, WF, QT, true, false, 1>(p, ex_lds, h, it, it.w);
+  else ex_item<DP, WF, QT, false, false, EX_WAVES>(p, ex_lds, h, it, it.w);
+}
+
+// Join of a cut tile's partials, in part order: a workgroup per (cut tile, kv
+// head, 4 EX_THREADS / D of its rows), four dims of one row per thread.
+template <typename QT>
+__global__ __launch_bounds__(EX_THREADS) void extend_merge_kernel(ExtendParams p, int32_t rows_per_wg) {
+  const int c = int(blockIdx.x) / p.kv_heads, h = int(blockIdx.x) - c * p.kv_heads;
+  if (c >= p.head[1]) return;
+  const int2 cut = p.cut[c];
+  if (cut.y < 0) return;
+  const int4 it = p.item[cut.y];
+  const int b = it.x, tile = it.y & 0x3fffffff, parts = it.z >> 16;
+  const int G = p.groups, D = p.D, rows = p.seq[b].w * G;
+  const int D4 = D / 4;
+  const int rr = int(blockIdx.y) * rows_per_wg + int(threadIdx.x) / D4, d = 4 * (int(threadIdx.x) % D4);
+  const int row = tile * EX_WIDE + rr;
+  if (int(threadIdx.x) >= rows_per_wg * D4 || rr >= p.part_rows || row >= rows) return;
+  constexpr int AHEAD = 8;   // partials loaded together
+  const int64_t step = int64_t(p.kv_heads) * p.part_rows;
+  const int64_t at = (int64_t(cut.x) * p.kv_heads + h) * p.part_rows + rr;
+  ExJoin j;
+  for (int k0 = 0; k0 < parts; k0 += AHEAD) j.take<AHEAD>(p, parts - k0, d, [&](int k) { return at + (k0 + k) * step; });
+  const int tk = row / G;
+  j.put<QT>(p, ex_rows(p, b).x + tk, h * G + row - tk * G, d);
+}
+
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
@@ -48,10 +244,10 @@ static ExLayout ex_layout(int64_t batch, int64_t rows, int64_t max_tokens, int64
 template <int DP, int WF, typename QT>
 static void ex_launch(const ExtendParams& p, hipStream_t stream) {
   const int lds = ex_lds_bytes<DP>();
-  hipLaunchKernelGGL(extend_plan_kernel<false>, dim3(p.batch), dim3(EX_PLAN), 0, stream, p);
+  hipLaunchKernelGGL(extend_plan_kernel, dim3(p.batch), dim3(EX_PLAN), 0, stream, p);
   const dim3 grid(p.max_items * p.kv_heads);
-  if (p.part_rows > EX_NARROW) hipLaunchKernelGGL((extend_kernel<DP, WF, QT, true, false>), grid, dim3(EX_THREADS), lds, stream, p);
-  else hipLaunchKernelGGL((extend_kernel<DP, WF, QT, false, false>), grid, dim3(EX_THREADS), lds, stream, p);
+  if (p.part_rows > EX_NARROW) hipLaunchKernelGGL((extend_kernel<DP, WF, QT, true>), grid, dim3(EX_THREADS), lds, stream, p);
+  else hipLaunchKernelGGL((extend_kernel<DP, WF, QT, false>), grid, dim3(EX_THREADS), lds, stream, p);
   const int rows_per_wg = 4 * EX_THREADS / p.D;
   hipLaunchKernelGGL(extend_merge_kernel<QT>,
                      dim3(p.max_cut * p.kv_heads, (p.part_rows + rows_per_wg - 1) / rows_per_wg), dim3(EX_THREADS), 0,

@@ -132,18 +132,19 @@ struct ExtendParams {
   int32_t max_items, max_cut, max_part, part_rows;
   int64_t subs_per_seq;
   // Calls with shared prefixes (SHARED) alone.  Their segments are the
-  // prefixes, then the requests; a prefix's rows are those of its requests.
+  // prefixes, then the requests; a prefix's rows are those of the requests
+  // that take it together (prefix_attention.hip).
   const int32_t* prefix_of;    // [batch] a request's prefix, or none
   const int32_t* pre_table;
   const int32_t* pre_states;
   const int32_t* pre_lengths;
   int64_t pre_stride;
   const int32_t* pre_nblocks;
-  int32_t pre_blocks, prefixes, max_tiles;
+  int32_t pre_blocks, prefixes, max_tiles, max_lone;
   int64_t pre_subs;        // sub-tiles of a prefix's list
   int32_t* row_list;       // [rows] packed rows by prefix, request and row
-  int2* row_home;          // [rows] {request, place among its prefix's rows or -1}
-  int2* seg;               // [segments] {first tile, place of its first row (prefixes: in row_list)}
+  int4* row_home;          // [rows] {request, row of it, prefix, place among the prefix's rows}, -1 for none
+  int2* seg;               // [segments] {first tile, where its first row (prefixes: in row_list) or its list is}
   int2* tile;              // [max_tiles] {first partial or -1 (the item wrote the rows itself), parts}
 };
 
@@ -196,37 +197,11 @@ __device__ __forceinline__ int2 ex_rows(const ExtendParams& p, int b, int* all =
   return make_int2(lo, min(min(end, p.rows) - lo, p.max_tokens));
 }
 
-template <bool SHARED>
-__device__ __forceinline__ bool ex_is_prefix(const ExtendParams& p, int s) {
-  if constexpr (SHARED) return s < p.prefixes;
-  return false;
-}
-
-// The request of a segment that is no prefix.
-template <bool SHARED>
-__device__ __forceinline__ int ex_request(const ExtendParams& p, int s) {
-  return SHARED ? s - p.prefixes : s;
-}
-
-template <bool SHARED>
-__device__ __forceinline__ int64_t ex_list_at(const ExtendParams& p, int s) {
-  if constexpr (SHARED)
-    return s < p.prefixes ? s * p.pre_subs : p.prefixes * p.pre_subs + (s - p.prefixes) * p.subs_per_seq;
-  return int64_t(s) * p.subs_per_seq;
-}
-
-// A request's prefix, -1 for none (also for a number that no prefix has).
-__device__ __forceinline__ int ex_prefix(const ExtendParams& p, int b) {
-  const int g = p.prefix_of[b];
-  return g >= 0 && g < p.prefixes ? g : -1;
-}
-
 __device__ __forceinline__ int ex_tiles(int rows) { return rows <= EX_NARROW ? (rows > 0) : (rows + EX_WIDE - 1) / EX_WIDE; }
 
 // Sub-tiles that a tile's last row sees (of `subs`), within one of each
 // sub-tile behind it: exact when the tokens after it fill whole sub-tiles.
-__device__ __forceinline__ int ex_work(int subs, int rows, int tile, bool wide, int groups, bool causal) {
-  if (!causal) return max(subs, 1);
+__device__ __forceinline__ int ex_work(int subs, int rows, int tile, bool wide, int groups) {
   const int last = wide ? min((tile + 1) * EX_WIDE, rows) - 1 : rows - 1;
   const int hidden = (rows - 1) / groups - last / groups;
   return max(subs - hidden / EX_SUB, 1);
@@ -251,74 +226,24 @@ __device__ __forceinline__ ExTileId ex_tile_id(int segments, int f, const int2* 
   return {lo, ex_tiles(rows[lo]) - 1 - (f - first[lo].x), rows[lo] > EX_NARROW};
 }
 
-template <bool SHARED>
-__global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
-  __shared__ Ex3 sh[EX_PLAN / 64];
-  __shared__ int s_last;
-  __shared__ int2 s_tile[EX_MAX_BATCH];   // a request's first tile, its sub-tiles
-  __shared__ int s_rows[EX_MAX_BATCH];    // its query rows per kv head
-  __shared__ float s_work[EX_PLAN / 64];
-  const int tid = threadIdx.x, s_id = blockIdx.x;
-  const bool pre = ex_is_prefix<SHARED>(p, s_id);
-  const int b = ex_request<SHARED>(p, s_id);
-  const int segments = SHARED ? p.batch + p.prefixes : p.batch;
-  int nb = pre ? p.pre_blocks : p.num_blocks;
-  if (pre ? p.pre_nblocks != nullptr : p.seq_nblocks != nullptr) nb = min(max(pre ? p.pre_nblocks[s_id] : p.seq_nblocks[b], 0), nb);
-  const int64_t row = pre ? s_id * p.pre_stride : int64_t(b) * p.stride;
-  const int32_t* const of_table = pre ? p.pre_table : p.table;
-  const int32_t* const of_states = pre ? p.pre_states : p.states;
-  const int32_t* const of_lengths = pre ? p.pre_lengths : p.lengths;
-  int tokens = 0;
+// Lists the resident sub-tiles of a table row of nb blocks behind those that
+// `w` counts: sub-tiles, tokens and COLD tokens that every row sees, of those
+// below the ordinal all_see (with cold_zero; the others become sub-tiles of zeros).
+struct ExWalk {
+  int at = 0, ordinal = 0, cold = 0;
+};
+__device__ __forceinline__ void ex_walk(const ExtendParams& p, const int32_t* table, const int32_t* states,
+                                        const int32_t* lengths, int nb, int all_see_until, int4* out,
+                                        Ex3 (&sh)[EX_PLAN / 64], ExWalk& w) {
+  const int tid = threadIdx.x;
   Ex3 total;
-  int n_all, n, place = 0;   // the request's new tokens, of which the first n are computed
-  if constexpr (SHARED) {
-    // A prefix's rows are its requests' one after another; each request
-    // enters its own.
-    const int g = pre ? s_id : ex_prefix(p, b);
-    Ex3 sum = {0, 0, 0};       // rows of prefixes before, of this one's requests before, of this one
-    if (g >= 0) {
-      for (int i = tid; i < p.batch; i += EX_PLAN) {
-        const int k = ex_prefix(p, i), rows = ex_rows(p, i).y;
-        if (k >= 0 && k < g) sum.a += rows;
-        if (k == g && !pre && i < b) sum.b += rows;
-        if (k == g) sum.c += rows;
-      }
-    }
-    ex_scan3(sum, sh, &total);
-    // (packed ranges that overlap have more rows than there are)
-    place = min(total.a, p.rows);
-    if (pre) {
-      n = n_all = min(total.c, p.rows - place);
-      if (n < total.c && tid == 0) atomicOr(p.err, 4);
-    } else {
-      const int2 r = ex_rows(p, b, &n_all);
-      n = r.y;
-      const int end = min(n_all, p.rows - r.x);
-      for (int i = tid; i < end; i += EX_PLAN) {
-        int mine = g >= 0 && i < n ? total.b + i : -1;
-        if (mine >= p.rows - place) mine = -1;
-        if (mine >= 0) p.row_list[place + mine] = r.x + i;
-        p.row_home[r.x + i] = make_int2(i < n ? b : -1, mine);
-      }
-    }
-  } else {
-    n = ex_rows(p, b, &n_all).y;
-  }
-  if (p.cold_zero) {   // COLD sub-tiles need the distance to the row's end
-    int sum = 0;
-    for (int i = tid; i < nb; i += EX_PLAN) sum += min(max(of_lengths[row + i], 0), p.bs);
-    ex_scan3({sum, 0, 0}, sh, &total);
-    tokens = total.a;
-  }
-  int at = 0, ordinal = 0, cold = 0;   // sub-tiles, tokens and COLD tokens before this chunk
-  int4* out = p.subtile + ex_list_at<SHARED>(p, s_id);
   for (int i0 = 0; i0 < nb; i0 += EX_PLAN) {
     const int i = i0 + tid;
     int len = 0, state = COLD, slot = 0, keep = 0;
     if (i < nb) {
-      len = min(max(of_lengths[row + i], 0), p.bs);
-      state = of_states[row + i];
-      slot = of_table[row + i];
+      len = min(max(lengths[i], 0), p.bs);
+      state = states[i];
+      slot = table[i];
     }
     if (len > 0) {
       if (state == HOT || state == WARM) {
@@ -333,172 +258,22 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
     }
     int count = keep ? (len + EX_SUB - 1) / EX_SUB : 0;
     Ex3 s = ex_scan3({len, keep == 2 ? 0 : count, 0}, sh, &total);
-    const int first = ordinal + s.a - len;
-    int pos = at + s.b - (keep == 2 ? 0 : count);
-    ordinal += total.a;
+    const int first = w.ordinal + s.a - len;
+    int pos = w.at + s.b - (keep == 2 ? 0 : count);
+    w.ordinal += total.a;
     if (p.cold_zero) {
-      const bool all_see = keep == 2 && (pre || first + len <= tokens - n_all + 1);
+      const bool all_see = keep == 2 && first + len <= all_see_until;
       if (all_see) count = 0;
       const Ex3 z = ex_scan3({count, all_see ? len : 0, 0}, sh, &total);
-      pos = at + z.a - count;
-      at += total.a;
-      cold += total.b;
+      pos = w.at + z.a - count;
+      w.at += total.a;
+      w.cold += total.b;
     } else {
-      at += total.b;
+      w.at += total.b;
     }
     const int code = state == COLD ? EX_STATE_ZERO : state;
     for (int j = 0; j < count; ++j)
       out[pos + j] = make_int4(slot, min(len - j * EX_SUB, EX_SUB) | (code << 8) | (j << 16), first + j * EX_SUB, 0);
-  }
-  if (tid == 0) {
-    // Agent-scope stores: the last workgroup may read them from another XCD.
-    int32_t* s = reinterpret_cast<int32_t*>(p.seq + s_id);
-    if (n < n_all) atomicOr(p.err, 4);
-    // (every row of a prefix's sees all of it: a limit past its tokens)
-    const int v[4] = {at, pre ? ordinal + n : ordinal - (n_all - n), cold, n};
-    if constexpr (SHARED) p.seg[s_id].y = place;
-    for (int k = 0; k < 4; ++k) __hip_atomic_store(s + k, v[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __builtin_amdgcn_s_waitcnt(0);
-    s_last = __hip_atomic_fetch_add(p.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == gridDim.x;
-  }
-  __syncthreads();
-  if (!s_last) return;
-  if (tid == 0) __hip_atomic_store(p.arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // The requests' tiles and an upper bound of the sum of the tiles' works:
-  // each is at most g(t) = max(f(t), 1) with f linear, g is convex, and a
-  // convex sum lies below its chord's.
-  const int G = p.groups;
-  float work = 0.f;
-  int tiles_all = 0;
-  for (int i0 = 0; i0 < segments; i0 += EX_PLAN) {
-    const int i = i0 + tid;
-    int rows = 0, subs = 0;
-    if (i < segments) {
-      int32_t* s = reinterpret_cast<int32_t*>(p.seq + i);
-      subs = __hip_atomic_load(s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      rows = __hip_atomic_load(s + 3, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) * G;
-    }
-    const int tiles = ex_tiles(rows);
-    const bool wide = rows > EX_NARROW;
-    if (tiles > 0) {
-      auto g = [&](int t) {
-        if (ex_is_prefix<SHARED>(p, i)) return float(subs) + 1.f;
-        const float last = wide ? float(t + 1) * EX_WIDE : float(rows);
-        return fmaxf(float(subs) + 1.f - fmaxf((float(rows) - last) / float(G) - 1.f, 0.f) / EX_SUB, 1.f);
-      };
-      work += 0.5f * (g(0) + g(tiles - 1)) * float(tiles);
-    }
-    const Ex3 s = ex_scan3({tiles, 0, 0}, sh, &total);
-    if (i < segments) {
-      s_tile[i] = make_int2(tiles_all + s.a - tiles, subs);
-      s_rows[i] = rows;
-    }
-    tiles_all += total.a;
-  }
-  work = wave_sum(work);
-  if ((tid & 63) == 0) s_work[tid >> 6] = work;
-  __syncthreads();
-  work = 0.f;
-  for (int i = 0; i < EX_PLAN / 64; ++i) work += s_work[i];
-  work = work * 1.001f + 1.f;   // the rounding of these sums
-  // Sub-tiles per item: each wave rates one choice.  P = longest / (w + 1) for
-  // the first eight waves, a few sizes around an even share for the others;
-  // with the items' count and the longest of them the time is the rounds over
-  // the slots, or the even share and a quarter of an item where the items are
-  // of mixed lengths and fill each other's gaps, and the cost of the partials.
-  // Measured with the whole call: 2048 tokens on 32768, 32 tiles on as many
-  // slots, are left whole, 973 us against 1221 cut in two (the tiles of a head
-  // then also walk the same keys at the same time, in one L2); a single token
-  // on 100000 in 32 parts 85 us, in 64 99; a cost of 24 per partial leaves 512
-  // tokens beside 15 single ones whole, 98 us against 78 cut in four.
-  __shared__ float s_time[EX_PLAN / 64];
-  __shared__ int s_per[EX_PLAN / 64];
-  const float slots = fmaxf(float(EX_SLOTS / p.kv_heads), 1.f);
-  const int least = max(EX_MIN_SUBS, int(ceilf(work / fmaxf(float(EX_TARGET / p.kv_heads), 1.f))));
-  {
-    const int w = tid >> 6, lane = tid & 63;
-    auto tile_work = [&](int f) {
-      const ExTileId x = ex_tile_id(segments, f, s_tile, s_rows);
-      return ex_work(s_tile[x.request].y, s_rows[x.request], x.tile, x.wide, G, !ex_is_prefix<SHARED>(p, x.request));
-    };
-    float longest = 0.f;
-    for (int i = lane; i < segments; i += 64)
-      if (s_rows[i] > 0) longest = fmaxf(longest, float(s_tile[i].y));
-    longest = wave_max(longest);
-    const float share = work / slots;
-    const float f = w == 8 ? 0.34f : w == 9 ? 0.51f : w == 10 ? 0.68f : w == 11 ? 0.8f : w == 12 ? 1.02f
-                  : w == 13 ? 1.25f : w == 14 ? 1.5f : 2.f;
-    const int per = max(least, int(ceilf(w < 8 ? longest / float(w + 1) : share * f)));
-    float items = 0.f, partials = 0.f, len = 0.f;
-    for (int i = lane; i < tiles_all; i += 64) {
-      const int v = tile_work(i), k = ex_parts(v, per);
-      items += float(k);
-      if (k > 1) partials += float(k);
-      len = fmaxf(len, float(v) / float(k));
-    }
-    items = wave_sum(items);
-    partials = wave_sum(partials);
-    len = wave_max(len) + EX_ITEM_COST;
-    const float even = (work + EX_ITEM_COST * items) / slots;
-    const float time = fmaxf(len, fminf(ceilf(items / slots) * len, even + 0.25f * len)) + EX_PART_COST * partials / slots;
-    if (lane == 0) {
-      s_time[w] = time;
-      s_per[w] = per;
-    }
-  }
-  __syncthreads();
-  int per_item = s_per[0];
-  {
-    float best = s_time[0];
-    for (int i = 1; i < EX_PLAN / 64; ++i)
-      if (s_time[i] < best) {
-        best = s_time[i];
-        per_item = s_per[i];
-      }
-  }
-  // Items, tile by tile; each request's longest tiles first.
-  int items = 0, cuts = 0, partials = 0;
-  for (int f0 = 0; f0 < tiles_all; f0 += EX_PLAN) {
-    const int f = f0 + tid;
-    int i = 0, t = 0, parts = 0;
-    bool wide = false;
-    if (f < tiles_all) {
-      const ExTileId x = ex_tile_id(segments, f, s_tile, s_rows);
-      i = x.request;
-      t = x.tile;
-      wide = x.wide;
-      parts = ex_parts(ex_work(s_tile[i].y, s_rows[i], t, wide, G, !ex_is_prefix<SHARED>(p, i)), per_item);
-    }
-    // Rows that also have a prefix's part keep partials in any case.
-    const bool joined = SHARED && parts > 0 && (ex_is_prefix<SHARED>(p, i) || ex_prefix(p, ex_request<SHARED>(p, i)) >= 0);
-    const int cut = parts > 1 || joined ? 1 : 0;
-    const int each = SHARED && wide ? EX_WIDE / EX_UNIT : 1;   // of a part
-    const Ex3 s = ex_scan3({parts, cut, cut ? parts * each : 0}, sh, &total);
-    const int at_item = items + s.a - parts, at_cut = cuts + s.b - cut, at_part = partials + s.c - (cut ? parts * each : 0);
-    items += total.a;
-    cuts += total.b;
-    partials += total.c;
-    if (parts > 0) {
-      // The host's bounds hold for packed ranges that do not overlap; items of others may be left out (-1).
-      const bool fits = at_item + parts <= p.max_items && (SHARED ? f < p.max_tiles : !cut || at_cut < p.max_cut) &&
-                        (!cut || at_part + parts * each <= p.max_part);
-      if (!fits) atomicOr(p.err, 4);
-      for (int k = 0; k < parts; ++k)
-        if (at_item + k < p.max_items)
-          p.item[at_item + k] = make_int4(fits ? i : -1, t | (wide ? 1 << 30 : 0), k | (parts << 16), cut ? at_part + k * each : -1);
-      if constexpr (SHARED) {
-        if (f < p.max_tiles) p.tile[f] = make_int2(cut ? at_part : -1, fits ? parts : 0);
-      } else {
-        if (cut && at_cut < p.max_cut) p.cut[at_cut] = make_int2(at_part, fits ? at_item : -1);
-      }
-    }
-  }
-  if constexpr (SHARED) {
-    for (int i = tid; i < segments; i += EX_PLAN) p.seg[i].x = s_tile[i].x;
-  }
-  if (tid == 0) {
-    p.head[0] = min(items, p.max_items);
-    p.head[1] = min(cuts, p.max_cut);
   }
 }
 
@@ -528,6 +303,13 @@ typedef const __attribute__((address_space(4))) ex_int4* ExList;
 struct ExSub {
   int slot, valid, state, sub, ordinal;
 };
+
+// Where the list of request b's sub-tiles is: behind the prefixes', or, for
+// ~where >= 0, among those of requests that walk their prefix themselves.
+__device__ __forceinline__ int64_t ex_list_of(const ExtendParams& p, int b, int where) {
+  const int64_t own = p.prefixes * p.pre_subs + b * p.subs_per_seq;
+  return where >= 0 ? own : p.prefixes * p.pre_subs + p.batch * p.subs_per_seq + ~where * (p.pre_subs + p.subs_per_seq);
+}
 
 // Sub-tile i of a list; from `end` on an empty one.  (Lists have EX_PAD spare
 // entries behind them, which may be read.)
@@ -1036,22 +818,38 @@ constexpr int ex_lds_bytes() {
 //   WIDE  every wave holds 32 rows of its own and all share 64 keys at a time,
 //         each wave staging the K or the V of one sub-tile; else all hold the
 //         same 32 rows and each stages and takes 32 keys of its own
-template <int DP, int WF, typename QT, bool WIDE, bool SHARED>
-__device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h, const ex_int4 it, int64_t partial) {
+//   KW    waves that split the keys of narrow rows; the workgroup holds
+//         EX_WAVES / KW items side by side, each of its own arguments, `dead`
+//         where there is none (it only meets the others' barriers)
+template <int DP, int WF, typename QT, bool WIDE, bool SHARED, int KW>
+__device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h, const ex_int4 it, int64_t partial,
+                                        bool dead = false) {
   constexpr int TK = WIDE ? 64 : 32;
   constexpr int NS = WIDE ? 1 : 4;          // halves a wave stages
-  constexpr int KW = WIDE ? 1 : EX_WAVES;   // waves that split the keys
   const int tid = threadIdx.x, lane = tid & 63, w = ex_uniform(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int b = it.x, tile = it.y & 0x3fffffff;
   const int part = it.z & 0xffff, parts = it.z >> 16;
   const int4 seq = p.seq[b];
-  const bool pre = ex_is_prefix<SHARED>(p, b);
-  const int q0 = pre ? p.seg[b].y : ex_rows(p, ex_request<SHARED>(p, b)).x, n = seq.w, G = p.groups, D = p.D;
+  bool pre = false;                         // a prefix's rows: through the list
+  int q0, n = seq.w;
+  int64_t list_at;
+  if constexpr (SHARED) {
+    const int where = p.seg[b].y;
+    pre = b < p.prefixes;
+    q0 = pre ? where : ex_rows(p, b - p.prefixes).x;
+    list_at = pre ? b * p.pre_subs : ex_list_of(p, b - p.prefixes, where);
+    if (dead) n = 0;
+  } else {
+    q0 = ex_rows(p, b).x;
+    list_at = int64_t(b) * p.subs_per_seq;
+  }
+  const int G = p.groups, D = p.D, kw = w % KW;   // kw: the wave's place among those of its item
+
   const int rows = n * G;
   const int row_first = tile * EX_WIDE, row_last = min(row_first + (WIDE ? EX_WIDE : 32), rows) - 1;
   const int lim_min = seq.y - n + row_first / G, lim_max = seq.y - n + row_last / G;
-  const int4* raw_list = p.subtile + ex_list_at<SHARED>(p, b);
+  const int4* raw_list = p.subtile + list_at;
   const ExList list = (ExList)(uintptr_t)raw_list;
 
   // This lane's row.
@@ -1121,12 +919,12 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
   for (int dt = 0; dt < DP / 32; ++dt) a.o[dt] = f32x16{};
   a.m = EX_NONE;
   a.l = 0.f;
-  if (part == 0 && seq.z > 0 && (KW == 1 || w == 0)) {   // COLD tokens with logit 0 that every row sees
+  if (part == 0 && seq.z > 0 && (KW == 1 || kw == 0)) {   // COLD tokens with logit 0 that every row sees
     a.m = 0.f;
     a.l = half == 0 ? float(seq.z) * exp2f(EX_BOOST) : 0.f;
   }
 
-  const int visible = ex_uniform(ex_visible(raw_list, seq.x, lim_max));
+  const int visible = dead ? 0 : ex_uniform(ex_visible(raw_list, seq.x, lim_max));
   constexpr int ROUND = TK / 16 * KW;       // sub-tiles per round of the workgroup
   const int chunk = ((visible + parts - 1) / parts + ROUND - 1) & ~(ROUND - 1);
   const int lo = min(part * chunk, visible), hi = min(lo + chunk, visible);
@@ -1135,7 +933,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
   // and the one after it loads.  Narrow: a tile per wave, stored between its
   // steps in the wave's own order.
   ExTile<DP, TK>* tiles = reinterpret_cast<ExTile<DP, TK>*>(lds);
-  const int first = WIDE ? lo : lo + w * (TK / 16);
+  const int first = WIDE ? lo : lo + kw * (TK / 16);
   ExHalf<DP> st[NS];
   ExSub sub[WIDE ? 1 : 2];
   bool wild = false;
@@ -1290,7 +1088,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
     // The waves' states of the same rows meet in LDS: 32 rows of DP sums each.
     __syncthreads();
     float* so = reinterpret_cast<float*>(lds);
-    float* sml = so + KW * 32 * (DP + 4);
+    float* sml = so + EX_WAVES * 32 * (DP + 4);
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -1304,15 +1102,15 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
     }
     __syncthreads();
     // Row x / (DP / 4), dims 4 (x % (DP / 4)) ..
-    for (int x = tid; x < 32 * (DP / 4); x += EX_THREADS) {
-      const int rr = x / (DP / 4), d = 4 * (x % (DP / 4));
+    for (int x = tid % (64 * KW); x < 32 * (DP / 4); x += 64 * KW) {
+      const int rr = x / (DP / 4), d = 4 * (x % (DP / 4)), k0 = w - kw;
       float m = EX_NONE;
 #pragma unroll
-      for (int k = 0; k < KW; ++k) m = fmaxf(m, sml[(k * 32 + rr) * 2]);
+      for (int k = k0; k < k0 + KW; ++k) m = fmaxf(m, sml[(k * 32 + rr) * 2]);
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
       float l = 0.f;
 #pragma unroll
-      for (int k = 0; k < KW; ++k) {
+      for (int k = k0; k < k0 + KW; ++k) {
         const float c = __builtin_amdgcn_exp2f(sml[(k * 32 + rr) * 2] - m);
         if (c > 0.f) {   // (a state of no weight may hold an infinity's product)
           l += sml[(k * 32 + rr) * 2 + 1] * c;
@@ -1369,49 +1167,36 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
   }
 }
 
-// MIXED: calls that may hold wide tiles; the others' kernel is without their code.
-template <int DP, int WF, typename QT, bool MIXED, bool SHARED>
-__global__ __launch_bounds__(EX_THREADS, 2) void extend_kernel(ExtendParams p) {
-  extern __shared__ __attribute__((aligned(16))) char ex_lds[];
-  const int i = int(blockIdx.x) / p.kv_heads, h = int(blockIdx.x) - i * p.kv_heads;
-  if (i >= p.head[0]) return;
-  const ex_int4 it = ((ExList)(uintptr_t)p.item)[i];
-  if (it.x < 0) return;
-  if (MIXED && (it.y & (1 << 30))) ex_item<DP, WF, QT, true, SHARED>(p, ex_lds, h, it, it.w);
-  else ex_item<DP, WF, QT, false, SHARED>(p, ex_lds, h, it, it.w);
-}
-
-// Sums of four dims of one row over partials, `step` rows apart from row `at`
-// on, in order.
+// Sums of four dims of one row over partials.
 struct ExJoin {
   float m = EX_NONE, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
 
-  __device__ __forceinline__ void add(const ExtendParams& p, int64_t at, int64_t step, int parts, int d) {
-    constexpr int AHEAD = 8;   // partials loaded together
-    for (int k0 = 0; k0 < parts; k0 += AHEAD) {
-      float2 ml[AHEAD];
-      f32x4 v[AHEAD];
+  // N partials, of which `count` count, at place(k): their loads are in flight
+  // together, and they are added in order.
+  template <int N, typename F>
+  __device__ __forceinline__ void take(const ExtendParams& p, int count, int d, F place) {
+    float2 ml[N];
+    f32x4 v[N];
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int64_t x = at + min(k0 + k, parts - 1) * step;
-        ml[k] = reinterpret_cast<const float2*>(p.part_ml)[x];
-        v[k] = *reinterpret_cast<const f32x4*>(p.part_o + x * p.D + d);
-      }
-      float top = m;
+    for (int k = 0; k < N; ++k) {
+      const int64_t x = place(min(k, count - 1));
+      ml[k] = reinterpret_cast<const float2*>(p.part_ml)[x];
+      v[k] = *reinterpret_cast<const f32x4*>(p.part_o + x * p.D + d);
+    }
+    float top = m;
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) top = fmaxf(top, ml[k].x);
-      const float f0 = __builtin_amdgcn_exp2f(m - top);
-      m = top;
-      l *= f0;
-      o *= f0;
+    for (int k = 0; k < N; ++k) top = fmaxf(top, ml[k].x);
+    const float f0 = __builtin_amdgcn_exp2f(m - top);
+    m = top;
+    l *= f0;
+    o *= f0;
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const float f = k0 + k < parts ? __builtin_amdgcn_exp2f(ml[k].x - m) : 0.f;
-        if (f > 0.f) {   // (a partial of no weight may hold an infinity's product)
-          l += ml[k].y * f;
-          o += v[k] * f;
-        }
+    for (int k = 0; k < N; ++k) {
+      const float f = k < count ? __builtin_amdgcn_exp2f(ml[k].x - m) : 0.f;
+      if (f > 0.f) {   // (a partial of no weight may hold an infinity's product)
+        l += ml[k].y * f;
+        o += v[k] * f;
       }
     }
   }
@@ -1424,63 +1209,6 @@ struct ExJoin {
     *reinterpret_cast<uint2*>(dst) = make_uint2(ex_out2<QT>(o[0] * inv, o[1] * inv), ex_out2<QT>(o[2] * inv, o[3] * inv));
   }
 };
-
-// Join of a cut tile's partials, in part order: a workgroup per (cut tile, kv
-// head, 4 EX_THREADS / D of its rows), four dims of one row per thread.
-template <typename QT>
-__global__ __launch_bounds__(EX_THREADS) void extend_merge_kernel(ExtendParams p, int32_t rows_per_wg) {
-  const int c = int(blockIdx.x) / p.kv_heads, h = int(blockIdx.x) - c * p.kv_heads;
-  if (c >= p.head[1]) return;
-  const int2 cut = p.cut[c];
-  if (cut.y < 0) return;
-  const int4 it = p.item[cut.y];
-  const int b = it.x, tile = it.y & 0x3fffffff, parts = it.z >> 16;
-  const int G = p.groups, D = p.D, rows = p.seq[b].w * G;
-  const int D4 = D / 4;
-  const int rr = int(blockIdx.y) * rows_per_wg + int(threadIdx.x) / D4, d = 4 * (int(threadIdx.x) % D4);
-  const int row = tile * EX_WIDE + rr;
-  if (int(threadIdx.x) >= rows_per_wg * D4 || rr >= p.part_rows || row >= rows) return;
-  ExJoin j;
-  j.add(p, (int64_t(cut.x) * p.kv_heads + h) * p.part_rows + rr, int64_t(p.kv_heads) * p.part_rows, parts, d);
-  const int tk = row / G;
-  j.put<QT>(p, ex_rows(p, b).x + tk, h * G + row - tk * G, d);
-}
-
-// The same with shared prefixes: four dims of one packed row and head per
-// thread, the request's own partials, then those of its prefix.
-template <typename QT>
-__global__ __launch_bounds__(EX_THREADS) void extend_join_kernel(ExtendParams p) {
-  const int D4 = p.D / 4, G = p.groups;
-  const int64_t x = int64_t(blockIdx.x) * EX_THREADS + threadIdx.x;
-  const int64_t rh = x / D4;
-  const int d = 4 * int(x - rh * D4);
-  const int64_t r = rh / p.heads;
-  if (r >= p.rows) return;
-  const int hd = int(rh - r * p.heads), h = hd / G;
-  const int2 home = p.row_home[r];
-  // (a row of no request has whatever the workspace held)
-  if (home.x < 0 || home.x >= p.batch) return;
-  const int s = p.prefixes + home.x, i = int(r) - ex_rows(p, home.x).x, n = p.seq[s].w;
-  if (i < 0 || i >= n) return;
-  auto add = [&](ExJoin& j, int seg, int rows, int row) {
-    const int t = row / EX_WIDE, f = p.seg[seg].x + ex_tiles(rows) - 1 - t;
-    if (f >= p.max_tiles) return false;
-    const int2 tile = p.tile[f];
-    if (tile.x < 0 || tile.y <= 0) return false;   // its item wrote the rows, or there was no room for it
-    const int rr = row - t * EX_WIDE;
-    const int64_t step = int64_t(rows > EX_NARROW ? EX_WIDE / EX_UNIT : 1) * p.kv_heads * EX_UNIT;
-    j.add(p, ex_unit_row(p, tile.x, h, rr), step, tile.y, d);
-    return true;
-  };
-  ExJoin j;
-  if (!add(j, s, n * G, i * G + hd - h * G)) return;
-  const int g = ex_prefix(p, home.x);
-  if (g >= 0) {
-    const int all = p.seq[g].w;
-    if (home.y < 0 || home.y >= all || !add(j, g, all * G, home.y * G + hd - h * G)) return;
-  }
-  j.put<QT>(p, r, hd, d);
-}
 
 // ---------------------------------------------------------------------------
 // Host

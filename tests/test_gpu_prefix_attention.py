@@ -132,6 +132,9 @@ CASES = [
     ([90], [0, 0], [6, 2], [5, 0], 4, 2, 64, 16),                          # more rows than tokens; nothing of its own
     ([2500], [0, 0, 0], [1, 1, 3], [12, 600, 3], 4, 1, 64, 16),            # cut
     ([40, 60], [0, 1], [12, 3], [50, 33], 4, 2, 8, 1),
+    ([700], [0, 0, -1], [130, 33, 140], [130, 300, 200], 8, 2, 64, 16),    # requests that walk their prefix themselves,
+    ([90, 0, 40], [2, 0, 1, 0], [300, 1, 129, 2], [333, 20, 129, 9], 8, 1, 128, 16),   # beside others
+    ([1800], [0, 0], [171, 1], [171, 20], 12, 4, 96, 16),
 ]
 
 
