@@ -165,6 +165,15 @@ __global__ __launch_bounds__(EX_PLAN) void extend_plan_kernel(ExtendParams p) {
   }
 }
 
+// An item of the plan.
+template <int DP, int WF, typename QT, bool WIDE>
+__device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h, const ex_int4 it) {
+  const int b = it.x, q0 = ex_rows(p, b).x;
+  const ExWorkspaceList list = {p.subtile + int64_t(b) * p.subs_per_seq};
+  ex_tile_part<DP, WF, QT, WIDE, false, WIDE ? 1 : EX_WAVES>(p, lds, h, it.y & 0x3fffffff, it.z & 0xffff, it.z >> 16, p.seq[b],
+                                                             list, [&](int t) { return q0 + t; }, it.w);
+}
+
 // MIXED: calls that may hold wide tiles; the others' kernel is without their code.
 template <int DP, int WF, typename QT, bool MIXED>
 __global__ __launch_bounds__(EX_THREADS, 2) void extend_kernel(ExtendParams p) {
@@ -173,8 +182,8 @@ __global__ __launch_bounds__(EX_THREADS, 2) void extend_kernel(ExtendParams p) {
   if (i >= p.head[0]) return;
   const ex_int4 it = ((ExList)(uintptr_t)p.item)[i];
   if (it.x < 0) return;
-  if (MIXED && (it.y & (1 << 30))) ex_item<DP, WF, QT, true, false, 1>(p, ex_lds, h, it, it.w);
-  else ex_item<DP, WF, QT, false, false, EX_WAVES>(p, ex_lds, h, it, it.w);
+  if (MIXED && (it.y & (1 << 30))) ex_item<DP, WF, QT, true>(p, ex_lds, h, it);
+  else ex_item<DP, WF, QT, false>(p, ex_lds, h, it);
 }
 
 // Join of a cut tile's partials, in part order: a workgroup per (cut tile, kv

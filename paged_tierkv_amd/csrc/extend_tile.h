@@ -146,6 +146,10 @@ struct ExtendParams {
   int4* row_home;          // [rows] {request, row of it, prefix, place among the prefix's rows}, -1 for none
   int2* seg;               // [segments] {first tile, where its first row (prefixes: in row_list) or its list is}
   int2* tile;              // [max_tiles] {first partial or -1 (the item wrote the rows itself), parts}
+  // Steps that the host lays out.
+  int2* row_pre;           // [rows] {request, place of its first row among the slots' rows}
+  int32_t pre_slots, pre_parts, own_parts, own_side;
+  int64_t own_unit;        // the requests' own first partial
 };
 
 // A partial's rows are kept 32 at a time where tiles of both sizes have them.
@@ -304,17 +308,19 @@ struct ExSub {
   int slot, valid, state, sub, ordinal;
 };
 
-// Where the list of request b's sub-tiles is: behind the prefixes', or, for
-// ~where >= 0, among those of requests that walk their prefix themselves.
-__device__ __forceinline__ int64_t ex_list_of(const ExtendParams& p, int b, int where) {
-  const int64_t own = p.prefixes * p.pre_subs + b * p.subs_per_seq;
-  return where >= 0 ? own : p.prefixes * p.pre_subs + p.batch * p.subs_per_seq + ~where * (p.pre_subs + p.subs_per_seq);
-}
+// A list of sub-tiles in the workspace: any(i) is entry i, each lane's own;
+// one(i) the same for an i that the wave shares.
+struct ExWorkspaceList {
+  const int4* list;
+  __device__ __forceinline__ int4 any(int i) const { return list[i]; }
+  __device__ __forceinline__ ex_int4 one(int i) const { return ((ExList)(uintptr_t)list)[i]; }
+};
 
-// Sub-tile i of a list; from `end` on an empty one.  (Lists have EX_PAD spare
-// entries behind them, which may be read.)
-__device__ __forceinline__ ExSub ex_sub(ExList list, int i, int end) {
-  const ex_int4 v = list[i];
+// Sub-tile i of a list; from `end` on an empty one.  (Lists have spare entries
+// behind them, which may be read.)
+template <typename LIST>
+__device__ __forceinline__ ExSub ex_sub(const LIST& list, int i, int end) {
+  const ex_int4 v = list.one(i);
   ExSub s;
   const bool in = i < end;
   s.slot = in ? v.x : 0;
@@ -326,8 +332,8 @@ __device__ __forceinline__ ExSub ex_sub(ExList list, int i, int end) {
 }
 
 // Keys of each sub-tile of a tile that a row with the given limit sees.
-template <int TK>
-__device__ __forceinline__ void ex_ends(ExList list, int at, int hi, int lim, int (&end)[TK / 16]) {
+template <int TK, typename LIST>
+__device__ __forceinline__ void ex_ends(const LIST& list, int at, int hi, int lim, int (&end)[TK / 16]) {
 #pragma unroll
   for (int i = 0; i < TK / 16; ++i) {
     const ExSub s = ex_sub(list, at + i, hi);
@@ -601,13 +607,14 @@ __device__ __forceinline__ float ex_value(const ExtendParams& p, int h, const Ex
 
 // Sub-tiles of a list whose first ordinal is at most `limit` (ordinals grow):
 // 64 samples at a time by one wave, all waves alike.
-__device__ __forceinline__ int ex_visible(const int4* list, int count, int limit) {
+template <typename LIST>
+__device__ __forceinline__ int ex_visible(const LIST& list, int count, int limit) {
   int lo = 0, hi = count;   // sub-tiles before lo are visible, from hi on hidden
   const int lane = threadIdx.x & 63;
   while (hi > lo) {
     const int step = (hi - lo + 63) / 64;
     const int i = lo + lane * step;
-    const bool vis = i < hi && list[i].z <= limit;
+    const bool vis = i < hi && list.any(i).z <= limit;
     const int seen = __popcll(__ballot(vis));
     if (seen == 0) return lo;
     const int last = lo + (seen - 1) * step;   // visible
@@ -619,14 +626,15 @@ __device__ __forceinline__ int ex_visible(const int4* list, int count, int limit
 
 // The first sub-tile of [lo, hi) that is not full, or not seen by every row
 // (from the limit lim on): tiles before it need no masks.  By one wave.
-__device__ __forceinline__ int ex_full_until(const int4* list, int lo, int hi, int lim) {
+template <typename LIST>
+__device__ __forceinline__ int ex_full_until(const LIST& list, int lo, int hi, int lim) {
   const int lane = threadIdx.x & 63;
   for (int i0 = lo; i0 < hi; i0 += 256) {
     uint64_t odd[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = min(i0 + k * 64 + lane, hi - 1);
-      const int4 v = list[i];
+      const int4 v = list.any(i);
       odd[k] = __ballot((v.y & 0xff) != EX_SUB || v.z + EX_SUB - 1 > lim);
     }
 #pragma unroll
@@ -814,43 +822,29 @@ constexpr int ex_lds_bytes() {
   return wide > narrow ? (wide > merge ? wide : merge) : (narrow > merge ? narrow : merge);
 }
 
-// An item: query rows of one tile, sub-tiles [part / parts) of what it sees.
+// Query rows of one tile, sub-tiles [part / parts) of what they see.
 //   WIDE  every wave holds 32 rows of its own and all share 64 keys at a time,
 //         each wave staging the K or the V of one sub-tile; else all hold the
 //         same 32 rows and each stages and takes 32 keys of its own
 //   KW    waves that split the keys of narrow rows; the workgroup holds
-//         EX_WAVES / KW items side by side, each of its own arguments, `dead`
+//         EX_WAVES / KW tiles side by side, each of its own arguments, `dead`
 //         where there is none (it only meets the others' barriers)
-template <int DP, int WF, typename QT, bool WIDE, bool SHARED, int KW>
-__device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h, const ex_int4 it, int64_t partial,
-                                        bool dead = false) {
+//   UNITS how partials lie: ex_unit_row, or part_rows for each
+//   seq   {sub-tiles, tokens up to the last row, COLD tokens that every row
+//         sees, query tokens n}; packed(t): the packed row of token t
+template <int DP, int WF, typename QT, bool WIDE, bool UNITS, int KW, typename LIST, typename MAP>
+__device__ __forceinline__ void ex_tile_part(const ExtendParams& p, char* lds, int h, int tile, int part, int parts,
+                                             const int4 seq, const LIST& list, MAP packed, int64_t partial,
+                                             bool dead = false) {
   constexpr int TK = WIDE ? 64 : 32;
   constexpr int NS = WIDE ? 1 : 4;          // halves a wave stages
   const int tid = threadIdx.x, lane = tid & 63, w = ex_uniform(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int b = it.x, tile = it.y & 0x3fffffff;
-  const int part = it.z & 0xffff, parts = it.z >> 16;
-  const int4 seq = p.seq[b];
-  bool pre = false;                         // a prefix's rows: through the list
-  int q0, n = seq.w;
-  int64_t list_at;
-  if constexpr (SHARED) {
-    const int where = p.seg[b].y;
-    pre = b < p.prefixes;
-    q0 = pre ? where : ex_rows(p, b - p.prefixes).x;
-    list_at = pre ? b * p.pre_subs : ex_list_of(p, b - p.prefixes, where);
-    if (dead) n = 0;
-  } else {
-    q0 = ex_rows(p, b).x;
-    list_at = int64_t(b) * p.subs_per_seq;
-  }
-  const int G = p.groups, D = p.D, kw = w % KW;   // kw: the wave's place among those of its item
-
+  const int n = dead ? 0 : seq.w;
+  const int G = p.groups, D = p.D, kw = w % KW;   // kw: the wave's place among those of its tile
   const int rows = n * G;
   const int row_first = tile * EX_WIDE, row_last = min(row_first + (WIDE ? EX_WIDE : 32), rows) - 1;
   const int lim_min = seq.y - n + row_first / G, lim_max = seq.y - n + row_last / G;
-  const int4* raw_list = p.subtile + list_at;
-  const ExList list = (ExList)(uintptr_t)raw_list;
 
   // This lane's row.
   const int r = row_first + (WIDE ? w * 32 : 0) + col;
@@ -860,8 +854,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
   f16x8 q[DP / 16];
   float qscale = fabsf(p.scale_log2);       // (its sign goes to the query)
   {
-    const int packed = pre ? p.row_list[q0 + tok] : q0 + tok;
-    const QT* src = reinterpret_cast<const QT*>(p.q) + int64_t(packed) * p.qs_t + int64_t(head) * p.qs_h;
+    const QT* src = reinterpret_cast<const QT*>(p.q) + int64_t(packed(tok)) * p.qs_t + int64_t(head) * p.qs_h;
     uint4 raw[DP / 16];
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
@@ -924,7 +917,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
     a.l = half == 0 ? float(seq.z) * exp2f(EX_BOOST) : 0.f;
   }
 
-  const int visible = dead ? 0 : ex_uniform(ex_visible(raw_list, seq.x, lim_max));
+  const int visible = dead ? 0 : ex_uniform(ex_visible(list, seq.x, lim_max));
   constexpr int ROUND = TK / 16 * KW;       // sub-tiles per round of the workgroup
   const int chunk = ((visible + parts - 1) / parts + ROUND - 1) & ~(ROUND - 1);
   const int lo = min(part * chunk, visible), hi = min(lo + chunk, visible);
@@ -986,7 +979,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
     const int tiles_n = (hi - lo + 3) / 4;
     int full = 0;
     if (tiles_n > 0) {
-      full = ex_uniform(ex_full_until(raw_list, lo, hi, lim_min));
+      full = ex_uniform(ex_full_until(list, lo, hi, lim_min));
       find(lo);
       load();
       store(tiles[0], sub, lo + 4 <= full);
@@ -1032,7 +1025,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
       }
     }
   } else if (first < hi) {
-    const int full = ex_uniform(ex_full_until(raw_list, lo, hi, lim_min));
+    const int full = ex_uniform(ex_full_until(list, lo, hi, lim_min));
     find(first);
     load();
     store(tiles[w], sub, first + TK / 16 <= full);
@@ -1061,7 +1054,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
   // Infinities and NaN of the tiles with hidden keys, for the rows that see them.
   if constexpr (WIDE) wild = __syncthreads_or(wild);
   if (wild) {
-    const int full = ex_full_until(raw_list, lo, hi, lim_min);
+    const int full = ex_full_until(list, lo, hi, lim_min);
 #pragma unroll 1
     for (int at = first; at < hi; at += ROUND) {
       if (at + TK / 16 <= full) continue;
@@ -1120,7 +1113,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
       const int row = row_first + rr;
       if (row >= rows || d >= D) continue;
       if (partial >= 0) {
-        const int64_t at = SHARED ? ex_unit_row(p, partial, h, rr) : (partial * p.kv_heads + h) * p.part_rows + rr;
+        const int64_t at = UNITS ? ex_unit_row(p, partial, h, rr) : (partial * p.kv_heads + h) * p.part_rows + rr;
         *reinterpret_cast<f32x4*>(p.part_o + at * D + d) = o;
         if (d == 0) {
           p.part_ml[at * 2] = m;
@@ -1129,14 +1122,14 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
       } else {
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
         const int tk = row / G, hd = h * G + row - tk * G;
-        QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t(q0 + tk) * p.heads + hd) * D + d;
+        QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t(packed(tk)) * p.heads + hd) * D + d;
         *reinterpret_cast<uint2*>(dst) = make_uint2(ex_out2<QT>(o[0] * inv, o[1] * inv), ex_out2<QT>(o[2] * inv, o[3] * inv));
       }
     }
   } else {
     if (!live) return;
     if (partial >= 0) {
-      const int64_t at = SHARED ? ex_unit_row(p, partial, h, r - row_first)
+      const int64_t at = UNITS ? ex_unit_row(p, partial, h, r - row_first)
                                 : (partial * p.kv_heads + h) * p.part_rows + (r - row_first);
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
@@ -1152,7 +1145,7 @@ __device__ __forceinline__ void ex_item(const ExtendParams& p, char* lds, int h,
       }
     } else {
       const float inv = a.l > 0.f ? 1.f / a.l : (a.l == 0.f ? 0.f : a.l);
-      QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t(q0 + tok) * p.heads + head) * D;
+      QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t(packed(tok)) * p.heads + head) * D;
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll

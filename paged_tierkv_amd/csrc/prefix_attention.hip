@@ -30,17 +30,15 @@
 
 namespace tierkv {
 
-#ifndef PX_LONE_
-#define PX_LONE_ 512
-#endif
-#ifndef PX_KW_
-#define PX_KW_ 2
-#endif
-constexpr int PX_LONE = PX_LONE_;       // rows (tokens times heads of a kv head) from which a request walks its prefix itself
-constexpr int PX_KW = PX_KW_;           // waves of a narrow item
+constexpr int PX_LONE = 512;            // rows (tokens times heads of a kv head) from which a request walks its prefix itself
+constexpr int PX_KW = 2;                // waves of a narrow item
 constexpr int PX_SIDE = EX_WAVES / PX_KW;   // narrow items side by side
 constexpr int PX_MIN_NARROW = 8;        // sub-tiles of a narrow item, at least, when a tile is cut
 constexpr float PX_NARROW_COST = 0.5f;  // a narrow item's sub-tile, in wide sub-tiles' time
+// A step's workgroup, in microseconds: its start and end, a wide sub-tile, a
+// round of narrow ones (alone, and how much more beside others), and what each part
+// adds to the join; and the bytes of partials per microsecond.
+constexpr double PX_COST = 7., PX_COST_WIDE = 0.5, PX_COST_ROUND = 1.7, PX_COST_SIDE = 1.8, PX_COST_PART = 0.08, PX_COST_BYTES = 3e6;
 
 // A request's prefix, -1 for none (also for a number that no prefix has).
 __device__ __forceinline__ int px_prefix(const ExtendParams& p, int b) {
@@ -50,6 +48,13 @@ __device__ __forceinline__ int px_prefix(const ExtendParams& p, int b) {
 
 __device__ __forceinline__ bool px_lone(const ExtendParams& p, int b) {
   return px_prefix(p, b) >= 0 && ex_rows(p, b).y * p.groups >= PX_LONE;
+}
+
+// Where the list of request b's sub-tiles is: behind the prefixes', or, for
+// ~where >= 0, among those of requests that walk their prefix themselves.
+__device__ __forceinline__ int64_t px_list_of(const ExtendParams& p, int b, int where) {
+  const int64_t own = p.prefixes * p.pre_subs + b * p.subs_per_seq;
+  return where >= 0 ? own : p.prefixes * p.pre_subs + p.batch * p.subs_per_seq + ~where * (p.pre_subs + p.subs_per_seq);
 }
 
 __global__ __launch_bounds__(EX_PLAN) void prefix_plan_kernel(ExtendParams p) {
@@ -120,7 +125,7 @@ __global__ __launch_bounds__(EX_PLAN) void prefix_plan_kernel(ExtendParams p) {
     tokens = total.a;
   }
   const int all_see = pre ? 0x7fffffff : tokens - n_all + 1;
-  int4* const out = p.subtile + (pre ? seg * p.pre_subs : ex_list_of(p, b, fits ? where : 0));
+  int4* const out = p.subtile + (pre ? seg * p.pre_subs : px_list_of(p, b, fits ? where : 0));
   if (pre_blocks && fits) ex_walk(p, p.pre_table + pre_row, p.pre_states + pre_row, p.pre_lengths + pre_row, pre_blocks, all_see, out, sh, list);
   if (own_blocks && fits) ex_walk(p, p.table + row, p.states + row, p.lengths + row, own_blocks, all_see, out, sh, list);
   if (tid == 0) {
@@ -274,6 +279,16 @@ __global__ __launch_bounds__(EX_PLAN) void prefix_plan_kernel(ExtendParams p) {
   }
 }
 
+template <int DP, int WF, typename QT, bool WIDE>
+__device__ __forceinline__ void px_item(const ExtendParams& p, char* lds, int h, const ex_int4 it, bool dead) {
+  const int s = it.x, where = p.seg[s].y;
+  const bool pre = s < p.prefixes;
+  const int q0 = pre ? where : ex_rows(p, s - p.prefixes).x;
+  const ExWorkspaceList list = {p.subtile + (pre ? s * p.pre_subs : px_list_of(p, s - p.prefixes, where))};
+  ex_tile_part<DP, WF, QT, WIDE, true, WIDE ? 1 : PX_KW>(p, lds, h, it.y, it.z & 0xffff, it.z >> 16, p.seq[s], list,
+                                                         [&](int t) { return pre ? p.row_list[q0 + t] : q0 + t; }, it.w, dead);
+}
+
 // Workgroups take wide items one by one, then narrow ones PX_SIDE at a time,
 // until none is left: the first by their number, the others from a counter.
 template <int DP, int WF, typename QT, bool MIXED>
@@ -289,14 +304,14 @@ __global__ __launch_bounds__(EX_THREADS, 2) void prefix_kernel(ExtendParams p) {
     if (MIXED && j < wide) {
       const int i = j / p.kv_heads, h = j - i * p.kv_heads;
       const ex_int4 it = ((ExList)(uintptr_t)p.item)[i];
-      if (it.x >= 0) ex_item<DP, WF, QT, true, true, 1>(p, px_lds, h, it, it.w);
+      if (it.x >= 0) px_item<DP, WF, QT, true>(p, px_lds, h, it, false);
     } else {
       const int u = (j - wide) * PX_SIDE + ex_uniform(threadIdx.x >> 6) / PX_KW;
       const int x = min(u, narrow - 1), i = x / p.kv_heads, h = x - i * p.kv_heads;
       ex_int4 it = ((ExList)(uintptr_t)p.item)[p.max_items - 1 - i];
       const bool dead = u >= narrow || it.x < 0;
       if (it.x < 0) it.x = 0;
-      ex_item<DP, WF, QT, false, true, PX_KW>(p, px_lds, h, it, it.w, dead);
+      px_item<DP, WF, QT, false>(p, px_lds, h, it, dead);
     }
     if (threadIdx.x == 0) s_next = next;
     __syncthreads();
@@ -353,6 +368,298 @@ __global__ __launch_bounds__(EX_THREADS) void prefix_join_kernel(ExtendParams p)
   j.put<QT>(p, r, hd, d);
 }
 
+// ---------------------------------------------------------------------------
+// Steps of a few tokens per request
+// ---------------------------------------------------------------------------
+// Where no request brings more than 32 rows (single tokens, drafts), the plan
+// would cost as much as the attention: a launch of its own, and five dependent
+// reads between it and an item's first key.  These calls are laid out on the
+// host, from sizes alone: every request's table row is cut into own_parts
+// ranges of blocks, every prefix's into pre_parts, and a workgroup lists the
+// sub-tiles of its range in LDS itself.  A prefix's rows fill tiles ("slots")
+// of 256; how many there are follows from the requests' prefixes, which each
+// workgroup of a slot reads.  Two launches: the parts, and their join.
+
+constexpr int PX_LIST = 416;       // sub-tiles that a workgroup lists
+constexpr int PX_MOST = 8;         // requests' parts side by side in a workgroup, where it is not one
+
+// A step's workgroup's LDS beside the tiles'.
+struct PxShared {
+  int4 list[PX_LIST + 4 * PX_MOST];   // (spare entries behind each part's, which may be read)
+  int rows[EX_WIDE + 4];              // packed rows of a tile's tokens
+  int2 scan[EX_WAVES];
+  int found[4];
+};
+static_assert(ex_lds_bytes<128>() + sizeof(PxShared) + 256 <= 160 * 1024 && ex_lds_bytes<64>() <= ex_lds_bytes<128>(),
+              "a CU's LDS, 256 bytes of it for a vote of the workgroup");
+
+// Sub-tiles in LDS.
+struct PxList {
+  const int4* list;
+  __device__ __forceinline__ int4 any(int i) const { return list[i]; }
+  __device__ __forceinline__ ex_int4 one(int i) const {
+    const int4 v = list[i];
+    return ex_int4{ex_uniform(v.x), ex_uniform(v.y), ex_uniform(v.z), 0};
+  }
+};
+
+struct PxBlock {
+  int len, slot, state, keep, count;   // keep: 1 resident, 2 COLD that enters with logit 0; sub-tiles
+};
+
+// Block i of a table row, from `end` on an empty one.
+__device__ __forceinline__ PxBlock px_block(const ExtendParams& p, const int32_t* table, const int32_t* states,
+                                            const int32_t* lengths, int i, int end) {
+  PxBlock o = {0, 0, COLD, 0, 0};
+  if (i < end) {
+    o.len = min(max(lengths[i], 0), p.bs);
+    o.state = states[i];
+    o.slot = table[i];
+  }
+  if (o.len > 0) {
+    if (o.state == HOT || o.state == WARM) {
+      const int64_t slots = o.state == HOT ? p.hot_slots : p.warm_slots;
+      if (o.slot >= 0 && o.slot < slots) o.keep = 1;
+      else atomicOr(p.err, 1);
+    } else if (o.state != COLD) {
+      atomicOr(p.err, 2);
+    } else if (p.cold_zero) {
+      o.keep = 2;
+    }
+  }
+  o.count = o.keep ? (o.len + EX_SUB - 1) / EX_SUB : 0;
+  return o;
+}
+
+__device__ __forceinline__ void px_enter(int4* list, const PxBlock& k, int count, int first) {
+  const int code = k.state == COLD ? EX_STATE_ZERO : k.state;
+  for (int j = 0; j < count; ++j)
+    list[j] = make_int4(k.slot, min(k.len - j * EX_SUB, EX_SUB) | (code << 8) | (j << 16), first + j * EX_SUB, 0);
+}
+
+// Inclusive sums of two values over groups of W waves, and the groups' sums.
+template <int W>
+__device__ __forceinline__ int2 px_scan(int a, int b, int2 (&sh)[EX_WAVES], int2* total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, w0 = w / W * W;
+  int2 v = make_int2(wave_inclusive_scan(a), wave_inclusive_scan(b));
+  __syncthreads();
+  if (lane == 63) sh[w] = v;
+  __syncthreads();
+  int2 all = make_int2(0, 0);
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const int2 t = sh[w0 + i];
+    if (w0 + i < w) {
+      v.x += t.x;
+      v.y += t.y;
+    }
+    all.x += t.x;
+    all.y += t.y;
+  }
+  *total = all;
+  return v;
+}
+
+// What a part of a step takes: one of a slot's rows, for one kv head, or of a
+// request's own.
+struct PxPart {
+  int h, tile, rows;       // rows: of the slot's prefix or of the request
+  int4 seq;
+  const int4* list;
+  int64_t unit;
+  int first;               // packed row of token 0, or, with a map, the token of its first entry
+  const int* map;
+  bool dead;
+};
+
+// A slot's; dead where there is none.
+template <bool MIXED>
+__device__ __forceinline__ PxPart px_step_prefix(const ExtendParams& p, char* lds, PxShared& s, int x) {
+  const int tid = threadIdx.x, G = p.groups;
+  const int h = x % p.kv_heads, part = x / p.kv_heads % p.pre_parts, slot = x / p.kv_heads / p.pre_parts;
+  // The slot's prefix g, its tile of it, and the prefix's rows.
+  int* const counts = reinterpret_cast<int*>(lds);
+  for (int i = tid; i < p.prefixes; i += EX_THREADS) counts[i] = 0;
+  if (tid == 0) s.found[0] = -1;
+  __syncthreads();
+  for (int i = tid; i < p.batch; i += EX_THREADS) {
+    const int k = px_prefix(p, i);
+    if (k >= 0) atomicAdd(counts + k, ex_rows(p, i).y);
+  }
+  __syncthreads();
+  int2 total;
+  int before = 0;
+  for (int i0 = 0; i0 < p.prefixes; i0 += EX_THREADS) {
+    const int i = i0 + tid, n = i < p.prefixes ? counts[i] : 0;
+    const int tiles = (n * G + EX_WIDE - 1) / EX_WIDE;
+    const int2 v = px_scan<EX_WAVES>(tiles, 0, s.scan, &total);
+    const int first = before + v.x - tiles;
+    if (slot >= first && slot < first + tiles) {
+      s.found[0] = i;
+      s.found[1] = slot - first;
+      s.found[2] = n;
+    }
+    before += total.x;
+  }
+  if (before > p.pre_slots && tid == 0) atomicOr(p.err, 4);   // (packed ranges that overlap)
+  __syncthreads();
+  const int g = ex_uniform(s.found[0]), t = ex_uniform(s.found[1]), n = ex_uniform(s.found[2]);
+  PxPart o{};
+  o.dead = g < 0;
+  if (g < 0) return o;
+  // The tile's tokens, in the order of their requests.
+  const int row0 = t * EX_WIDE, t0 = row0 / G, t1 = min((min(row0 + EX_WIDE, n * G) + G - 1) / G, n);
+  before = 0;
+  for (int i0 = 0; i0 < p.batch; i0 += EX_THREADS) {
+    const int i = i0 + tid;
+    int2 r = make_int2(0, 0);
+    if (i < p.batch && px_prefix(p, i) == g) r = ex_rows(p, i);
+    const int2 v = px_scan<EX_WAVES>(r.y, 0, s.scan, &total);
+    const int place = before + v.x - r.y;
+    for (int k = max(t0 - place, 0); k < min(t1 - place, r.y); ++k) {
+      s.rows[place + k - t0] = r.x + k;
+      // Where its rows are among the slots', by the tile that its first is in.
+      if (h == 0 && part == 0 && (place + k) * G >= row0) p.row_pre[r.x + k] = make_int2(i, (slot - t) * EX_WIDE + (place + k) * G);
+    }
+    before += total.x;
+  }
+  // The part's sub-tiles.
+  const int nb = p.pre_nblocks ? min(max(p.pre_nblocks[g], 0), p.pre_blocks) : p.pre_blocks;
+  const int per = (nb + p.pre_parts - 1) / p.pre_parts, k0 = min(part * per, nb), k1 = min(k0 + per, nb);
+  const int64_t row = g * p.pre_stride;
+  int subs = 0, cold = 0;
+  for (int i0 = k0; i0 < k1; i0 += EX_THREADS) {
+    const PxBlock k = px_block(p, p.pre_table + row, p.pre_states + row, p.pre_lengths + row, i0 + tid, k1);
+    const int count = k.keep == 2 ? 0 : k.count;   // (every row sees them: a count)
+    const int2 v = px_scan<EX_WAVES>(count, k.keep == 2 ? k.len : 0, s.scan, &total);
+    px_enter(s.list + subs + v.x - count, k, count, 0);
+    subs += total.x;
+    cold += total.y;
+  }
+  __syncthreads();
+  o.h = h;
+  o.tile = t;
+  o.rows = n * G;
+  o.seq = make_int4(subs, n + 64, cold, n);   // (every row sees every token: limits past a sub-tile's end)
+  o.list = s.list;
+  o.unit = (int64_t(slot) * p.pre_parts + part) * (MIXED ? EX_WIDE / EX_UNIT : 1);
+  o.first = t0;
+  o.map = s.rows;
+  return o;
+}
+
+// A request's, EX_WAVES / KW side by side.
+template <int KW>
+__device__ __forceinline__ PxPart px_step_own(const ExtendParams& p, PxShared& s, int x) {
+  constexpr int SIDE = EX_WAVES / KW, THREADS = 64 * KW;
+  const int w = ex_uniform(threadIdx.x >> 6), mine = w / KW, tid = threadIdx.x % THREADS;
+  const int64_t units = int64_t(p.batch) * p.own_parts * p.kv_heads;
+  const int64_t u = int64_t(x) * SIDE + mine;
+  const bool dead = u >= units;
+  const int64_t v0 = min(u, units - 1);
+  const int h = int(v0 % p.kv_heads), part = int(v0 / p.kv_heads % p.own_parts), b = int(v0 / p.kv_heads / p.own_parts);
+  int n_all;
+  const int2 rows = ex_rows(p, b, &n_all);
+  const int q0 = rows.x, n = rows.y, g = px_prefix(p, b);
+  if (h == 0 && part == 0 && !dead) {
+    for (int i = tid; i < min(n_all, p.rows - q0); i += THREADS) p.row_home[q0 + i] = make_int4(i < n ? b : -1, i, g, 0);
+    if (n < n_all && tid == 0) atomicOr(p.err, 4);
+  }
+  const int nb = p.seq_nblocks ? min(max(p.seq_nblocks[b], 0), p.num_blocks) : p.num_blocks;
+  const int per = (nb + p.own_parts - 1) / p.own_parts, k0 = min(part * per, nb), k1 = min(k0 + per, nb);
+  const int64_t row = int64_t(b) * p.stride;
+  const PxBlock k = px_block(p, p.table + row, p.states + row, p.lengths + row, k0 + tid, k1);   // (per <= THREADS)
+  // Tokens before the part and in all.
+  int2 total;
+  int below = 0, held = 0;
+  for (int i = tid; i < nb; i += THREADS) {
+    const int len = min(max(p.lengths[row + i], 0), p.bs);
+    held += len;
+    if (i < k0) below += len;
+  }
+  px_scan<KW>(below, held, s.scan, &total);
+  const int base = total.x, tokens = total.y;
+  const int2 lens = px_scan<KW>(k.len, 0, s.scan, &total);
+  const int first = base + lens.x - k.len;
+  const bool all_see = k.keep == 2 && first + k.len <= tokens - n_all + 1;
+  const int count = all_see ? 0 : k.count;
+  const int2 v = px_scan<KW>(count, all_see ? k.len : 0, s.scan, &total);
+  int4* const list = s.list + mine * (PX_LIST / SIDE + 4);
+  px_enter(list + v.x - count, k, count, first);
+  __syncthreads();
+  PxPart o{};
+  o.h = h;
+  o.rows = n * p.groups;
+  o.seq = make_int4(total.x, tokens - (n_all - n), total.y, n);
+  o.list = list;
+  o.unit = p.own_unit + int64_t(b) * p.own_parts + part;
+  o.first = q0;
+  o.dead = dead || n == 0;
+  return o;
+}
+
+// MIXED: calls that may hold wide tiles; the others' kernel is without their code.
+template <int DP, int WF, typename QT, bool MIXED>
+__global__ __launch_bounds__(EX_THREADS, 2) void prefix_step_kernel(ExtendParams p) {
+  extern __shared__ __attribute__((aligned(16))) char px_lds[];
+  __shared__ PxShared s;
+  const int pre = p.pre_slots * p.pre_parts * p.kv_heads, x = blockIdx.x;
+  PxPart o;
+  int side = 1;
+  if (x < pre) {
+    o = px_step_prefix<MIXED>(p, px_lds, s, x);
+    if (o.dead) return;
+  } else {
+    side = p.own_side;
+    if (side == 1) o = px_step_own<EX_WAVES>(p, s, x - pre);
+    else o = px_step_own<EX_WAVES / PX_MOST>(p, s, x - pre);
+  }
+  auto packed = [&](int t) { return o.map ? o.map[max(t - o.first, 0)] : o.first + t; };
+  const PxList list = {o.list};
+  if (MIXED && o.rows > EX_NARROW) ex_tile_part<DP, WF, QT, true, true, 1>(p, px_lds, o.h, o.tile, 0, 1, o.seq, list, packed, o.unit);
+  else if (side == 1) ex_tile_part<DP, WF, QT, false, true, EX_WAVES>(p, px_lds, o.h, o.tile, 0, 1, o.seq, list, packed, o.unit, o.dead);
+  else ex_tile_part<DP, WF, QT, false, true, EX_WAVES / PX_MOST>(p, px_lds, o.h, o.tile, 0, 1, o.seq, list, packed, o.unit, o.dead);
+}
+
+template <typename QT>
+__global__ __launch_bounds__(EX_THREADS) void prefix_step_join_kernel(ExtendParams p, int32_t each) {
+  const int D4 = p.D / 4, G = p.groups;
+  const int64_t x = int64_t(blockIdx.x) * EX_THREADS + threadIdx.x;
+  const int64_t rh = x / D4;
+  const int d = 4 * int(x - rh * D4);
+  const int64_t r = rh / p.heads;
+  if (r >= p.rows) return;
+  const int hd = int(rh - r * p.heads), h = hd / G;
+  const int4 home = p.row_home[r];
+  const int2 of = p.row_pre[r];
+  // (a row of no request has whatever the workspace held)
+  if (home.x < 0 || home.x >= p.batch) return;
+  const int2 rows_of = ex_rows(p, home.x);
+  if (home.y < 0 || home.y >= rows_of.y || int(r) - rows_of.x != home.y) return;
+  const int64_t step = int64_t(p.kv_heads) * EX_UNIT;
+  const int64_t at = ex_unit_row(p, p.own_unit + int64_t(home.x) * p.own_parts, h, home.y * G + hd - h * G);
+  int pre_count = 0;
+  int64_t pre_at = 0;
+  if (home.z >= 0) {
+    const int64_t row = int64_t(of.y) + hd - h * G, slot = row / EX_WIDE;
+    if (of.x != home.x || of.y < 0 || slot >= p.pre_slots) return;
+    pre_count = p.pre_parts;
+    pre_at = ex_unit_row(p, slot * p.pre_parts * each, h, int(row - slot * EX_WIDE));
+  }
+  const int count = p.own_parts + pre_count;
+  auto place = [&](int k) { return k < p.own_parts ? at + k * step : pre_at + (k - p.own_parts) * each * step; };
+  ExJoin j;
+  int k0 = 0;
+  for (; count - k0 > 4; k0 += 8) j.take<8>(p, count - k0, d, [&](int k) { return place(k0 + k); });
+  if (count - k0 > 2) j.take<4>(p, count - k0, d, [&](int k) { return place(k0 + k); });
+  else if (count - k0 > 0) j.take<2>(p, count - k0, d, [&](int k) { return place(k0 + k); });
+  j.put<QT>(p, r, hd, d);
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+
 struct PrefixLayout {
   int64_t arrived, head, seq, seg, tile, row_list, row_home, subtile, item, part_o, part_ml, total;
   int64_t subs, pre_subs, lone, tiles, wide_items, items, units;
@@ -396,6 +703,66 @@ static PrefixLayout prefix_layout(int64_t batch, int64_t prefixes, int64_t rows,
   return l;
 }
 
+// A step's layout: how many ranges the tables' rows are cut into, and where
+// its workspace lies.  parts are rated by the time of their workgroups, one per
+// CU at a time, in microseconds measured on steps of 1 to 256 requests.
+struct StepLayout {
+  int64_t row_home, row_pre, part_o, part_ml, total;
+  int64_t slots, pre_parts, own_parts, side, each, own_unit, units, workgroups;
+  bool use;
+};
+
+static StepLayout step_layout(int64_t batch, int64_t prefixes, int64_t rows, int64_t max_tokens, int64_t groups,
+                              int64_t kv_heads, int64_t num_blocks, int64_t pre_blocks, int64_t bs, int64_t D) {
+  StepLayout l{};
+  const int64_t all = std::min(rows, batch * max_tokens) * groups, longest = std::min(rows, max_tokens) * groups;
+  l.use = longest <= EX_NARROW;
+  if (!l.use || rows == 0) return l;
+  auto up = [](int64_t x) { return (x + 255) & ~int64_t(255); };
+  auto div = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const int64_t subs = div(bs, EX_SUB), fit = PX_LIST / subs;
+  const bool wide = all > EX_NARROW;
+  l.each = wide ? EX_WIDE / EX_UNIT : 1;
+  const int64_t groups_n = std::min(prefixes, batch);
+  l.slots = all / EX_WIDE + groups_n;
+  // The slots there are when the requests are spread evenly over the prefixes.
+  const int64_t live = groups_n * div(div(all, groups_n), EX_WIDE);
+  const bool pre_wide = div(all, groups_n) > EX_NARROW;
+  double best = 0;
+  for (int64_t side : {1, PX_MOST}) {
+    const int64_t own_fit = fit / side, least_own = div(num_blocks, own_fit), least_pre = div(pre_blocks, fit);
+    const int64_t waves = EX_WAVES / side;
+    for (int64_t own = least_own; own <= std::max<int64_t>(least_own, 8); own *= 2) {
+      for (int64_t pre = least_pre, last = 0; last == 0; pre = pre < 4 ? pre + 1 : pre + pre * 2 / 5) {
+        if (pre >= std::max<int64_t>(least_pre, 64)) last = 1;
+        const double pre_subs = double(div(pre_blocks, pre) * subs), own_subs = double(div(num_blocks, own) * subs);
+        const double c_pre = PX_COST + (pre_wide ? PX_COST_WIDE * pre_subs : PX_COST_ROUND * std::ceil(pre_subs / (2 * EX_WAVES)));
+        const double c_own = PX_COST + PX_COST_ROUND * std::ceil(own_subs / (2 * waves)) * (side > 1 ? PX_COST_SIDE : 1.);
+        const double n_pre = double(live * pre * kv_heads), n_own = double(div(batch * own * kv_heads, side));
+        const double sum = (n_pre * c_pre + n_own * c_own) / EX_SLOTS, most = std::max(c_pre, c_own);
+        const double makespan = n_pre + n_own <= EX_SLOTS ? most : std::max(most, sum + 0.5 * std::min(c_pre, c_own));
+        const double bytes = (double(all) * pre + double(batch) * longest * own) * kv_heads * D * 4;
+        const double time = makespan + PX_COST_PART * (pre + own) + 2 * bytes / PX_COST_BYTES;
+        if (best == 0 || time < best) {
+          best = time;
+          l.side = side;
+          l.own_parts = own;
+          l.pre_parts = pre;
+        }
+      }
+    }
+  }
+  l.own_unit = l.slots * l.pre_parts * l.each;
+  l.units = l.own_unit + batch * l.own_parts;
+  l.workgroups = l.slots * l.pre_parts * kv_heads + div(batch * l.own_parts * kv_heads, l.side);
+  l.row_home = EX_WS_HEAD;
+  l.row_pre = up(l.row_home + rows * 16);
+  l.part_ml = up(l.row_pre + rows * 8);
+  l.part_o = up(l.part_ml + l.units * kv_heads * EX_UNIT * 8);
+  l.total = up(l.part_o + l.units * kv_heads * EX_UNIT * D * 4);
+  return l;
+}
+
 template <int DP, int WF, typename QT>
 static void prefix_launch(const ExtendParams& p, bool wide, hipStream_t stream) {
   const int lds = ex_lds_bytes<DP>();
@@ -409,13 +776,31 @@ static void prefix_launch(const ExtendParams& p, bool wide, hipStream_t stream) 
                      stream, p);
 }
 
+template <int DP, int WF, typename QT>
+static void step_launch(const ExtendParams& p, const StepLayout& l, hipStream_t stream) {
+  const int lds = ex_lds_bytes<DP>();
+  const dim3 grid(uint32_t(l.workgroups));
+  if (l.each > 1) hipLaunchKernelGGL((prefix_step_kernel<DP, WF, QT, true>), grid, dim3(EX_THREADS), lds, stream, p);
+  else hipLaunchKernelGGL((prefix_step_kernel<DP, WF, QT, false>), grid, dim3(EX_THREADS), lds, stream, p);
+  const int64_t threads = int64_t(p.rows) * p.heads * (p.D / 4);
+  hipLaunchKernelGGL(prefix_step_join_kernel<QT>, dim3(uint32_t((threads + EX_THREADS - 1) / EX_THREADS)), dim3(EX_THREADS), 0,
+                     stream, p, int32_t(l.each));
+}
+
+// step: NULL for calls that are planned on the device.
+template <int DP, int WF, typename QT>
+static void prefix_start(const ExtendParams& p, const StepLayout* step, bool wide, hipStream_t stream) {
+  if (step) step_launch<DP, WF, QT>(p, *step, stream);
+  else prefix_launch<DP, WF, QT>(p, wide, stream);
+}
+
 template <int DP>
-static void prefix_dispatch(const ExtendParams& p, bool wide, int wf, int dtype, hipStream_t stream) {
+static void prefix_dispatch(const ExtendParams& p, const StepLayout* step, bool wide, int wf, int dtype, hipStream_t stream) {
   const bool bf = dtype == TIERKV_DTYPE_BF16, i8 = wf == TIERKV_WARM_ABSMAX_I8;
-  if (bf && i8) prefix_launch<DP, TIERKV_WARM_ABSMAX_I8, __hip_bfloat16>(p, wide, stream);
-  else if (bf) prefix_launch<DP, TIERKV_WARM_REF_U8, __hip_bfloat16>(p, wide, stream);
-  else if (i8) prefix_launch<DP, TIERKV_WARM_ABSMAX_I8, __half>(p, wide, stream);
-  else prefix_launch<DP, TIERKV_WARM_REF_U8, __half>(p, wide, stream);
+  if (bf && i8) prefix_start<DP, TIERKV_WARM_ABSMAX_I8, __hip_bfloat16>(p, step, wide, stream);
+  else if (bf) prefix_start<DP, TIERKV_WARM_REF_U8, __hip_bfloat16>(p, step, wide, stream);
+  else if (i8) prefix_start<DP, TIERKV_WARM_ABSMAX_I8, __half>(p, step, wide, stream);
+  else prefix_start<DP, TIERKV_WARM_REF_U8, __half>(p, step, wide, stream);
 }
 
 }  // namespace tierkv
@@ -429,8 +814,12 @@ extern "C" int64_t tierkv_prefix_workspace_bytes(int32_t batch, int32_t num_pref
   if (batch <= 0 || num_prefixes <= 0 || num_rows < 0 || max_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
       num_heads % num_kv_heads != 0 || num_blocks <= 0 || num_prefix_blocks <= 0 || block_size <= 0 || head_dim <= 0)
     return -1;
-  return prefix_layout(batch, num_prefixes, num_rows, max_tokens, num_heads / num_kv_heads, num_kv_heads, num_blocks,
-                       num_prefix_blocks, block_size, head_dim).total;
+  const int groups = num_heads / num_kv_heads;
+  const StepLayout s = step_layout(batch, num_prefixes, num_rows, max_tokens, groups, num_kv_heads, num_blocks,
+                                   num_prefix_blocks, block_size, head_dim);
+  if (s.use) return std::max<int64_t>(s.total, EX_WS_HEAD);
+  return prefix_layout(batch, num_prefixes, num_rows, max_tokens, groups, num_kv_heads, num_blocks, num_prefix_blocks,
+                       block_size, head_dim).total;
 }
 
 extern "C" int32_t tierkv_prefix_attention(
@@ -461,34 +850,50 @@ extern "C" int32_t tierkv_prefix_attention(
     return fail(TIERKV_ERR_UNSUPPORTED, "more than 4096 requests and prefixes");
   if (int64_t(num_prefix_blocks) * block_size + num_rows > 0x7fffffff - EX_SUB)
     return fail(TIERKV_ERR_UNSUPPORTED, "prefixes of 2^31 tokens or more");
-  const PrefixLayout l = prefix_layout(batch, num_prefixes, num_rows, max_tokens, p.groups, num_kv_heads, num_blocks,
-                                       num_prefix_blocks, block_size, head_dim);
+  const StepLayout step = step_layout(batch, num_prefixes, num_rows, max_tokens, p.groups, num_kv_heads, num_blocks,
+                                      num_prefix_blocks, block_size, head_dim);
+  const PrefixLayout l = step.use ? PrefixLayout{}
+                                  : prefix_layout(batch, num_prefixes, num_rows, max_tokens, p.groups, num_kv_heads,
+                                                  num_blocks, num_prefix_blocks, block_size, head_dim);
   // (a launch has fewer than 2^32 threads)
-  if (l.items * num_kv_heads > 0x7fffffff ||
-      int64_t(num_rows) * num_heads > (0xffffffffll - EX_THREADS) / (head_dim / 4) || l.units > 0x7fffffff)
+  if (l.items * num_kv_heads > 0x7fffffff || step.workgroups > 0xffffffffll / EX_THREADS ||
+      int64_t(num_rows) * num_heads > (0xffffffffll - EX_THREADS) / (head_dim / 4) || std::max(l.units, step.units) > 0x7fffffff)
     return fail(TIERKV_ERR_UNSUPPORTED, "grid too large");
-  if (workspace_bytes < l.total) return fail(TIERKV_ERR_WORKSPACE, "workspace too small");
+  if (workspace_bytes < (step.use ? std::max<int64_t>(step.total, EX_WS_HEAD) : l.total))
+    return fail(TIERKV_ERR_WORKSPACE, "workspace too small");
   if (num_rows == 0 || max_tokens == 0) return TIERKV_OK;
   char* ws = reinterpret_cast<char*>(workspace);
   p.err = reinterpret_cast<int32_t*>(ws);
-  p.arrived = reinterpret_cast<uint32_t*>(ws + l.arrived);
-  p.head = reinterpret_cast<int32_t*>(ws + l.head);
-  p.seq = reinterpret_cast<int4*>(ws + l.seq);
-  p.seg = reinterpret_cast<int2*>(ws + l.seg);
-  p.tile = reinterpret_cast<int2*>(ws + l.tile);
-  p.row_list = reinterpret_cast<int32_t*>(ws + l.row_list);
-  p.row_home = reinterpret_cast<int4*>(ws + l.row_home);
-  p.subtile = reinterpret_cast<int4*>(ws + l.subtile);
-  p.item = reinterpret_cast<int4*>(ws + l.item);
-  p.part_o = reinterpret_cast<float*>(ws + l.part_o);
-  p.part_ml = reinterpret_cast<float*>(ws + l.part_ml);
-  p.max_items = int32_t(l.items);
-  p.max_cut = int32_t(l.wide_items);
-  p.max_lone = int32_t(l.lone);
-  p.max_tiles = int32_t(l.tiles);
-  p.max_part = int32_t(l.units);
-  p.subs_per_seq = l.subs;
-  p.pre_subs = l.pre_subs;
+  if (step.use) {
+    p.row_home = reinterpret_cast<int4*>(ws + step.row_home);
+    p.row_pre = reinterpret_cast<int2*>(ws + step.row_pre);
+    p.part_o = reinterpret_cast<float*>(ws + step.part_o);
+    p.part_ml = reinterpret_cast<float*>(ws + step.part_ml);
+    p.pre_slots = int32_t(step.slots);
+    p.pre_parts = int32_t(step.pre_parts);
+    p.own_parts = int32_t(step.own_parts);
+    p.own_side = int32_t(step.side);
+    p.own_unit = step.own_unit;
+  } else {
+    p.arrived = reinterpret_cast<uint32_t*>(ws + l.arrived);
+    p.head = reinterpret_cast<int32_t*>(ws + l.head);
+    p.seq = reinterpret_cast<int4*>(ws + l.seq);
+    p.seg = reinterpret_cast<int2*>(ws + l.seg);
+    p.tile = reinterpret_cast<int2*>(ws + l.tile);
+    p.row_list = reinterpret_cast<int32_t*>(ws + l.row_list);
+    p.row_home = reinterpret_cast<int4*>(ws + l.row_home);
+    p.subtile = reinterpret_cast<int4*>(ws + l.subtile);
+    p.item = reinterpret_cast<int4*>(ws + l.item);
+    p.part_o = reinterpret_cast<float*>(ws + l.part_o);
+    p.part_ml = reinterpret_cast<float*>(ws + l.part_ml);
+    p.max_items = int32_t(l.items);
+    p.max_cut = int32_t(l.wide_items);
+    p.max_lone = int32_t(l.lone);
+    p.max_tiles = int32_t(l.tiles);
+    p.max_part = int32_t(l.units);
+    p.subs_per_seq = l.subs;
+    p.pre_subs = l.pre_subs;
+  }
   p.prefix_of = prefix_of;
   p.pre_table = prefix_table;
   p.pre_states = prefix_states;
@@ -498,7 +903,8 @@ extern "C" int32_t tierkv_prefix_attention(
   p.pre_blocks = num_prefix_blocks;
   p.prefixes = num_prefixes;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  if (head_dim <= 64) prefix_dispatch<64>(p, l.wide, warm_format, query_dtype, stream);
-  else prefix_dispatch<128>(p, l.wide, warm_format, query_dtype, stream);
+  const StepLayout* of = step.use ? &step : nullptr;
+  if (head_dim <= 64) prefix_dispatch<64>(p, of, l.wide, warm_format, query_dtype, stream);
+  else prefix_dispatch<128>(p, of, l.wide, warm_format, query_dtype, stream);
   return check_launch("tierkv_prefix_attention");
 }

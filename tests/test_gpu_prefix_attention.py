@@ -330,7 +330,7 @@ def test_replays_match_eager_calls(device):
         check(out, r, "masked")
     assert ws.error_word() == 0
     with pytest.raises(RuntimeError):
-        launch(t, s, "masked", workspace=extend_workspace(device, 4, 7, 8, 2, 1, 64))
+        launch(t, s, "masked", workspace=DecodeWorkspace(device, 4096, growable=False))
 
 
 def test_threads_and_streams_get_their_own_results(device):
