@@ -373,7 +373,9 @@ extern "C" int32_t tierkv_rotate_rows(
     return fail(TIERKV_ERR_INVALID, "attention_scaling must be finite and eps finite and not negative");
   const bool pools = slots || hot_k || hot_v || value;
   if (pools) {
-    if (!slots || !hot_k || !hot_v || !value) return fail(TIERKV_ERR_INVALID, "slots, value and both HOT pools go together");
+    // (no rows: their tensors have no address)
+    if (!hot_k || !hot_v || (num_rows > 0 && (!slots || !value)))
+      return fail(TIERKV_ERR_INVALID, "slots, value and both HOT pools go together");
     if (block_size <= 0 || block_size > 64) return fail(TIERKV_ERR_UNSUPPORTED, "block_size must be in [1, 64]");
     if (hot_slots <= 0 || hot_slots * block_size > 0x7fffffff)
       return fail(TIERKV_ERR_UNSUPPORTED, "pool rows must lie in (0, 2^31)");

@@ -361,44 +361,68 @@ def write_slots(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, hot
 _HALVES = (torch.float16, torch.bfloat16)
 
 
-def _packed_rows(t, name: str, rows: int, heads: int, dim: int, dtype, index: int):
+def _is(t, dtype, shape, index: int) -> bool:
+    """Whether t is a contiguous tensor of this dtype, shape and device."""
+    return (isinstance(t, torch.Tensor) and t.dtype == dtype and t.get_device() == index and t.shape == shape
+            and t.is_contiguous())
+
+
+def _packed_rows(t, name: str, shape, dtype, index: int):
     """Packed rows [rows, heads, dim] with the last dim contiguous (copied
     where it is not)."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != (rows, heads, dim):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name} must be [tokens, heads, head_dim] of the step's geometry and the rows' dtype.")
     if t.get_device() != index:
         raise ValueError("rows, tables and pools must be on one device.")
-    return t if t.stride(2) == 1 or dim == 1 else t.contiguous()
+    return t if t.stride(2) == 1 or shape[2] == 1 else t.contiguous()
 
 
-def _out_rows(t, name: str, shape, dtype, device):
+def _out_rows(t, name: str, shape, dtype, device, index: int):
     if t is None:
         return torch.empty(shape, dtype=dtype, device=device)
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
+    if not _is(t, dtype, shape, index):
         raise ValueError(f"{name} must be a contiguous tensor of the rows' shape, dtype and device.")
     return t
 
 
+def _step_i32(t, name: str, shape, index: int) -> None:
+    if not _is(t, torch.int32, shape, index):
+        _require_i32(t, name, shape)
+        raise ValueError("rows, tables and pools must be on one device.")
+
+
+def _hot_pools(hot_k, hot_v, index: int) -> None:
+    if not (isinstance(hot_k, torch.Tensor) and hot_k.ndim == 4 and _is(hot_k, torch.float16, hot_k.shape, index)
+            and _is(hot_v, torch.float16, hot_k.shape, index)):
+        _check_tiles(hot_k, "hot_k", torch.float16)
+        _check_tiles(hot_v, "hot_v", torch.float16)
+        if hot_v.shape != hot_k.shape:
+            raise ValueError("K and V pools must have identical shapes.")
+        raise ValueError("rows, tables and pools must be on one device.")
+
+
 def _warm_pools(warm_k, warm_v, k_scale, k_zero, v_scale, v_zero, fmt: int, index: int) -> None:
     """Check WARM pools and their metadata (``fmt``: WARM_FORMATS' value)."""
-    dtype = torch.uint8 if fmt == _lib.WARM_REF_U8 else torch.int8
-    _check_tiles(warm_k, "warm_k", dtype)
-    _check_tiles(warm_v, "warm_v", dtype)
-    if warm_v.shape != warm_k.shape:
-        raise ValueError("K and V pools must have identical shapes.")
-    slots, kv_heads, bs, _ = warm_k.shape
     ref = fmt == _lib.WARM_REF_U8
-    metas = (k_scale, k_zero, v_scale, v_zero) if ref else (k_scale, v_scale)
-    if any(t is None for t in metas):
-        raise ValueError("WARM pools need their scales, reference-format ones their zero points.")
-    for t in metas:
+    dtype = torch.uint8 if ref else torch.int8
+    if not (isinstance(warm_k, torch.Tensor) and warm_k.ndim == 4 and _is(warm_k, dtype, warm_k.shape, index)
+            and _is(warm_v, dtype, warm_k.shape, index)):
+        _check_tiles(warm_k, "warm_k", dtype)
+        _check_tiles(warm_v, "warm_v", dtype)
+        if warm_v.shape != warm_k.shape:
+            raise ValueError("K and V pools must have identical shapes.")
+        raise ValueError("rows, tables and pools must be on one device.")
+    slots, kv_heads, bs, _ = warm_k.shape
+    entries, kind = (slots * kv_heads * bs, torch.float16) if ref else (slots * kv_heads, torch.float32)
+    for t in (k_scale, k_zero, v_scale, v_zero) if ref else (k_scale, v_scale):
+        if t is None:
+            raise ValueError("WARM pools need their scales, reference-format ones their zero points.")
         _lib.require_gpu_tensor(t, "warm metadata")
-        if (t.dtype != (torch.float16 if ref else torch.float32) or not t.is_contiguous()
-                or t.numel() != slots * kv_heads * (bs if ref else 1)):
+        if t.dtype != kind or t.numel() != entries or not t.is_contiguous():
             raise ValueError("WARM metadata must be contiguous: fp16 per token and head (ref_u8), fp32 per slot and "
                              "head (absmax_i8).")
-    if any(t.get_device() != index for t in (warm_k, warm_v, *metas)):
-        raise ValueError("rows, tables and pools must be on one device.")
+        if t.get_device() != index:
+            raise ValueError("rows, tables and pools must be on one device.")
 
 
 def rotate_rows(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
@@ -426,47 +450,46 @@ def rotate_rows(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor,
     _lib.require_gpu_tensor(key, "key")
     if query.ndim != 3 or key.ndim != 3 or query.dtype not in _HALVES:
         raise ValueError("query and key must be fp16 / bf16 [tokens, heads, head_dim].")
-    rows, heads, dim = query.shape
+    shape = query.shape
+    rows, heads, dim = shape
     kv_heads = key.shape[1]
+    kv_shape = (rows, kv_heads, dim)
     index, device, dtype = query.get_device(), query.device, query.dtype
-    q = _packed_rows(query, "query", rows, heads, dim, dtype, index)
-    k = _packed_rows(key, "key", rows, kv_heads, dim, dtype, index)
-    _require_i32(positions, "positions", (rows,))
-    _lib.require_gpu_tensor(inv_freq, "inv_freq")
-    if inv_freq.dtype != torch.float32 or inv_freq.ndim != 1 or not inv_freq.is_contiguous() or 2 * len(inv_freq) > dim:
-        raise ValueError("inv_freq must be contiguous fp32 [rotary_dim / 2], rotary_dim at most head_dim.")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        _lib.require_gpu_tensor(w, "norm weight")
-        if (w.dtype not in (dtype, torch.float32) or w.dtype != weights[0].dtype or tuple(w.shape) != (dim,)
-                or not w.is_contiguous()):
+    q = _packed_rows(query, "query", shape, dtype, index)
+    k = _packed_rows(key, "key", kv_shape, dtype, index)
+    _step_i32(positions, "positions", (rows,), index)
+    half = inv_freq.numel() if isinstance(inv_freq, torch.Tensor) else 0
+    if not _is(inv_freq, torch.float32, (half,), index) or 2 * half > dim:
+        raise ValueError("inv_freq must be contiguous fp32 [rotary_dim / 2] on the rows' device, rotary_dim at most head_dim.")
+    of = q_weight if q_weight is not None else k_weight
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dtype not in (dtype, torch.float32) or not _is(w, of.dtype, (dim,), index)):
             raise ValueError("norm weights must be contiguous [head_dim] tensors of the rows' dtype or fp32, both alike.")
-    given = [t is not None for t in (value, slots, hot_k, hot_v)]
-    if any(given) != all(given):
-        raise ValueError("value, slots, hot_k and hot_v go together.")
     bs, pool, v, vt, vh = 1, 0, None, 0, 0
-    if slots is not None:
-        _check_tiles(hot_k, "hot_k", torch.float16)
-        _check_tiles(hot_v, "hot_v", torch.float16)
-        if hot_v.shape != hot_k.shape or (hot_k.shape[1], hot_k.shape[3]) != (kv_heads, dim):
-            raise ValueError("K and V pools must have identical shapes, of the rows' geometry.")
-        pool, bs = hot_k.shape[0], hot_k.shape[2]
-        _require_i32(slots, "slots", (rows,))
-        v = _packed_rows(value, "value", rows, kv_heads, dim, dtype, index)
+    if slots is None:
+        if value is not None or hot_k is not None or hot_v is not None:
+            raise ValueError("value, slots, hot_k and hot_v go together.")
+    else:
+        if value is None or hot_k is None or hot_v is None:
+            raise ValueError("value, slots, hot_k and hot_v go together.")
+        _hot_pools(hot_k, hot_v, index)
+        pool, pool_heads, bs, pool_dim = hot_k.shape
+        if pool_heads != kv_heads or pool_dim != dim:
+            raise ValueError("the pools must have the rows' geometry.")
+        _step_i32(slots, "slots", (rows,), index)
+        v = _packed_rows(value, "value", kv_shape, dtype, index)
         vt, vh, _ = v.stride()
-    on = (positions, inv_freq, *weights, *((slots, hot_k, hot_v) if slots is not None else ()))
-    if any(t.get_device() != index for t in on):
-        raise ValueError("rows, tables and pools must be on one device.")
-    q_out = _out_rows(q_out, "q_out", (rows, heads, dim), dtype, device)
+    q_out = _out_rows(q_out, "q_out", shape, dtype, device, index)
     if k_out is not None or slots is None:
-        k_out = _out_rows(k_out, "k_out", (rows, kv_heads, dim), dtype, device)
+        k_out = _out_rows(k_out, "k_out", kv_shape, dtype, device, index)
+    qt, qh, _ = q.stride()
+    kt, kh, _ = k.stride()
     code = _lib.DTYPE_BF16 if dtype == torch.bfloat16 else _lib.DTYPE_F16
     ptr = _lib.ptr
-    rc = _on_device(device, lib.tierkv_rotate_rows, ptr(q), q.stride(0), q.stride(1), ptr(q_out), ptr(k), k.stride(0),
-                    k.stride(1), ptr(k_out), ptr(v), vt, vh, code, ptr(positions), rows, ptr(inv_freq),
-                    2 * len(inv_freq), int(bool(interleaved)), float(attention_scaling), ptr(q_weight), ptr(k_weight),
-                    _lib.DTYPE_F32 if weights and weights[0].dtype == torch.float32 else code, float(eps), ptr(slots),
-                    ptr(hot_k), ptr(hot_v), pool, heads, kv_heads, bs, dim)
+    rc = _on_device(device, lib.tierkv_rotate_rows, ptr(q), qt, qh, ptr(q_out), ptr(k), kt, kh, ptr(k_out), ptr(v), vt,
+                    vh, code, ptr(positions), rows, ptr(inv_freq), 2 * half, 1 if interleaved else 0, attention_scaling,
+                    ptr(q_weight), ptr(k_weight), _lib.DTYPE_F32 if of is not None and of.dtype == torch.float32 else code,
+                    eps, ptr(slots), ptr(hot_k), ptr(hot_v), pool, heads, kv_heads, bs, dim)
     _lib.check(rc, "tierkv_rotate_rows")
     return q_out, k_out
 
@@ -493,17 +516,17 @@ def quantize_rows(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, w
     pool, kv_heads, bs, dim = warm_k.shape
     if key.ndim != 3 or key.dtype not in _HALVES:
         raise ValueError("key and value must be fp16 / bf16 [tokens, kv_heads, head_dim].")
-    rows = key.shape[0]
-    k = _packed_rows(key, "key", rows, kv_heads, dim, key.dtype, index)
-    v = _packed_rows(value, "value", rows, kv_heads, dim, key.dtype, index)
-    _require_i32(slots, "slots", (rows,))
-    if slots.get_device() != index:
-        raise ValueError("rows, tables and pools must be on one device.")
+    rows, dtype = key.shape[0], key.dtype
+    k = _packed_rows(key, "key", (rows, kv_heads, dim), dtype, index)
+    v = _packed_rows(value, "value", (rows, kv_heads, dim), dtype, index)
+    _step_i32(slots, "slots", (rows,), index)
     if rows == 0:
         return
+    kt, kh, _ = k.stride()
+    vt, vh, _ = v.stride()
     ptr, ref = _lib.ptr, fmt == _lib.WARM_REF_U8
-    rc = _on_device(key.device, lib.tierkv_quantize_rows, ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0),
-                    v.stride(1), _lib.DTYPE_BF16 if k.dtype == torch.bfloat16 else _lib.DTYPE_F16, ptr(slots), rows,
+    rc = _on_device(key.device, lib.tierkv_quantize_rows, ptr(k), kt, kh, ptr(v), vt, vh,
+                    _lib.DTYPE_BF16 if dtype == torch.bfloat16 else _lib.DTYPE_F16, ptr(slots), rows,
                     ptr(warm_k), ptr(warm_v), pool, ptr(k_scale), ptr(k_zero) if ref else None, ptr(v_scale),
                     ptr(v_zero) if ref else None, fmt, kv_heads, bs, dim)
     _lib.check(rc, "tierkv_quantize_rows")
@@ -529,36 +552,34 @@ def read_rows(start: torch.Tensor, cu_tokens: torch.Tensor, num_tokens: int, blo
     shape = block_table.shape
     batch, stride = shape
     index, device = block_table.get_device(), block_table.device
-    ints = [("block_table", block_table, shape), ("block_states", block_states, shape),
-            ("block_lengths", block_lengths, shape), ("start", start, shape[:1]), ("cu_tokens", cu_tokens, (batch + 1,))]
+    _step_i32(block_table, "block_table", shape, index)
+    _step_i32(block_states, "block_states", shape, index)
+    _step_i32(block_lengths, "block_lengths", shape, index)
+    _step_i32(start, "start", (batch,), index)
+    _step_i32(cu_tokens, "cu_tokens", (batch + 1,), index)
     if seq_num_blocks is not None:
-        ints.append(("seq_num_blocks", seq_num_blocks, shape[:1]))
-    for name, t, want in ints:
-        _require_i32(t, name, want)
-        if t.get_device() != index:
-            raise ValueError("rows, tables and pools must be on one device.")
+        _step_i32(seq_num_blocks, "seq_num_blocks", (batch,), index)
     if dtype not in _LOGIT_DTYPES:
         raise ValueError("dtype must be fp16, bf16 or fp32.")
     rows = int(num_tokens)
     if rows < 0:
         raise ValueError("num_tokens must not be negative.")
-    _check_tiles(hot_k, "hot_k", torch.float16)
-    _check_tiles(hot_v, "hot_v", torch.float16)
+    _hot_pools(hot_k, hot_v, index)
     _lib.require_gpu_tensor(warm_k, "warm_k")
     fmt = _lib.WARM_ABSMAX_I8 if warm_k.dtype == torch.int8 else _lib.WARM_REF_U8
     _warm_pools(warm_k, warm_v, k_scale, k_zero, v_scale, v_zero, fmt, index)
-    if hot_v.shape != hot_k.shape or warm_k.shape[1:] != hot_k.shape[1:]:
+    hot, kv_heads, bs, dim = hot_k.shape
+    warm, *geometry = warm_k.shape
+    if geometry != [kv_heads, bs, dim]:
         raise ValueError("HOT and WARM pools must have one geometry.")
-    if hot_k.get_device() != index or hot_v.get_device() != index:
-        raise ValueError("rows, tables and pools must be on one device.")
-    kv_heads, bs, dim = hot_k.shape[1:]
+    want = (rows, kv_heads, dim)
     k_rows, v_rows = (None, None) if out is None else out
-    k_rows = _out_rows(k_rows, "out", (rows, kv_heads, dim), dtype, device)
-    v_rows = _out_rows(v_rows, "out", (rows, kv_heads, dim), dtype, device)
+    k_rows = _out_rows(k_rows, "out", want, dtype, device, index)
+    v_rows = _out_rows(v_rows, "out", want, dtype, device, index)
     ptr, ref = _lib.ptr, fmt == _lib.WARM_REF_U8
     rc = _on_device(device, lib.tierkv_read_rows, ptr(start), ptr(cu_tokens), rows, ptr(block_table), ptr(block_states),
-                    ptr(block_lengths), stride, ptr(seq_num_blocks), stride, ptr(hot_k), ptr(hot_v), hot_k.shape[0],
-                    ptr(warm_k), ptr(warm_v), warm_k.shape[0], ptr(k_scale), ptr(k_zero) if ref else None, ptr(v_scale),
+                    ptr(block_lengths), stride, ptr(seq_num_blocks), stride, ptr(hot_k), ptr(hot_v), hot,
+                    ptr(warm_k), ptr(warm_v), warm, ptr(k_scale), ptr(k_zero) if ref else None, ptr(v_scale),
                     ptr(v_zero) if ref else None, fmt, ptr(k_rows), ptr(v_rows), _LOGIT_DTYPES[dtype], batch, kv_heads,
                     bs, dim)
     _lib.check(rc, "tierkv_read_rows")

@@ -21,7 +21,8 @@ resident on the device:
 * ``extend_layer`` takes several new tokens per sequence on top of what the
   cache holds (a follow-up prompt): slot map, row write,
   ``tierkv_extend_attention``, and the tick by the scores of the last token.
-  They stay: nothing takes tokens back out of the cache.
+  They stay: nothing takes tokens back out of the cache;
+* ``read_layer`` gives a layer's tokens back as dense K/V.
 
 Budgets are fractions of each sequence's current block count (workload
 C5: 15 % HOT, 55 % WARM, the rest evicted), evaluated on the host from the
@@ -521,12 +522,17 @@ class BatchedTieredKVRuntime:
 
     def extend_layer(self, layer: int, query_states: torch.Tensor, key_states: torch.Tensor,
                      value_states: torch.Tensor, num_key_value_groups: int, scaling: float,
-                     policy_step: bool = True) -> torch.Tensor:
+                     policy_step: bool = True, rotary: dict | None = None) -> torch.Tensor:
         """Several new tokens per sequence of one layer: append K/V [B, kv_heads,
         T, D], attend with query [B, H, T, D] (rotated, as K; each token sees
         the cache and the new tokens up to itself) and, with ``policy_step``,
         re-tier the layer by the scores of the last token.  T is at most
         ``extend_tokens``.  Returns the attention output [B, T, H, D].
+        rotary: None (q and k already rotated), or what ``kernels.rotate_rows``
+        takes beside the rows (``inv_freq``, and where the model has them
+        ``q_weight``, ``k_weight``, ``eps``, ``attention_scaling``,
+        ``interleaved``) -- then q and k are the projections, of v's type, and
+        are normed and rotated by their positions on the way into the cache.
         A call that cannot be taken raises before anything changes: ValueError
         for its tensors, RuntimeError when the tokens exceed max_seq_len or the
         free HOT slots (tokens of several calls without a tick), and under
@@ -561,12 +567,19 @@ class BatchedTieredKVRuntime:
                                "(a call with policy_step, or tick_layer).")
         rows = lambda t: t.transpose(1, 2).reshape(B * T, t.shape[1], d)   # noqa: E731
         q, k, v = rows(query_states), rows(key_states), rows(value_states)
-        if k.dtype not in halves:
+        if rotary is not None:   # its checks, on no rows
+            none = st.nblocks[:0]
+            kernels.rotate_rows(q[:0], k[:0], none, value=v[:0], slots=none, hot_k=st.hot_k, hot_v=st.hot_v, **rotary)
+        elif k.dtype not in halves:
             k, v = k.to(torch.float16), v.to(torch.float16)
         new = torch.full((B,), T, dtype=torch.int32, device=self.device)
         m = kernels.build_slot_map(new, st.table, st.states, st.lengths, st.nblocks, st.open, st.hot_free, st.ctl,
                                    self.block_size, B * T)
-        kernels.write_slots(k, v, m.slots, st.hot_k, st.hot_v)
+        if rotary is not None:
+            q, _ = kernels.rotate_rows(q, k, m.positions, value=v, slots=m.slots, hot_k=st.hot_k, hot_v=st.hot_v,
+                                       q_out=torch.zeros_like(q, memory_format=torch.contiguous_format), **rotary)
+        else:
+            kernels.write_slots(k, v, m.slots, st.hot_k, st.hot_v)
         num_blocks = min(self._advance_blocks(layer, T), self.max_blocks)
         # Zeros: what a step gives that the device refuses all the same (after
         # an earlier error that check_errors reports).
@@ -576,8 +589,9 @@ class BatchedTieredKVRuntime:
             st.k_zero, st.v_scale, st.v_zero, num_blocks, num_key_value_groups, scaling, cold_mode=self.cold_mode,
             seq_num_blocks=st.nblocks, max_tokens=T, out=out)
         if policy_step:
+            last = query_states[:, :, -1:] if rotary is None else q.view(B, T, -1, d)[:, -1, :, None]
             _, sums = tierkv_decode_attention(
-                query_states[:, :, -1:].contiguous(), st.table, st.states, st.lengths, st.hot_k, st.hot_v, st.warm_k,
+                last.contiguous(), st.table, st.states, st.lengths, st.hot_k, st.hot_v, st.warm_k,
                 st.warm_v, st.k_scale, st.k_zero, st.v_scale, st.v_zero, num_blocks, num_key_value_groups, scaling,
                 return_scores=True, cold_mode=self.cold_mode, seq_num_blocks=st.nblocks,
                 workspace=self.reserve_decode_workspace(query_states.shape[1]), deterministic=self.deterministic)
@@ -586,6 +600,21 @@ class BatchedTieredKVRuntime:
         if layer == self.num_layers - 1:
             self.seq_len += T
         return out.view(B, T, -1, d)
+
+    def read_layer(self, layer: int, start: int, tokens: int, dtype: torch.dtype = torch.float16):
+        """K and V of tokens [start, start + tokens) of every sequence of a
+        layer, as the cache holds them ([B, kv_heads, tokens, D]; evicted
+        tokens, and those past what it holds, are 0): what moves a prompt to
+        another cache, or an attention of the caller's own reads.  Nothing is
+        read back to the host."""
+        if start < 0 or tokens < 0:
+            raise ValueError("start and tokens must not be negative.")
+        st = self.layers[layer]
+        begin = torch.full((self.batch,), start, dtype=torch.int32, device=self.device)
+        cu = torch.arange(self.batch + 1, dtype=torch.int32, device=self.device) * tokens
+        out = kernels.read_rows(begin, cu, self.batch * tokens, st.table, st.states, st.lengths, st.nblocks, st.hot_k,
+                                st.hot_v, st.warm_k, st.warm_v, st.k_scale, st.k_zero, st.v_scale, st.v_zero, dtype)
+        return tuple(t.view(self.batch, tokens, self.kv_heads, self.head_dim).transpose(1, 2) for t in out)
 
     def tick_layer(self, layer: int, score_sums: torch.Tensor, num_blocks: int) -> None:
         st = self.layers[layer]

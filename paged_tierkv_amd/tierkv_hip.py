@@ -707,17 +707,20 @@ def _attend_packed(query_states, cu_tokens, block_table, block_states, block_len
     if prefix is not None:
         prefix_of, *tables, counts = prefix
         _lib.require_gpu_tensor(prefix_of, "prefix_of")
-        if prefix_of.dtype != torch.int32 or not prefix_of.is_contiguous() or tuple(prefix_of.shape) != (batch,):
+        if prefix_of.dtype != torch.int32 or not prefix_of.is_contiguous() or prefix_of.shape != (batch,):
             raise ValueError("prefix_of must be a contiguous int32 tensor with one entry per request.")
+        if prefix_of.get_device() != index:
+            raise ValueError("queries, tables and pools must be on one device.")
         for name, t in zip(("prefix_table", "prefix_states", "prefix_lengths"), tables):
             _lib.require_gpu_tensor(t, name)
-            if t.dtype != torch.int32 or not t.is_contiguous() or t.ndim != 2 or t.shape != tables[0].shape:
+            if t.dtype != torch.int32 or t.ndim != 2 or t.shape != tables[0].shape or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous int32 tensor [prefixes, max_prefix_blocks].")
-        if any(t.get_device() != index for t in (prefix_of, *tables)):
-            raise ValueError("queries, tables and pools must be on one device.")
-        prefixes, width = (int(x) for x in tables[0].shape)
+            if t.get_device() != index:
+                raise ValueError("queries, tables and pools must be on one device.")
+        prefixes, width = tables[0].shape
         counts = _block_counts(counts, prefixes, index, device)
-        pre = (_lib.ptr(prefix_of), *(_lib.ptr(t) for t in tables), width, _lib.ptr(counts), width, prefixes)
+        ptr = _lib.ptr
+        pre = (ptr(prefix_of), ptr(tables[0]), ptr(tables[1]), ptr(tables[2]), width, ptr(counts), width, prefixes)
     bound = rows if max_tokens is None else min(int(max_tokens), rows)
     if bound < 0:
         raise ValueError("max_tokens must not be negative.")

@@ -176,6 +176,9 @@ def test_empty_steps_and_refusals(device):
     i = lambda n: torch.zeros(n, dtype=torch.int32, device=device)   # noqa: E731
     q, k = kernels.rotate_rows(z(0, 4, 64), z(0, 2, 64), i(0), f)
     assert q.shape == (0, 4, 64) and k.shape == (0, 2, 64)
+    pool = z(2, 2, 16, 64)
+    q, k = kernels.rotate_rows(z(0, 4, 64), z(0, 2, 64), i(0), f, value=z(0, 2, 64), slots=i(0), hot_k=pool, hot_v=pool)
+    assert q.shape == (0, 4, 64) and k is None
     ok = dict(query=z(3, 4, 64), key=z(3, 2, 64), positions=i(3), inv_freq=f)
     pools = dict(value=z(3, 2, 64), slots=i(3), hot_k=z(2, 2, 16, 64), hot_v=z(2, 2, 16, 64))
     kernels.rotate_rows(**ok, **{**pools, "slots": torch.arange(3, dtype=torch.int32, device=device)})
