@@ -20,6 +20,9 @@ it follows.  Modules:
 * ``runtime``       -- the batched runtime's allocation order and tick rules
                        (per-sequence rules of the reference runtime; the
                        batch-level order has no counterpart there).
+* ``serving``       -- a serving step over requests of different lengths.
+* ``shared_prompt`` -- rows rotated, quantized and read back, attention over
+                       shared prefixes.
 
 The reference-API pools and runtime (paged_tierkv_amd.tierkv_policy) have no
 restatement here: they are pinned directly against trajectories the

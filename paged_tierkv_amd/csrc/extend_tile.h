@@ -48,7 +48,11 @@
 // value, as the probabilities have one when they become fp16 operands: the
 // matrix units take 16-bit operands at sixteen times the rate of 32-bit ones.
 // (Values past fp16's range become infinite, as the format's own
-// dequantization makes them, tierkv_policy.py:39-44.)
+// dequantization makes them, tierkv_policy.py:39-44.)  Calls with shared
+// prefixes round less: there V of an absmax block goes in as code * 2^e, exact,
+// and the rest of the scale m, scale = m 2^e, multiplies the probabilities
+// before their rounding (fp16 outputs 1.4 times as far from 64 bits as a
+// product in 32 bits rounded once, with both rounded 1.65 times).
 // Probabilities carry a factor 2^6 so that small ones stay normal fp16.
 // bf16 queries become fp16 after division by a power of two near the row's
 // largest value, which the logits get back in 32 bits.
@@ -148,7 +152,7 @@ struct ExtendParams {
   int2* tile;              // [max_tiles] {first partial or -1 (the item wrote the rows itself), parts}
   // Steps that the host lays out.
   int2* row_pre;           // [rows] {request, place of its first row among the slots' rows}
-  int32_t pre_slots, pre_parts, own_parts, own_side;
+  int32_t pre_slots, pre_parts, own_parts, own_tiles, own_side;
   int64_t own_unit;        // the requests' own first partial
 };
 
@@ -491,9 +495,25 @@ __device__ __forceinline__ void ex_store_k(const ExtendParams& p, const ExSub& s
   }
 }
 
+// A block's scale as m 2^e: the power of two (code * 2^e is exact in fp16 over
+// its range) and m in [1, 2) with the sign.  Scales that are zero, below the
+// normal numbers or not finite stay whole.
+__device__ __forceinline__ float2 ex_split(float scale) {
+  const uint32_t bits = __float_as_uint(scale), e = bits & 0x7f800000u;
+  if (e == 0 || e == 0x7f800000u) return make_float2(scale, 1.f);
+  return make_float2(__uint_as_float(e), __uint_as_float((bits & 0x807fffffu) | 0x3f800000u));
+}
+
+// Where a sub-tile's m is: behind its first row of K.
+template <int DP, int TK>
+__device__ __forceinline__ float* ex_factor(ExTile<DP, TK>& t, int sub) {
+  return reinterpret_cast<float*>(t.k + ex_k_at<DP>(sub * EX_SUB, DP / 8));
+}
+
 // The same of a V half, transposed; returns, when asked to check, the largest
-// magnitude bits of its values (two halves).
-template <int DP, int WF, int TK>
+// magnitude bits of its values (two halves).  EXACT (absmax): codes times the
+// scale's power of two; the rest of the scale goes to the probabilities.
+template <int DP, int WF, int TK, bool EXACT>
 __device__ __forceinline__ uint32_t ex_store_v(const ExtendParams& p, const ExSub& s, const ExHalf<DP>& st, int at,
                                                bool check, ExTile<DP, TK>& t) {
   typedef ExHalf<DP> St;
@@ -505,6 +525,11 @@ __device__ __forceinline__ uint32_t ex_store_v(const ExtendParams& p, const ExSu
   uint2* const dst = reinterpret_cast<uint2*>(t.v + ex_v_at<TK>(St::DL * n, at * 2 + (g & 1))) + (g >> 1);
   constexpr int NEXT = 2 * (TK / 8 + 1);             // the next dim's row
   uint32_t largest = 0;
+  float2 split = make_float2(1.f, 1.f);
+  if constexpr (EXACT) {
+    if (!zero && !hot) split = ex_split(__uint_as_float(st.meta[0]));
+    if (lane == 0) *ex_factor<DP, TK>(t, at) = split.y;
+  }
   auto put = [&](int i, uint2 o) {
     dst[i * NEXT] = o;
     if (check) largest = ex_max_u16(largest, ex_max_u16(o.x & 0x7fff7fffu, o.y & 0x7fff7fffu));
@@ -537,7 +562,7 @@ __device__ __forceinline__ uint32_t ex_store_v(const ExtendParams& p, const ExSu
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
-      mul[j] = off[j] ? 0.f : __uint_as_float(st.meta[0]);
+      mul[j] = off[j] ? 0.f : (EXACT ? split.x : __uint_as_float(st.meta[0]));
       add[j] = -128.f * mul[j];
       w[j][0] = st.r[j].x ^ 0x80808080u;
       w[j][1] = st.r[j].y ^ 0x80808080u;
@@ -589,7 +614,7 @@ __device__ __attribute__((noinline)) void ex_clear_wild(int at, ExTile<DP, TK>* 
 
 // V of token t of a sub-tile (its row in the block), one dim, as the product
 // takes it.
-template <int WF>
+template <int WF, bool EXACT>
 __device__ __forceinline__ float ex_value(const ExtendParams& p, int h, const ExSub& s, int t, int d) {
   const int64_t row = (int64_t(s.slot) * p.kv_heads + h) * p.bs + s.sub * EX_SUB + t;
   if (s.state == HOT) return __half2float(p.hot_v[row * p.D + d]);
@@ -597,7 +622,12 @@ __device__ __forceinline__ float ex_value(const ExtendParams& p, int h, const Ex
   const uint8_t c = p.warm_v[row * p.D + d];
   float f;
   if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
-    f = float(int8_t(c)) * reinterpret_cast<const float*>(p.v_scale)[int64_t(s.slot) * p.kv_heads + h];
+    const float scale = reinterpret_cast<const float*>(p.v_scale)[int64_t(s.slot) * p.kv_heads + h];
+    if constexpr (EXACT) {
+      const float2 split = ex_split(scale);
+      return __half2float(__float2half_rn(float(int8_t(c)) * split.x)) * split.y;
+    }
+    f = float(int8_t(c)) * scale;
   } else {
     f = (float(c) - __half2float(reinterpret_cast<const __half*>(p.v_zero)[row])) *
         __half2float(reinterpret_cast<const __half*>(p.v_scale)[row]);
@@ -713,12 +743,16 @@ __device__ __forceinline__ void ex_logits(const ExTile<DP, TK>& t, const f16x8 (
 // so the largest logit is the factor times the largest unscaled one and the
 // factor's product joins the exponential's subtraction (absmax; the reference
 // format has a factor per key and takes the product first, as masked tiles do).
-template <int DP, int WF, int TK>
-__device__ __forceinline__ void ex_softmax(const ExTile<DP, TK>& t, float qscale, const int (&end)[TK / 16], bool whole,
+template <int DP, int WF, int TK, bool EXACT>
+__device__ __forceinline__ void ex_softmax(ExTile<DP, TK>& t, float qscale, const int (&end)[TK / 16], bool whole,
                                            f32x16 (&s)[TK / 32], ExAcc<DP>& a) {
   constexpr int KT = TK / 32;
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
-  float c[KT * 2];
+  float c[KT * 2], vm[KT * 2];
+  if constexpr (EXACT) {
+#pragma unroll
+    for (int sub = 0; sub < KT * 2; ++sub) vm[sub] = *ex_factor<DP, TK>(t, sub);
+  }
   if constexpr (WF == TIERKV_WARM_ABSMAX_I8) {
 #pragma unroll
     for (int sub = 0; sub < KT * 2; ++sub) c[sub] = t.kscale[sub] * qscale;
@@ -782,7 +816,7 @@ __device__ __forceinline__ void ex_softmax(const ExTile<DP, TK>& t, float qscale
     for (int r = 0; r < 8; ++r) {
       const float e = __builtin_amdgcn_exp2f(fmaf(s[sub / 2][(sub & 1) * 8 + r], c[sub], base));
       a.l += e;
-      pr[sub & 1][r] = _Float16(e);
+      pr[sub & 1][r] = EXACT ? _Float16(e * vm[sub]) : _Float16(e);
     }
   };
   __builtin_amdgcn_sched_barrier(0);
@@ -838,12 +872,13 @@ __device__ __forceinline__ void ex_tile_part(const ExtendParams& p, char* lds, i
                                              bool dead = false) {
   constexpr int TK = WIDE ? 64 : 32;
   constexpr int NS = WIDE ? 1 : 4;          // halves a wave stages
+  constexpr bool EXACT = UNITS && WF == TIERKV_WARM_ABSMAX_I8;   // (extend attention keeps the bits that it had)
   const int tid = threadIdx.x, lane = tid & 63, w = ex_uniform(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int n = dead ? 0 : seq.w;
   const int G = p.groups, D = p.D, kw = w % KW;   // kw: the wave's place among those of its tile
   const int rows = n * G;
-  const int row_first = tile * EX_WIDE, row_last = min(row_first + (WIDE ? EX_WIDE : 32), rows) - 1;
+  const int row_first = tile * (WIDE || !UNITS ? EX_WIDE : EX_NARROW), row_last = min(row_first + (WIDE ? EX_WIDE : 32), rows) - 1;
   const int lim_min = seq.y - n + row_first / G, lim_max = seq.y - n + row_last / G;
 
   // This lane's row.
@@ -951,7 +986,7 @@ __device__ __forceinline__ void ex_tile_part(const ExtendParams& p, char* lds, i
     }
   };
   auto store_v = [&](ExTile<DP, TK>& t, const ExSub& of, const ExHalf<DP>& v, int place, bool whole) {
-    const uint32_t largest = ex_store_v<DP, WF, TK>(p, of, v, place, !whole, t);
+    const uint32_t largest = ex_store_v<DP, WF, TK, EXACT>(p, of, v, place, !whole, t);
     if (!whole && __any(ex_wild(largest))) {
       ex_clear_wild<DP, TK>(place, &t);
       wild = true;
@@ -987,11 +1022,11 @@ __device__ __forceinline__ void ex_tile_part(const ExtendParams& p, char* lds, i
       load();
       __syncthreads();
     }
-    auto output = [&](int at, f32x16 (&s)[TK / 32], const ExTile<DP, TK>& t) {
+    auto output = [&](int at, f32x16 (&s)[TK / 32], ExTile<DP, TK>& t) {
       const bool whole = at + 4 <= full;
       int end[TK / 16] = {};
       if (!whole) ex_ends<TK>(list, at, hi, lim, end);
-      ex_softmax<DP, WF, TK>(t, qscale, end, whole, s, a);
+      ex_softmax<DP, WF, TK, EXACT>(t, qscale, end, whole, s, a);
     };
     // Two barriers per tile; every wave meets 2 tiles_n + 1 of them.
     int buf = 0;
@@ -1042,7 +1077,7 @@ __device__ __forceinline__ void ex_tile_part(const ExtendParams& p, char* lds, i
       ex_logits<DP, WF, TK>(tiles[w], q, qsum, s);
       int end[TK / 16] = {};
       if (!whole) ex_ends<TK>(list, at, hi, lim, end);
-      ex_softmax<DP, WF, TK>(tiles[w], qscale, end, whole, s, a);
+      ex_softmax<DP, WF, TK, EXACT>(tiles[w], qscale, end, whole, s, a);
       if (at + ROUND < hi) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         store(tiles[w], held, at + ROUND + TK / 16 <= full);
@@ -1068,7 +1103,7 @@ __device__ __forceinline__ void ex_tile_part(const ExtendParams& p, char* lds, i
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int d = dt * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-              const float v = d < D ? ex_value<WF>(p, h, sb, x, d) : 0.f;
+              const float v = d < D ? ex_value<WF, EXACT>(p, h, sb, x, d) : 0.f;
               if (!(fabsf(v) < INFINITY)) a.o[dt][i] += v;
             }
         }

@@ -33,6 +33,7 @@ namespace tierkv {
 constexpr int PX_LONE = 512;            // rows (tokens times heads of a kv head) from which a request walks its prefix itself
 constexpr int PX_KW = 2;                // waves of a narrow item
 constexpr int PX_SIDE = EX_WAVES / PX_KW;   // narrow items side by side
+constexpr int PX_TAIL = 4;              // items that cutting the last tiles adds, at most, for each place
 constexpr int PX_MIN_NARROW = 8;        // sub-tiles of a narrow item, at least, when a tile is cut
 constexpr float PX_NARROW_COST = 0.5f;  // a narrow item's sub-tile, in wide sub-tiles' time
 // A step's workgroup, in microseconds: its start and end, a wide sub-tile, a
@@ -199,7 +200,7 @@ __global__ __launch_bounds__(EX_PLAN) void prefix_plan_kernel(ExtendParams p) {
   };
   // Sub-tiles per wide item: each wave rates one choice, as extend attention's
   // plan does; the narrow items fill what the wide ones leave.
-  __shared__ float s_time[EX_PLAN / 64];
+  __shared__ float s_time[EX_PLAN / 64], s_items[EX_PLAN / 64], s_len[EX_PLAN / 64];
   __shared__ int s_per[EX_PLAN / 64];
   const int least = max(EX_MIN_SUBS, int(ceilf(wide_work / fmaxf(float(EX_TARGET / p.kv_heads), 1.f))));
   {
@@ -227,20 +228,36 @@ __global__ __launch_bounds__(EX_PLAN) void prefix_plan_kernel(ExtendParams p) {
     if (lane == 0) {
       s_time[w] = time;
       s_per[w] = per;
+      s_items[w] = items;
+      s_len[w] = len;
     }
   }
   __syncthreads();
-  int per_wide = s_per[0];
+  int choice = 0;
+  for (int i = 1; i < EX_PLAN / 64; ++i)
+    if (s_time[i] < s_time[choice]) choice = i;
+  const int per_wide = s_per[choice];
+  // Whole tiles that would begin a last round of the slots, not full, are cut
+  // by `tail`, so that the round is shorter (113 tiles on 32 places: 2147 us
+  // with four rounds, 1920 with the last 17 tiles cut).
+  int tail = 1, tail_from = 0x7fffffff;
   {
-    float best = s_time[0];
-    for (int i = 1; i < EX_PLAN / 64; ++i)
-      if (s_time[i] < best) {
-        best = s_time[i];
-        per_wide = s_per[i];
+    const int places = int(slots), items = int(s_items[choice]);
+    const int rest = places > 0 ? items % places : 0;
+    if (items > places && rest > 0) {
+      float best = 1.f;
+      for (int k = 2; k <= 8; ++k) {
+        const float t = ceilf(float(rest * k) / float(places)) / float(k) + float(k) * EX_ITEM_COST / s_len[choice];
+        if (rest * (k - 1) <= places * PX_TAIL && t < best) {
+          best = t;
+          tail = k;
+          tail_from = items - rest;
+        }
       }
+    }
   }
   // Items, tile by tile: wide ones from the front, narrow ones from the back.
-  int wide_items = 0, narrow_items = 0, units = 0;
+  int wide_items = 0, narrow_items = 0, units = 0, before = 0;   // before: wide items without the tail's cuts
   for (int f0 = 0; f0 < tiles_all; f0 += EX_PLAN) {
     const int f = f0 + tid;
     ExTileId x = {0, 0, false};
@@ -248,6 +265,11 @@ __global__ __launch_bounds__(EX_PLAN) void prefix_plan_kernel(ExtendParams p) {
     if (f < tiles_all) {
       x = ex_tile_id(segments, f, s_tile, s_rows);
       parts = ex_parts(tile_work(x), x.wide ? per_wide : per_narrow);
+    }
+    if (tail > 1) {
+      const Ex3 s = ex_scan3({x.wide ? parts : 0, 0, 0}, sh, &total);
+      if (x.wide && parts == 1 && before + s.a - parts >= tail_from) parts = tail;
+      before += total.a;
     }
     // Rows that also have a prefix's part keep partials in any case.
     const int rb = x.request - p.prefixes;
@@ -371,7 +393,7 @@ __global__ __launch_bounds__(EX_THREADS) void prefix_join_kernel(ExtendParams p)
 // ---------------------------------------------------------------------------
 // Steps of a few tokens per request
 // ---------------------------------------------------------------------------
-// Where no request brings more than 32 rows (single tokens, drafts), the plan
+// Where no request brings more than PX_STEP rows (single tokens, drafts), the plan
 // would cost as much as the attention: a launch of its own, and five dependent
 // reads between it and an item's first key.  These calls are laid out on the
 // host, from sizes alone: every request's table row is cut into own_parts
@@ -380,6 +402,7 @@ __global__ __launch_bounds__(EX_THREADS) void prefix_join_kernel(ExtendParams p)
 // of 256; how many there are follows from the requests' prefixes, which each
 // workgroup of a slot reads.  Two launches: the parts, and their join.
 
+constexpr int PX_STEP = 64;        // rows of a request, at most: tiles of 32
 constexpr int PX_LIST = 416;       // sub-tiles that a workgroup lists
 constexpr int PX_MOST = 8;         // requests' parts side by side in a workgroup, where it is not one
 
@@ -553,15 +576,15 @@ template <int KW>
 __device__ __forceinline__ PxPart px_step_own(const ExtendParams& p, PxShared& s, int x) {
   constexpr int SIDE = EX_WAVES / KW, THREADS = 64 * KW;
   const int w = ex_uniform(threadIdx.x >> 6), mine = w / KW, tid = threadIdx.x % THREADS;
-  const int64_t units = int64_t(p.batch) * p.own_parts * p.kv_heads;
+  const int64_t units = int64_t(p.batch) * p.own_tiles * p.own_parts * p.kv_heads;
   const int64_t u = int64_t(x) * SIDE + mine;
   const bool dead = u >= units;
-  const int64_t v0 = min(u, units - 1);
-  const int h = int(v0 % p.kv_heads), part = int(v0 / p.kv_heads % p.own_parts), b = int(v0 / p.kv_heads / p.own_parts);
+  const int64_t v0 = min(u, units - 1), v1 = v0 / p.kv_heads, v2 = v1 / p.own_parts;
+  const int h = int(v0 % p.kv_heads), part = int(v1 % p.own_parts), tile = int(v2 % p.own_tiles), b = int(v2 / p.own_tiles);
   int n_all;
   const int2 rows = ex_rows(p, b, &n_all);
   const int q0 = rows.x, n = rows.y, g = px_prefix(p, b);
-  if (h == 0 && part == 0 && !dead) {
+  if (h == 0 && part == 0 && tile == 0 && !dead) {
     for (int i = tid; i < min(n_all, p.rows - q0); i += THREADS) p.row_home[q0 + i] = make_int4(i < n ? b : -1, i, g, 0);
     if (n < n_all && tid == 0) atomicOr(p.err, 4);
   }
@@ -589,12 +612,13 @@ __device__ __forceinline__ PxPart px_step_own(const ExtendParams& p, PxShared& s
   __syncthreads();
   PxPart o{};
   o.h = h;
+  o.tile = tile;
   o.rows = n * p.groups;
   o.seq = make_int4(total.x, tokens - (n_all - n), total.y, n);
   o.list = list;
-  o.unit = p.own_unit + int64_t(b) * p.own_parts + part;
+  o.unit = p.own_unit + v1;
   o.first = q0;
-  o.dead = dead || n == 0;
+  o.dead = dead || tile * EX_NARROW >= n * p.groups;
   return o;
 }
 
@@ -616,7 +640,7 @@ __global__ __launch_bounds__(EX_THREADS, 2) void prefix_step_kernel(ExtendParams
   }
   auto packed = [&](int t) { return o.map ? o.map[max(t - o.first, 0)] : o.first + t; };
   const PxList list = {o.list};
-  if (MIXED && o.rows > EX_NARROW) ex_tile_part<DP, WF, QT, true, true, 1>(p, px_lds, o.h, o.tile, 0, 1, o.seq, list, packed, o.unit);
+  if (MIXED && x < pre && o.rows > EX_NARROW) ex_tile_part<DP, WF, QT, true, true, 1>(p, px_lds, o.h, o.tile, 0, 1, o.seq, list, packed, o.unit);
   else if (side == 1) ex_tile_part<DP, WF, QT, false, true, EX_WAVES>(p, px_lds, o.h, o.tile, 0, 1, o.seq, list, packed, o.unit, o.dead);
   else ex_tile_part<DP, WF, QT, false, true, EX_WAVES / PX_MOST>(p, px_lds, o.h, o.tile, 0, 1, o.seq, list, packed, o.unit, o.dead);
 }
@@ -637,7 +661,9 @@ __global__ __launch_bounds__(EX_THREADS) void prefix_step_join_kernel(ExtendPara
   const int2 rows_of = ex_rows(p, home.x);
   if (home.y < 0 || home.y >= rows_of.y || int(r) - rows_of.x != home.y) return;
   const int64_t step = int64_t(p.kv_heads) * EX_UNIT;
-  const int64_t at = ex_unit_row(p, p.own_unit + int64_t(home.x) * p.own_parts, h, home.y * G + hd - h * G);
+  const int mine = home.y * G + hd - h * G;   // (in tile mine / 32)
+  const int64_t tile = int64_t(home.x) * p.own_tiles + mine / EX_NARROW;
+  const int64_t at = ex_unit_row(p, p.own_unit + tile * p.own_parts, h, mine % EX_NARROW);
   int pre_count = 0;
   int64_t pre_at = 0;
   if (home.z >= 0) {
@@ -668,8 +694,8 @@ struct PrefixLayout {
 
 // Tiles as ex_layout counts them, for the requests' rows and once more for the
 // prefixes'.  An item is a tile or a part of one: wide tiles are cut into
-// EX_TARGET / kv_heads more parts at most, narrow ones into as many as there are
-// places for them.  Partials in units of 32 rows: eight for every wide item.
+// EX_TARGET / kv_heads more parts at most, and the last of them into PX_TAIL
+// more for each place, narrow ones into as many as there are places for them.  Partials in units of 32 rows: eight for every wide item.
 static PrefixLayout prefix_layout(int64_t batch, int64_t prefixes, int64_t rows, int64_t max_tokens, int64_t groups,
                                   int64_t kv_heads, int64_t num_blocks, int64_t pre_blocks, int64_t bs, int64_t D) {
   PrefixLayout l{};
@@ -682,7 +708,7 @@ static PrefixLayout prefix_layout(int64_t batch, int64_t prefixes, int64_t rows,
   };
   const int64_t wide = wide_tiles(batch, longest) + wide_tiles(prefixes, all), narrow = batch + prefixes;
   l.tiles = wide + narrow;
-  l.wide_items = l.wide ? wide + std::max<int64_t>(EX_TARGET / kv_heads, 1) : 0;
+  l.wide_items = l.wide ? wide + std::max<int64_t>(EX_TARGET / kv_heads, 1) + (EX_SLOTS / kv_heads + 1) * PX_TAIL : 0;
   l.items = l.wide_items + narrow + (EX_SLOTS / kv_heads + 1) * PX_SIDE;
   l.units = l.wide_items * (EX_WIDE / EX_UNIT) + (l.items - l.wide_items);
   l.lone = longest >= PX_LONE ? std::min(batch, all / PX_LONE) : 0;
@@ -708,7 +734,7 @@ static PrefixLayout prefix_layout(int64_t batch, int64_t prefixes, int64_t rows,
 // CU at a time, in microseconds measured on steps of 1 to 256 requests.
 struct StepLayout {
   int64_t row_home, row_pre, part_o, part_ml, total;
-  int64_t slots, pre_parts, own_parts, side, each, own_unit, units, workgroups;
+  int64_t slots, pre_parts, own_parts, own_tiles, side, each, own_unit, units, workgroups;
   bool use;
 };
 
@@ -716,12 +742,13 @@ static StepLayout step_layout(int64_t batch, int64_t prefixes, int64_t rows, int
                               int64_t kv_heads, int64_t num_blocks, int64_t pre_blocks, int64_t bs, int64_t D) {
   StepLayout l{};
   const int64_t all = std::min(rows, batch * max_tokens) * groups, longest = std::min(rows, max_tokens) * groups;
-  l.use = longest <= EX_NARROW;
+  l.use = longest <= PX_STEP;
   if (!l.use || rows == 0) return l;
   auto up = [](int64_t x) { return (x + 255) & ~int64_t(255); };
   auto div = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const int64_t subs = div(bs, EX_SUB), fit = PX_LIST / subs;
   const bool wide = all > EX_NARROW;
+  l.own_tiles = std::max<int64_t>(div(longest, EX_NARROW), 1);
   l.each = wide ? EX_WIDE / EX_UNIT : 1;
   const int64_t groups_n = std::min(prefixes, batch);
   l.slots = all / EX_WIDE + groups_n;
@@ -738,7 +765,7 @@ static StepLayout step_layout(int64_t batch, int64_t prefixes, int64_t rows, int
         const double pre_subs = double(div(pre_blocks, pre) * subs), own_subs = double(div(num_blocks, own) * subs);
         const double c_pre = PX_COST + (pre_wide ? PX_COST_WIDE * pre_subs : PX_COST_ROUND * std::ceil(pre_subs / (2 * EX_WAVES)));
         const double c_own = PX_COST + PX_COST_ROUND * std::ceil(own_subs / (2 * waves)) * (side > 1 ? PX_COST_SIDE : 1.);
-        const double n_pre = double(live * pre * kv_heads), n_own = double(div(batch * own * kv_heads, side));
+        const double n_pre = double(live * pre * kv_heads), n_own = double(div(batch * l.own_tiles * own * kv_heads, side));
         const double sum = (n_pre * c_pre + n_own * c_own) / EX_SLOTS, most = std::max(c_pre, c_own);
         const double makespan = n_pre + n_own <= EX_SLOTS ? most : std::max(most, sum + 0.5 * std::min(c_pre, c_own));
         const double bytes = (double(all) * pre + double(batch) * longest * own) * kv_heads * D * 4;
@@ -753,8 +780,8 @@ static StepLayout step_layout(int64_t batch, int64_t prefixes, int64_t rows, int
     }
   }
   l.own_unit = l.slots * l.pre_parts * l.each;
-  l.units = l.own_unit + batch * l.own_parts;
-  l.workgroups = l.slots * l.pre_parts * kv_heads + div(batch * l.own_parts * kv_heads, l.side);
+  l.units = l.own_unit + batch * l.own_tiles * l.own_parts;
+  l.workgroups = l.slots * l.pre_parts * kv_heads + div(batch * l.own_tiles * l.own_parts * kv_heads, l.side);
   l.row_home = EX_WS_HEAD;
   l.row_pre = up(l.row_home + rows * 16);
   l.part_ml = up(l.row_pre + rows * 8);
@@ -872,6 +899,7 @@ extern "C" int32_t tierkv_prefix_attention(
     p.pre_slots = int32_t(step.slots);
     p.pre_parts = int32_t(step.pre_parts);
     p.own_parts = int32_t(step.own_parts);
+    p.own_tiles = int32_t(step.own_tiles);
     p.own_side = int32_t(step.side);
     p.own_unit = step.own_unit;
   } else {

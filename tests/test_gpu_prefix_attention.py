@@ -373,3 +373,28 @@ def test_refusals(device):
                 dict(scaling=float("nan")), dict(query_states=t["q"].float()), dict(max_tokens=-1), dict(cold_mode="other")):
         with pytest.raises(ValueError):
             tierkv_prefix_attention(**{**ok, **bad})
+
+
+@pytest.mark.parametrize("fmt,dtype", [("absmax_i8", torch.float16), ("ref_u8", torch.bfloat16)])
+def test_tiles_for_more_than_a_round_equal_extend_attention(device, fmt, dtype):
+    """Requests of many wide tiles each, the last of which are cut, beside
+    single tokens: the same tokens in every request's own row."""
+    s = step(31, [300], [0, 0, -1, 0], [1500, 1, 1100, 700], [1500, 40, 1100, 701], 32, 32, 64, fmt=fmt, dtype=dtype, pad=0)
+    t = tensors(s, device)
+    got = launch(t, s, "masked")
+    rows = [[], [], []]
+    for b, g in enumerate(s["member"]):
+        for out, p, m in zip(rows, s["pre"], s["own"]):
+            out.append(list(p[g][:s["pre"][3][g]] if g >= 0 else []) + list(m[b][:s["own"][3][b]]))
+    nb = torch.tensor([len(x) for x in rows[0]], dtype=torch.int32, device=device)
+    width = int(nb.max())
+    joined = [torch.tensor([x + [0] * (width - len(x)) for x in r], dtype=torch.int32, device=device) for r in rows]
+    ref = tierkv_extend_attention(t["q"], t["cu"], *joined, *t["pools"], width, s["groups"], s["scaling"], cold_mode="masked",
+                                  seq_num_blocks=nb)
+    # Both round probabilities and WARM values once: each is off the exact
+    # output by 2 * 2^-11 of sum p |v|, at most the largest |v| (normal values,
+    # below 8 here), and by its own rounding.
+    tol = 2 * (2 * 2.0 ** -11 * 8) + ref.abs().float() * torch.finfo(dtype).eps
+    assert ((got.float() - ref.float()).abs() <= tol).all()
+    again = launch(t, s, "masked")
+    assert torch.equal(again, got)
