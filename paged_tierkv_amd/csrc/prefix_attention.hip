@@ -90,14 +90,14 @@ __global__ __launch_bounds__(EX_PLAN) void prefix_plan_kernel(ExtendParams p) {
   int n, n_all, where = 0;
   bool fits = true;
   if (pre) {
-    // (packed ranges that overlap have more rows than there are)
-    where = min(total.a, p.rows);
-    n = n_all = min(total.c, p.rows - where);
+    // (packed ranges that overlap have more rows than there are, perhaps more than 2^31)
+    where = min(max(total.a, 0), p.rows);
+    n = n_all = min(max(total.c, 0), p.rows - where);
     fits = n == total.c;
   } else {
     const int2 r = ex_rows(p, b, &n_all);
     n = r.y;
-    const int place = min(total.a, p.rows), end = min(n_all, p.rows - r.x);
+    const int place = min(max(total.a, 0), p.rows), end = min(n_all, p.rows - r.x);
     if (lone) {
       where = ~total.a;
       if (total.a >= p.max_lone) {   // (the same)
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(EX_PLAN) void prefix_plan_kernel(ExtendParams p) {
     }
     for (int i = tid; i < end; i += EX_PLAN) {
       const int mine = g >= 0 && !lone ? total.b + i : -1;
-      const bool in = i < n && mine < p.rows - place;
+      const bool in = i < n && mine < p.rows - place;   // (mine: -1 or less for none)
       if (in && mine >= 0) p.row_list[place + mine] = r.x + i;
       p.row_home[r.x + i] = make_int4(in ? b : -1, i, mine >= 0 ? g : -1, mine);
     }
@@ -839,7 +839,8 @@ extern "C" int64_t tierkv_prefix_workspace_bytes(int32_t batch, int32_t num_pref
                                                  int32_t num_blocks, int32_t num_prefix_blocks, int32_t block_size,
                                                  int32_t head_dim) {
   if (batch <= 0 || num_prefixes <= 0 || num_rows < 0 || max_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
-      num_heads % num_kv_heads != 0 || num_blocks <= 0 || num_prefix_blocks <= 0 || block_size <= 0 || head_dim <= 0)
+      num_heads % num_kv_heads != 0 || num_blocks <= 0 || num_prefix_blocks <= 0 || block_size <= 0 || block_size > 64 ||
+      head_dim <= 0 || head_dim > 128)
     return -1;
   const int groups = num_heads / num_kv_heads;
   const StepLayout s = step_layout(batch, num_prefixes, num_rows, max_tokens, groups, num_kv_heads, num_blocks,

@@ -1300,7 +1300,7 @@ extern "C" int32_t tierkv_quantize_rows(
     return fail(TIERKV_ERR_INVALID, "unknown warm format");
   if (num_kv_heads <= 0 || num_kv_heads > 65535 || block_size <= 0 || block_size > 64 || head_dim <= 0 || head_dim > 256)
     return fail(TIERKV_ERR_UNSUPPORTED, "1 to 65535 heads, block_size in [1, 64] and head_dim in [1, 256]");
-  if (warm_slots <= 0 || warm_slots * block_size > 0x7fffffff)
+  if (warm_slots <= 0 || warm_slots > 0x7fffffff / block_size)
     return fail(TIERKV_ERR_UNSUPPORTED, "pool rows must lie in (0, 2^31)");
   if (num_rows == 0) return TIERKV_OK;
   if (!key || !value || !slots || !warm_k || !warm_v || !k_scale || !v_scale)

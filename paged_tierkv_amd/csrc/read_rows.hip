@@ -109,7 +109,7 @@ __global__ __launch_bounds__(RR_THREADS) void read_rows_scalar_kernel(ReadParams
   const int width = p.kv_heads * p.D;
   if (part.any) {
     const ReadBlock k = rr_block(p, b, i, n, part.at);
-    const int count = k.end - k.first;
+    const int count = max(k.end - k.first, 0);   // (far behind the last token asked for, its product would pass 32 bits)
     for (int x = threadIdx.x; x < 2 * count * width; x += RR_THREADS) {
       const int kv = x >= count * width, y = x - kv * count * width;
       const int h = y / (count * p.D), z = y - h * count * p.D;

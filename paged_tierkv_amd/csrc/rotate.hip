@@ -377,7 +377,7 @@ extern "C" int32_t tierkv_rotate_rows(
     if (!hot_k || !hot_v || (num_rows > 0 && (!slots || !value)))
       return fail(TIERKV_ERR_INVALID, "slots, value and both HOT pools go together");
     if (block_size <= 0 || block_size > 64) return fail(TIERKV_ERR_UNSUPPORTED, "block_size must be in [1, 64]");
-    if (hot_slots <= 0 || hot_slots * block_size > 0x7fffffff)
+    if (hot_slots <= 0 || hot_slots > 0x7fffffff / block_size)
       return fail(TIERKV_ERR_UNSUPPORTED, "pool rows must lie in (0, 2^31)");
   } else if (!k_out && num_rows > 0) {
     return fail(TIERKV_ERR_INVALID, "the keys need HOT pools or k_out");

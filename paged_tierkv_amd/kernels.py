@@ -562,8 +562,8 @@ def read_rows(start: torch.Tensor, cu_tokens: torch.Tensor, num_tokens: int, blo
     if dtype not in _LOGIT_DTYPES:
         raise ValueError("dtype must be fp16, bf16 or fp32.")
     rows = int(num_tokens)
-    if rows < 0:
-        raise ValueError("num_tokens must not be negative.")
+    if not 0 <= rows < 1 << 31:
+        raise ValueError("num_tokens must not be negative or pass 2^31.")
     _hot_pools(hot_k, hot_v, index)
     _lib.require_gpu_tensor(warm_k, "warm_k")
     fmt = _lib.WARM_ABSMAX_I8 if warm_k.dtype == torch.int8 else _lib.WARM_REF_U8

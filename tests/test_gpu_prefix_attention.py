@@ -280,6 +280,26 @@ def test_bad_slots_are_reported_and_max_tokens_leaves_rows_out(device):
     assert (out[7:9] == 7).all() and (out[10:] == 7).all()
 
 
+@pytest.mark.parametrize("most", [1, 24])       # a step's way and a plan's
+def test_row_ranges_that_overlap_do_no_harm(device, most):
+    """Ranges out of order, so that requests' rows overlap: rows of no request
+    stay as they are, the error word says so if any row was left out, and the
+    next call finds nothing of it."""
+    s = step(17, [60, 40], [0, 1, 0, 0], [3 * most, most, 4 * most, most], [200, 30, 210, 60], 4, 2, 64, spare=0)
+    t = tensors(s, device)
+    ws = DecodeWorkspace(device)
+    want = launch(t, s, "masked", workspace=ws).clone()
+    n = int(s["cu"][-1])
+    good = t["cu"].clone()
+    for cu in ([0, n - 1, 0, n, n], [5 * n, -3, 7, 2, n], [n, n - 1, 1, 0, n]):
+        t["cu"].copy_(torch.tensor(cu, dtype=torch.int32))
+        out = torch.full_like(t["q"], 7.0)
+        launch(t, s, "masked", workspace=ws, out=out)
+        assert (out[n:] == 7).all() and ws.error_word() in (0, 4)
+    t["cu"].copy_(good)
+    assert torch.equal(launch(t, s, "masked", workspace=ws)[:n], want[:n]) and ws.error_word() == 0
+
+
 def test_no_rows_and_no_tokens(device):
     s = step(12, [30], [0, 0], [0, 0], [5, 20], 4, 2, 64, pad=3)
     out = torch.full(s["q"].shape, 7.0, dtype=torch.float16, device=device)

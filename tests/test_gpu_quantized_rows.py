@@ -239,6 +239,28 @@ def test_bad_slots_read_as_evicted_and_counts_default_to_the_table(device):
     assert (got[0][:32] == 0).all() and (got[0][48:] == 0).all() and (got[0][32:48] != 0).any()
 
 
+@pytest.mark.parametrize("d", [20, 24])
+def test_a_short_window_of_a_very_long_context(device, d):
+    """Ten tokens at the front and in the middle of 2^20 (evicted ones but for
+    two blocks): what lies far behind a window writes nothing."""
+    kv, bs, n = 64, 64, 1 << 14
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)   # noqa: E731
+    states = torch.full((1, n), 2, dtype=torch.int32, device=device)
+    states[0, [0, 9000]] = 0
+    table = torch.zeros_like(states)
+    table[0, 9000] = 1
+    lengths = torch.full_like(states, bs)
+    hot = torch.arange(2 * 2 * kv * bs * d, device=device).remainder(501).half().view(2, 2, kv, bs, d)
+    codes, scale = torch.zeros((1, kv, bs, d), dtype=torch.int8, device=device), torch.zeros((1, kv), device=device)
+    for start, slot in ((3, 0), (9000 * bs + 3, 1), (5 * bs, None)):
+        out = torch.full((2, 30, kv, d), 7.0, dtype=torch.float16, device=device)
+        kernels.read_rows(i32(start), i32(10, 20), 30, table, states, lengths, None, hot[0], hot[1], codes, codes, scale, None, scale,
+                  None, out=(out[0], out[1]))
+        want = torch.full_like(out, 7.0)
+        want[:, 10:20] = 0 if slot is None else hot[:, slot, :, 3:13].transpose(1, 2)
+        assert torch.equal(out, want)
+
+
 def test_values_outside_the_tokens_do_not_matter(device):
     c = cache(3, [[5, 16]], 2, 64, 16, "absmax_i8", spare=0)
     c["states"][0], c["table"][0] = [HOT, HOT], [0, 1]

@@ -34,7 +34,7 @@ NO_POOLS = dict(v=None, slots=None, hk=None, hv=None)
     (dict(vh=-8), 1), (dict(amp=float("nan")), 1), (dict(eps=-1.0), 1), (dict(eps=float("nan")), 1),
     (dict(eps=float("inf")), 1), (dict(slots=None), 1), (dict(hv=None), 1), (dict(v=None), 1), (NO_POOLS, 1),
     (dict(heads=0), 2), (dict(kv=0), 2), (dict(heads=65536), 2), (dict(d=0), 2), (dict(d=257), 2), (dict(bs=0), 2),
-    (dict(bs=65), 2), (dict(pool=0), 2), (dict(pool=1 << 27), 2), (dict(rows=1 << 26, heads=64), 2),
+    (dict(bs=65), 2), (dict(pool=0), 2), (dict(pool=1 << 27), 2), (dict(pool=1 << 60), 2), (dict(rows=1 << 26, heads=64), 2),
     (dict(rows=0), 0), (dict(rows=0, q=None, **NO_POOLS), 0),
 ])
 def test_rotate_rows_refusals(kw, code):
@@ -54,7 +54,7 @@ def quantize(**kw):
 @pytest.mark.parametrize("kw,code", [
     (dict(k=None), 1), (dict(slots=None), 1), (dict(wv=None), 1), (dict(ks=None), 1), (dict(kz=None), 1), (dict(dtype=2), 1),
     (dict(fmt=2), 1), (dict(rows=-1), 1), (dict(kt=-1), 1), (dict(kv=0), 2), (dict(kv=65536), 2), (dict(bs=0), 2),
-    (dict(bs=65), 2), (dict(d=257), 2), (dict(pool=0), 2), (dict(pool=1 << 27), 2), (dict(rows=1 << 26), 2),
+    (dict(bs=65), 2), (dict(d=257), 2), (dict(pool=0), 2), (dict(pool=1 << 27), 2), (dict(pool=1 << 60), 2), (dict(rows=1 << 26), 2),
     (dict(rows=0), 0), (dict(rows=0, k=None, fmt=1, kz=None), 0),
 ])
 def test_quantize_rows_refusals(kw, code):
@@ -127,6 +127,9 @@ def test_prefix_workspace_sizes():
     size = lambda *a: _lib.lib().tierkv_prefix_workspace_bytes(*a)   # noqa: E731
     assert size(2, 0, 8, 8, 8, 2, 8, 8, 16, 64) < 0 and size(2, 1, 8, 8, 7, 2, 8, 8, 16, 64) < 0
     assert size(2, 1, 8, 8, 8, 2, 8, 0, 16, 64) < 0
+    # geometries that no call takes: blocks longer than a workgroup's list of one request's range among them
+    assert size(2, 1, 8, 8, 8, 2, 8, 8, 2000, 64) < 0 and size(2, 1, 8, 8, 8, 2, 8, 8, 65, 64) < 0
+    assert size(2, 1, 8, 8, 8, 2, 8, 8, 16, 136) < 0 and size(2, 1, 8, 8, 8, 2, 8, 8, 64, 128) > 0
     small = size(2, 1, 8, 8, 8, 2, 8, 8, 16, 64)
     assert 0 < small <= size(2, 1, 800, 800, 8, 2, 8, 8, 16, 64) and small < size(2, 3, 8, 8, 8, 2, 8, 800, 16, 64)
     assert prefix(nbytes=small - 1, pblocks=8, prefixes=1) == 4
