@@ -585,9 +585,12 @@ TIERKV_API int32_t tierkv_extend_attention(
  *      requests' tables, and a prefix may have no request
  * batch + num_prefixes <= 4096.  The prefix adds no position of its own: the
  * keys are in the cache with the positions that they were rotated by.
- * workspace: as there, tierkv_prefix_workspace_bytes(...) bytes (2 (D + 2) * 4
- * bytes for each row and head, and what cut tiles take).  Other arguments,
- * limits, errors and roundings as there; the same inputs give the same bits. */
+ * workspace: as there, tierkv_prefix_workspace_bytes(...) bytes of these
+ * sizes (-1 for sizes that no call takes; fewer rows may take more, since
+ * their tables are cut into more parts).  absmax values enter the products
+ * exactly, code * 2^e with the rest of the scale on the probabilities; other
+ * roundings, arguments, limits and errors as there.  The same inputs give the
+ * same bits. */
 TIERKV_API int64_t tierkv_prefix_workspace_bytes(int32_t batch, int32_t num_prefixes, int32_t num_rows,
                                                  int32_t max_tokens, int32_t num_heads, int32_t num_kv_heads,
                                                  int32_t num_blocks, int32_t num_prefix_blocks, int32_t block_size,

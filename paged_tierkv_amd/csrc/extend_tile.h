@@ -153,6 +153,7 @@ struct ExtendParams {
   // Steps that the host lays out.
   int2* row_pre;           // [rows] {request, place of its first row among the slots' rows}
   int32_t pre_slots, pre_parts, own_parts, own_tiles, own_side;
+  int32_t pre_least, own_least;   // blocks of a part, at least
   int64_t own_unit;        // the requests' own first partial
 };
 

@@ -406,6 +406,16 @@ constexpr int PX_STEP = 64;        // rows of a request, at most: tiles of 32
 constexpr int PX_LIST = 416;       // sub-tiles that a workgroup lists
 constexpr int PX_MOST = 8;         // requests' parts side by side in a workgroup, where it is not one
 
+// What a workgroup of a step takes, or one of several side by side: parts of
+// one slot's rows, for one kv head, or of a request's own.
+struct PxWork {
+  int h, tile, rows, n;    // rows: of the slot's prefix or of the request, n: their tokens
+  int row, nb, per, used;  // of the tables: row, its blocks, how they are cut (used 0: nothing to do)
+  int hidden;              // tokens of the request in all
+  int first;               // packed row of token 0, or, of a slot, the token of its first entry
+  int unit;                // of part 0
+};
+
 // A step's workgroup's LDS beside the tiles'.
 struct PxShared {
   int4 list[PX_LIST + 4 * PX_MOST];   // (spare entries behind each part's, which may be read)
@@ -483,23 +493,30 @@ __device__ __forceinline__ int2 px_scan(int a, int b, int2 (&sh)[EX_WAVES], int2
   return v;
 }
 
-// What a part of a step takes: one of a slot's rows, for one kv head, or of a
-// request's own.
+// How a table row of nb blocks is cut: blocks of a part, and parts, at least
+// one.  (The host's parts are for rows of the table's width; shorter ones have
+// fewer, so that a part stays worth its workgroup's time.)
+__device__ __forceinline__ int2 px_cut(int nb, int parts, int least) {
+  const int per = max((nb + parts - 1) / parts, least);
+  return make_int2(per, max((nb + per - 1) / per, 1));
+}
+
+__device__ __forceinline__ int px_own_blocks(const ExtendParams& p, int b) {
+  return p.seq_nblocks ? min(max(p.seq_nblocks[b], 0), p.num_blocks) : p.num_blocks;
+}
+
+__device__ __forceinline__ int px_pre_blocks(const ExtendParams& p, int g) {
+  return p.pre_nblocks ? min(max(p.pre_nblocks[g], 0), p.pre_blocks) : p.pre_blocks;
+}
+
 struct PxPart {
-  int h, tile, rows;       // rows: of the slot's prefix or of the request
   int4 seq;
   const int4* list;
-  int64_t unit;
-  int first;               // packed row of token 0, or, with a map, the token of its first entry
-  const int* map;
-  bool dead;
 };
 
-// A slot's; dead where there is none.
-template <bool MIXED>
-__device__ __forceinline__ PxPart px_step_prefix(const ExtendParams& p, char* lds, PxShared& s, int x) {
+// A slot's.
+__device__ __forceinline__ PxWork px_step_prefix(const ExtendParams& p, char* lds, PxShared& s, int h, int slot, bool enters, int each) {
   const int tid = threadIdx.x, G = p.groups;
-  const int h = x % p.kv_heads, part = x / p.kv_heads % p.pre_parts, slot = x / p.kv_heads / p.pre_parts;
   // The slot's prefix g, its tile of it, and the prefix's rows.
   int* const counts = reinterpret_cast<int*>(lds);
   for (int i = tid; i < p.prefixes; i += EX_THREADS) counts[i] = 0;
@@ -527,8 +544,7 @@ __device__ __forceinline__ PxPart px_step_prefix(const ExtendParams& p, char* ld
   if (before > p.pre_slots && tid == 0) atomicOr(p.err, 4);   // (packed ranges that overlap)
   __syncthreads();
   const int g = ex_uniform(s.found[0]), t = ex_uniform(s.found[1]), n = ex_uniform(s.found[2]);
-  PxPart o{};
-  o.dead = g < 0;
+  PxWork o{};
   if (g < 0) return o;
   // The tile's tokens, in the order of their requests.
   const int row0 = t * EX_WIDE, t0 = row0 / G, t1 = min((min(row0 + EX_WIDE, n * G) + G - 1) / G, n);
@@ -542,17 +558,31 @@ __device__ __forceinline__ PxPart px_step_prefix(const ExtendParams& p, char* ld
     for (int k = max(t0 - place, 0); k < min(t1 - place, r.y); ++k) {
       s.rows[place + k - t0] = r.x + k;
       // Where its rows are among the slots', by the tile that its first is in.
-      if (h == 0 && part == 0 && (place + k) * G >= row0) p.row_pre[r.x + k] = make_int2(i, (slot - t) * EX_WIDE + (place + k) * G);
+      if (enters && (place + k) * G >= row0) p.row_pre[r.x + k] = make_int2(i, (slot - t) * EX_WIDE + (place + k) * G);
     }
     before += total.x;
   }
-  // The part's sub-tiles.
-  const int nb = p.pre_nblocks ? min(max(p.pre_nblocks[g], 0), p.pre_blocks) : p.pre_blocks;
-  const int per = (nb + p.pre_parts - 1) / p.pre_parts, k0 = min(part * per, nb), k1 = min(k0 + per, nb);
-  const int64_t row = g * p.pre_stride;
+  o.nb = px_pre_blocks(p, g);
+  const int2 cut = px_cut(o.nb, p.pre_parts, p.pre_least);
+  o.h = h;
+  o.tile = t;
+  o.rows = n * G;
+  o.n = n;
+  o.row = g;
+  o.per = cut.x;
+  o.used = cut.y;
+  o.first = t0;
+  o.unit = slot * p.pre_parts * each;
+  return o;
+}
+
+__device__ __forceinline__ PxPart px_prefix_part(const ExtendParams& p, PxShared& s, const PxWork& o, int part) {
+  const int k0 = min(part * o.per, o.nb), k1 = min(k0 + o.per, o.nb);
+  const int64_t row = o.row * p.pre_stride;
+  int2 total;
   int subs = 0, cold = 0;
   for (int i0 = k0; i0 < k1; i0 += EX_THREADS) {
-    const PxBlock k = px_block(p, p.pre_table + row, p.pre_states + row, p.pre_lengths + row, i0 + tid, k1);
+    const PxBlock k = px_block(p, p.pre_table + row, p.pre_states + row, p.pre_lengths + row, i0 + int(threadIdx.x), k1);
     const int count = k.keep == 2 ? 0 : k.count;   // (every row sees them: a count)
     const int2 v = px_scan<EX_WAVES>(count, k.keep == 2 ? k.len : 0, s.scan, &total);
     px_enter(s.list + subs + v.x - count, k, count, 0);
@@ -560,42 +590,49 @@ __device__ __forceinline__ PxPart px_step_prefix(const ExtendParams& p, char* ld
     cold += total.y;
   }
   __syncthreads();
-  o.h = h;
-  o.tile = t;
-  o.rows = n * G;
-  o.seq = make_int4(subs, n + 64, cold, n);   // (every row sees every token: limits past a sub-tile's end)
-  o.list = s.list;
-  o.unit = (int64_t(slot) * p.pre_parts + part) * (MIXED ? EX_WIDE / EX_UNIT : 1);
-  o.first = t0;
-  o.map = s.rows;
+  return {make_int4(subs, o.n + 64, cold, o.n), s.list};   // (every row sees every token: limits past a sub-tile's end)
+}
+
+// A request's, EX_WAVES / KW side by side: unit u of (request, tile, kv head).
+template <int KW>
+__device__ __forceinline__ PxWork px_step_own(const ExtendParams& p, int x, bool enters) {
+  const int units = p.batch * p.own_tiles * p.kv_heads;
+  const int u = x * (EX_WAVES / KW) + ex_uniform(threadIdx.x >> 6) / KW;
+  const bool dead = u >= units;
+  const int v0 = min(u, units - 1), v1 = v0 / p.kv_heads, tile = v1 % p.own_tiles, b = v1 / p.own_tiles;
+  PxWork o{};
+  const int2 rows = ex_rows(p, b, &o.hidden);
+  o.h = v0 - v1 * p.kv_heads;
+  o.tile = tile;
+  o.n = rows.y;
+  o.rows = o.n * p.groups;
+  o.first = rows.x;
+  if (enters && o.h == 0 && tile == 0 && !dead) {
+    const int g = px_prefix(p, b);
+    for (int i = threadIdx.x % (64 * KW); i < min(o.hidden, p.rows - rows.x); i += 64 * KW)
+      p.row_home[rows.x + i] = make_int4(i < o.n ? b : -1, i, g, 0);
+    if (o.n < o.hidden && threadIdx.x % (64 * KW) == 0) atomicOr(p.err, 4);
+  }
+  o.row = b;
+  o.nb = px_own_blocks(p, b);
+  const int2 cut = px_cut(o.nb, p.own_parts, p.own_least);
+  o.per = cut.x;
+  o.used = dead || tile * EX_NARROW >= o.rows ? 0 : cut.y;
+  o.unit = int(p.own_unit) + v1 * p.own_parts;
   return o;
 }
 
-// A request's, EX_WAVES / KW side by side.
 template <int KW>
-__device__ __forceinline__ PxPart px_step_own(const ExtendParams& p, PxShared& s, int x) {
+__device__ __forceinline__ PxPart px_own_part(const ExtendParams& p, PxShared& s, const PxWork& o, int part) {
   constexpr int SIDE = EX_WAVES / KW, THREADS = 64 * KW;
-  const int w = ex_uniform(threadIdx.x >> 6), mine = w / KW, tid = threadIdx.x % THREADS;
-  const int64_t units = int64_t(p.batch) * p.own_tiles * p.own_parts * p.kv_heads;
-  const int64_t u = int64_t(x) * SIDE + mine;
-  const bool dead = u >= units;
-  const int64_t v0 = min(u, units - 1), v1 = v0 / p.kv_heads, v2 = v1 / p.own_parts;
-  const int h = int(v0 % p.kv_heads), part = int(v1 % p.own_parts), tile = int(v2 % p.own_tiles), b = int(v2 / p.own_tiles);
-  int n_all;
-  const int2 rows = ex_rows(p, b, &n_all);
-  const int q0 = rows.x, n = rows.y, g = px_prefix(p, b);
-  if (h == 0 && part == 0 && tile == 0 && !dead) {
-    for (int i = tid; i < min(n_all, p.rows - q0); i += THREADS) p.row_home[q0 + i] = make_int4(i < n ? b : -1, i, g, 0);
-    if (n < n_all && tid == 0) atomicOr(p.err, 4);
-  }
-  const int nb = p.seq_nblocks ? min(max(p.seq_nblocks[b], 0), p.num_blocks) : p.num_blocks;
-  const int per = (nb + p.own_parts - 1) / p.own_parts, k0 = min(part * per, nb), k1 = min(k0 + per, nb);
-  const int64_t row = int64_t(b) * p.stride;
+  const int mine = ex_uniform(threadIdx.x >> 6) / KW, tid = threadIdx.x % THREADS;
+  const int k0 = min(part * o.per, o.nb), k1 = min(k0 + o.per, o.nb);
+  const int64_t row = o.row * p.stride;
   const PxBlock k = px_block(p, p.table + row, p.states + row, p.lengths + row, k0 + tid, k1);   // (per <= THREADS)
   // Tokens before the part and in all.
   int2 total;
   int below = 0, held = 0;
-  for (int i = tid; i < nb; i += THREADS) {
+  for (int i = tid; i < o.nb; i += THREADS) {
     const int len = min(max(p.lengths[row + i], 0), p.bs);
     held += len;
     if (i < k0) below += len;
@@ -604,22 +641,13 @@ __device__ __forceinline__ PxPart px_step_own(const ExtendParams& p, PxShared& s
   const int base = total.x, tokens = total.y;
   const int2 lens = px_scan<KW>(k.len, 0, s.scan, &total);
   const int first = base + lens.x - k.len;
-  const bool all_see = k.keep == 2 && first + k.len <= tokens - n_all + 1;
+  const bool all_see = k.keep == 2 && first + k.len <= tokens - o.hidden + 1;
   const int count = all_see ? 0 : k.count;
   const int2 v = px_scan<KW>(count, all_see ? k.len : 0, s.scan, &total);
   int4* const list = s.list + mine * (PX_LIST / SIDE + 4);
   px_enter(list + v.x - count, k, count, first);
   __syncthreads();
-  PxPart o{};
-  o.h = h;
-  o.tile = tile;
-  o.rows = n * p.groups;
-  o.seq = make_int4(total.x, tokens - (n_all - n), total.y, n);
-  o.list = list;
-  o.unit = p.own_unit + v1;
-  o.first = q0;
-  o.dead = dead || tile * EX_NARROW >= n * p.groups;
-  return o;
+  return {make_int4(total.x, tokens - (o.hidden - o.n), total.y, o.n), list};
 }
 
 // MIXED: calls that may hold wide tiles; the others' kernel is without their code.
@@ -627,22 +655,34 @@ template <int DP, int WF, typename QT, bool MIXED>
 __global__ __launch_bounds__(EX_THREADS, 2) void prefix_step_kernel(ExtendParams p) {
   extern __shared__ __attribute__((aligned(16))) char px_lds[];
   __shared__ PxShared s;
-  const int pre = p.pre_slots * p.pre_parts * p.kv_heads, x = blockIdx.x;
-  PxPart o;
-  int side = 1;
-  if (x < pre) {
-    o = px_step_prefix<MIXED>(p, px_lds, s, x);
-    if (o.dead) return;
-  } else {
-    side = p.own_side;
-    if (side == 1) o = px_step_own<EX_WAVES>(p, s, x - pre);
-    else o = px_step_own<EX_WAVES / PX_MOST>(p, s, x - pre);
+  constexpr int KW_SIDE = EX_WAVES / PX_MOST;
+  const int pre = p.pre_slots * p.pre_parts * p.kv_heads, x = blockIdx.x, each = MIXED ? EX_WIDE / EX_UNIT : 1;
+  const bool shared = x < pre;
+  const int side = shared ? 1 : p.own_side;
+  PxWork o;
+  int part;
+  if (shared) {
+    const int v = x / p.kv_heads, h = x - v * p.kv_heads, slot = v / p.pre_parts;
+    part = v - slot * p.pre_parts;
+    o = px_step_prefix(p, px_lds, s, h, slot, h == 0 && part == 0, each);
+  } else {   // (part by part: those that are not there come last)
+    const int groups = (p.batch * p.own_tiles * p.kv_heads + side - 1) / side, y = x - pre;
+    part = y / groups;
+    if (side == 1) o = px_step_own<EX_WAVES>(p, y - part * groups, part == 0);
+    else o = px_step_own<KW_SIDE>(p, y - part * groups, part == 0);
   }
-  auto packed = [&](int t) { return o.map ? o.map[max(t - o.first, 0)] : o.first + t; };
-  const PxList list = {o.list};
-  if (MIXED && x < pre && o.rows > EX_NARROW) ex_tile_part<DP, WF, QT, true, true, 1>(p, px_lds, o.h, o.tile, 0, 1, o.seq, list, packed, o.unit);
-  else if (side == 1) ex_tile_part<DP, WF, QT, false, true, EX_WAVES>(p, px_lds, o.h, o.tile, 0, 1, o.seq, list, packed, o.unit, o.dead);
-  else ex_tile_part<DP, WF, QT, false, true, EX_WAVES / PX_MOST>(p, px_lds, o.h, o.tile, 0, 1, o.seq, list, packed, o.unit, o.dead);
+  const bool dead = part >= o.used;
+  if (side == 1 ? dead : !__syncthreads_or(!dead)) return;
+  PxPart of;
+  if (shared) of = px_prefix_part(p, s, o, part);
+  else if (side == 1) of = px_own_part<EX_WAVES>(p, s, o, part);
+  else of = px_own_part<KW_SIDE>(p, s, o, part);
+  const PxList list = {of.list};
+  auto packed = [&](int t) { return shared ? s.rows[max(t - o.first, 0)] : o.first + t; };
+  const int64_t unit = o.unit + part * (shared ? each : 1);
+  if (MIXED && shared && o.rows > EX_NARROW) ex_tile_part<DP, WF, QT, true, true, 1>(p, px_lds, o.h, o.tile, 0, 1, of.seq, list, packed, unit);
+  else if (side == 1) ex_tile_part<DP, WF, QT, false, true, EX_WAVES>(p, px_lds, o.h, o.tile, 0, 1, of.seq, list, packed, unit);
+  else ex_tile_part<DP, WF, QT, false, true, KW_SIDE>(p, px_lds, o.h, o.tile, 0, 1, of.seq, list, packed, unit, dead);
 }
 
 template <typename QT>
@@ -668,12 +708,12 @@ __global__ __launch_bounds__(EX_THREADS) void prefix_step_join_kernel(ExtendPara
   int64_t pre_at = 0;
   if (home.z >= 0) {
     const int64_t row = int64_t(of.y) + hd - h * G, slot = row / EX_WIDE;
-    if (of.x != home.x || of.y < 0 || slot >= p.pre_slots) return;
-    pre_count = p.pre_parts;
+    if (of.x != home.x || of.y < 0 || slot >= p.pre_slots || home.z >= p.prefixes) return;
+    pre_count = px_cut(px_pre_blocks(p, home.z), p.pre_parts, p.pre_least).y;
     pre_at = ex_unit_row(p, slot * p.pre_parts * each, h, int(row - slot * EX_WIDE));
   }
-  const int count = p.own_parts + pre_count;
-  auto place = [&](int k) { return k < p.own_parts ? at + k * step : pre_at + (k - p.own_parts) * each * step; };
+  const int own_count = px_cut(px_own_blocks(p, home.x), p.own_parts, p.own_least).y, count = own_count + pre_count;
+  auto place = [&](int k) { return k < own_count ? at + k * step : pre_at + (k - own_count) * each * step; };
   ExJoin j;
   int k0 = 0;
   for (; count - k0 > 4; k0 += 8) j.take<8>(p, count - k0, d, [&](int k) { return place(k0 + k); });
@@ -735,6 +775,7 @@ static PrefixLayout prefix_layout(int64_t batch, int64_t prefixes, int64_t rows,
 struct StepLayout {
   int64_t row_home, row_pre, part_o, part_ml, total;
   int64_t slots, pre_parts, own_parts, own_tiles, side, each, own_unit, units, workgroups;
+  int64_t pre_least, own_least;
   bool use;
 };
 
@@ -781,7 +822,10 @@ static StepLayout step_layout(int64_t batch, int64_t prefixes, int64_t rows, int
   }
   l.own_unit = l.slots * l.pre_parts * l.each;
   l.units = l.own_unit + batch * l.own_tiles * l.own_parts;
-  l.workgroups = l.slots * l.pre_parts * kv_heads + div(batch * l.own_tiles * l.own_parts * kv_heads, l.side);
+  // Least parts: one round of narrow sub-tiles, and eight wide sub-tiles.
+  l.own_least = std::max<int64_t>(2 * (EX_WAVES / l.side) / subs, 1);
+  l.pre_least = std::max<int64_t>(8 / subs, 1);
+  l.workgroups = l.slots * l.pre_parts * kv_heads + div(batch * l.own_tiles * kv_heads, l.side) * l.own_parts;
   l.row_home = EX_WS_HEAD;
   l.row_pre = up(l.row_home + rows * 16);
   l.part_ml = up(l.row_pre + rows * 8);
@@ -885,6 +929,7 @@ extern "C" int32_t tierkv_prefix_attention(
                                                   num_blocks, num_prefix_blocks, block_size, head_dim);
   // (a launch has fewer than 2^32 threads)
   if (l.items * num_kv_heads > 0x7fffffff || step.workgroups > 0xffffffffll / EX_THREADS ||
+      batch * step.own_tiles * num_kv_heads > 0x7fffff00 ||
       int64_t(num_rows) * num_heads > (0xffffffffll - EX_THREADS) / (head_dim / 4) || std::max(l.units, step.units) > 0x7fffffff)
     return fail(TIERKV_ERR_UNSUPPORTED, "grid too large");
   if (workspace_bytes < (step.use ? std::max<int64_t>(step.total, EX_WS_HEAD) : l.total))
@@ -903,6 +948,8 @@ extern "C" int32_t tierkv_prefix_attention(
     p.own_tiles = int32_t(step.own_tiles);
     p.own_side = int32_t(step.side);
     p.own_unit = step.own_unit;
+    p.pre_least = int32_t(step.pre_least);
+    p.own_least = int32_t(step.own_least);
   } else {
     p.arrived = reinterpret_cast<uint32_t*>(ws + l.arrived);
     p.head = reinterpret_cast<int32_t*>(ws + l.head);

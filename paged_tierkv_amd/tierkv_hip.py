@@ -780,7 +780,9 @@ def extend_workspace(device, batch: int, num_tokens: int, num_heads: int, kv_hea
                      prefix_blocks: int = 0) -> DecodeWorkspace:
     """A fixed workspace for ``tierkv_extend_attention`` calls of this
     geometry, as captured steps need one; with ``prefixes`` rows of
-    ``prefix_blocks`` blocks, for ``tierkv_prefix_attention``."""
+    ``prefix_blocks`` blocks, for ``tierkv_prefix_attention`` (calls of these
+    sizes: fewer tokens may take more, their tables being cut into more
+    parts)."""
     need = _extend_bytes(int(batch), int(num_tokens), int(num_tokens if max_tokens is None else min(max_tokens, num_tokens)),
                          int(num_heads), int(kv_heads), int(num_blocks), int(block_size), int(head_dim), int(prefixes),
                          int(prefix_blocks))
