@@ -151,7 +151,7 @@ struct ExtendParams {
   int2* seg;               // [segments] {first tile, where its first row (prefixes: in row_list) or its list is}
   int2* tile;              // [max_tiles] {first partial or -1 (the item wrote the rows itself), parts}
   // Steps that the host lays out.
-  int2* row_pre;           // [rows] {request, place of its first row among the slots' rows}
+  int4* row_pre;           // [rows] {request, place of its first row among the slots' rows, parts of the prefix, 0}
   int32_t pre_slots, pre_parts, own_parts, own_tiles, own_side;
   int32_t pre_least, own_least;   // blocks of a part, at least
   int64_t own_unit;        // the requests' own first partial

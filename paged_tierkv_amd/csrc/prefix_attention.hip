@@ -501,14 +501,6 @@ __device__ __forceinline__ int2 px_cut(int nb, int parts, int least) {
   return make_int2(per, max((nb + per - 1) / per, 1));
 }
 
-__device__ __forceinline__ int px_own_blocks(const ExtendParams& p, int b) {
-  return p.seq_nblocks ? min(max(p.seq_nblocks[b], 0), p.num_blocks) : p.num_blocks;
-}
-
-__device__ __forceinline__ int px_pre_blocks(const ExtendParams& p, int g) {
-  return p.pre_nblocks ? min(max(p.pre_nblocks[g], 0), p.pre_blocks) : p.pre_blocks;
-}
-
 struct PxPart {
   int4 seq;
   const int4* list;
@@ -546,6 +538,8 @@ __device__ __forceinline__ PxWork px_step_prefix(const ExtendParams& p, char* ld
   const int g = ex_uniform(s.found[0]), t = ex_uniform(s.found[1]), n = ex_uniform(s.found[2]);
   PxWork o{};
   if (g < 0) return o;
+  o.nb = p.pre_nblocks ? min(max(p.pre_nblocks[g], 0), p.pre_blocks) : p.pre_blocks;
+  const int2 cut = px_cut(o.nb, p.pre_parts, p.pre_least);
   // The tile's tokens, in the order of their requests.
   const int row0 = t * EX_WIDE, t0 = row0 / G, t1 = min((min(row0 + EX_WIDE, n * G) + G - 1) / G, n);
   before = 0;
@@ -558,12 +552,10 @@ __device__ __forceinline__ PxWork px_step_prefix(const ExtendParams& p, char* ld
     for (int k = max(t0 - place, 0); k < min(t1 - place, r.y); ++k) {
       s.rows[place + k - t0] = r.x + k;
       // Where its rows are among the slots', by the tile that its first is in.
-      if (enters && (place + k) * G >= row0) p.row_pre[r.x + k] = make_int2(i, (slot - t) * EX_WIDE + (place + k) * G);
+      if (enters && (place + k) * G >= row0) p.row_pre[r.x + k] = make_int4(i, (slot - t) * EX_WIDE + (place + k) * G, cut.y, 0);
     }
     before += total.x;
   }
-  o.nb = px_pre_blocks(p, g);
-  const int2 cut = px_cut(o.nb, p.pre_parts, p.pre_least);
   o.h = h;
   o.tile = t;
   o.rows = n * G;
@@ -607,15 +599,15 @@ __device__ __forceinline__ PxWork px_step_own(const ExtendParams& p, int x, bool
   o.n = rows.y;
   o.rows = o.n * p.groups;
   o.first = rows.x;
+  o.nb = p.seq_nblocks ? min(max(p.seq_nblocks[b], 0), p.num_blocks) : p.num_blocks;
+  const int2 cut = px_cut(o.nb, p.own_parts, p.own_least);
   if (enters && o.h == 0 && tile == 0 && !dead) {
     const int g = px_prefix(p, b);
     for (int i = threadIdx.x % (64 * KW); i < min(o.hidden, p.rows - rows.x); i += 64 * KW)
-      p.row_home[rows.x + i] = make_int4(i < o.n ? b : -1, i, g, 0);
+      p.row_home[rows.x + i] = make_int4(i < o.n ? b : -1, i, g, cut.y);
     if (o.n < o.hidden && threadIdx.x % (64 * KW) == 0) atomicOr(p.err, 4);
   }
   o.row = b;
-  o.nb = px_own_blocks(p, b);
-  const int2 cut = px_cut(o.nb, p.own_parts, p.own_least);
   o.per = cut.x;
   o.used = dead || tile * EX_NARROW >= o.rows ? 0 : cut.y;
   o.unit = int(p.own_unit) + v1 * p.own_parts;
@@ -695,7 +687,7 @@ __global__ __launch_bounds__(EX_THREADS) void prefix_step_join_kernel(ExtendPara
   if (r >= p.rows) return;
   const int hd = int(rh - r * p.heads), h = hd / G;
   const int4 home = p.row_home[r];
-  const int2 of = p.row_pre[r];
+  const int4 of = p.row_pre[r];
   // (a row of no request has whatever the workspace held)
   if (home.x < 0 || home.x >= p.batch) return;
   const int2 rows_of = ex_rows(p, home.x);
@@ -708,11 +700,11 @@ __global__ __launch_bounds__(EX_THREADS) void prefix_step_join_kernel(ExtendPara
   int64_t pre_at = 0;
   if (home.z >= 0) {
     const int64_t row = int64_t(of.y) + hd - h * G, slot = row / EX_WIDE;
-    if (of.x != home.x || of.y < 0 || slot >= p.pre_slots || home.z >= p.prefixes) return;
-    pre_count = px_cut(px_pre_blocks(p, home.z), p.pre_parts, p.pre_least).y;
+    if (of.x != home.x || of.y < 0 || slot >= p.pre_slots) return;
+    pre_count = min(max(of.z, 0), p.pre_parts);
     pre_at = ex_unit_row(p, slot * p.pre_parts * each, h, int(row - slot * EX_WIDE));
   }
-  const int own_count = px_cut(px_own_blocks(p, home.x), p.own_parts, p.own_least).y, count = own_count + pre_count;
+  const int own_count = min(max(home.w, 0), p.own_parts), count = own_count + pre_count;
   auto place = [&](int k) { return k < own_count ? at + k * step : pre_at + (k - own_count) * each * step; };
   ExJoin j;
   int k0 = 0;
@@ -828,7 +820,7 @@ static StepLayout step_layout(int64_t batch, int64_t prefixes, int64_t rows, int
   l.workgroups = l.slots * l.pre_parts * kv_heads + div(batch * l.own_tiles * kv_heads, l.side) * l.own_parts;
   l.row_home = EX_WS_HEAD;
   l.row_pre = up(l.row_home + rows * 16);
-  l.part_ml = up(l.row_pre + rows * 8);
+  l.part_ml = up(l.row_pre + rows * 16);
   l.part_o = up(l.part_ml + l.units * kv_heads * EX_UNIT * 8);
   l.total = up(l.part_o + l.units * kv_heads * EX_UNIT * D * 4);
   return l;
@@ -939,7 +931,7 @@ extern "C" int32_t tierkv_prefix_attention(
   p.err = reinterpret_cast<int32_t*>(ws);
   if (step.use) {
     p.row_home = reinterpret_cast<int4*>(ws + step.row_home);
-    p.row_pre = reinterpret_cast<int2*>(ws + step.row_pre);
+    p.row_pre = reinterpret_cast<int4*>(ws + step.row_pre);
     p.part_o = reinterpret_cast<float*>(ws + step.part_o);
     p.part_ml = reinterpret_cast<float*>(ws + step.part_ml);
     p.pre_slots = int32_t(step.slots);
