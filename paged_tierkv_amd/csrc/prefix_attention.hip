@@ -422,6 +422,7 @@ struct PxShared {
   int rows[EX_WIDE + 4];              // packed rows of a tile's tokens
   int2 scan[EX_WAVES];
   int found[4];
+  int dead[EX_WAVES];
 };
 static_assert(ex_lds_bytes<128>() + sizeof(PxShared) + 256 <= 160 * 1024 && ex_lds_bytes<64>() <= ex_lds_bytes<128>(),
               "a CU's LDS, 256 bytes of it for a vote of the workgroup");
@@ -664,13 +665,24 @@ __global__ __launch_bounds__(EX_THREADS, 2) void prefix_step_kernel(ExtendParams
     else o = px_step_own<KW_SIDE>(p, y - part * groups, part == 0);
   }
   const bool dead = part >= o.used;
-  if (side == 1 ? dead : !__syncthreads_or(!dead)) return;
+  if (side == 1) {
+    if (dead) return;
+  } else {
+    if ((threadIdx.x & 63) == 0) s.dead[threadIdx.x >> 6] = dead;
+    __syncthreads();
+    int all = 1;
+    for (int w = 0; w < EX_WAVES; ++w) all &= s.dead[w];
+    if (all) return;
+  }
   PxPart of;
   if (shared) of = px_prefix_part(p, s, o, part);
   else if (side == 1) of = px_own_part<EX_WAVES>(p, s, o, part);
   else of = px_own_part<KW_SIDE>(p, s, o, part);
+  // (a wave's all alike: scalar registers)
+  for (int* v : {&of.seq.x, &of.seq.y, &of.seq.z, &of.seq.w, &o.h, &o.tile, &o.rows, &o.first, &o.unit}) *v = ex_uniform(*v);
   const PxList list = {of.list};
-  auto packed = [&](int t) { return shared ? s.rows[max(t - o.first, 0)] : o.first + t; };
+  const int first = o.first;
+  auto packed = [&](int t) { return shared ? s.rows[max(t - first, 0)] : first + t; };
   const int64_t unit = o.unit + part * (shared ? each : 1);
   if (MIXED && shared && o.rows > EX_NARROW) ex_tile_part<DP, WF, QT, true, true, 1>(p, px_lds, o.h, o.tile, 0, 1, of.seq, list, packed, unit);
   else if (side == 1) ex_tile_part<DP, WF, QT, false, true, EX_WAVES>(p, px_lds, o.h, o.tile, 0, 1, of.seq, list, packed, unit);
