@@ -52,7 +52,9 @@
 // prefixes round less: there V of an absmax block goes in as code * 2^e, exact,
 // and the rest of the scale m, scale = m 2^e, multiplies the probabilities
 // before their rounding (fp16 outputs 1.4 times as far from 64 bits as a
-// product in 32 bits rounded once, with both rounded 1.65 times).
+// product in 32 bits rounded once, with both rounded 1.65 times; 16 prompts of
+// up to 512 tokens on 16384: 2047 us against 1904, 1933 once the compiler left
+// loop-invariant code where it was; single tokens level).
 // Probabilities carry a factor 2^6 so that small ones stay normal fp16.
 // bf16 queries become fp16 after division by a power of two near the row's
 // largest value, which the logits get back in 32 bits.

@@ -16,15 +16,22 @@
 // sharing: its tiles walk the prefix and then its own tokens, as if its table
 // held both, and have no parts to join.
 //
-// Three launches:
+// Steps of a few tokens per request are laid out by the host (below).  Others
+// take three launches:
 //   * prefix_plan_kernel, a workgroup per segment, lists its sub-tiles and
 //     enters its rows; the last to finish cuts the segments' tiles into items;
 //   * prefix_kernel, up to one workgroup per CU, which take items until none is
 //     left: wide ones (256 rows, eight waves together) first, then narrow ones
-//     (up to 32 rows), four side by side with two waves each.  Single tokens on
-//     short contexts are most of a decode step's items, and each is a chain
-//     of reads; one at a time per workgroup took three times as long;
+//     (up to 32 rows), four side by side with two waves each, since each is a
+//     chain of reads; one at a time per workgroup took three times as long;
 //   * prefix_join_kernel adds up the parts of rows that have several.
+//
+// Bound: vector instructions beside the matrix products for prompts (16 of up
+// to 512 tokens on a prefix of 16384, 32 heads on 8 kv heads of 128: 1933 us,
+// 667 TFLOP/s); for steps the requests' own tokens at the memory rate, and 7 us
+// that a workgroup takes to start and end, one at a time per CU (64 single
+// tokens on a prefix of 8192: 42 us; 256 on 4 of 4096: 80; 24 x 5 on
+// 1501: 27; 2 on 600: 17).
 
 #include "extend_tile.h"
 
@@ -239,7 +246,8 @@ __global__ __launch_bounds__(EX_PLAN) void prefix_plan_kernel(ExtendParams p) {
   const int per_wide = s_per[choice];
   // Whole tiles that would begin a last round of the slots, not full, are cut
   // by `tail`, so that the round is shorter (113 tiles on 32 places: 2147 us
-  // with four rounds, 1920 with the last 17 tiles cut).
+  // with four rounds, 1920 with the last 17 tiles cut, before absmax values
+  // entered the products exactly).
   int tail = 1, tail_from = 0x7fffffff;
   {
     const int places = int(slots), items = int(s_items[choice]);
@@ -396,8 +404,8 @@ __global__ __launch_bounds__(EX_THREADS) void prefix_join_kernel(ExtendParams p)
 // Where no request brings more than PX_STEP rows (single tokens, drafts), the plan
 // would cost as much as the attention: a launch of its own, and five dependent
 // reads between it and an item's first key.  These calls are laid out on the
-// host, from sizes alone: every request's table row is cut into own_parts
-// ranges of blocks, every prefix's into pre_parts, and a workgroup lists the
+// host, from sizes alone: a request's table row is cut into up to own_parts
+// ranges of blocks, a prefix's into up to pre_parts, and a workgroup lists the
 // sub-tiles of its range in LDS itself.  A prefix's rows fill tiles ("slots")
 // of 256; how many there are follows from the requests' prefixes, which each
 // workgroup of a slot reads.  Two launches: the parts, and their join.
@@ -495,8 +503,9 @@ __device__ __forceinline__ int2 px_scan(int a, int b, int2 (&sh)[EX_WAVES], int2
 }
 
 // How a table row of nb blocks is cut: blocks of a part, and parts, at least
-// one.  (The host's parts are for rows of the table's width; shorter ones have
-// fewer, so that a part stays worth its workgroup's time.)
+// one.  The host's parts are for rows of the table's width; shorter ones have
+// fewer, and the workgroups of the others, last in the launch, end at once (64
+// requests of 250 tokens in tables of 16384 blocks: 143 us, 611 with all parts).
 __device__ __forceinline__ int2 px_cut(int nb, int parts, int least) {
   const int per = max((nb + parts - 1) / parts, least);
   return make_int2(per, max((nb + per - 1) / per, 1));

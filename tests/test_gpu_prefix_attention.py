@@ -226,6 +226,23 @@ def test_visible_infinities_arrive_where_they_belong(device):
     assert torch.equal(out[~hit], clean[~hit])
 
 
+@pytest.mark.parametrize("bs,spare,many", [(16, 900, 1), (16, 5000, 1), (64, 700, 1), (16, 3000, 12)])
+@pytest.mark.parametrize("cold", ["masked", "zero_logit"])
+def test_tables_far_wider_than_their_rows(device, bs, spare, many, cold):
+    """Rows of few blocks and of many in tables of thousands, which a step cuts
+    by their width: its parts that a row does not have are left out."""
+    s = step(18, [30, 4000, 0], [0, 1, 1, 2, -1] * many, [1, 3, 1, 0, 2] * many, [20, 5000, 64, 9, 300] + [20, 50, 64, 9, 300] * (many - 1),
+             8, 2, 64, bs=bs, spare=spare)
+    t = tensors(s, device)
+    ws = DecodeWorkspace(device)
+    out = launch(t, s, cold, workspace=ws, max_tokens=3)
+    assert ws.error_word() == 0
+    check(out, s, cold)
+    t["own"][3].zero_()                                  # no blocks of their own: the prefix alone
+    s["own"][3][:] = 0
+    check(launch(t, s, cold, workspace=ws, max_tokens=3), s, cold)
+
+
 def test_order_of_requests_and_repeated_calls_keep_the_bits(device):
     """The same inputs twice give the same bits; a request's result does not
     depend on where its rows stand, up to the joins' rounding."""
