@@ -321,7 +321,7 @@ __device__ __forceinline__ void px_item(const ExtendParams& p, char* lds, int h,
 
 // Workgroups take wide items one by one, then narrow ones PX_SIDE at a time,
 // until none is left: the first by their number, the others from a counter.
-template <int DP, int WF, typename QT, bool MIXED>
+template <int DP, int WF, typename QT>
 __global__ __launch_bounds__(EX_THREADS, 2) void prefix_kernel(ExtendParams p) {
   extern __shared__ __attribute__((aligned(16))) char px_lds[];
   __shared__ int s_next;
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(EX_THREADS, 2) void prefix_kernel(ExtendParams p) {
   while (j < all) {
     int next = 0;
     if (threadIdx.x == 0) next = atomicAdd(p.head + 2, 1) + int(gridDim.x);
-    if (MIXED && j < wide) {
+    if (j < wide) {
       const int i = j / p.kv_heads, h = j - i * p.kv_heads;
       const ex_int4 it = ((ExList)(uintptr_t)p.item)[i];
       if (it.x >= 0) px_item<DP, WF, QT, true>(p, px_lds, h, it, false);
@@ -742,7 +742,6 @@ __global__ __launch_bounds__(EX_THREADS) void prefix_step_join_kernel(ExtendPara
 struct PrefixLayout {
   int64_t arrived, head, seq, seg, tile, row_list, row_home, subtile, item, part_o, part_ml, total;
   int64_t subs, pre_subs, lone, tiles, wide_items, items, units;
-  bool wide;
 };
 
 // Tiles as ex_layout counts them, for the requests' rows and once more for the
@@ -754,14 +753,11 @@ static PrefixLayout prefix_layout(int64_t batch, int64_t prefixes, int64_t rows,
   PrefixLayout l{};
   auto up = [](int64_t x) { return (x + 255) & ~int64_t(255); };
   const int64_t all = rows * groups, longest = std::min(rows, max_tokens) * groups;
-  l.wide = all > EX_NARROW;
   // Segments of more than 32 rows, and their tiles of up to 256.
-  auto wide_tiles = [&](int64_t segments, int64_t most) {
-    return most <= EX_NARROW ? 0 : all / EX_WIDE + std::min(segments, all / (EX_NARROW + 1));
-  };
-  const int64_t wide = wide_tiles(batch, longest) + wide_tiles(prefixes, all), narrow = batch + prefixes;
+  auto wide_tiles = [&](int64_t segments) { return all / EX_WIDE + std::min(segments, all / (EX_NARROW + 1)); };
+  const int64_t wide = wide_tiles(batch) + wide_tiles(prefixes), narrow = batch + prefixes;
   l.tiles = wide + narrow;
-  l.wide_items = l.wide ? wide + std::max<int64_t>(EX_TARGET / kv_heads, 1) + (EX_SLOTS / kv_heads + 1) * PX_TAIL : 0;
+  l.wide_items = wide + std::max<int64_t>(EX_TARGET / kv_heads, 1) + (EX_SLOTS / kv_heads + 1) * PX_TAIL;
   l.items = l.wide_items + narrow + (EX_SLOTS / kv_heads + 1) * PX_SIDE;
   l.units = l.wide_items * (EX_WIDE / EX_UNIT) + (l.items - l.wide_items);
   l.lone = longest >= PX_LONE ? std::min(batch, all / PX_LONE) : 0;
@@ -848,13 +844,12 @@ static StepLayout step_layout(int64_t batch, int64_t prefixes, int64_t rows, int
 }
 
 template <int DP, int WF, typename QT>
-static void prefix_launch(const ExtendParams& p, bool wide, hipStream_t stream) {
+static void prefix_launch(const ExtendParams& p, hipStream_t stream) {
   const int lds = ex_lds_bytes<DP>();
   hipLaunchKernelGGL(prefix_plan_kernel, dim3(p.batch + p.prefixes), dim3(EX_PLAN), 0, stream, p);
   const int64_t most = (int64_t(p.max_cut) + (p.max_items - p.max_cut + PX_SIDE - 1) / PX_SIDE) * p.kv_heads;
   const dim3 grid(uint32_t(std::min<int64_t>(most, EX_SLOTS)));
-  if (wide) hipLaunchKernelGGL((prefix_kernel<DP, WF, QT, true>), grid, dim3(EX_THREADS), lds, stream, p);
-  else hipLaunchKernelGGL((prefix_kernel<DP, WF, QT, false>), grid, dim3(EX_THREADS), lds, stream, p);
+  hipLaunchKernelGGL((prefix_kernel<DP, WF, QT>), grid, dim3(EX_THREADS), lds, stream, p);
   const int64_t threads = int64_t(p.rows) * p.heads * (p.D / 4);
   hipLaunchKernelGGL(prefix_join_kernel<QT>, dim3(uint32_t((threads + EX_THREADS - 1) / EX_THREADS)), dim3(EX_THREADS), 0,
                      stream, p);
@@ -873,18 +868,18 @@ static void step_launch(const ExtendParams& p, const StepLayout& l, hipStream_t 
 
 // step: NULL for calls that are planned on the device.
 template <int DP, int WF, typename QT>
-static void prefix_start(const ExtendParams& p, const StepLayout* step, bool wide, hipStream_t stream) {
+static void prefix_start(const ExtendParams& p, const StepLayout* step, hipStream_t stream) {
   if (step) step_launch<DP, WF, QT>(p, *step, stream);
-  else prefix_launch<DP, WF, QT>(p, wide, stream);
+  else prefix_launch<DP, WF, QT>(p, stream);
 }
 
 template <int DP>
-static void prefix_dispatch(const ExtendParams& p, const StepLayout* step, bool wide, int wf, int dtype, hipStream_t stream) {
+static void prefix_dispatch(const ExtendParams& p, const StepLayout* step, int wf, int dtype, hipStream_t stream) {
   const bool bf = dtype == TIERKV_DTYPE_BF16, i8 = wf == TIERKV_WARM_ABSMAX_I8;
-  if (bf && i8) prefix_start<DP, TIERKV_WARM_ABSMAX_I8, __hip_bfloat16>(p, step, wide, stream);
-  else if (bf) prefix_start<DP, TIERKV_WARM_REF_U8, __hip_bfloat16>(p, step, wide, stream);
-  else if (i8) prefix_start<DP, TIERKV_WARM_ABSMAX_I8, __half>(p, step, wide, stream);
-  else prefix_start<DP, TIERKV_WARM_REF_U8, __half>(p, step, wide, stream);
+  if (bf && i8) prefix_start<DP, TIERKV_WARM_ABSMAX_I8, __hip_bfloat16>(p, step, stream);
+  else if (bf) prefix_start<DP, TIERKV_WARM_REF_U8, __hip_bfloat16>(p, step, stream);
+  else if (i8) prefix_start<DP, TIERKV_WARM_ABSMAX_I8, __half>(p, step, stream);
+  else prefix_start<DP, TIERKV_WARM_REF_U8, __half>(p, step, stream);
 }
 
 }  // namespace tierkv
@@ -993,7 +988,7 @@ extern "C" int32_t tierkv_prefix_attention(
   p.prefixes = num_prefixes;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   const StepLayout* of = step.use ? &step : nullptr;
-  if (head_dim <= 64) prefix_dispatch<64>(p, of, l.wide, warm_format, query_dtype, stream);
-  else prefix_dispatch<128>(p, of, l.wide, warm_format, query_dtype, stream);
+  if (head_dim <= 64) prefix_dispatch<64>(p, of, warm_format, query_dtype, stream);
+  else prefix_dispatch<128>(p, of, warm_format, query_dtype, stream);
   return check_launch("tierkv_prefix_attention");
 }
