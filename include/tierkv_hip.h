@@ -587,7 +587,8 @@ TIERKV_API int32_t tierkv_extend_attention(
  * keys are in the cache with the positions that they were rotated by.
  * workspace: as there, tierkv_prefix_workspace_bytes(...) bytes of these
  * sizes (-1 for sizes that no call takes; fewer rows may take more, since
- * their tables are cut into more parts).  absmax values enter the products
+ * their tables are cut into more parts; a small max_tokens takes at most
+ * twice what a large one does).  absmax values enter the products
  * exactly, code * 2^e with the rest of the scale on the probabilities; other
  * roundings, arguments, limits and errors as there.  The same inputs give the
  * same bits. */

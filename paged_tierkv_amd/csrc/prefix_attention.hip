@@ -16,8 +16,8 @@
 // sharing: its tiles walk the prefix and then its own tokens, as if its table
 // held both, and have no parts to join.
 //
-// Steps of a few tokens per request are laid out by the host (below).  Others
-// take three launches:
+// Steps of a few tokens per request are laid out by the host (below), unless
+// their tables are very wide (prefix_call).  Others take three launches:
 //   * prefix_plan_kernel, a workgroup per segment, lists its sub-tiles and
 //     enters its rows; the last to finish cuts the segments' tiles into items;
 //   * prefix_kernel, up to one workgroup per CU, which take items until none is
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(EX_THREADS) void prefix_join_kernel(ExtendParams p)
 // of 256; how many there are follows from the requests' prefixes, which each
 // workgroup of a slot reads.  Two launches: the parts, and their join.
 
-constexpr int PX_STEP = 64;        // rows of a request, at most: tiles of 32
+constexpr int PX_STEP = 64;        // rows of a request, at most: tiles of 32 (and what prefix_call says)
 constexpr int PX_LIST = 416;       // sub-tiles that a workgroup lists
 constexpr int PX_MOST = 8;         // requests' parts side by side in a workgroup, where it is not one
 
@@ -786,6 +786,7 @@ struct StepLayout {
   int64_t slots, pre_parts, own_parts, own_tiles, side, each, own_unit, units, workgroups;
   int64_t pre_least, own_least;
   bool use;
+  int64_t bytes() const { return std::max<int64_t>(total, EX_WS_HEAD); }
 };
 
 static StepLayout step_layout(int64_t batch, int64_t prefixes, int64_t rows, int64_t max_tokens, int64_t groups,
@@ -843,6 +844,31 @@ static StepLayout step_layout(int64_t batch, int64_t prefixes, int64_t rows, int
   return l;
 }
 
+// The way that a call of these sizes takes, and its workspace.  A step's parts
+// and partials follow the tables' width, the plan's the rows there are: past
+// PX_STEP_MEMORY of the plan's workspace, or of a launch's 2^32 threads, calls
+// of few tokens are planned too.  Around that size tables are mostly far wider
+// than their rows, which a step's workgroups pay for and the plan's do not: 256
+// single tokens with 256 of their own in tables of 16384 blocks, 1.4 GB, 501 us as a step and
+// 131 planned; full rows lose by it (64 whose tables of 16384 are full, 1.4
+// times the plan's: 11.0 ms as a step, 20.9 planned).
+constexpr int64_t PX_STEP_MEMORY = 2;
+struct PrefixCall {
+  StepLayout step;
+  PrefixLayout plan;
+  int64_t bytes() const { return step.use ? step.bytes() : plan.total; }
+};
+
+static PrefixCall prefix_call(int64_t batch, int64_t prefixes, int64_t rows, int64_t max_tokens, int64_t groups,
+                              int64_t kv_heads, int64_t num_blocks, int64_t pre_blocks, int64_t bs, int64_t D) {
+  PrefixCall c{};
+  c.step = step_layout(batch, prefixes, rows, max_tokens, groups, kv_heads, num_blocks, pre_blocks, bs, D);
+  c.plan = prefix_layout(batch, prefixes, rows, max_tokens, groups, kv_heads, num_blocks, pre_blocks, bs, D);
+  c.step.use = c.step.use && c.step.workgroups <= 0xffffffffll / EX_THREADS && c.step.units <= 0x7fffffff &&
+               batch * c.step.own_tiles * kv_heads <= 0x7fffff00 && c.step.bytes() <= PX_STEP_MEMORY * c.plan.total;
+  return c;
+}
+
 template <int DP, int WF, typename QT>
 static void prefix_launch(const ExtendParams& p, hipStream_t stream) {
   const int lds = ex_lds_bytes<DP>();
@@ -895,11 +921,8 @@ extern "C" int64_t tierkv_prefix_workspace_bytes(int32_t batch, int32_t num_pref
       head_dim <= 0 || head_dim > 128)
     return -1;
   const int groups = num_heads / num_kv_heads;
-  const StepLayout s = step_layout(batch, num_prefixes, num_rows, max_tokens, groups, num_kv_heads, num_blocks,
-                                   num_prefix_blocks, block_size, head_dim);
-  if (s.use) return std::max<int64_t>(s.total, EX_WS_HEAD);
-  return prefix_layout(batch, num_prefixes, num_rows, max_tokens, groups, num_kv_heads, num_blocks, num_prefix_blocks,
-                       block_size, head_dim).total;
+  return prefix_call(batch, num_prefixes, num_rows, max_tokens, groups, num_kv_heads, num_blocks, num_prefix_blocks,
+                     block_size, head_dim).bytes();
 }
 
 extern "C" int32_t tierkv_prefix_attention(
@@ -930,18 +953,15 @@ extern "C" int32_t tierkv_prefix_attention(
     return fail(TIERKV_ERR_UNSUPPORTED, "more than 4096 requests and prefixes");
   if (int64_t(num_prefix_blocks) * block_size + num_rows > 0x7fffffff - EX_SUB)
     return fail(TIERKV_ERR_UNSUPPORTED, "prefixes of 2^31 tokens or more");
-  const StepLayout step = step_layout(batch, num_prefixes, num_rows, max_tokens, p.groups, num_kv_heads, num_blocks,
-                                      num_prefix_blocks, block_size, head_dim);
-  const PrefixLayout l = step.use ? PrefixLayout{}
-                                  : prefix_layout(batch, num_prefixes, num_rows, max_tokens, p.groups, num_kv_heads,
-                                                  num_blocks, num_prefix_blocks, block_size, head_dim);
+  const PrefixCall way = prefix_call(batch, num_prefixes, num_rows, max_tokens, p.groups, num_kv_heads, num_blocks,
+                                     num_prefix_blocks, block_size, head_dim);
+  const StepLayout& step = way.step;
+  const PrefixLayout& l = way.plan;
   // (a launch has fewer than 2^32 threads)
-  if (l.items * num_kv_heads > 0x7fffffff || step.workgroups > 0xffffffffll / EX_THREADS ||
-      batch * step.own_tiles * num_kv_heads > 0x7fffff00 ||
-      int64_t(num_rows) * num_heads > (0xffffffffll - EX_THREADS) / (head_dim / 4) || std::max(l.units, step.units) > 0x7fffffff)
+  if ((!step.use && (l.items * num_kv_heads > 0x7fffffff || l.units > 0x7fffffff)) ||
+      int64_t(num_rows) * num_heads > (0xffffffffll - EX_THREADS) / (head_dim / 4))
     return fail(TIERKV_ERR_UNSUPPORTED, "grid too large");
-  if (workspace_bytes < (step.use ? std::max<int64_t>(step.total, EX_WS_HEAD) : l.total))
-    return fail(TIERKV_ERR_WORKSPACE, "workspace too small");
+  if (workspace_bytes < way.bytes()) return fail(TIERKV_ERR_WORKSPACE, "workspace too small");
   if (num_rows == 0 || max_tokens == 0) return TIERKV_OK;
   char* ws = reinterpret_cast<char*>(workspace);
   p.err = reinterpret_cast<int32_t*>(ws);
