@@ -1245,6 +1245,17 @@ struct ExJoin {
 // Host
 // ---------------------------------------------------------------------------
 
+// Why the calls with and without shared prefixes do not take these sizes, NULL
+// where they do.
+inline const char* ex_refused(int64_t batch, int64_t rows, int64_t groups, int64_t num_blocks, int64_t bs, int64_t D) {
+  if (bs <= 0 || bs > 64 || D <= 0 || D > 128 || D % 8 != 0)
+    return "block_size must be in [1, 64] and head_dim a multiple of 8 up to 128";
+  if (num_blocks * bs > 0x7fffffff - EX_SUB) return "rows of 2^31 tokens or more";
+  if (batch > EX_MAX_BATCH) return "more than 4096 requests";
+  if (rows * groups > (int64_t(1) << 29)) return "more than 2^29 query rows per kv head";
+  return nullptr;
+}
+
 // Checks the arguments that the calls with and without shared prefixes have in
 // common, and enters them.
 inline int32_t ex_arguments(
@@ -1273,8 +1284,8 @@ inline int32_t ex_arguments(
     return fail(TIERKV_ERR_INVALID, "unknown warm format");
   if (cold_mode != TIERKV_COLD_ZERO_LOGIT && cold_mode != TIERKV_COLD_MASKED)
     return fail(TIERKV_ERR_INVALID, "unknown cold mode");
-  if (block_size <= 0 || block_size > 64 || head_dim <= 0 || head_dim > 128 || head_dim % 8 != 0)
-    return fail(TIERKV_ERR_UNSUPPORTED, "block_size must be in [1, 64] and head_dim a multiple of 8 up to 128");
+  if (const char* why = ex_refused(batch, num_rows, num_heads / num_kv_heads, num_blocks, block_size, head_dim))
+    return fail(TIERKV_ERR_UNSUPPORTED, why);
   if (!hot_k || !hot_v || hot_slots <= 0) return fail(TIERKV_ERR_INVALID, "HOT pools are required");
   if (!warm_k || !warm_v || !k_scale || !v_scale || warm_slots <= 0)
     return fail(TIERKV_ERR_INVALID, "WARM pools and scales are required (pass 1-slot placeholders when empty)");
@@ -1286,11 +1297,6 @@ inline int32_t ex_arguments(
   if (!aligned16(query) || !aligned16(out) || !aligned16(hot_k) || !aligned16(hot_v) || !aligned16(warm_k) ||
       !aligned16(warm_v) || !aligned16(workspace))
     return fail(TIERKV_ERR_INVALID, "query, out, pools and workspace must be 16-byte aligned");
-  if (int64_t(num_blocks) * block_size > 0x7fffffff - EX_SUB)
-    return fail(TIERKV_ERR_UNSUPPORTED, "rows of 2^31 tokens or more");
-  if (batch > EX_MAX_BATCH) return fail(TIERKV_ERR_UNSUPPORTED, "more than 4096 requests");
-  if (int64_t(num_rows) * (num_heads / num_kv_heads) > (int64_t(1) << 29))
-    return fail(TIERKV_ERR_UNSUPPORTED, "more than 2^29 query rows per kv head");
   p.q = query;
   p.qs_t = q_stride_t;
   p.qs_h = q_stride_h;

@@ -856,16 +856,25 @@ constexpr int64_t PX_STEP_MEMORY = 2;
 struct PrefixCall {
   StepLayout step;
   PrefixLayout plan;
+  const char* refused;   // why no such call is taken, or NULL
   int64_t bytes() const { return step.use ? step.bytes() : plan.total; }
 };
 
 static PrefixCall prefix_call(int64_t batch, int64_t prefixes, int64_t rows, int64_t max_tokens, int64_t groups,
                               int64_t kv_heads, int64_t num_blocks, int64_t pre_blocks, int64_t bs, int64_t D) {
   PrefixCall c{};
+  c.refused = ex_refused(batch, rows, groups, num_blocks, bs, D);
+  if (!c.refused && batch + prefixes > EX_MAX_BATCH) c.refused = "more than 4096 requests and prefixes";
+  if (!c.refused && pre_blocks * bs + rows > 0x7fffffff - EX_SUB) c.refused = "prefixes of 2^31 tokens or more";
+  if (c.refused) return c;
   c.step = step_layout(batch, prefixes, rows, max_tokens, groups, kv_heads, num_blocks, pre_blocks, bs, D);
   c.plan = prefix_layout(batch, prefixes, rows, max_tokens, groups, kv_heads, num_blocks, pre_blocks, bs, D);
   c.step.use = c.step.use && c.step.workgroups <= 0xffffffffll / EX_THREADS && c.step.units <= 0x7fffffff &&
                batch * c.step.own_tiles * kv_heads <= 0x7fffff00 && c.step.bytes() <= PX_STEP_MEMORY * c.plan.total;
+  // (a launch has fewer than 2^32 threads)
+  if ((!c.step.use && (c.plan.items * kv_heads > 0x7fffffff || c.plan.units > 0x7fffffff)) ||
+      rows * groups * kv_heads > (0xffffffffll - EX_THREADS) / (D / 4))
+    c.refused = "grid too large";
   return c;
 }
 
@@ -917,12 +926,11 @@ extern "C" int64_t tierkv_prefix_workspace_bytes(int32_t batch, int32_t num_pref
                                                  int32_t num_blocks, int32_t num_prefix_blocks, int32_t block_size,
                                                  int32_t head_dim) {
   if (batch <= 0 || num_prefixes <= 0 || num_rows < 0 || max_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
-      num_heads % num_kv_heads != 0 || num_blocks <= 0 || num_prefix_blocks <= 0 || block_size <= 0 || block_size > 64 ||
-      head_dim <= 0 || head_dim > 128)
-    return -1;
-  const int groups = num_heads / num_kv_heads;
-  return prefix_call(batch, num_prefixes, num_rows, max_tokens, groups, num_kv_heads, num_blocks, num_prefix_blocks,
-                     block_size, head_dim).bytes();
+      num_heads % num_kv_heads != 0 || num_blocks <= 0 || num_prefix_blocks <= 0)
+    return fail(-1, "sizes must be positive, and num_heads a multiple of num_kv_heads");
+  const PrefixCall way = prefix_call(batch, num_prefixes, num_rows, max_tokens, num_heads / num_kv_heads, num_kv_heads,
+                                     num_blocks, num_prefix_blocks, block_size, head_dim);
+  return way.refused ? fail(-1, way.refused) : way.bytes();
 }
 
 extern "C" int32_t tierkv_prefix_attention(
@@ -949,18 +957,11 @@ extern "C" int32_t tierkv_prefix_attention(
     return fail(TIERKV_ERR_INVALID, "null prefix tables");
   if (num_prefixes <= 0 || num_prefix_blocks <= 0 || num_prefix_blocks > prefix_stride)
     return fail(TIERKV_ERR_INVALID, "num_prefixes must be positive and num_prefix_blocks within the prefix tables");
-  if (int64_t(batch) + num_prefixes > EX_MAX_BATCH)
-    return fail(TIERKV_ERR_UNSUPPORTED, "more than 4096 requests and prefixes");
-  if (int64_t(num_prefix_blocks) * block_size + num_rows > 0x7fffffff - EX_SUB)
-    return fail(TIERKV_ERR_UNSUPPORTED, "prefixes of 2^31 tokens or more");
   const PrefixCall way = prefix_call(batch, num_prefixes, num_rows, max_tokens, p.groups, num_kv_heads, num_blocks,
                                      num_prefix_blocks, block_size, head_dim);
+  if (way.refused) return fail(TIERKV_ERR_UNSUPPORTED, way.refused);
   const StepLayout& step = way.step;
   const PrefixLayout& l = way.plan;
-  // (a launch has fewer than 2^32 threads)
-  if ((!step.use && (l.items * num_kv_heads > 0x7fffffff || l.units > 0x7fffffff)) ||
-      int64_t(num_rows) * num_heads > (0xffffffffll - EX_THREADS) / (head_dim / 4))
-    return fail(TIERKV_ERR_UNSUPPORTED, "grid too large");
   if (workspace_bytes < way.bytes()) return fail(TIERKV_ERR_WORKSPACE, "workspace too small");
   if (num_rows == 0 || max_tokens == 0) return TIERKV_OK;
   char* ws = reinterpret_cast<char*>(workspace);

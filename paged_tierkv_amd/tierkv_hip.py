@@ -768,6 +768,8 @@ def _extend_bytes(batch, rows, bound, num_heads, kv_heads, num_blocks, block_siz
     if prefixes or prefix_blocks:
         need = lib.tierkv_prefix_workspace_bytes(batch, prefixes, rows, bound, num_heads, kv_heads, num_blocks,
                                                  prefix_blocks, block_size, head_dim)
+        if need < 0:
+            raise ValueError(f"invalid attention geometry: {_lib.last_error()}.")
     else:
         need = lib.tierkv_extend_workspace_bytes(batch, rows, bound, num_heads, kv_heads, num_blocks, block_size, head_dim)
     if need < 0:

@@ -45,3 +45,29 @@ def test_ordinary_steps_keep_their_way():
     assert size(256, 4, 256, 1, 32, 8, 13, 256, 16, 128) < 64 * MB
     assert size(24, 2, 120, 5, 32, 4, 6, 94, 16, 64) < 16 * MB
     assert size(2, 1, 2, 1, 32, 8, 2, 38, 16, 128) < MB
+
+
+OK = dict(batch=2, prefixes=1, rows=8, most=8, heads=8, kv=2, blocks=8, pblocks=8, bs=16, d=64)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(d=20), dict(d=4), dict(d=132), dict(bs=65),
+    dict(batch=4096), dict(batch=5000, rows=5000, most=1), dict(prefixes=4095), dict(batch=2000, prefixes=2097),
+    dict(blocks=(1 << 27)), dict(pblocks=(1 << 27)), dict(pblocks=(1 << 27) - 1, rows=1 << 20),
+    dict(rows=1 << 28), dict(rows=1 << 27, heads=2), dict(batch=1 << 30, rows=1 << 30), dict(prefixes=1 << 30),
+    dict(blocks=(1 << 31) - 1, pblocks=(1 << 31) - 1),
+])
+def test_sizes_that_no_call_takes_have_no_workspace(kw):
+    """Whatever the call refuses for its sizes has no workspace, and the other
+    way round."""
+    a = {**OK, **kw}
+    assert size(*a.values()) == -1
+    assert call(*a.values(), 1 << 62) in (1, 2) and _lib.last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(d=8), dict(d=128), dict(bs=64), dict(batch=4095), dict(prefixes=4094),
+                                dict(blocks=(1 << 27) - 2), dict(rows=1 << 26, heads=2)])
+def test_sizes_at_the_limits_have_one(kw):
+    a = {**OK, **kw}
+    need = size(*a.values())
+    assert need > 0 and call(*a.values(), need - 1) == 4
