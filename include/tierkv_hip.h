@@ -583,13 +583,15 @@ TIERKV_API int32_t tierkv_extend_attention(
  *      prefix_stride], of the same pools, with prefix_num_blocks (NULL: all
  *      num_prefix_blocks of them) as seq_num_blocks; blocks may also be in
  *      requests' tables, and a prefix may have no request
- * batch + num_prefixes <= 4096.  The prefix adds no position of its own: the
- * keys are in the cache with the positions that they were rotated by.
+ * batch + num_prefixes <= 4096; where max_tokens is 512 rows per kv head or
+ * more, prefix and own tables together hold fewer than 2^31 tokens.  The
+ * prefix adds no position of its own: the keys are in the cache with the
+ * positions that they were rotated by.
  * workspace: as there, tierkv_prefix_workspace_bytes(...) bytes of these
  * sizes (-1 for sizes that no call takes; fewer rows may take more, since
  * their tables are cut into more parts; a small max_tokens takes at most
- * twice what a large one does).  absmax values enter the products
- * exactly, code * 2^e with the rest of the scale on the probabilities; other
+ * twice what a large one does).  absmax values enter the products exactly,
+ * code * 2^e with the rest of the scale on the probabilities; other
  * roundings, arguments, limits and errors as there.  The same inputs give the
  * same bits. */
 TIERKV_API int64_t tierkv_prefix_workspace_bytes(int32_t batch, int32_t num_prefixes, int32_t num_rows,

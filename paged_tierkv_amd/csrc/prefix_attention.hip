@@ -871,6 +871,9 @@ static PrefixCall prefix_call(int64_t batch, int64_t prefixes, int64_t rows, int
   c.plan = prefix_layout(batch, prefixes, rows, max_tokens, groups, kv_heads, num_blocks, pre_blocks, bs, D);
   c.step.use = c.step.use && c.step.workgroups <= 0xffffffffll / EX_THREADS && c.step.units <= 0x7fffffff &&
                batch * c.step.own_tiles * kv_heads <= 0x7fffff00 && c.step.bytes() <= PX_STEP_MEMORY * c.plan.total;
+  // (a lone request's tokens are its prefix's and its own)
+  if (!c.step.use && c.plan.lone > 0 && (pre_blocks + num_blocks) * bs + rows > 0x7fffffff - EX_SUB)
+    c.refused = "prefixes and rows of 2^31 tokens or more together, walked by requests of 512 rows or more";
   // (a launch has fewer than 2^32 threads)
   if ((!c.step.use && (c.plan.items * kv_heads > 0x7fffffff || c.plan.units > 0x7fffffff)) ||
       rows * groups * kv_heads > (0xffffffffll - EX_THREADS) / (D / 4))

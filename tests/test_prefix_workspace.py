@@ -71,3 +71,16 @@ def test_sizes_at_the_limits_have_one(kw):
     a = {**OK, **kw}
     need = size(*a.values())
     assert need > 0 and call(*a.values(), need - 1) == 4
+
+
+def test_a_prefix_and_own_tokens_that_are_walked_together_count_together():
+    """A request of 512 rows per kv head and more walks its prefix and its own
+    tokens as one row, whose places are 32-bit numbers."""
+    half = dict(OK, blocks=1 << 26, pblocks=1 << 26, rows=600)
+    for most, taken in ((600, False), (128, False), (127, True), (16, True)):
+        a = dict(half, most=most)
+        need = size(*a.values())
+        assert (need > 0) == taken, most
+        assert call(*a.values(), need - 1 if taken else 1 << 62) == (4 if taken else 2)
+    a = dict(half, most=600, pblocks=(1 << 26) - 64)      # 1024 tokens fewer
+    assert size(*a.values()) > 0
