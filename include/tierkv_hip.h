@@ -484,7 +484,8 @@ TIERKV_API int32_t tierkv_write_slots(
  * Rows whose position is negative are left out: nothing of them is written.
  * 32-bit arithmetic, one rounding.  apply_rotary_pos_emb and write_hot_tokens
  * (modeling_llama.py:376-377, tierkv_policy.py:934-967) by rows; the norms
- * have no counterpart in the reference.  head_dim up to 256. */
+ * have no counterpart in the reference.  head_dim up to 256, fewer than 2^26
+ * rows. */
 TIERKV_API int32_t tierkv_rotate_rows(
     const void* query, int64_t q_stride_t, int64_t q_stride_h, void* q_out,
     const void* key, int64_t k_stride_t, int64_t k_stride_h, void* k_out,
