@@ -503,12 +503,16 @@ TIERKV_API int32_t tierkv_rotate_rows(
  * written are distinct.
  *   REF_U8: each (row, head) by itself, the codes, scale and zero point of
  *     tierkv_demote_to_warm.
- *   ABSMAX_I8: a block's rows are consecutive in the call.  With p the lowest
+ *   ABSMAX_I8: a block's rows are consecutive in the call, with no skipped row
+ *     among them (what a block's rows in several places of one call give is
+ *     not defined).  With p the lowest
  *     position written of a block and s its scale (0 where p = 0, a block that
  *     starts anew), the scale becomes s' = max(|s|, max|x| / 127) of the rows
  *     written; the rows before p, which the block holds, become rint(code * s /
  *     s') and those written rint(x / s').  Every other row of the block holds
- *     nothing afterwards.
+ *     nothing afterwards.  Each growth rounds held codes again, by up to half
+ *     a step of the scale then: in a block of b tokens filled one by one, the
+ *     values of position p end within (b - p) / 2 steps of the last scale.
  * write_warm_block (tierkv_policy.py:969-1002) by rows.  head_dim up to 256. */
 TIERKV_API int32_t tierkv_quantize_rows(
     const void* key, int64_t k_stride_t, int64_t k_stride_h, const void* value, int64_t v_stride_t, int64_t v_stride_h,

@@ -502,8 +502,10 @@ def quantize_rows(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, w
     position; negative: skipped), as a step writes them
     (``tierkv_quantize_rows``).  ``ref_u8``: each row and head by itself, as
     ``demote_to_warm`` does.  ``absmax_i8``: a block's rows are consecutive in
-    the call; the block's scale grows where they ask for it, and the rows that
-    it holds before them are brought to the new scale."""
+    the call, with no skipped row among them; the block's scale grows where
+    they ask for it, and the rows that it holds before them are brought to the
+    new scale, rounded once more: in a block of b tokens filled one by one, the
+    values of position p end within (b - p) / 2 steps of the last scale."""
     lib = _lib.lib()
     if warm_format not in WARM_FORMATS:
         raise ValueError('warm_format must be "absmax_i8" or "ref_u8".')
