@@ -57,8 +57,8 @@ HIP_SOURCES = {
     # tier branches of its tile loader as in the decode kernel.
     "extend_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-simplifycfg-sink-common=false"],
     # The same tiles, in a loop over items: constants and addresses that the
-    # compiler moved out of it pushed 19 registers to scratch memory (16 prompts
-    # of 512 tokens on 16384: 2046 us, 1933 without).
+    # compiler moved out of it pushed 19 registers to scratch memory, 6 where it
+    # leaves them (16 prompts of 512 tokens on 16384, absmax: 2046 us, 1933).
     "prefix_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-simplifycfg-sink-common=false",
                              "-mllvm", "-disable-machine-licm"],
     "slot_map.hip": [],

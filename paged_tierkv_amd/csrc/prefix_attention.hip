@@ -27,17 +27,22 @@
 //   * prefix_join_kernel adds up the parts of rows that have several.
 //
 // Bound: vector instructions beside the matrix products for prompts (16 of up
-// to 512 tokens on a prefix of 16384, 32 heads on 8 kv heads of 128: 1933 us,
-// 667 TFLOP/s); for steps the requests' own tokens at the memory rate, and 7 us
-// that a workgroup takes to start and end, one at a time per CU (64 single
-// tokens on a prefix of 8192: 42 us; 256 on 4 of 4096: 80; 24 x 5 on
-// 1501: 27; 2 on 600: 17).
+// to 512 tokens on a prefix of 16384, 32 heads on 8 kv heads of 128: 1937 us,
+// 665 TFLOP/s; the reference format 2460); for steps the requests' own tokens
+// at the memory rate, and 7 us that a workgroup takes to start and end, one at
+// a time per CU (64 single tokens on a prefix of 8192: 44 us; 256 on 4 of 4096,
+// reference format: 83; 24 x 5 on 1501: 27; 2 on 600: 17); between them the
+// plan and wide tiles that are not full (32 requests of 100 tokens on 4096: 368
+// us, 109 at the products' rate).  All of calls replayed from a graph.
 
 #include "extend_tile.h"
 
 namespace tierkv {
 
-constexpr int PX_LONE = 512;            // rows (tokens times heads of a kv head) from which a request walks its prefix itself
+// Rows (tokens times heads of a kv head) from which a request walks its prefix
+// itself (32 requests on a prefix of 4096, 4 heads per kv head: 127 tokens each,
+// shared, 397 us; 128, by themselves, 343).
+constexpr int PX_LONE = 512;
 constexpr int PX_KW = 2;                // waves of a narrow item
 constexpr int PX_SIDE = EX_WAVES / PX_KW;   // narrow items side by side
 constexpr int PX_TAIL = 4;              // items that cutting the last tiles adds, at most, for each place
@@ -410,7 +415,10 @@ __global__ __launch_bounds__(EX_THREADS) void prefix_join_kernel(ExtendParams p)
 // of 256; how many there are follows from the requests' prefixes, which each
 // workgroup of a slot reads.  Two launches: the parts, and their join.
 
-constexpr int PX_STEP = 64;        // rows of a request, at most: tiles of 32 (and what prefix_call says)
+// Rows of a request, at most: tiles of 32 (32 requests on a prefix of 4096, 4
+// heads per kv head: 16 tokens each, a step, 74 us; 17, planned, 105), and what
+// prefix_call says.
+constexpr int PX_STEP = 64;
 constexpr int PX_LIST = 416;       // sub-tiles that a workgroup lists
 constexpr int PX_MOST = 8;         // requests' parts side by side in a workgroup, where it is not one
 

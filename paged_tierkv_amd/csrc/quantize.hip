@@ -803,8 +803,8 @@ int32_t launch_promote(const DequantJobs& q, int n_grid, hipStream_t stream) {
 // k / v [rows, kv_heads, D] becomes row slots[r] = slot * bs + position of the
 // WARM pools.  bf16 rows become fp16 first, as where they are written HOT.
 // Bound: memory and one chain of slots, rows, scale and codes.  8191 bf16 rows
-// of 8 heads of 128, 51 MB, take 14 us (reference format) and 19 us (absmax);
-// 96 single tokens in open absmax blocks 8 us.  One element per thread took 240 and 60.
+// of 8 heads of 128, 51 MB, take 13 us (reference format) and 19 us (absmax);
+// 96 single tokens in open absmax blocks 6 us.  One element per thread took 240 and 60.
 // ---------------------------------------------------------------------------
 struct QuantRows {
   const void* src[2];

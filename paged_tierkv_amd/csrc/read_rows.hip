@@ -12,10 +12,14 @@
 // 7), and blocks that end before the first token asked for, even if full, end
 // at once (64 windows of 64 tokens in 2000: 21 -> 14 us).
 // Bound: memory.  32768 tokens of 8 heads of 128, a tenth HOT, six tenths WARM
-// and the rest zeros, 188 MB, take 36 us where the inputs are not in the caches
-// and 31 where they are; with one element per thread 334.  Two blocks per
-// workgroup take 11 us for 500 tokens where one takes 7, and four 36 for
-// 32768.
+// and the rest zeros, 188 MB, take 41 to 43 us where two contexts are read in
+// turn and 35 where one is read again; with one element per thread 334.  Two
+// blocks per workgroup take 11 us for 500 tokens where one takes 7, and four 36
+// for 32768 (read again).
+// The sums grow with the square of the context, the launch with the tables'
+// width: 262144 tokens take 493 us (3.1 TB/s), 2^20 2775 (2.2), their last 300
+// 23 and 72; 250 tokens of each of 32 requests 14 us in tables of 16 blocks, 24
+// of 1024 and 118 of 8192.
 
 #include "tierkv_common.h"
 

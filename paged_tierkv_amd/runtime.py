@@ -533,6 +533,10 @@ class BatchedTieredKVRuntime:
         ``q_weight``, ``k_weight``, ``eps``, ``attention_scaling``,
         ``interleaved``) -- then q and k are the projections, of v's type, and
         are normed and rotated by their positions on the way into the cache.
+        Their angles are formed in 64 bits, while ``decode_layer(rope=)`` turns
+        by the 16-bit cos and sin that it is given, in the model library's
+        order of 16-bit operations: keys of one cache that both have written
+        are turned by angles that differ by those roundings.
         A call that cannot be taken raises before anything changes: ValueError
         for its tensors, RuntimeError when the tokens exceed max_seq_len or the
         free HOT slots (tokens of several calls without a tick), and under
