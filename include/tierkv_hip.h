@@ -594,11 +594,11 @@ TIERKV_API int32_t tierkv_extend_attention(
  * positions that they were rotated by.
  * workspace: as there, tierkv_prefix_workspace_bytes(...) bytes of these
  * sizes (-1 for sizes that no call takes; fewer rows may take more, since
- * their tables are cut into more parts; a small max_tokens takes at most
- * twice what a large one does).  absmax values enter the products exactly,
- * code * 2^e with the rest of the scale on the probabilities; other
- * roundings, arguments, limits and errors as there.  The same inputs give the
- * same bits. */
+ * their tables are cut into more parts; a max_tokens of up to 64 rows per kv
+ * head takes at most twice what a larger one does).  absmax values enter the
+ * products exactly, code * 2^e with the rest of the scale on the
+ * probabilities; other roundings, arguments, limits and errors as there.  The
+ * same inputs give the same bits. */
 TIERKV_API int64_t tierkv_prefix_workspace_bytes(int32_t batch, int32_t num_prefixes, int32_t num_rows,
                                                  int32_t max_tokens, int32_t num_heads, int32_t num_kv_heads,
                                                  int32_t num_blocks, int32_t num_prefix_blocks, int32_t block_size,

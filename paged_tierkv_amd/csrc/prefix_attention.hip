@@ -857,9 +857,9 @@ static StepLayout step_layout(int64_t batch, int64_t prefixes, int64_t rows, int
 // PX_STEP_MEMORY of the plan's workspace, or of a launch's 2^32 threads, calls
 // of few tokens are planned too.  Around that size tables are mostly far wider
 // than their rows, which a step's workgroups pay for and the plan's do not: 256
-// single tokens with 256 of their own in tables of 16384 blocks, 1.4 GB, 501 us as a step and
-// 131 planned; full rows lose by it (64 whose tables of 16384 are full, 1.4
-// times the plan's: 11.0 ms as a step, 20.9 planned).
+// single tokens with 256 of their own in tables of 16384 blocks, 1.4 GB, 501 us
+// as a step and 131 planned; full rows lose by it (64 whose tables of 16384 are
+// full, 1.4 times the plan's: 11.0 ms as a step, 20.9 planned).
 constexpr int64_t PX_STEP_MEMORY = 2;
 struct PrefixCall {
   StepLayout step;
